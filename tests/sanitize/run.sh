@@ -21,5 +21,5 @@ done
 for p in $pids; do wait $p; done
 clang=/opt/rocm/lib/llvm/bin/clang++
 $clang -fsanitize=address -fsanitize=undefined -fno-sanitize-recover=undefined -g -O1 -std=c++17 -c "$here/abi_driver.cpp" -o "$out/abi_driver.o"
-$HIPCC --offload-arch=gfx950 -fsanitize=address -fsanitize=undefined "$out"/*.o -o "$out/abi_driver"
+$HIPCC --offload-arch=gfx950 -Xarch_host -fsanitize=address -Xarch_host -fsanitize=undefined "$out"/*.o -o "$out/abi_driver"
 ASAN_OPTIONS=detect_leaks=0:abort_on_error=1 UBSAN_OPTIONS=print_stacktrace=1:halt_on_error=1 "$out/abi_driver" "${1:-3000}"
