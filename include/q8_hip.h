@@ -381,6 +381,39 @@ int q8_attn_fwd(const void* q, const void* k, const void* v, void* o, const int3
  */
 int q8_attn_set_config(int cfg);
 
+/*
+ * Layer norm over the last dimension and its backward (no counterpart in the reference, whose norm is q8_rmsnorm's).
+ *   mu = mean_j x[r,j];  rstd = 1 / sqrt(mean_j (x[r,j] - mu)^2 + eps);  h = (x - mu) * rstd;  y = h * w + b
+ *   u = g * w;  dx = rstd * (u - mean(u) - h * mean(u * h));  dw_j = sum_r g h;  db_j = sum_r g   (fixed order, no atomics)
+ * x, y, grad, dx of element type dt in {BF16, F16, F32}; y, dx [rows, dim] contiguous; x and grad with a row stride in
+ * elements (at least dim; any value for one row). w, b, dw, db [dim], all of w_dtype: F32 or dt; NULL = 1, 0, not wanted.
+ * mean, rstd fp32 [rows] (forward: both or neither). 1 <= dim <= 32768; every pointer aligned to its element (rows that are
+ * 16-byte aligned with dim % 8 == 0 run on 16-byte accesses). The backward with dw or db takes a workspace of
+ * q8_layernorm_backward_workspace(rows, dim) bytes (negative: an error code) that it writes before it reads it.
+ */
+int q8_layernorm(const void* x, int dt, int64_t x_row_stride, const void* w, const void* b, int w_dtype, void* y, float* mean,
+                 float* rstd, int64_t rows, int dim, float eps, q8_stream_t stream);
+int64_t q8_layernorm_backward_workspace(int64_t rows, int dim);
+int q8_layernorm_backward(const void* grad, int64_t grad_row_stride, const void* x, int dt, int64_t x_row_stride, const void* w,
+                          int w_dtype, const float* mean, const float* rstd, void* dx, void* dw, void* db, void* workspace,
+                          int64_t workspace_bytes, int64_t rows, int dim, q8_stream_t stream);
+
+/*
+ * Rotary positions from positions and frequencies (q8_rope takes tables of x's shape instead), queries and keys in one launch.
+ *   a = position * inv_freq[i], i < rotary_dim / 2;  (u, v) -> factor * (u cos a - v sin a, v cos a + u sin a)
+ *   (u, v): elements (i, i + rotary_dim / 2) with half_layout, else (2 i, 2 i + 1); elements from rotary_dim on are copied;
+ *   backward: the transposed rotation (-sin a).
+ * q, k [batch, heads, tokens, dim] of dt in {BF16, F16, F32} with element strides {batch, head, token} (0 or more, unit last
+ * stride); the strides are read by the call, on the host. An output may be its input; it may not overlap it otherwise.
+ * q_heads or k_heads 0: without that tensor. positions: int32 / int64 (pos_bits) [batch, tokens] with pos_row_stride elements
+ * between batch rows (0: one row for all), NULL = 0 .. tokens - 1. inv_freq: fp64, radians per position.
+ * dim <= 512, rotary_dim even and 2 .. dim. The angle is formed in fp64 and reduced there; sine, cosine and products are fp32.
+ */
+int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int q_heads, const void* k,
+              const int64_t* k_strides, void* k_out, const int64_t* k_out_strides, int k_heads, int dt, const void* positions,
+              int pos_bits, int64_t pos_row_stride, const double* inv_freq, int rotary_dim, int half_layout, float factor,
+              int backward, int64_t batch, int64_t tokens, int dim, q8_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,6 +3,8 @@ pybind11 modules (q8_kernels_cuda.{gemm,quantizer,ops,flash_attention}._C), impl
 C ABI of libq8_hip.so. Outputs are allocated here with torch (as the reference's C++ glue does), inputs
 are borrowed, launches go to the current torch stream of the input's device and do not synchronise.
 """
+import contextlib
+import ctypes
 from typing import List, Optional
 
 import torch
@@ -45,6 +47,11 @@ def _as_rows(x):
     if x2.stride(-1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
         x2 = x2.contiguous()
     return x2
+
+
+def _on(device):
+    """The context in which calls go to `device`: nothing to do where it is the current one (the guard costs microseconds)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 # ----------------------------------------------------------------------------- quantizer._C
@@ -759,3 +766,126 @@ def rms_norm_backward(x_normed: torch.Tensor, x_norms: torch.Tensor, grad_out: t
                                                   _DT[g2.dtype], _ptr(w),
                                                   out.data_ptr(), _DT[out_type], rows, dim, _stream(x_normed)))
     return out.reshape(x_normed.shape)
+
+
+# ----------------------------------------------------------------------------- layer norm
+
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _norm_params(x, weight, bias, who):
+    """The parameters, contiguous, and their type's code; both are float32 or both of x's type."""
+    out, dt = [], None
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            if t.device != x.device:
+                raise RuntimeError("%s: %s must be on %s" % (who, name, x.device))
+            if t.dim() != 1 or t.shape[0] != x.shape[-1]:
+                raise RuntimeError("%s: %s must have shape [%d], got %s" % (who, name, x.shape[-1], list(t.shape)))
+            if t.dtype not in (torch.float32, x.dtype) or (dt is not None and t.dtype != dt):
+                raise RuntimeError("%s: weight and bias must both be float32 or both of x's type %s" % (who, x.dtype))
+            dt = t.dtype
+            t = t.contiguous()
+        out.append(t)
+    return out[0], out[1], _DT[torch.float32 if dt is None else dt]
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5, *,
+               stats: bool = True) -> List[Optional[torch.Tensor]]:
+    """[y (x.shape, x's type), mean, rstd (x.shape[:-1], float32)]; stats=False: the last two are None."""
+    _require_gpu(x, "x")
+    if x.dtype not in _FLOATS:
+        raise RuntimeError("layer_norm: x must be bfloat16, float16 or float32, got %s" % x.dtype)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError("layer_norm: x must have a last dimension of one element or more")
+    weight, bias, wd = _norm_params(x, weight, bias, "layer_norm")
+    x2 = _as_rows(x)
+    rows, dim = x2.shape
+    with _on(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2)) if stats else (None, None)
+        _lib.check(_lib.lib().q8_layernorm(x2.data_ptr(), _DT[x.dtype], x2.stride(0), _ptr(weight), _ptr(bias), wd, y.data_ptr(), _ptr(mean),
+                                           _ptr(rstd), rows, dim, float(eps), _stream(x)))
+    return [y, mean, rstd]
+
+
+def layer_norm_backward(grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                        mean: torch.Tensor, rstd: torch.Tensor, needs=(True, True, True)) -> List[Optional[torch.Tensor]]:
+    """[dx, dweight, dbias] of layer_norm, None where not needed or absent; x, mean and rstd as the forward had and gave them."""
+    _require_gpu(grad, "grad")
+    if grad.shape != x.shape or grad.dtype != x.dtype or grad.device != x.device:
+        raise RuntimeError("layer_norm_backward: grad must match x")
+    weight, bias, wd = _norm_params(x, weight, bias, "layer_norm_backward")
+    if any(t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device or not t.is_contiguous() for t in (mean, rstd)):
+        raise RuntimeError("layer_norm_backward: mean and rstd must be the forward's")
+    x2, g2 = _as_rows(x), _as_rows(grad)
+    rows, dim = x2.shape
+    L = _lib.lib()
+    with _on(x.device):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
+        dw = torch.empty_like(weight) if needs[1] and weight is not None else None
+        db = torch.empty_like(bias) if needs[2] and bias is not None else None
+        size = L.q8_layernorm_backward_workspace(rows, dim) if dw is not None or db is not None else 0
+        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size > 0 else None
+        _lib.check(L.q8_layernorm_backward(g2.data_ptr(), g2.stride(0), x2.data_ptr(), _DT[x.dtype], x2.stride(0), _ptr(weight), wd, mean.data_ptr(),
+                                           rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(work), max(size, 0), rows, dim, _stream(x)))
+    return [dx, dw, db]
+
+
+# ----------------------------------------------------------------------------- rotary positions by position and frequency
+
+_Strides3 = ctypes.c_int64 * 3
+
+
+def _unit_last(t):
+    """t itself where its last stride is 1 (a size of one element counts), else a contiguous copy."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _like(t):
+    """An uninitialised tensor in t's memory order with unit last stride."""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Optional[torch.Tensor], inv_freq: torch.Tensor,
+           half: bool = True, factor: float = 1.0, *, backward: bool = False) -> List[Optional[torch.Tensor]]:
+    """[q', k'] of q [B, H, T, D] and k [B, Hkv, T, D] (either may be None), see functional.rotary.apply_rotary; backward: the
+    transposed rotation, which takes the gradients of q' and k' to those of q and k."""
+    x = q if q is not None else k
+    if x is None:
+        raise RuntimeError("rotary: q or k is needed")
+    for t, name in ((q, "q"), (k, "k")):
+        if t is None:
+            continue
+        _require_gpu(t, name)
+        if t.dim() != 4 or t.dtype not in _FLOATS:
+            raise RuntimeError("rotary: %s must be [B, heads, T, D] in bfloat16, float16 or float32" % name)
+        if t.dtype != x.dtype or t.device != x.device or (t.shape[0], t.shape[2], t.shape[3]) != (x.shape[0], x.shape[2], x.shape[3]):
+            raise RuntimeError("rotary: q and k must agree in type, device, batch, tokens and head size")
+    batch, _, tokens, dim = x.shape
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != x.device:
+        raise RuntimeError("rotary: inv_freq must be float64 [R / 2] on %s" % x.device)
+    inv_freq = inv_freq.contiguous()
+    bits, row = 0, 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != x.device:
+            raise RuntimeError("rotary: positions must be int32 or int64 on %s" % x.device)
+        if positions.shape != (tokens,) and positions.shape != (batch, tokens) and positions.shape != (1, tokens):
+            raise RuntimeError("rotary: positions must be [%d] or [%d, %d], got %s" % (tokens, batch, tokens, list(positions.shape)))
+        bits = 32 if positions.dtype == torch.int32 else 64
+        if tokens > 1 and positions.stride(-1) != 1:
+            positions = positions.contiguous()
+        if positions.dim() == 2 and positions.shape[0] > 1:
+            row = positions.stride(0)
+            if 0 < row < tokens:
+                positions = positions.contiguous()
+                row = tokens
+    with _on(x.device):
+        q, k = (None if t is None else _unit_last(t) for t in (q, k))
+        q_out, k_out = (None if t is None else _like(t) for t in (q, k))
+        st = [None if t is None else _Strides3(*t.stride()[:3]) for t in (q, q_out, k, k_out)]
+        _lib.check(_lib.lib().q8_rotary(_ptr(q), st[0], _ptr(q_out), st[1], 0 if q is None else q.shape[1], _ptr(k), st[2], _ptr(k_out), st[3],
+                                        0 if k is None else k.shape[1], _DT[x.dtype], _ptr(positions), bits, row, inv_freq.data_ptr(),
+                                        2 * inv_freq.shape[0], int(half), factor, int(backward), batch, tokens, dim, _stream(x)))
+    return [q_out, k_out]

@@ -21,6 +21,7 @@ Q8_GEMM_KERNEL_PERSIST256, Q8_GEMM_KERNEL_PERSIST192, Q8_GEMM_KERNEL_RESIDUAL = 
 
 _c = ctypes
 _vp, _i, _i64, _f = _c.c_void_p, _c.c_int, _c.c_int64, _c.c_float
+_i64p = _c.POINTER(_i64)
 
 # name -> (restype, argtypes): every symbol include/q8_hip.h declares
 SIGNATURES = {
@@ -54,6 +55,10 @@ SIGNATURES = {
     "q8_gemm_set_config": (_i, [_i]),
     "q8_attn_set_config": (_i, [_i]),
     "q8_gemm_last_kernel": (_i, []),
+    "q8_layernorm": (_i, [_vp, _i, _i64, _vp, _vp, _i, _vp, _vp, _vp, _i64, _i, _f, _vp]),
+    "q8_layernorm_backward_workspace": (_i64, [_i64, _i]),
+    "q8_layernorm_backward": (_i, [_vp, _i64, _vp, _i, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _vp]),
+    "q8_rotary": (_i, [_vp, _i64p, _vp, _i64p, _i, _vp, _i64p, _vp, _i64p, _i, _i, _vp, _i, _i64, _vp, _i, _i, _f, _i, _i64, _i64, _i, _vp]),
     "q8_attn_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _f, _i, _i, _vp]),
 }
 
