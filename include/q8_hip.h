@@ -414,6 +414,33 @@ int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_
               int pos_bits, int64_t pos_row_stride, const double* inv_freq, int rotary_dim, int half_layout, float factor,
               int backward, int64_t batch, int64_t tokens, int dim, q8_stream_t stream);
 
+/*
+ * 16-bit cross attention and its backward (no counterpart in the reference, whose attention is q8_attn_fwd's).
+ *   s_ij = softmax_scale q_i . k_j over the keys j that count;  p = softmax(s);  o_i = sum_j p_ij v_j  (zeros if none counts)
+ *   lse_i = log2 sum_j exp2(log2(e) s_ij)  (+inf if none counts), what the backward forms p from again
+ *   dv = p^T do;  dp = do v^T;  ds = p (dp - rowsum(do o));  dq = softmax_scale ds k;  dk = softmax_scale ds^T q
+ * q, o, grad, dq [B, H, M, D]; k, v, dk, dv [B, Hkv, N, D]: BF16 or F16, element strides {batch, head, token} (read by the call,
+ * on the host; 0 or more, multiples of 8 where there is more than one index), unit last stride, 16-byte aligned. H a multiple
+ * of Hkv: heads h (H / Hkv) .. share key head h, whose gradients are summed over them. D a multiple of 8 up to 128.
+ * kv_lens: int32 [B], clamped to 0 .. N, or NULL = N; key_mask: one byte per key [B, N] with a row stride in bytes, 0 = does
+ * not count, or NULL. Keys and values that do not count are not read into any result; their gradients are zeros.
+ * lse: fp32 [B, H, M] (forward: NULL = not wanted). softmax_scale positive and finite.
+ * The workspaces hold partial sums (the forward's: 0 bytes where none are needed); a negative size is an error code. They are
+ * written before they are read and may be reused as soon as the call's work on the stream is done.
+ */
+int64_t q8_cross_attn_workspace(int64_t B, int H, int Hkv, int M, int N, int D);
+int q8_cross_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                  const int64_t* v_strides, void* o, const int64_t* o_strides, float* lse, const int32_t* kv_lens,
+                  const uint8_t* key_mask, int64_t mask_row_stride, int dt, float softmax_scale, int64_t B, int H, int Hkv, int M,
+                  int N, int D, void* workspace, int64_t workspace_bytes, q8_stream_t stream);
+int64_t q8_cross_attn_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D);
+int q8_cross_attn_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides, const void* k,
+                           const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* o,
+                           const int64_t* o_strides, const float* lse, void* dq, const int64_t* dq_strides, void* dk,
+                           const int64_t* dk_strides, void* dv, const int64_t* dv_strides, const int32_t* kv_lens,
+                           const uint8_t* key_mask, int64_t mask_row_stride, int dt, float softmax_scale, int64_t B, int H, int Hkv,
+                           int M, int N, int D, void* workspace, int64_t workspace_bytes, q8_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

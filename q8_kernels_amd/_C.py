@@ -889,3 +889,91 @@ def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Opti
                                         0 if k is None else k.shape[1], _DT[x.dtype], _ptr(positions), bits, row, inv_freq.data_ptr(),
                                         2 * inv_freq.shape[0], int(half), factor, int(backward), batch, tokens, dim, _stream(x)))
     return [q_out, k_out]
+
+
+# ----------------------------------------------------------------------------- 16-bit cross attention
+
+def _chunks(t):
+    """t itself where its rows are 16-byte chunks the kernels can address (unit last stride, the others multiples of 8
+    elements, 16-byte aligned), else a contiguous copy."""
+    st, shape = t.stride(), t.shape
+    if (st[3] == 1 and t.data_ptr() % 16 == 0 and (st[0] % 8 == 0 or shape[0] == 1) and (st[1] % 8 == 0 or shape[1] == 1)
+            and (st[2] % 8 == 0 or shape[2] == 1)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _attn_check(q, k, v, kv_lens, key_mask, who):
+    """(kv_lens, key_mask with unit last stride, its row stride) after the checks the C entry points cannot make"""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _require_gpu(t, name)
+        if t.dim() != 4:
+            raise RuntimeError("%s: %s must be [B, heads, tokens, D], got %s" % (who, name, list(t.shape)))
+        if t.dtype not in (torch.bfloat16, torch.float16) or t.dtype != q.dtype or t.device != q.device:
+            raise RuntimeError("%s: q, k and v must be bfloat16 or float16, all of one type, on one device" % who)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise RuntimeError("%s: q %s does not go with k %s and v %s" % (who, list(q.shape), list(k.shape), list(v.shape)))
+    b, n = k.shape[0], k.shape[2]
+    if kv_lens is not None:
+        if kv_lens.dtype != torch.int32 or kv_lens.shape != (b,) or kv_lens.device != q.device:
+            raise RuntimeError("%s: kv_lens must be int32 [%d] on %s" % (who, b, q.device))
+        kv_lens = kv_lens.contiguous()
+    row = 0
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or key_mask.shape != (b, n) or key_mask.device != q.device:
+            raise RuntimeError("%s: key_mask must be bool [%d, %d] on %s" % (who, b, n, q.device))
+        if n > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        row = key_mask.stride(0)
+    return kv_lens, key_mask, row
+
+
+def _strides(t):
+    return _Strides3(*t.stride()[:3])
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, kv_lens: Optional[torch.Tensor] = None,
+                    key_mask: Optional[torch.Tensor] = None, *, stats: bool = True) -> List[Optional[torch.Tensor]]:
+    """[o (q's shape, type and memory order), lse (float32 [B, H, M], log2 of the sum of 2^(score * log2 e); +inf where no key
+    counts; None without stats)], see functional.cross_attention.cross_attention."""
+    kv_lens, key_mask, row = _attn_check(q, k, v, kv_lens, key_mask, "cross_attention")
+    (b, h, m, d), hk, n = q.shape, k.shape[1], k.shape[2]
+    L = _lib.lib()
+    with _on(q.device):
+        size = L.q8_cross_attn_workspace(b, h, hk, m, n, d)
+        if size < 0:
+            _lib.check(size)
+        q, k, v = _chunks(q), _chunks(k), _chunks(v)
+        o = _like(q)
+        lse = torch.empty((b, h, m), dtype=torch.float32, device=q.device) if stats else None
+        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        _lib.check(L.q8_cross_attn(q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(), _strides(o),
+                                   _ptr(lse), _ptr(kv_lens), _ptr(key_mask), row, _DT[q.dtype], softmax_scale, b, h, hk, m, n, d, _ptr(work), size,
+                                   _stream(q)))
+    return [o, lse]
+
+
+def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                             softmax_scale: float, kv_lens: Optional[torch.Tensor] = None,
+                             key_mask: Optional[torch.Tensor] = None) -> List[torch.Tensor]:
+    """[dq, dk, dv] in the memory orders of q, k and v; o and lse as the forward gave them."""
+    who = "cross_attention_backward"
+    kv_lens, key_mask, row = _attn_check(q, k, v, kv_lens, key_mask, who)
+    (b, h, m, d), hk, n = q.shape, k.shape[1], k.shape[2]
+    if any(t.shape != q.shape or t.dtype != q.dtype or t.device != q.device for t in (grad, o)):
+        raise RuntimeError("%s: grad and o must match q" % who)
+    if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        raise RuntimeError("%s: lse must be the forward's" % who)
+    L = _lib.lib()
+    with _on(q.device):
+        size = L.q8_cross_attn_backward_workspace(b, h, hk, m, n, d)
+        if size < 0:
+            _lib.check(size)
+        q, k, v, o, grad = _chunks(q), _chunks(k), _chunks(v), _chunks(o), _chunks(grad)
+        dq, dk, dv = _like(q), _like(k), _like(v)
+        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        args = [x for t in (grad, q, k, v, o) for x in (t.data_ptr(), _strides(t))] + [lse.data_ptr()]
+        args += [x for t in (dq, dk, dv) for x in (t.data_ptr(), _strides(t))]
+        _lib.check(L.q8_cross_attn_backward(*args, _ptr(kv_lens), _ptr(key_mask), row, _DT[q.dtype], softmax_scale, b, h, hk, m, n, d, _ptr(work), size,
+                                            _stream(q)))
+    return [dq, dk, dv]

@@ -1,0 +1,274 @@
+// 16-bit cross attention, forward: O = softmax(scale Q K^T) V over the keys that count, any number of queries and keys.
+//
+// One pass over the keys with the running maximum and sum of the softmax. A workgroup holds 128 query rows, 32 a wave; Q^T
+// stays in registers, K and V go through LDS in tiles of 64 keys (double-buffered, the next tile's loads in flight during the
+// present one's arithmetic). S^T = K Q^T leaves a query's scores in one lane pair, P^T = exp2(S^T c - m) goes on as the B
+// operand of O^T = V^T P^T without leaving registers. Scores, maxima, sums and O are fp32; P is rounded to 16 bits for the
+// product (as its operand has to be), relative to a maximum that trails the running one by at most 2^8, so the rounding is
+// a relative one. O is rescaled only when the maximum has grown beyond that.
+//
+// Few row blocks: the keys of a unit are divided over several workgroups, whose unnormalised results, maxima and sums a
+// second kernel joins.
+#include "cross_attn_common.h"
+
+namespace q8 {
+
+struct XFwd {
+    XTensor q, k, v;
+    XOut o;
+    float* lse;          // [units, R]: log2 of the sum of exp2 (c s); +inf: no key counts. NULL: not wanted
+    XKeys keys;
+    float c;             // softmax scale * log2 e
+    int Hkv, G, M, D, R;
+    int units, row_blocks, splits;
+    float *part, *pm, *pl;  // splits > 1: [splits, units, R, D], [splits, units, R] twice
+};
+
+template <int DT, int DP>
+__global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
+    constexpr int LD = DP + 16, KS = DP / 16, DTL = DP / 32;
+    __shared__ __align__(16) uint16_t kt[2][kXTile * LD], vt[2][kXTile * LD];
+    __shared__ __align__(16) float bias[2][kXTile];
+    unsigned item;
+    if (!xcd_item((unsigned)a.units * a.row_blocks * a.splits, item)) return;
+    const int rb = item % a.row_blocks, split = (item / a.row_blocks) % a.splits, unit = item / (a.row_blocks * a.splits);
+    const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
+
+    const int len = a.keys.length(b);
+    const uint8_t* mask = a.keys.row(b);
+    const int tiles = (len + kXTile - 1) / kXTile, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+
+    v4u qf[KS];
+    {
+        const int g = row < a.R ? row / a.M : 0, m = row - g * a.M;
+        const uint16_t* p = a.q.p + b * a.q.sb + (int64_t)(hk * a.G + g) * a.q.sh + m * a.q.st + half * 8;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = (row < a.R && s * 16 + half * 8 < a.D) ? *reinterpret_cast<const v4u*>(p + s * 16) : v4u{0u, 0u, 0u, 0u};
+    }
+    const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+    const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+    Stage<DP> ks, vs;
+    auto load = [&](int t) {
+        auto at = [&](const uint16_t* p, int64_t st) {
+            return [=](int r) -> const uint16_t* {
+                const int key = t * kXTile + r;
+                return key < len && (mask == nullptr || mask[key]) ? p + key * st : nullptr;
+            };
+        };
+        ks.load(at(kp, a.k.st), a.D);
+        vs.load(at(vp, a.v.st), a.D);
+    };
+    auto store = [&](int t) {
+        ks.store(kt[t & 1]);
+        vs.store(vt[t & 1]);
+        if (threadIdx.x < kXTile) {
+            const int key = t * kXTile + threadIdx.x;
+            bias[t & 1][threadIdx.x] = key < len && (mask == nullptr || mask[key]) ? 0.f : -__builtin_inff();
+        }
+    };
+
+    v16f acc[DTL];
+#pragma unroll
+    for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
+    float m = -3.0e38f, l = 0.f;  // in units of log2; the sum over this lane's half of the keys
+
+    if (t0 < t1) {
+        load(t0);
+        store(t0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        if (t + 1 < t1) load(t + 1);
+        const uint16_t *kl = kt[t & 1], *vl = vt[t & 1];
+        const bool masked = mask != nullptr || (t + 1) * kXTile > len;
+        v16f s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[u] = splat16(0.f);
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v4f w = *reinterpret_cast<const v4f*>(&bias[t & 1][u * 32 + i * 8 + half * 4]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[u][i * 4 + j] = w[j];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<LD>(kl, u * 32, e * 16, lane), qf[e], s[u]);
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = max_ieee(top, s[0][i]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = max_ieee(top, s[1][i]);
+        top = half_pair_max(top) * a.c;
+        const bool grown = top > m + 8.f;
+        if (__builtin_amdgcn_ballot_w64(grown) != 0) {
+            const float next = grown ? top : m, f = __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DTL; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], a.c, -m));
+                l += s[u][i];
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const v4u p = pack_step<DT>(s[u], k);
+#pragma unroll
+                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<LD>(vl, u * 32 + k * 16, d * 32, lane), p, acc[d]);
+            }
+        }
+        if (t + 1 < t1) store(t + 1);
+        __syncthreads();
+    }
+    {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (a.splits > 1) {
+        if (row < a.R) {
+            const int64_t at = ((int64_t)split * a.units + unit) * a.R + row;
+            if (half == 0) { a.pm[at] = m; a.pl[at] = l; }
+            float* p = a.part + at * a.D;
+#pragma unroll
+            for (int d = 0; d < DTL; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = d * 32 + i * 8 + half * 4;
+                    if (e < a.D) *reinterpret_cast<v4f*>(p + e) = v4f{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                }
+        }
+        return;
+    }
+    if (a.lse != nullptr && row < a.R && half == 0)
+        a.lse[(int64_t)unit * a.R + row] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    // (the tile buffers are free: every wave has passed the last barrier of the loop)
+    static_assert(kXWaves * 32 * (DP + 8) <= 2 * kXTile * LD, "the output tiles fit the K buffers");
+    store_tile<DT, DP>(acc, inv, kt[0] + wave * 32 * (DP + 8), a.D, lane, [&](int r) -> uint16_t* {
+        const int n = row0 + r;
+        if (n >= a.R) return nullptr;
+        const int g = n / a.M;
+        return a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (n - g * a.M) * a.o.st;
+    });
+}
+
+// Joins the parts of a row: weights exp2(m_i - max m). 32 lanes a row, 4 elements a lane.
+template <int DT>
+__global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
+    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), all = (int64_t)a.units * a.R;
+    if (n >= all) return;
+    const int e = (threadIdx.x & 31) * 4;
+    float m = -3.0e38f, l = 0.f;
+    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.pm[i * all + n]);
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < a.splits; ++i) {
+        const float w = __builtin_amdgcn_exp2f(a.pm[i * all + n] - m);
+        l += w * a.pl[i * all + n];
+        if (e < a.D) {
+            const v4f p = *reinterpret_cast<const v4f*>(a.part + (i * all + n) * a.D + e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += w * p[j];
+        }
+    }
+    if (a.lse != nullptr && e == 0) a.lse[n] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
+    if (e >= a.D) return;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int unit = (int)(n / a.R), r = (int)(n - (int64_t)unit * a.R), g = r / a.M, b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    uint16_t* p = a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (r - g * a.M) * a.o.st;
+    *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
+}
+
+// Workgroups that share the keys of a row block: until about 512 run (two on every CU), four tiles each or more.
+static int fwd_splits(int64_t blocks, int N) {
+    const int64_t tiles = ((int64_t)N + kXTile - 1) / kXTile, want = blocks ? (512 + blocks - 1) / blocks : 1, most = (tiles + 3) / 4;
+    const int64_t s = want < most ? want : most;
+    return s < 1 ? 1 : (int)s;
+}
+
+}  // namespace q8
+
+using namespace q8;
+
+extern "C" int64_t q8_cross_attn_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
+    if (int e = x_sizes("q8_cross_attn_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
+    const int64_t units = B * Hkv, rows = (int64_t)(H / Hkv) * M, blocks = units * ((rows + 127) / 128);
+    const int splits = fwd_splits(blocks, N);
+    return splits == 1 ? 0 : splits * units * rows * (D + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                             void* o, const int64_t* o_strides, float* lse, const int32_t* kv_lens, const uint8_t* key_mask, int64_t mask_row_stride,
+                             int dt, float softmax_scale, int64_t B, int H, int Hkv, int M, int N, int D, void* workspace, int64_t workspace_bytes,
+                             q8_stream_t stream) {
+    const char* who = "q8_cross_attn";
+    if (int e = x_sizes(who, dt, B, H, Hkv, M, N, D, softmax_scale)) return e;
+    if (B == 0 || M == 0) return Q8_OK;
+    if (int e = x_tensor(who, "q", q, q_strides, B, H, M, D)) return e;
+    if (int e = x_tensor(who, "o", o, o_strides, B, H, M, D)) return e;
+    if (N) {
+        if (int e = x_tensor(who, "k", k, k_strides, B, Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "v", v, v_strides, B, Hkv, N, D)) return e;
+    }
+    if ((reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(kv_lens) & 3)) return fail(Q8_ERR_ALIGN, "%s: lse or kv_lens not aligned", who);
+    if (key_mask && (mask_row_stride < 0 || (B > 1 && mask_row_stride > INT64_MAX / 2 / B))) return fail(Q8_ERR_SHAPE, "%s: row stride of the mask", who);
+    XFwd a{};
+    static const int64_t none[3] = {0, 0, 0};
+    const int64_t *ksr = N ? k_strides : none, *vsr = N ? v_strides : none;
+    a.q = XTensor{static_cast<const uint16_t*>(q), q_strides[0], q_strides[1], q_strides[2]};
+    a.k = XTensor{static_cast<const uint16_t*>(k), ksr[0], ksr[1], ksr[2]};
+    a.v = XTensor{static_cast<const uint16_t*>(v), vsr[0], vsr[1], vsr[2]};
+    a.o = XOut{static_cast<uint16_t*>(o), o_strides[0], o_strides[1], o_strides[2]};
+    a.lse = lse;
+    a.keys = XKeys{kv_lens, key_mask, mask_row_stride, N};
+    a.c = softmax_scale * kLog2e;
+    a.Hkv = Hkv;
+    a.G = H / Hkv;
+    a.M = M;
+    a.D = D;
+    a.R = a.G * M;
+    a.units = (int)(B * Hkv);
+    a.row_blocks = (a.R + 127) / 128;
+    a.splits = fwd_splits((int64_t)a.units * a.row_blocks, N);
+    if ((int64_t)a.units * a.row_blocks * a.splits > 0x7ffffff0) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
+    if (a.splits > 1) {
+        const int64_t need = q8_cross_attn_workspace(B, H, Hkv, M, N, D);
+        if (workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
+        if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
+        if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+        const int64_t n = (int64_t)a.splits * a.units * a.R;
+        a.part = static_cast<float*>(workspace);
+        a.pm = a.part + n * D;
+        a.pl = a.pm + n;
+    }
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const unsigned grid = xcd_grid((unsigned)a.units * a.row_blocks * a.splits);
+#define X_FWD(DT)                                                                       \
+    switch (padded_head(D)) {                                                           \
+        case 32: cross_attn_fwd_kernel<DT, 32><<<grid, kXThreads, 0, st>>>(a); break;   \
+        case 64: cross_attn_fwd_kernel<DT, 64><<<grid, kXThreads, 0, st>>>(a); break;   \
+        case 96: cross_attn_fwd_kernel<DT, 96><<<grid, kXThreads, 0, st>>>(a); break;   \
+        default: cross_attn_fwd_kernel<DT, 128><<<grid, kXThreads, 0, st>>>(a);         \
+    }
+    if (dt == Q8_BF16) { X_FWD(Q8_BF16) } else { X_FWD(Q8_F16) }
+#undef X_FWD
+    if (int e = launch_status(who)) return e;
+    if (a.splits > 1) {
+        const unsigned n = (unsigned)(((int64_t)a.units * a.R + 7) / 8);
+        if (dt == Q8_BF16) cross_attn_join_kernel<Q8_BF16><<<n, 256, 0, st>>>(a);
+        else cross_attn_join_kernel<Q8_F16><<<n, 256, 0, st>>>(a);
+        return launch_status(who);
+    }
+    return Q8_OK;
+}

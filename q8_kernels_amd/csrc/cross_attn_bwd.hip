@@ -1,0 +1,461 @@
+// 16-bit cross attention, backward. With P = exp2(c S - lse) formed again from Q, K and the forward's log-sums:
+//   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta),  delta = rowsum(dO O),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// Two kernels, so that every sum has one owner and a fixed order (no atomics), at the price of forming S and dP twice (seven
+// products instead of five; partial sums of dQ per key tile would move more time's worth of bytes than the two products
+// cost). The first owns 128 query rows and walks over the keys: it forms delta, writes it for the second, and dQ. The second
+// owns 128 keys and walks over the rows of all query heads of the group, so dK and dV of a shared head come out summed. P and
+// dS are rounded to 16 bits for the products they enter; scores, dP, sums and delta are fp32.
+//
+// A key that does not count: in the first kernel its score is -infinity (P = 0 exactly, whatever lse is) and its rows of K
+// and V are zeros; in the second a key is a column of every product, whose garbage stays in its column, and its gradient is
+// written as zeros. A row without keys has lse = +infinity, which makes its P zero everywhere.
+//
+// Few workgroups: the walk is divided over several of them, their fp32 sums are added by a third kernel in order.
+#include "cross_attn_common.h"
+
+namespace q8 {
+
+struct XBwd {
+    XTensor q, k, v, o, g;
+    XOut dq, dk, dv;
+    const float* lse;    // [units, R]
+    float* delta;        // [units, R], workspace
+    XKeys keys;
+    float c, scale;
+    int Hkv, G, M, N, D, R;
+    int units, blocks, splits;  // blocks of 128 rows (keys in the second kernel) in a unit
+    float* part;         // splits > 1: [splits, units, R, D], or [splits, units, N, 2 D] (dK, dV)
+};
+
+template <int DT, int DP>
+__global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
+    constexpr int LD = DP + 16, KS = DP / 16, DTL = DP / 32;
+    __shared__ __align__(16) uint16_t kt[2][kXTile * LD], vt[2][kXTile * LD];
+    __shared__ __align__(16) float bias[2][kXTile];
+    unsigned item;
+    if (!xcd_item((unsigned)a.units * a.blocks * a.splits, item)) return;
+    const int rb = item % a.blocks, split = (item / a.blocks) % a.splits, unit = item / (a.blocks * a.splits);
+    const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
+
+    const int len = a.keys.length(b);
+    const uint8_t* mask = a.keys.row(b);
+    const int tiles = (len + kXTile - 1) / kXTile, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+
+    v4u qf[KS], gf[KS];
+    float delta = 0.f, lse = __builtin_inff();
+    {
+        const bool ok = row < a.R;
+        const int g = ok ? row / a.M : 0, m = row - g * a.M;
+        const uint16_t* qp = a.q.p + b * a.q.sb + (int64_t)(hk * a.G + g) * a.q.sh + m * a.q.st + half * 8;
+        const uint16_t* gp = a.g.p + b * a.g.sb + (int64_t)(hk * a.G + g) * a.g.sh + m * a.g.st + half * 8;
+        const uint16_t* op = a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + m * a.o.st + half * 8;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const bool in = ok && s * 16 + half * 8 < a.D;
+            qf[s] = in ? *reinterpret_cast<const v4u*>(qp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            gf[s] = in ? *reinterpret_cast<const v4u*>(gp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            const v4u of = in ? *reinterpret_cast<const v4u*>(op + s * 16) : v4u{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                delta += unpack<DT>(gf[s][i] & 0xffffu) * unpack<DT>(of[i] & 0xffffu);
+                delta += unpack<DT>(gf[s][i] >> 16) * unpack<DT>(of[i] >> 16);
+            }
+        }
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(delta), __float_as_uint(delta), false, false);
+        delta = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        if (ok) {
+            const int64_t at = (int64_t)unit * a.R + row;
+            lse = a.lse[at];
+            if (split == 0 && half == 0) a.delta[at] = delta;
+        }
+    }
+    const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+    const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+    Stage<DP> ks, vs;
+    auto load = [&](int t) {
+        auto at = [&](const uint16_t* p, int64_t st) {
+            return [=](int r) -> const uint16_t* {
+                const int key = t * kXTile + r;
+                return key < len && (mask == nullptr || mask[key]) ? p + key * st : nullptr;
+            };
+        };
+        ks.load(at(kp, a.k.st), a.D);
+        vs.load(at(vp, a.v.st), a.D);
+    };
+    auto store = [&](int t) {
+        ks.store(kt[t & 1]);
+        vs.store(vt[t & 1]);
+        if (threadIdx.x < kXTile) {
+            const int key = t * kXTile + threadIdx.x;
+            bias[t & 1][threadIdx.x] = key < len && (mask == nullptr || mask[key]) ? 0.f : -__builtin_inff();
+        }
+    };
+
+    v16f acc[DTL];
+#pragma unroll
+    for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
+    if (t0 < t1) {
+        load(t0);
+        store(t0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        if (t + 1 < t1) load(t + 1);
+        const uint16_t *kl = kt[t & 1], *vl = vt[t & 1];
+        const bool masked = mask != nullptr || (t + 1) * kXTile > len;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            v16f s = splat16(0.f), dp = splat16(-delta);
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v4f w = *reinterpret_cast<const v4f*>(&bias[t & 1][u * 32 + i * 8 + half * 4]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[i * 4 + j] = w[j];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<LD>(kl, u * 32, e * 16, lane), qf[e], s);
+#pragma unroll
+            for (int e = 0; e < KS; ++e) dp = mfma16<DT>(lds_rows<LD>(vl, u * 32, e * 16, lane), gf[e], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const v4u p = pack_step<DT>(dp, k);
+#pragma unroll
+                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<LD>(kl, u * 32 + k * 16, d * 32, lane), p, acc[d]);
+            }
+        }
+        if (t + 1 < t1) store(t + 1);
+        __syncthreads();
+    }
+    if (a.splits > 1) {
+        if (row < a.R) {
+            float* p = a.part + (((int64_t)split * a.units + unit) * a.R + row) * a.D;
+#pragma unroll
+            for (int d = 0; d < DTL; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = d * 32 + i * 8 + half * 4;
+                    if (e < a.D) *reinterpret_cast<v4f*>(p + e) = v4f{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                }
+        }
+        return;
+    }
+    static_assert(kXWaves * 32 * (DP + 8) <= 2 * kXTile * LD, "the output tiles fit the K buffers");
+    store_tile<DT, DP>(acc, a.scale, kt[0] + wave * 32 * (DP + 8), a.D, lane, [&](int r) -> uint16_t* {
+        const int n = row0 + r;
+        if (n >= a.R) return nullptr;
+        const int g = n / a.M;
+        return a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (n - g * a.M) * a.dq.st;
+    });
+}
+
+template <int DT, int DP>
+__global__ __launch_bounds__(kXThreads, DP > 64 ? 1 : 2) void cross_attn_dkdv_kernel(XBwd a) {
+    constexpr int LD = DP + 16, KS = DP / 16, DTL = DP / 32;
+    __shared__ __align__(16) uint16_t qt[2][kXTile * LD], gt[2][kXTile * LD];
+    __shared__ __align__(16) float lt[2][kXTile], dt[2][kXTile];  // -lse and -delta of the tile's rows
+    unsigned item;
+    if (!xcd_item((unsigned)a.units * a.blocks * a.splits, item)) return;
+    const int kb = item % a.blocks, split = (item / a.blocks) % a.splits, unit = item / (a.blocks * a.splits);
+    const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int key0 = kb * 128 + wave * 32, key = key0 + (lane & 31);
+
+    const int len = a.keys.length(b);
+    const uint8_t* mask = a.keys.row(b);
+    const bool counts = key < len && (mask == nullptr || mask[key]);
+    const int tiles = (a.R + kXTile - 1) / kXTile, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = split * per;
+    int t1 = t0 + per < tiles ? t0 + per : tiles;
+    if (kb * 128 >= len) t1 = t0;  // no key of this workgroup counts: zeros
+
+    v4u kf[KS], vf[KS];
+    {
+        const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh + key * a.k.st + half * 8;
+        const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh + key * a.v.st + half * 8;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const bool in = counts && s * 16 + half * 8 < a.D;
+            kf[s] = in ? *reinterpret_cast<const v4u*>(kp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            vf[s] = in ? *reinterpret_cast<const v4u*>(vp + s * 16) : v4u{0u, 0u, 0u, 0u};
+        }
+    }
+    Stage<DP> qs, gs;
+    float row_lse = 0.f, row_delta = 0.f;
+    auto load = [&](int t) {
+        auto at = [&](const XTensor& x) {
+            const uint16_t* p = x.p + b * x.sb + (int64_t)hk * a.G * x.sh;
+            return [&, p](int r) -> const uint16_t* {
+                const int n = t * kXTile + r;
+                if (n >= a.R) return nullptr;
+                const int g = n / a.M;
+                return p + g * x.sh + (n - g * a.M) * x.st;
+            };
+        };
+        qs.load(at(a.q), a.D);
+        gs.load(at(a.g), a.D);
+        const int n = t * kXTile + (threadIdx.x & 63);
+        if (threadIdx.x < 2 * kXTile) {
+            row_lse = -__builtin_inff();
+            row_delta = 0.f;
+            if (n < a.R) {
+                row_lse = -a.lse[(int64_t)unit * a.R + n];
+                row_delta = -a.delta[(int64_t)unit * a.R + n];
+            }
+        }
+    };
+    auto store = [&](int t) {
+        qs.store(qt[t & 1]);
+        gs.store(gt[t & 1]);
+        if (threadIdx.x < kXTile) {
+            lt[t & 1][threadIdx.x] = row_lse;
+            dt[t & 1][threadIdx.x] = row_delta;
+        }
+    };
+
+    v16f dk[DTL], dv[DTL];
+#pragma unroll
+    for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
+    if (t0 < t1) {
+        load(t0);
+        store(t0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        if (t + 1 < t1) load(t + 1);
+        const uint16_t *ql = qt[t & 1], *gl = gt[t & 1];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            v16f s = splat16(0.f), dp;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const v4f w = *reinterpret_cast<const v4f*>(&dt[t & 1][u * 32 + i * 8 + half * 4]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dp[i * 4 + j] = w[j];
+            }
+#pragma unroll
+            for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<LD>(ql, u * 32, e * 16, lane), kf[e], s);
+#pragma unroll
+            for (int e = 0; e < KS; ++e) dp = mfma16<DT>(lds_rows<LD>(gl, u * 32, e * 16, lane), vf[e], dp);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const v4f w = *reinterpret_cast<const v4f*>(&lt[t & 1][u * 32 + i * 8 + half * 4]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[i * 4 + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * 4 + j], a.c, w[j]));
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const v4u p = pack_step<DT>(s, k);
+#pragma unroll
+                for (int d = 0; d < DTL; ++d) dv[d] = mfma16<DT>(lds_cols<LD>(gl, u * 32 + k * 16, d * 32, lane), p, dv[d]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const v4u p = pack_step<DT>(dp, k);
+#pragma unroll
+                for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(lds_cols<LD>(ql, u * 32 + k * 16, d * 32, lane), p, dk[d]);
+            }
+        }
+        if (t + 1 < t1) store(t + 1);
+        __syncthreads();
+    }
+    if (!counts) {  // a key that does not count has no gradient, whatever its column holds
+#pragma unroll
+        for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
+    }
+    if (a.splits > 1) {
+        if (key < a.N) {
+            float* p = a.part + (((int64_t)split * a.units + unit) * a.N + key) * 2 * a.D;
+#pragma unroll
+            for (int d = 0; d < DTL; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = d * 32 + i * 8 + half * 4;
+                    if (e < a.D) {
+                        *reinterpret_cast<v4f*>(p + e) = v4f{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
+                        *reinterpret_cast<v4f*>(p + a.D + e) = v4f{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
+                    }
+                }
+        }
+        return;
+    }
+    static_assert(kXWaves * 32 * (DP + 8) <= 2 * kXTile * LD, "the output tiles fit the tile buffers");
+    auto at = [&](const XOut& x) {
+        uint16_t* p = x.p + b * x.sb + hk * x.sh;
+        return [&, p](int r) -> uint16_t* { return key0 + r < a.N ? p + (key0 + r) * x.st : nullptr; };
+    };
+    store_tile<DT, DP>(dk, a.scale, qt[0] + wave * 32 * (DP + 8), a.D, lane, at(a.dk));
+    store_tile<DT, DP>(dv, 1.0f, gt[0] + wave * 32 * (DP + 8), a.D, lane, at(a.dv));
+}
+
+// Adds the parts of dQ (WIDTH = 1) or of dK and dV (WIDTH = 2): one thread for 4 elements of a row.
+template <int DT, int WIDTH>
+__global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
+    const int64_t rows = (int64_t)a.units * (WIDTH == 1 ? a.R : a.N);
+    const int quads = WIDTH * a.D / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = i / quads;
+    if (n >= rows) return;
+    int e = (int)(i - n * quads) * 4;
+    v4f s = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < a.splits; ++k) {
+        const v4f p = *reinterpret_cast<const v4f*>(a.part + ((int64_t)k * rows + n) * (WIDTH * a.D) + e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += p[j];
+    }
+    const bool is_v = WIDTH == 2 && e >= a.D;
+    const float f = is_v ? 1.0f : a.scale;
+    if (is_v) e -= a.D;
+    const int len = WIDTH == 1 ? a.R : a.N, unit = (int)(n / len), r = (int)(n - (int64_t)unit * len), b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    uint16_t* p;
+    if constexpr (WIDTH == 1) {
+        const int g = r / a.M;
+        p = a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (r - g * a.M) * a.dq.st;
+    } else {
+        const XOut& x = is_v ? a.dv : a.dk;
+        p = x.p + b * x.sb + hk * x.sh + r * x.st;
+    }
+    *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(s[0] * f, s[1] * f), (int)pack2<DT>(s[2] * f, s[3] * f)};
+}
+
+// Workgroups that share the walk of a block: until about 512 run, four tiles each or more.
+static int bwd_splits(int64_t blocks, int64_t length) {
+    const int64_t tiles = (length + kXTile - 1) / kXTile, want = blocks ? (512 + blocks - 1) / blocks : 1, most = (tiles + 3) / 4;
+    const int64_t s = want < most ? want : most;
+    return s < 1 ? 1 : (int)s;
+}
+
+struct XPlan {
+    int64_t units, rows, dq_blocks, kv_blocks, dq_part, kv_part;  // parts in floats
+    int dq_splits, kv_splits;
+};
+static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
+    XPlan p{};
+    p.units = B * Hkv;
+    p.rows = (int64_t)(H / Hkv) * M;
+    p.dq_blocks = (p.rows + 127) / 128;
+    p.kv_blocks = ((int64_t)N + 127) / 128;
+    p.dq_splits = bwd_splits(p.units * p.dq_blocks, N);
+    p.kv_splits = bwd_splits(p.units * p.kv_blocks, p.rows);
+    p.dq_part = p.dq_splits > 1 ? p.dq_splits * p.units * p.rows * D : 0;
+    p.kv_part = p.kv_splits > 1 ? p.kv_splits * p.units * N * 2 * D : 0;
+    return p;
+}
+static int64_t delta_floats(const XPlan& p) { return (p.units * p.rows + 3) / 4 * 4; }
+
+}  // namespace q8
+
+using namespace q8;
+
+extern "C" int64_t q8_cross_attn_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
+    if (int e = x_sizes("q8_cross_attn_backward_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
+    const XPlan p = plan(B, H, Hkv, M, N, D);
+    return (delta_floats(p) + (p.dq_part > p.kv_part ? p.dq_part : p.kv_part)) * (int64_t)sizeof(float);
+}
+
+extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides, const void* k,
+                                      const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* o, const int64_t* o_strides,
+                                      const float* lse, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                                      const int64_t* dv_strides, const int32_t* kv_lens, const uint8_t* key_mask, int64_t mask_row_stride, int dt,
+                                      float softmax_scale, int64_t B, int H, int Hkv, int M, int N, int D, void* workspace, int64_t workspace_bytes,
+                                      q8_stream_t stream) {
+    const char* who = "q8_cross_attn_backward";
+    if (int e = x_sizes(who, dt, B, H, Hkv, M, N, D, softmax_scale)) return e;
+    if (B == 0 || (M == 0 && N == 0)) return Q8_OK;
+    static const int64_t none[3] = {0, 0, 0};
+    if (M) {
+        if (int e = x_tensor(who, "grad", grad, grad_strides, B, H, M, D)) return e;
+        if (int e = x_tensor(who, "q", q, q_strides, B, H, M, D)) return e;
+        if (int e = x_tensor(who, "o", o, o_strides, B, H, M, D)) return e;
+        if (int e = x_tensor(who, "dq", dq, dq_strides, B, H, M, D)) return e;
+        if (lse == nullptr) return fail(Q8_ERR_NULL, "%s: lse is NULL", who);
+    }
+    if (N) {
+        if (int e = x_tensor(who, "k", k, k_strides, B, Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "v", v, v_strides, B, Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "dk", dk, dk_strides, B, Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "dv", dv, dv_strides, B, Hkv, N, D)) return e;
+    }
+    if ((reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(kv_lens) & 3)) return fail(Q8_ERR_ALIGN, "%s: lse or kv_lens not aligned", who);
+    if (key_mask && (mask_row_stride < 0 || (B > 1 && mask_row_stride > INT64_MAX / 2 / B))) return fail(Q8_ERR_SHAPE, "%s: row stride of the mask", who);
+    const int64_t need = q8_cross_attn_backward_workspace(B, H, Hkv, M, N, D);
+    if (need && workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
+    if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
+    if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+    const XPlan p = plan(B, H, Hkv, M, N, D);
+    if (p.units * p.dq_blocks * p.dq_splits > 0x7ffffff0 || p.units * p.kv_blocks * p.kv_splits > 0x7ffffff0) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
+    XBwd a{};
+    auto in = [&](const void* x, const int64_t* s, int n) {
+        const int64_t* t = n ? s : none;
+        return XTensor{static_cast<const uint16_t*>(x), t[0], t[1], t[2]};
+    };
+    auto out = [&](void* x, const int64_t* s, int n) {
+        const int64_t* t = n ? s : none;
+        return XOut{static_cast<uint16_t*>(x), t[0], t[1], t[2]};
+    };
+    a.q = in(q, q_strides, M);
+    a.o = in(o, o_strides, M);
+    a.g = in(grad, grad_strides, M);
+    a.k = in(k, k_strides, N);
+    a.v = in(v, v_strides, N);
+    a.dq = out(dq, dq_strides, M);
+    a.dk = out(dk, dk_strides, N);
+    a.dv = out(dv, dv_strides, N);
+    a.lse = lse;
+    a.delta = static_cast<float*>(workspace);
+    a.part = a.delta + delta_floats(p);
+    a.keys = XKeys{kv_lens, key_mask, mask_row_stride, N};
+    a.c = softmax_scale * kLog2e;
+    a.scale = softmax_scale;
+    a.Hkv = Hkv;
+    a.G = H / Hkv;
+    a.M = M;
+    a.N = N;
+    a.D = D;
+    a.R = (int)p.rows;
+    a.units = (int)p.units;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+#define X_BWD(NAME, DT)                                                       \
+    switch (padded_head(D)) {                                                 \
+        case 32: NAME<DT, 32><<<grid, kXThreads, 0, st>>>(a); break;          \
+        case 64: NAME<DT, 64><<<grid, kXThreads, 0, st>>>(a); break;          \
+        case 96: NAME<DT, 96><<<grid, kXThreads, 0, st>>>(a); break;          \
+        default: NAME<DT, 128><<<grid, kXThreads, 0, st>>>(a);                \
+    }
+    if (M) {
+        a.blocks = (int)p.dq_blocks;
+        a.splits = p.dq_splits;
+        const unsigned grid = xcd_grid((unsigned)(p.units * p.dq_blocks * p.dq_splits));
+        if (dt == Q8_BF16) { X_BWD(cross_attn_dq_kernel, Q8_BF16) } else { X_BWD(cross_attn_dq_kernel, Q8_F16) }
+        if (int e = launch_status(who)) return e;
+        if (a.splits > 1) {
+            const unsigned n = (unsigned)((p.units * p.rows * (D / 4) + 255) / 256);
+            if (dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 1><<<n, 256, 0, st>>>(a);
+            else cross_attn_add_kernel<Q8_F16, 1><<<n, 256, 0, st>>>(a);
+            if (int e = launch_status(who)) return e;
+        }
+    }
+    if (N) {
+        a.blocks = (int)p.kv_blocks;
+        a.splits = p.kv_splits;
+        const unsigned grid = xcd_grid((unsigned)(p.units * p.kv_blocks * p.kv_splits));
+        if (dt == Q8_BF16) { X_BWD(cross_attn_dkdv_kernel, Q8_BF16) } else { X_BWD(cross_attn_dkdv_kernel, Q8_F16) }
+        if (int e = launch_status(who)) return e;
+        if (a.splits > 1) {
+            const unsigned n = (unsigned)((p.units * N * (D / 2) + 255) / 256);
+            if (dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 2><<<n, 256, 0, st>>>(a);
+            else cross_attn_add_kernel<Q8_F16, 2><<<n, 256, 0, st>>>(a);
+            if (int e = launch_status(who)) return e;
+        }
+    }
+#undef X_BWD
+    return Q8_OK;
+}
