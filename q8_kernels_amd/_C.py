@@ -3,8 +3,6 @@ pybind11 modules (q8_kernels_cuda.{gemm,quantizer,ops,flash_attention}._C), impl
 C ABI of libq8_hip.so. Outputs are allocated here with torch (as the reference's C++ glue does), inputs
 are borrowed, launches go to the current torch stream of the input's device and do not synchronise.
 """
-import contextlib
-import ctypes
 from typing import List, Optional
 
 import torch
@@ -47,11 +45,6 @@ def _as_rows(x):
     if x2.stride(-1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
         x2 = x2.contiguous()
     return x2
-
-
-def _on(device):
-    """The context in which calls go to `device`: nothing to do where it is the current one (the guard costs microseconds)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 # ----------------------------------------------------------------------------- quantizer._C
@@ -768,212 +761,38 @@ def rms_norm_backward(x_normed: torch.Tensor, x_norms: torch.Tensor, grad_out: t
     return out.reshape(x_normed.shape)
 
 
-# ----------------------------------------------------------------------------- layer norm
-
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
-
-
-def _norm_params(x, weight, bias, who):
-    """The parameters, contiguous, and their type's code; both are float32 or both of x's type."""
-    out, dt = [], None
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            if t.device != x.device:
-                raise RuntimeError("%s: %s must be on %s" % (who, name, x.device))
-            if t.dim() != 1 or t.shape[0] != x.shape[-1]:
-                raise RuntimeError("%s: %s must have shape [%d], got %s" % (who, name, x.shape[-1], list(t.shape)))
-            if t.dtype not in (torch.float32, x.dtype) or (dt is not None and t.dtype != dt):
-                raise RuntimeError("%s: weight and bias must both be float32 or both of x's type %s" % (who, x.dtype))
-            dt = t.dtype
-            t = t.contiguous()
-        out.append(t)
-    return out[0], out[1], _DT[torch.float32 if dt is None else dt]
-
+# ----------------------------------------------------------------------------- operators of _torch_ops (no counterpart in the reference)
+#
+# Checks, allocations and launches of these are native (csrc/torch_ops.cpp); functional has them with their gradients.
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5, *,
                stats: bool = True) -> List[Optional[torch.Tensor]]:
     """[y (x.shape, x's type), mean, rstd (x.shape[:-1], float32)]; stats=False: the last two are None."""
-    _require_gpu(x, "x")
-    if x.dtype not in _FLOATS:
-        raise RuntimeError("layer_norm: x must be bfloat16, float16 or float32, got %s" % x.dtype)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError("layer_norm: x must have a last dimension of one element or more")
-    weight, bias, wd = _norm_params(x, weight, bias, "layer_norm")
-    x2 = _as_rows(x)
-    rows, dim = x2.shape
-    with _on(x.device):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2)) if stats else (None, None)
-        _lib.check(_lib.lib().q8_layernorm(x2.data_ptr(), _DT[x.dtype], x2.stride(0), _ptr(weight), _ptr(bias), wd, y.data_ptr(), _ptr(mean),
-                                           _ptr(rstd), rows, dim, float(eps), _stream(x)))
-    return [y, mean, rstd]
+    return _lib.ops().layer_norm_forward(x, weight, bias, eps, stats)
 
 
 def layer_norm_backward(grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
                         mean: torch.Tensor, rstd: torch.Tensor, needs=(True, True, True)) -> List[Optional[torch.Tensor]]:
     """[dx, dweight, dbias] of layer_norm, None where not needed or absent; x, mean and rstd as the forward had and gave them."""
-    _require_gpu(grad, "grad")
-    if grad.shape != x.shape or grad.dtype != x.dtype or grad.device != x.device:
-        raise RuntimeError("layer_norm_backward: grad must match x")
-    weight, bias, wd = _norm_params(x, weight, bias, "layer_norm_backward")
-    if any(t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device or not t.is_contiguous() for t in (mean, rstd)):
-        raise RuntimeError("layer_norm_backward: mean and rstd must be the forward's")
-    x2, g2 = _as_rows(x), _as_rows(grad)
-    rows, dim = x2.shape
-    L = _lib.lib()
-    with _on(x.device):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
-        dw = torch.empty_like(weight) if needs[1] and weight is not None else None
-        db = torch.empty_like(bias) if needs[2] and bias is not None else None
-        size = L.q8_layernorm_backward_workspace(rows, dim) if dw is not None or db is not None else 0
-        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size > 0 else None
-        _lib.check(L.q8_layernorm_backward(g2.data_ptr(), g2.stride(0), x2.data_ptr(), _DT[x.dtype], x2.stride(0), _ptr(weight), wd, mean.data_ptr(),
-                                           rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(work), max(size, 0), rows, dim, _stream(x)))
-    return [dx, dw, db]
-
-
-# ----------------------------------------------------------------------------- rotary positions by position and frequency
-
-_Strides3 = ctypes.c_int64 * 3
-
-
-def _unit_last(t):
-    """t itself where its last stride is 1 (a size of one element counts), else a contiguous copy."""
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
-def _like(t):
-    """An uninitialised tensor in t's memory order with unit last stride."""
-    out = torch.empty_like(t)
-    return out if out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return _lib.ops().layer_norm_backward(grad, x, weight, bias, mean, rstd, list(needs))
 
 
 def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Optional[torch.Tensor], inv_freq: torch.Tensor,
            half: bool = True, factor: float = 1.0, *, backward: bool = False) -> List[Optional[torch.Tensor]]:
     """[q', k'] of q [B, H, T, D] and k [B, Hkv, T, D] (either may be None), see functional.rotary.apply_rotary; backward: the
     transposed rotation, which takes the gradients of q' and k' to those of q and k."""
-    x = q if q is not None else k
-    if x is None:
-        raise RuntimeError("rotary: q or k is needed")
-    for t, name in ((q, "q"), (k, "k")):
-        if t is None:
-            continue
-        _require_gpu(t, name)
-        if t.dim() != 4 or t.dtype not in _FLOATS:
-            raise RuntimeError("rotary: %s must be [B, heads, T, D] in bfloat16, float16 or float32" % name)
-        if t.dtype != x.dtype or t.device != x.device or (t.shape[0], t.shape[2], t.shape[3]) != (x.shape[0], x.shape[2], x.shape[3]):
-            raise RuntimeError("rotary: q and k must agree in type, device, batch, tokens and head size")
-    batch, _, tokens, dim = x.shape
-    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != x.device:
-        raise RuntimeError("rotary: inv_freq must be float64 [R / 2] on %s" % x.device)
-    inv_freq = inv_freq.contiguous()
-    bits, row = 0, 0
-    if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != x.device:
-            raise RuntimeError("rotary: positions must be int32 or int64 on %s" % x.device)
-        if positions.shape != (tokens,) and positions.shape != (batch, tokens) and positions.shape != (1, tokens):
-            raise RuntimeError("rotary: positions must be [%d] or [%d, %d], got %s" % (tokens, batch, tokens, list(positions.shape)))
-        bits = 32 if positions.dtype == torch.int32 else 64
-        if tokens > 1 and positions.stride(-1) != 1:
-            positions = positions.contiguous()
-        if positions.dim() == 2 and positions.shape[0] > 1:
-            row = positions.stride(0)
-            if 0 < row < tokens:
-                positions = positions.contiguous()
-                row = tokens
-    with _on(x.device):
-        q, k = (None if t is None else _unit_last(t) for t in (q, k))
-        q_out, k_out = (None if t is None else _like(t) for t in (q, k))
-        st = [None if t is None else _Strides3(*t.stride()[:3]) for t in (q, q_out, k, k_out)]
-        _lib.check(_lib.lib().q8_rotary(_ptr(q), st[0], _ptr(q_out), st[1], 0 if q is None else q.shape[1], _ptr(k), st[2], _ptr(k_out), st[3],
-                                        0 if k is None else k.shape[1], _DT[x.dtype], _ptr(positions), bits, row, inv_freq.data_ptr(),
-                                        2 * inv_freq.shape[0], int(half), factor, int(backward), batch, tokens, dim, _stream(x)))
-    return [q_out, k_out]
-
-
-# ----------------------------------------------------------------------------- 16-bit cross attention
-
-def _chunks(t):
-    """t itself where its rows are 16-byte chunks the kernels can address (unit last stride, the others multiples of 8
-    elements, 16-byte aligned), else a contiguous copy."""
-    st, shape = t.stride(), t.shape
-    if (st[3] == 1 and t.data_ptr() % 16 == 0 and (st[0] % 8 == 0 or shape[0] == 1) and (st[1] % 8 == 0 or shape[1] == 1)
-            and (st[2] % 8 == 0 or shape[2] == 1)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _attn_check(q, k, v, kv_lens, key_mask, who):
-    """(kv_lens, key_mask with unit last stride, its row stride) after the checks the C entry points cannot make"""
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _require_gpu(t, name)
-        if t.dim() != 4:
-            raise RuntimeError("%s: %s must be [B, heads, tokens, D], got %s" % (who, name, list(t.shape)))
-        if t.dtype not in (torch.bfloat16, torch.float16) or t.dtype != q.dtype or t.device != q.device:
-            raise RuntimeError("%s: q, k and v must be bfloat16 or float16, all of one type, on one device" % who)
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise RuntimeError("%s: q %s does not go with k %s and v %s" % (who, list(q.shape), list(k.shape), list(v.shape)))
-    b, n = k.shape[0], k.shape[2]
-    if kv_lens is not None:
-        if kv_lens.dtype != torch.int32 or kv_lens.shape != (b,) or kv_lens.device != q.device:
-            raise RuntimeError("%s: kv_lens must be int32 [%d] on %s" % (who, b, q.device))
-        kv_lens = kv_lens.contiguous()
-    row = 0
-    if key_mask is not None:
-        if key_mask.dtype != torch.bool or key_mask.shape != (b, n) or key_mask.device != q.device:
-            raise RuntimeError("%s: key_mask must be bool [%d, %d] on %s" % (who, b, n, q.device))
-        if n > 1 and key_mask.stride(1) != 1:
-            key_mask = key_mask.contiguous()
-        row = key_mask.stride(0)
-    return kv_lens, key_mask, row
-
-
-def _strides(t):
-    return _Strides3(*t.stride()[:3])
+    return _lib.ops().rotary(q, k, positions, inv_freq, half, factor, backward)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, kv_lens: Optional[torch.Tensor] = None,
                     key_mask: Optional[torch.Tensor] = None, *, stats: bool = True) -> List[Optional[torch.Tensor]]:
     """[o (q's shape, type and memory order), lse (float32 [B, H, M], log2 of the sum of 2^(score * log2 e); +inf where no key
     counts; None without stats)], see functional.cross_attention.cross_attention."""
-    kv_lens, key_mask, row = _attn_check(q, k, v, kv_lens, key_mask, "cross_attention")
-    (b, h, m, d), hk, n = q.shape, k.shape[1], k.shape[2]
-    L = _lib.lib()
-    with _on(q.device):
-        size = L.q8_cross_attn_workspace(b, h, hk, m, n, d)
-        if size < 0:
-            _lib.check(size)
-        q, k, v = _chunks(q), _chunks(k), _chunks(v)
-        o = _like(q)
-        lse = torch.empty((b, h, m), dtype=torch.float32, device=q.device) if stats else None
-        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        _lib.check(L.q8_cross_attn(q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(), _strides(o),
-                                   _ptr(lse), _ptr(kv_lens), _ptr(key_mask), row, _DT[q.dtype], softmax_scale, b, h, hk, m, n, d, _ptr(work), size,
-                                   _stream(q)))
-    return [o, lse]
+    return _lib.ops().cross_attention_forward(q, k, v, softmax_scale, kv_lens, key_mask, stats)
 
 
 def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                              softmax_scale: float, kv_lens: Optional[torch.Tensor] = None,
                              key_mask: Optional[torch.Tensor] = None) -> List[torch.Tensor]:
     """[dq, dk, dv] in the memory orders of q, k and v; o and lse as the forward gave them."""
-    who = "cross_attention_backward"
-    kv_lens, key_mask, row = _attn_check(q, k, v, kv_lens, key_mask, who)
-    (b, h, m, d), hk, n = q.shape, k.shape[1], k.shape[2]
-    if any(t.shape != q.shape or t.dtype != q.dtype or t.device != q.device for t in (grad, o)):
-        raise RuntimeError("%s: grad and o must match q" % who)
-    if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
-        raise RuntimeError("%s: lse must be the forward's" % who)
-    L = _lib.lib()
-    with _on(q.device):
-        size = L.q8_cross_attn_backward_workspace(b, h, hk, m, n, d)
-        if size < 0:
-            _lib.check(size)
-        q, k, v, o, grad = _chunks(q), _chunks(k), _chunks(v), _chunks(o), _chunks(grad)
-        dq, dk, dv = _like(q), _like(k), _like(v)
-        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        args = [x for t in (grad, q, k, v, o) for x in (t.data_ptr(), _strides(t))] + [lse.data_ptr()]
-        args += [x for t in (dq, dk, dv) for x in (t.data_ptr(), _strides(t))]
-        _lib.check(L.q8_cross_attn_backward(*args, _ptr(kv_lens), _ptr(key_mask), row, _DT[q.dtype], softmax_scale, b, h, hk, m, n, d, _ptr(work), size,
-                                            _stream(q)))
-    return [dq, dk, dv]
+    return _lib.ops().cross_attention_backward(grad, q, k, v, o, lse, softmax_scale, kv_lens, key_mask)

@@ -8,6 +8,7 @@ import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libq8_hip.so")
+OPS_PATH = os.path.join(HERE, "_torch_ops.so")
 
 # element types / flags, mirrored from include/q8_hip.h
 Q8_I8, Q8_E4M3, Q8_BF16, Q8_F16, Q8_F32 = 0, 1, 2, 3, 4
@@ -96,6 +97,24 @@ def lib():
                     fn.argtypes = args
                 _lib = handle
     return _lib
+
+
+_ops = None
+
+
+def ops():
+    """The native tensor-level operators (csrc/torch_ops.cpp, built next to the library); raises if they have not been built."""
+    global _ops
+    if _ops is None:
+        if not os.path.exists(OPS_PATH):
+            raise RuntimeError(
+                "_torch_ops.so not found at %s: build it with `python -m q8_kernels_amd.build` "
+                "(there is no fallback path)" % OPS_PATH)
+        import torch  # noqa: F401  (its libraries are what the module links against)
+        lib()
+        from . import _torch_ops
+        _ops = _torch_ops
+    return _ops
 
 
 def check(status):

@@ -8,9 +8,8 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from .._C import rotary
+from .. import _lib
 
 LAYOUTS = ("half", "interleaved")
 
@@ -52,29 +51,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return (f if device is None else f.to(device)), factor
 
 
-class Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, half, factor):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.half, ctx.factor = half, factor
-        q_out, k_out = rotary(q, k, positions, inv_freq, half, factor)
-        return q_out if k is None else (q_out, k_out)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_q, grad_k=None):
-        positions, inv_freq = ctx.saved_tensors
-        need_q, need_k = ctx.needs_input_grad[:2]
-        gq, gk = (grad_q if need_q else None), (grad_k if need_k else None)
-        if gq is not None or gk is not None:
-            gq, gk = rotary(gq, gk, positions, inv_freq, ctx.half, ctx.factor, backward=True)
-        return gq, gk, None, None, None, None
-
-
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor], inv_freq: torch.Tensor, *,
                  layout: str = "half", factor: float = 1.0):
-    """q [B, H, T, D] and k [B, Hkv, T, D] (or None), rotated: (q', k'), or q' alone without k. Differentiable in both.
+    """q [B, H, T, D] and k [B, Hkv, T, D] (or None), rotated: (q', k'), or q' alone without k. Differentiable in both (once).
 
     Any strides with unit last stride are read in place (token-major projections as `.view(B, T, H, D).transpose(1, 2)`);
     the results have the memory order of their inputs. bfloat16, float16 or float32, D up to 512. positions: int32 or
@@ -83,7 +62,5 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     Angles, sines and products are formed in float64 / float32 and rounded once."""
     if layout not in LAYOUTS:
         raise ValueError("apply_rotary: layout %r (one of %s)" % (layout, ", ".join(LAYOUTS)))
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return Rotary.apply(q, k, positions, inv_freq, layout == "half", float(factor))
-    out = rotary(q, k, positions, inv_freq, layout == "half", float(factor))
+    out = _lib.ops().apply_rotary(q, k, positions, inv_freq, layout == "half", factor)
     return out[0] if k is None else out
