@@ -7,9 +7,11 @@
 // product (as its operand has to be), relative to a maximum that trails the running one by at most 2^8, so the rounding is
 // a relative one. O is rescaled only when the maximum has grown beyond that.
 //
-// Few row blocks: the keys of a unit are divided over several workgroups, whose unnormalised results, maxima and sums a
-// second kernel joins.
+// Row blocks that do not fill the card: their keys are divided over several workgroups, whose unnormalised results, maxima and
+// sums a second kernel joins.
 #include "cross_attn_common.h"
+
+#include <type_traits>
 
 namespace q8 {
 
@@ -20,27 +22,36 @@ struct XFwd {
     XKeys keys;
     float c;             // softmax scale * log2 e
     int Hkv, G, M, D, R;
-    int units, row_blocks, splits;
-    float *part, *pm, *pl;  // splits > 1: [splits, units, R, D], [splits, units, R] twice
+    int row_blocks;         // of a unit
+    XSchedule plan;
+    float *part, *pm, *pl;  // divided blocks: [splits, tail, 128, D], [splits, tail, 128] twice
 };
 
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
-    constexpr int LD = DP + 16, KS = DP / 16, DTL = DP / 32;
-    __shared__ __align__(16) uint16_t kt[2][kXTile * LD], vt[2][kXTile * LD];
+    constexpr int KS = DP / 16, DTL = DP / 32, ELEMS = kXTile * DP;
+    __shared__ __align__(16) uint16_t tiles_lds[4 * ELEMS];  // K, K, V, V
     __shared__ __align__(16) float bias[2][kXTile];
-    unsigned item;
-    if (!xcd_item((unsigned)a.units * a.row_blocks * a.splits, item)) return;
-    const int rb = item % a.row_blocks, split = (item / a.row_blocks) % a.splits, unit = item / (a.row_blocks * a.splits);
+    unsigned block;
+    int split, of;
+    if (!a.plan.item(block, split, of)) return;
+    const int unit = block / a.row_blocks, rb = block - unit * a.row_blocks;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
 
-    const int len = a.keys.length(b);
-    const uint8_t* mask = a.keys.row(b);
-    const int tiles = (len + kXTile - 1) / kXTile, per = (tiles + a.splits - 1) / a.splits;
+    KVTiles<DP> kv;
+    kv.len = a.keys.length(b);
+    kv.mask = a.keys.row(b);
+    kv.D = a.D;
+    kv.kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+    kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+    kv.kst = a.k.st;
+    kv.vst = a.v.st;
+    const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
+    if (t0 < t1) kv.load(t0);
     v4u qf[KS];
     {
         const int g = row < a.R ? row / a.M : 0, m = row - g * a.M;
@@ -48,56 +59,39 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = (row < a.R && s * 16 + half * 8 < a.D) ? *reinterpret_cast<const v4u*>(p + s * 16) : v4u{0u, 0u, 0u, 0u};
     }
-    const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh;
-    const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh;
-    Stage<DP> ks, vs;
-    auto load = [&](int t) {
-        auto at = [&](const uint16_t* p, int64_t st) {
-            return [=](int r) -> const uint16_t* {
-                const int key = t * kXTile + r;
-                return key < len && (mask == nullptr || mask[key]) ? p + key * st : nullptr;
-            };
-        };
-        ks.load(at(kp, a.k.st), a.D);
-        vs.load(at(vp, a.v.st), a.D);
-    };
-    auto store = [&](int t) {
-        ks.store(kt[t & 1]);
-        vs.store(vt[t & 1]);
-        if (threadIdx.x < kXTile) {
-            const int key = t * kXTile + threadIdx.x;
-            bias[t & 1][threadIdx.x] = key < len && (mask == nullptr || mask[key]) ? 0.f : -__builtin_inff();
-        }
-    };
+    if (a.D < DP) {
+        clear_tiles<4 * ELEMS>(tiles_lds);
+        __syncthreads();
+    }
 
     v16f acc[DTL];
 #pragma unroll
     for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
     float m = -3.0e38f, l = 0.f;  // in units of log2; the sum over this lane's half of the keys
-
-    if (t0 < t1) {
-        load(t0);
-        store(t0);
-    }
+    uint64_t live = ~(uint64_t)0;
+    if (t0 < t1) live = kv.store(t0, tiles_lds, tiles_lds + 2 * ELEMS, bias[0]);
     __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        if (t + 1 < t1) load(t + 1);
-        const uint16_t *kl = kt[t & 1], *vl = vt[t & 1];
-        const bool masked = mask != nullptr || (t + 1) * kXTile > len;
+
+    auto step = [&](int t, auto buffer) {
+        constexpr int BUF = decltype(buffer)::value;
+        const uint16_t *kl = tiles_lds + BUF * ELEMS, *vl = tiles_lds + (2 + BUF) * ELEMS;
+        const bool more = t + 1 < t1;
+        if (more) kv.load(t + 1);
         v16f s[2];
+        if (live == ~(uint64_t)0) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            s[u] = splat16(0.f);
-            if (masked) {
+            for (int u = 0; u < 2; ++u) {
+                s[u] = splat16(0.f);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const v4f w = *reinterpret_cast<const v4f*>(&bias[t & 1][u * 32 + i * 8 + half * 4]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[u][i * 4 + j] = w[j];
-                }
+                for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, lane), qf[e], s[u]);
             }
+        } else {
 #pragma unroll
-            for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<LD>(kl, u * 32, e * 16, lane), qf[e], s[u]);
+            for (int u = 0; u < 2; ++u) {
+                s[u] = bias16(bias[BUF], u, half);
+#pragma unroll
+                for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, lane), qf[e], s[u]);
+            }
         }
         float top = s[0][0];
 #pragma unroll
@@ -126,19 +120,23 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(s[u], k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<LD>(vl, u * 32 + k * 16, d * 32, lane), p, acc[d]);
+                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(vl, u * 32 + k * 16, d, lane), p, acc[d]);
             }
         }
-        if (t + 1 < t1) store(t + 1);
+        if (more) live = kv.store(t + 1, tiles_lds + (1 - BUF) * ELEMS, tiles_lds + (3 - BUF) * ELEMS, bias[1 - BUF]);
         __syncthreads();
+    };
+    for (int t = t0; t < t1; t += 2) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
     }
     {
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
         l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
-    if (a.splits > 1) {
+    if (of > 1) {
         if (row < a.R) {
-            const int64_t at = ((int64_t)split * a.units + unit) * a.R + row;
+            const int64_t at = ((int64_t)split * a.plan.tail + (block - a.plan.full)) * 128 + wave * 32 + (lane & 31);
             if (half == 0) { a.pm[at] = m; a.pl[at] = l; }
             float* p = a.part + at * a.D;
 #pragma unroll
@@ -155,8 +153,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
         a.lse[(int64_t)unit * a.R + row] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     // (the tile buffers are free: every wave has passed the last barrier of the loop)
-    static_assert(kXWaves * 32 * (DP + 8) <= 2 * kXTile * LD, "the output tiles fit the K buffers");
-    store_tile<DT, DP>(acc, inv, kt[0] + wave * 32 * (DP + 8), a.D, lane, [&](int r) -> uint16_t* {
+    static_assert(kXWaves * 32 * (DP + 8) <= 4 * ELEMS, "the output tiles fit the tile buffers");
+    store_tile<DT, DP>(acc, inv, tiles_lds + wave * 32 * (DP + 8), a.D, lane, [&](int r) -> uint16_t* {
         const int n = row0 + r;
         if (n >= a.R) return nullptr;
         const int g = n / a.M;
@@ -167,13 +165,15 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
 // Joins the parts of a row: weights exp2(m_i - max m). 32 lanes a row, 4 elements a lane.
 template <int DT>
 __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
-    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), all = (int64_t)a.units * a.R;
-    if (n >= all) return;
+    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), all = (int64_t)a.plan.tail * 128;
+    const unsigned block = a.plan.full + (unsigned)(n >> 7);
+    const int unit = block / a.row_blocks, r = (block - unit * a.row_blocks) * 128 + (int)(n & 127);
+    if (n >= all || r >= a.R) return;
     const int e = (threadIdx.x & 31) * 4;
     float m = -3.0e38f, l = 0.f;
-    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.pm[i * all + n]);
+    for (int i = 0; i < a.plan.splits; ++i) m = fmaxf(m, a.pm[i * all + n]);
     v4f o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.splits; ++i) {
+    for (int i = 0; i < a.plan.splits; ++i) {
         const float w = __builtin_amdgcn_exp2f(a.pm[i * all + n] - m);
         l += w * a.pl[i * all + n];
         if (e < a.D) {
@@ -182,20 +182,16 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
             for (int j = 0; j < 4; ++j) o[j] += w * p[j];
         }
     }
-    if (a.lse != nullptr && e == 0) a.lse[n] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
+    if (a.lse != nullptr && e == 0) a.lse[(int64_t)unit * a.R + r] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
     if (e >= a.D) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    const int unit = (int)(n / a.R), r = (int)(n - (int64_t)unit * a.R), g = r / a.M, b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int g = r / a.M, b = unit / a.Hkv, hk = unit - b * a.Hkv;
     uint16_t* p = a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (r - g * a.M) * a.o.st;
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
-// Workgroups that share the keys of a row block: until about 512 run (two on every CU), four tiles each or more.
-static int fwd_splits(int64_t blocks, int N) {
-    const int64_t tiles = ((int64_t)N + kXTile - 1) / kXTile, want = blocks ? (512 + blocks - 1) / blocks : 1, most = (tiles + 3) / 4;
-    const int64_t s = want < most ? want : most;
-    return s < 1 ? 1 : (int)s;
-}
+// two workgroups on every CU (three with heads of 64 or less, whose registers allow it)
+static int fwd_slots(int D) { return D <= 64 ? 768 : 512; }
 
 }  // namespace q8
 
@@ -204,8 +200,7 @@ using namespace q8;
 extern "C" int64_t q8_cross_attn_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
     if (int e = x_sizes("q8_cross_attn_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
     const int64_t units = B * Hkv, rows = (int64_t)(H / Hkv) * M, blocks = units * ((rows + 127) / 128);
-    const int splits = fwd_splits(blocks, N);
-    return splits == 1 ? 0 : splits * units * rows * (D + 2) * (int64_t)sizeof(float);
+    return schedule(blocks, N, fwd_slots(D)).parts() * 128 * (D + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
@@ -238,22 +233,22 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
     a.M = M;
     a.D = D;
     a.R = a.G * M;
-    a.units = (int)(B * Hkv);
     a.row_blocks = (a.R + 127) / 128;
-    a.splits = fwd_splits((int64_t)a.units * a.row_blocks, N);
-    if ((int64_t)a.units * a.row_blocks * a.splits > 0x7ffffff0) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
-    if (a.splits > 1) {
+    const int64_t blocks = B * Hkv * a.row_blocks;
+    if (blocks > 0x7ffff000) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
+    a.plan = schedule(blocks, N, fwd_slots(D));
+    if (a.plan.parts()) {
         const int64_t need = q8_cross_attn_workspace(B, H, Hkv, M, N, D);
         if (workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
         if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
         if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
-        const int64_t n = (int64_t)a.splits * a.units * a.R;
+        const int64_t n = a.plan.parts() * 128;
         a.part = static_cast<float*>(workspace);
         a.pm = a.part + n * D;
         a.pl = a.pm + n;
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const unsigned grid = xcd_grid((unsigned)a.units * a.row_blocks * a.splits);
+    const unsigned grid = a.plan.grid();
 #define X_FWD(DT)                                                                       \
     switch (padded_head(D)) {                                                           \
         case 32: cross_attn_fwd_kernel<DT, 32><<<grid, kXThreads, 0, st>>>(a); break;   \
@@ -264,8 +259,8 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
     if (dt == Q8_BF16) { X_FWD(Q8_BF16) } else { X_FWD(Q8_F16) }
 #undef X_FWD
     if (int e = launch_status(who)) return e;
-    if (a.splits > 1) {
-        const unsigned n = (unsigned)(((int64_t)a.units * a.R + 7) / 8);
+    if (a.plan.parts()) {
+        const unsigned n = a.plan.tail * 16;
         if (dt == Q8_BF16) cross_attn_join_kernel<Q8_BF16><<<n, 256, 0, st>>>(a);
         else cross_attn_join_kernel<Q8_F16><<<n, 256, 0, st>>>(a);
         return launch_status(who);

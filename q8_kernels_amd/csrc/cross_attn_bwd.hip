@@ -14,6 +14,8 @@
 // Few workgroups: the walk is divided over several of them, their fp32 sums are added by a third kernel in order.
 #include "cross_attn_common.h"
 
+#include <type_traits>
+
 namespace q8 {
 
 struct XBwd {
@@ -24,27 +26,36 @@ struct XBwd {
     XKeys keys;
     float c, scale;
     int Hkv, G, M, N, D, R;
-    int units, blocks, splits;  // blocks of 128 rows (keys in the second kernel) in a unit
-    float* part;         // splits > 1: [splits, units, R, D], or [splits, units, N, 2 D] (dK, dV)
+    int blocks;          // of 128 rows (second kernel: keys) in a unit
+    XSchedule plan;
+    float* part;         // divided blocks: [splits, tail, 128, D], or [splits, tail, 128, 2 D] (dK, dV)
 };
 
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
-    constexpr int LD = DP + 16, KS = DP / 16, DTL = DP / 32;
-    __shared__ __align__(16) uint16_t kt[2][kXTile * LD], vt[2][kXTile * LD];
+    constexpr int KS = DP / 16, DTL = DP / 32, ELEMS = kXTile * DP;
+    __shared__ __align__(16) uint16_t tiles_lds[4 * ELEMS];  // K, K, V, V
     __shared__ __align__(16) float bias[2][kXTile];
-    unsigned item;
-    if (!xcd_item((unsigned)a.units * a.blocks * a.splits, item)) return;
-    const int rb = item % a.blocks, split = (item / a.blocks) % a.splits, unit = item / (a.blocks * a.splits);
+    unsigned block;
+    int split, of;
+    if (!a.plan.item(block, split, of)) return;
+    const int unit = block / a.blocks, rb = block - unit * a.blocks;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
 
-    const int len = a.keys.length(b);
-    const uint8_t* mask = a.keys.row(b);
-    const int tiles = (len + kXTile - 1) / kXTile, per = (tiles + a.splits - 1) / a.splits;
+    KVTiles<DP> kv;
+    kv.len = a.keys.length(b);
+    kv.mask = a.keys.row(b);
+    kv.D = a.D;
+    kv.kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+    kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+    kv.kst = a.k.st;
+    kv.vst = a.v.st;
+    const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
+    if (t0 < t1) kv.load(t0);
     v4u qf[KS], gf[KS];
     float delta = 0.f, lse = __builtin_inff();
     {
@@ -73,70 +84,56 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
             if (split == 0 && half == 0) a.delta[at] = delta;
         }
     }
-    const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh;
-    const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh;
-    Stage<DP> ks, vs;
-    auto load = [&](int t) {
-        auto at = [&](const uint16_t* p, int64_t st) {
-            return [=](int r) -> const uint16_t* {
-                const int key = t * kXTile + r;
-                return key < len && (mask == nullptr || mask[key]) ? p + key * st : nullptr;
-            };
-        };
-        ks.load(at(kp, a.k.st), a.D);
-        vs.load(at(vp, a.v.st), a.D);
-    };
-    auto store = [&](int t) {
-        ks.store(kt[t & 1]);
-        vs.store(vt[t & 1]);
-        if (threadIdx.x < kXTile) {
-            const int key = t * kXTile + threadIdx.x;
-            bias[t & 1][threadIdx.x] = key < len && (mask == nullptr || mask[key]) ? 0.f : -__builtin_inff();
-        }
-    };
+    if (a.D < DP) {
+        clear_tiles<4 * ELEMS>(tiles_lds);
+        __syncthreads();
+    }
 
     v16f acc[DTL];
 #pragma unroll
     for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
-    if (t0 < t1) {
-        load(t0);
-        store(t0);
-    }
+    uint64_t live = ~(uint64_t)0;
+    if (t0 < t1) live = kv.store(t0, tiles_lds, tiles_lds + 2 * ELEMS, bias[0]);
     __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        if (t + 1 < t1) load(t + 1);
-        const uint16_t *kl = kt[t & 1], *vl = vt[t & 1];
-        const bool masked = mask != nullptr || (t + 1) * kXTile > len;
+
+    auto step = [&](int t, auto buffer) {
+        constexpr int BUF = decltype(buffer)::value;
+        const uint16_t *kl = tiles_lds + BUF * ELEMS, *vl = tiles_lds + (2 + BUF) * ELEMS;
+        const bool more = t + 1 < t1;
+        if (more) kv.load(t + 1);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            v16f s = splat16(0.f), dp = splat16(-delta);
-            if (masked) {
+            v16f s, dp = splat16(-delta);
+            if (live == ~(uint64_t)0) {
+                s = splat16(0.f);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const v4f w = *reinterpret_cast<const v4f*>(&bias[t & 1][u * 32 + i * 8 + half * 4]);
+                for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, lane), qf[e], s);
+            } else {
+                s = bias16(bias[BUF], u, half);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[i * 4 + j] = w[j];
-                }
+                for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, lane), qf[e], s);
             }
 #pragma unroll
-            for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<LD>(kl, u * 32, e * 16, lane), qf[e], s);
-#pragma unroll
-            for (int e = 0; e < KS; ++e) dp = mfma16<DT>(lds_rows<LD>(vl, u * 32, e * 16, lane), gf[e], dp);
+            for (int e = 0; e < KS; ++e) dp = mfma16<DT>(lds_rows<DP>(vl, u * 32, e, lane), gf[e], dp);
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse));
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(dp, k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<LD>(kl, u * 32 + k * 16, d * 32, lane), p, acc[d]);
+                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(kl, u * 32 + k * 16, d, lane), p, acc[d]);
             }
         }
-        if (t + 1 < t1) store(t + 1);
+        if (more) live = kv.store(t + 1, tiles_lds + (1 - BUF) * ELEMS, tiles_lds + (3 - BUF) * ELEMS, bias[1 - BUF]);
         __syncthreads();
+    };
+    for (int t = t0; t < t1; t += 2) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
     }
-    if (a.splits > 1) {
+    if (of > 1) {
         if (row < a.R) {
-            float* p = a.part + (((int64_t)split * a.units + unit) * a.R + row) * a.D;
+            float* p = a.part + (((int64_t)split * a.plan.tail + (block - a.plan.full)) * 128 + wave * 32 + (lane & 31)) * a.D;
 #pragma unroll
             for (int d = 0; d < DTL; ++d)
 #pragma unroll
@@ -147,8 +144,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
         }
         return;
     }
-    static_assert(kXWaves * 32 * (DP + 8) <= 2 * kXTile * LD, "the output tiles fit the K buffers");
-    store_tile<DT, DP>(acc, a.scale, kt[0] + wave * 32 * (DP + 8), a.D, lane, [&](int r) -> uint16_t* {
+    static_assert(kXWaves * 32 * (DP + 8) <= 4 * ELEMS, "the output tiles fit the tile buffers");
+    store_tile<DT, DP>(acc, a.scale, tiles_lds + wave * 32 * (DP + 8), a.D, lane, [&](int r) -> uint16_t* {
         const int n = row0 + r;
         if (n >= a.R) return nullptr;
         const int g = n / a.M;
@@ -156,14 +153,19 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     });
 }
 
+// A head of more than 96 leaves no registers for V beside K and the two sums (two waves a SIMD have 256 each): V stays in LDS
+// and the rows are walked in tiles of 32.
 template <int DT, int DP>
-__global__ __launch_bounds__(kXThreads, DP > 64 ? 1 : 2) void cross_attn_dkdv_kernel(XBwd a) {
-    constexpr int LD = DP + 16, KS = DP / 16, DTL = DP / 32;
-    __shared__ __align__(16) uint16_t qt[2][kXTile * LD], gt[2][kXTile * LD];
-    __shared__ __align__(16) float lt[2][kXTile], dt[2][kXTile];  // -lse and -delta of the tile's rows
-    unsigned item;
-    if (!xcd_item((unsigned)a.units * a.blocks * a.splits, item)) return;
-    const int kb = item % a.blocks, split = (item / a.blocks) % a.splits, unit = item / (a.blocks * a.splits);
+__global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
+    constexpr int KS = DP / 16, DTL = DP / 32;
+    constexpr bool V_IN_LDS = DP > 96;
+    constexpr int TR = V_IN_LDS ? 32 : 64, ELEMS = TR * DP;
+    __shared__ __align__(16) uint16_t tiles_lds[4 * ELEMS + (V_IN_LDS ? 128 * DP : 0)];  // Q, Q, dO, dO, V
+    __shared__ __align__(16) float lt[2][TR], dt[2][TR];  // -lse and -delta of the tile's rows
+    unsigned block;
+    int split, of;
+    if (!a.plan.item(block, split, of)) return;
+    const int unit = block / a.blocks, kb = block - unit * a.blocks;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int key0 = kb * 128 + wave * 32, key = key0 + (lane & 31);
@@ -171,38 +173,31 @@ __global__ __launch_bounds__(kXThreads, DP > 64 ? 1 : 2) void cross_attn_dkdv_ke
     const int len = a.keys.length(b);
     const uint8_t* mask = a.keys.row(b);
     const bool counts = key < len && (mask == nullptr || mask[key]);
-    const int tiles = (a.R + kXTile - 1) / kXTile, per = (tiles + a.splits - 1) / a.splits;
+    const int tiles = (a.R + TR - 1) / TR, per = (tiles + of - 1) / of;
     const int t0 = split * per;
     int t1 = t0 + per < tiles ? t0 + per : tiles;
     if (kb * 128 >= len) t1 = t0;  // no key of this workgroup counts: zeros
 
-    v4u kf[KS], vf[KS];
-    {
-        const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh + key * a.k.st + half * 8;
-        const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh + key * a.v.st + half * 8;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const bool in = counts && s * 16 + half * 8 < a.D;
-            kf[s] = in ? *reinterpret_cast<const v4u*>(kp + s * 16) : v4u{0u, 0u, 0u, 0u};
-            vf[s] = in ? *reinterpret_cast<const v4u*>(vp + s * 16) : v4u{0u, 0u, 0u, 0u};
-        }
-    }
-    Stage<DP> qs, gs;
+    Stage<DP, TR> qs, gs;
     float row_lse = 0.f, row_delta = 0.f;
+    const uint16_t *qp = a.q.p + b * a.q.sb + (int64_t)hk * a.G * a.q.sh, *gp = a.g.p + b * a.g.sb + (int64_t)hk * a.G * a.g.sh;
     auto load = [&](int t) {
-        auto at = [&](const XTensor& x) {
-            const uint16_t* p = x.p + b * x.sb + (int64_t)hk * a.G * x.sh;
-            return [&, p](int r) -> const uint16_t* {
-                const int n = t * kXTile + r;
-                if (n >= a.R) return nullptr;
-                const int g = n / a.M;
-                return p + g * x.sh + (n - g * a.M) * x.st;
+        const int n0 = t * TR, g0 = n0 / a.M, m0 = n0 - g0 * a.M;
+        if (m0 + TR <= a.M) {  // all rows of one head
+            qs.load(qp + g0 * a.q.sh + m0 * a.q.st, a.q.st, a.D);
+            gs.load(gp + g0 * a.g.sh + m0 * a.g.st, a.g.st, a.D);
+        } else {
+            auto at = [&](const uint16_t* p, const XTensor& x) {
+                return [&, p](int r) {
+                    const int n = n0 + r < a.R ? n0 + r : a.R - 1, g = n / a.M;
+                    return p + g * x.sh + (n - g * a.M) * x.st;
+                };
             };
-        };
-        qs.load(at(a.q), a.D);
-        gs.load(at(a.g), a.D);
-        const int n = t * kXTile + (threadIdx.x & 63);
-        if (threadIdx.x < 2 * kXTile) {
+            qs.load_each(at(qp, a.q), a.D);
+            gs.load_each(at(gp, a.g), a.D);
+        }
+        const int n = n0 + (int)threadIdx.x;
+        if (threadIdx.x < TR) {
             row_lse = -__builtin_inff();
             row_delta = 0.f;
             if (n < a.R) {
@@ -211,42 +206,68 @@ __global__ __launch_bounds__(kXThreads, DP > 64 ? 1 : 2) void cross_attn_dkdv_ke
             }
         }
     };
-    auto store = [&](int t) {
-        qs.store(qt[t & 1]);
-        gs.store(gt[t & 1]);
-        if (threadIdx.x < kXTile) {
-            lt[t & 1][threadIdx.x] = row_lse;
-            dt[t & 1][threadIdx.x] = row_delta;
+    auto store = [&](int t, int buf) {
+        uint16_t *q = tiles_lds + buf * ELEMS, *g = tiles_lds + (2 + buf) * ELEMS;
+        const int left = a.R - t * TR;
+        if (left >= TR) {
+            qs.store(q, a.D);
+            gs.store(g, a.D);
+        } else {
+            const uint64_t live = ((uint64_t)1 << left) - 1;
+            qs.store_live(q, a.D, live);
+            gs.store_live(g, a.D, live);
+        }
+        if (threadIdx.x < TR) {
+            lt[buf][threadIdx.x] = row_lse;
+            dt[buf][threadIdx.x] = row_delta;
         }
     };
+    if (t0 < t1) load(t0);
+
+    v4u kf[KS], vf[V_IN_LDS ? 1 : KS];
+    uint16_t* vl = tiles_lds + 4 * ELEMS;
+    if (a.D < DP) {
+        clear_tiles<4 * ELEMS + (V_IN_LDS ? 128 * DP : 0)>(tiles_lds);
+        __syncthreads();
+    }
+    {
+        const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh + key * a.k.st + half * 8;
+        const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh + key * a.v.st + half * 8;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const bool in = counts && s * 16 + half * 8 < a.D;
+            kf[s] = in ? *reinterpret_cast<const v4u*>(kp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            const v4u v = in ? *reinterpret_cast<const v4u*>(vp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            if constexpr (V_IN_LDS) *reinterpret_cast<v4u*>(vl + wave * 32 * DP + tile_at<DP>(lane & 31, 2 * s + half)) = v;
+            else vf[s] = v;
+        }
+    }
 
     v16f dk[DTL], dv[DTL];
 #pragma unroll
     for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
-    if (t0 < t1) {
-        load(t0);
-        store(t0);
-    }
+    if (t0 < t1) store(t0, 0);
     __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        if (t + 1 < t1) load(t + 1);
-        const uint16_t *ql = qt[t & 1], *gl = gt[t & 1];
+    auto step = [&](int t, auto buffer) {
+        constexpr int BUF = decltype(buffer)::value;
+        const uint16_t *ql = tiles_lds + BUF * ELEMS, *gl = tiles_lds + (2 + BUF) * ELEMS;
+        const bool more = t + 1 < t1;
+        if (more) load(t + 1);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            v16f s = splat16(0.f), dp;
+        for (int u = 0; u < TR / 32; ++u) {
+            v16f s = splat16(0.f), dp = bias16(dt[BUF], u, half);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const v4f w = *reinterpret_cast<const v4f*>(&dt[t & 1][u * 32 + i * 8 + half * 4]);
+            for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(ql, u * 32, e, lane), kf[e], s);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) dp[i * 4 + j] = w[j];
+            for (int e = 0; e < KS; ++e) {
+                v4u v;
+                if constexpr (V_IN_LDS) v = lds_rows<DP>(vl, wave * 32, e, lane);
+                else v = vf[e];
+                dp = mfma16<DT>(lds_rows<DP>(gl, u * 32, e, lane), v, dp);
             }
 #pragma unroll
-            for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<LD>(ql, u * 32, e * 16, lane), kf[e], s);
-#pragma unroll
-            for (int e = 0; e < KS; ++e) dp = mfma16<DT>(lds_rows<LD>(gl, u * 32, e * 16, lane), vf[e], dp);
-#pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const v4f w = *reinterpret_cast<const v4f*>(&lt[t & 1][u * 32 + i * 8 + half * 4]);
+                const v4f w = *reinterpret_cast<const v4f*>(&lt[BUF][u * 32 + i * 8 + half * 4]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[i * 4 + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * 4 + j], a.c, w[j]));
             }
@@ -254,7 +275,7 @@ __global__ __launch_bounds__(kXThreads, DP > 64 ? 1 : 2) void cross_attn_dkdv_ke
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(s, k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) dv[d] = mfma16<DT>(lds_cols<LD>(gl, u * 32 + k * 16, d * 32, lane), p, dv[d]);
+                for (int d = 0; d < DTL; ++d) dv[d] = mfma16<DT>(lds_cols<DP>(gl, u * 32 + k * 16, d, lane), p, dv[d]);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] *= s[i];
@@ -262,19 +283,23 @@ __global__ __launch_bounds__(kXThreads, DP > 64 ? 1 : 2) void cross_attn_dkdv_ke
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(dp, k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(lds_cols<LD>(ql, u * 32 + k * 16, d * 32, lane), p, dk[d]);
+                for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(lds_cols<DP>(ql, u * 32 + k * 16, d, lane), p, dk[d]);
             }
         }
-        if (t + 1 < t1) store(t + 1);
+        if (more) store(t + 1, 1 - BUF);
         __syncthreads();
+    };
+    for (int t = t0; t < t1; t += 2) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
     }
     if (!counts) {  // a key that does not count has no gradient, whatever its column holds
 #pragma unroll
         for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
     }
-    if (a.splits > 1) {
+    if (of > 1) {
         if (key < a.N) {
-            float* p = a.part + (((int64_t)split * a.units + unit) * a.N + key) * 2 * a.D;
+            float* p = a.part + (((int64_t)split * a.plan.tail + (block - a.plan.full)) * 128 + wave * 32 + (lane & 31)) * 2 * a.D;
 #pragma unroll
             for (int d = 0; d < DTL; ++d)
 #pragma unroll
@@ -288,25 +313,30 @@ __global__ __launch_bounds__(kXThreads, DP > 64 ? 1 : 2) void cross_attn_dkdv_ke
         }
         return;
     }
-    static_assert(kXWaves * 32 * (DP + 8) <= 2 * kXTile * LD, "the output tiles fit the tile buffers");
+    static_assert(kXWaves * 32 * (DP + 8) <= 4 * ELEMS + (V_IN_LDS ? 128 * DP : 0), "the output tiles fit the tile buffers");
     auto at = [&](const XOut& x) {
         uint16_t* p = x.p + b * x.sb + hk * x.sh;
         return [&, p](int r) -> uint16_t* { return key0 + r < a.N ? p + (key0 + r) * x.st : nullptr; };
     };
-    store_tile<DT, DP>(dk, a.scale, qt[0] + wave * 32 * (DP + 8), a.D, lane, at(a.dk));
-    store_tile<DT, DP>(dv, 1.0f, gt[0] + wave * 32 * (DP + 8), a.D, lane, at(a.dv));
+    uint16_t* buf = tiles_lds + wave * 32 * (DP + 8);
+    store_tile<DT, DP>(dk, a.scale, buf, a.D, lane, at(a.dk));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    store_tile<DT, DP>(dv, 1.0f, buf, a.D, lane, at(a.dv));
 }
 
 // Adds the parts of dQ (WIDTH = 1) or of dK and dV (WIDTH = 2): one thread for 4 elements of a row.
 template <int DT, int WIDTH>
 __global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
-    const int64_t rows = (int64_t)a.units * (WIDTH == 1 ? a.R : a.N);
+    const int64_t rows = (int64_t)a.plan.tail * 128;
     const int quads = WIDTH * a.D / 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = i / quads;
-    if (n >= rows) return;
+    const unsigned block = a.plan.full + (unsigned)(n >> 7);
+    const int unit = block / a.blocks, r = (block - unit * a.blocks) * 128 + (int)(n & 127);
+    if (n >= rows || r >= (WIDTH == 1 ? a.R : a.N)) return;
     int e = (int)(i - n * quads) * 4;
     v4f s = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < a.splits; ++k) {
+    for (int k = 0; k < a.plan.splits; ++k) {
         const v4f p = *reinterpret_cast<const v4f*>(a.part + ((int64_t)k * rows + n) * (WIDTH * a.D) + e);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[j] += p[j];
@@ -314,7 +344,7 @@ __global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
     const bool is_v = WIDTH == 2 && e >= a.D;
     const float f = is_v ? 1.0f : a.scale;
     if (is_v) e -= a.D;
-    const int len = WIDTH == 1 ? a.R : a.N, unit = (int)(n / len), r = (int)(n - (int64_t)unit * len), b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
     uint16_t* p;
     if constexpr (WIDTH == 1) {
         const int g = r / a.M;
@@ -326,16 +356,12 @@ __global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(s[0] * f, s[1] * f), (int)pack2<DT>(s[2] * f, s[3] * f)};
 }
 
-// Workgroups that share the walk of a block: until about 512 run, four tiles each or more.
-static int bwd_splits(int64_t blocks, int64_t length) {
-    const int64_t tiles = (length + kXTile - 1) / kXTile, want = blocks ? (512 + blocks - 1) / blocks : 1, most = (tiles + 3) / 4;
-    const int64_t s = want < most ? want : most;
-    return s < 1 ? 1 : (int)s;
-}
+// two workgroups on every CU
+constexpr int kBwdSlots = 512;
 
 struct XPlan {
-    int64_t units, rows, dq_blocks, kv_blocks, dq_part, kv_part;  // parts in floats
-    int dq_splits, kv_splits;
+    int64_t units, rows, dq_blocks, kv_blocks, parts;  // blocks of a unit; floats of partial results
+    XSchedule dq, kv;
 };
 static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     XPlan p{};
@@ -343,10 +369,10 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     p.rows = (int64_t)(H / Hkv) * M;
     p.dq_blocks = (p.rows + 127) / 128;
     p.kv_blocks = ((int64_t)N + 127) / 128;
-    p.dq_splits = bwd_splits(p.units * p.dq_blocks, N);
-    p.kv_splits = bwd_splits(p.units * p.kv_blocks, p.rows);
-    p.dq_part = p.dq_splits > 1 ? p.dq_splits * p.units * p.rows * D : 0;
-    p.kv_part = p.kv_splits > 1 ? p.kv_splits * p.units * N * 2 * D : 0;
+    p.dq = schedule(p.units * p.dq_blocks, N, kBwdSlots);
+    p.kv = schedule(p.units * p.kv_blocks, p.rows, kBwdSlots);
+    const int64_t dq = p.dq.parts() * 128 * D, kv = p.kv.parts() * 256 * D;
+    p.parts = dq > kv ? dq : kv;  // one after the other in the same place
     return p;
 }
 static int64_t delta_floats(const XPlan& p) { return (p.units * p.rows + 3) / 4 * 4; }
@@ -358,7 +384,7 @@ using namespace q8;
 extern "C" int64_t q8_cross_attn_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
     if (int e = x_sizes("q8_cross_attn_backward_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
     const XPlan p = plan(B, H, Hkv, M, N, D);
-    return (delta_floats(p) + (p.dq_part > p.kv_part ? p.dq_part : p.kv_part)) * (int64_t)sizeof(float);
+    return (delta_floats(p) + p.parts) * (int64_t)sizeof(float);
 }
 
 extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides, const void* k,
@@ -391,7 +417,7 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
     if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
     if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
     const XPlan p = plan(B, H, Hkv, M, N, D);
-    if (p.units * p.dq_blocks * p.dq_splits > 0x7ffffff0 || p.units * p.kv_blocks * p.kv_splits > 0x7ffffff0) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
+    if (p.units * p.dq_blocks > 0x7ffff000 || p.units * p.kv_blocks > 0x7ffff000) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
     XBwd a{};
     auto in = [&](const void* x, const int64_t* s, int n) {
         const int64_t* t = n ? s : none;
@@ -421,7 +447,6 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
     a.N = N;
     a.D = D;
     a.R = (int)p.rows;
-    a.units = (int)p.units;
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define X_BWD(NAME, DT)                                                       \
     switch (padded_head(D)) {                                                 \
@@ -432,12 +457,12 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
     }
     if (M) {
         a.blocks = (int)p.dq_blocks;
-        a.splits = p.dq_splits;
-        const unsigned grid = xcd_grid((unsigned)(p.units * p.dq_blocks * p.dq_splits));
+        a.plan = p.dq;
+        const unsigned grid = a.plan.grid();
         if (dt == Q8_BF16) { X_BWD(cross_attn_dq_kernel, Q8_BF16) } else { X_BWD(cross_attn_dq_kernel, Q8_F16) }
         if (int e = launch_status(who)) return e;
-        if (a.splits > 1) {
-            const unsigned n = (unsigned)((p.units * p.rows * (D / 4) + 255) / 256);
+        if (a.plan.parts()) {
+            const unsigned n = a.plan.tail * (D / 8);  // 128 rows of D / 4 threads
             if (dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 1><<<n, 256, 0, st>>>(a);
             else cross_attn_add_kernel<Q8_F16, 1><<<n, 256, 0, st>>>(a);
             if (int e = launch_status(who)) return e;
@@ -445,12 +470,12 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
     }
     if (N) {
         a.blocks = (int)p.kv_blocks;
-        a.splits = p.kv_splits;
-        const unsigned grid = xcd_grid((unsigned)(p.units * p.kv_blocks * p.kv_splits));
+        a.plan = p.kv;
+        const unsigned grid = a.plan.grid();
         if (dt == Q8_BF16) { X_BWD(cross_attn_dkdv_kernel, Q8_BF16) } else { X_BWD(cross_attn_dkdv_kernel, Q8_F16) }
         if (int e = launch_status(who)) return e;
-        if (a.splits > 1) {
-            const unsigned n = (unsigned)((p.units * N * (D / 2) + 255) / 256);
+        if (a.plan.parts()) {
+            const unsigned n = a.plan.tail * (D / 4);
             if (dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 2><<<n, 256, 0, st>>>(a);
             else cross_attn_add_kernel<Q8_F16, 2><<<n, 256, 0, st>>>(a);
             if (int e = launch_status(who)) return e;

@@ -13,8 +13,10 @@
 // the group). K and V are read once for all of them, and dK, dV are sums over all R rows, which is the gradient of a shared
 // head. A unit is one (batch, key head).
 //
-// Tiles in LDS are row-major with rows of DP + 16 elements (DP: the head size D padded to 32, 64, 96 or 128): the 8 lanes of
-// one LDS cycle of a 16-byte read, and the 4 rows of a transposing read, then fall on different banks.
+// Tiles in LDS are row-major with rows of DP elements (DP: the head size D padded to 32, 64, 96 or 128) in 16-byte chunks, chunk
+// c of row r at c ^ f(r) (tile_at). LDS serves 16 lanes x 16 bytes, or 32 lanes x 8 bytes, at a time from 64 banks: the
+// operand reads take one chunk of 16 consecutive rows, the transposing reads 4 aligned chunks of 4 consecutive rows, and f
+// spreads either over all banks (rows padded by 32 bytes instead: 40 % of the LDS cycles were bank conflicts).
 #pragma once
 #include "q8_common.h"
 #include "q8_host.h"
@@ -64,17 +66,25 @@ __device__ __forceinline__ v16f splat16(float v) {
     return r;
 }
 
-// A operand: rows row0 + l % 32 of a row-major LDS tile, elements e0 + 8 (l / 32) .. + 7
-template <int LD>
-__device__ __forceinline__ v4u lds_rows(const uint16_t* tile, int row0, int e0, int lane) {
-    return *reinterpret_cast<const v4u*>(tile + (row0 + (lane & 31)) * LD + e0 + ((lane >> 5) << 3));
+// element offset of chunk c of row r
+template <int DP>
+__device__ __forceinline__ int tile_at(int r, int c) {
+    const int f = DP == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : DP == 64 ? ((r & 2) << 1) | ((r >> 2) & 3) : (r >> 2) & 3;
+    return r * DP + ((c ^ f) << 3);
 }
-// A operand of the transposed tile: column e0 + l % 32 over the 16 rows from row0, in the order of a score column's results
-template <int LD>
-__device__ __forceinline__ v4u lds_cols(const uint16_t* tile, int row0, int e0, int lane) {
-    const uint16_t* p = tile + (row0 + ((lane >> 5) << 2) + ((lane & 15) >> 2)) * LD + e0 + (lane & 16) + ((lane & 3) << 2);
+// A operand: rows row0 + l % 32 (row0 a multiple of 32), elements 16 s + 8 (l / 32) .. + 7
+template <int DP>
+__device__ __forceinline__ v4u lds_rows(const uint16_t* tile, int row0, int s, int lane) {
+    return *reinterpret_cast<const v4u*>(tile + row0 * DP + tile_at<DP>(lane & 31, 2 * s + (lane >> 5)));
+}
+// A operand of the transposed tile: column 32 d + l % 32 over the 16 rows from row0 (a multiple of 16), in the order of a
+// score column's results
+template <int DP>
+__device__ __forceinline__ v4u lds_cols(const uint16_t* tile, int row0, int d, int lane) {
+    const int r = ((lane >> 5) << 2) + ((lane & 15) >> 2), c = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), e = (lane & 1) << 2;
+    const uint16_t *p = tile + row0 * DP + tile_at<DP>(r, c) + e, *q = tile + row0 * DP + tile_at<DP>(r + 8, c) + e;
     const v4s16 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s16*)(p));
-    const v4s16 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s16*)(p + 8 * LD));
+    const v4s16 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s16*)(q));
     const v2i x = __builtin_bit_cast(v2i, a), y = __builtin_bit_cast(v2i, b);
     return v4u{(unsigned)x[0], (unsigned)x[1], (unsigned)y[0], (unsigned)y[1]};
 }
@@ -86,28 +96,54 @@ __device__ __forceinline__ v4u pack_step(const v16f& v, int s) {
                pack2<DT>(v[8 * s + 6], v[8 * s + 7])};
 }
 
-// 64 rows of a tensor on their way to LDS: requested early, written later. Rows or elements outside are zeros.
-template <int DP>
+// TR rows of a tensor on their way to LDS: requested early, written later. A thread's chunks (16 bytes) are chunk `ch` of rows
+// row + k RS, or, where a row's chunks do not divide the workgroup (DP = 96), each on its own. Chunks past the head size are
+// neither read nor written: clear_tiles has zeroed them once.
+template <int DP, int TR>
 struct Stage {
-    static constexpr int LD = DP + 16, CPR = DP / 8, N = kXTile * CPR / kXThreads;
+    static constexpr int CPR = DP / 8, N = TR * CPR / kXThreads, RS = kXThreads / CPR;
+    static constexpr bool EVEN = kXThreads % CPR == 0;
+    static_assert(TR * CPR % kXThreads == 0, "whole chunks for every thread");
     v4u r[N];
-    template <typename At>  // at(row): pointer to the row's first element, or NULL for a row of zeros
-    __device__ __forceinline__ void load(At at, int D) {
+    static __device__ __forceinline__ int row(int k) { return EVEN ? (int)threadIdx.x / CPR + k * RS : ((int)threadIdx.x + k * kXThreads) / CPR; }
+    static __device__ __forceinline__ int chunk(int k) { return EVEN ? (int)threadIdx.x % CPR : ((int)threadIdx.x + k * kXThreads) % CPR; }
+    // rows base + row * st (st below 2^25: a tile's offsets fit 32 bits), all of them there
+    __device__ __forceinline__ void load(const uint16_t* base, int64_t st, int D) {
+        const unsigned s = (unsigned)st;
 #pragma unroll
-        for (int c = 0; c < N; ++c) {
-            const int i = threadIdx.x + c * kXThreads, row = i / CPR, e = (i - row * CPR) * 8;
-            const uint16_t* p = at(row);
-            r[c] = (p != nullptr && e < D) ? *reinterpret_cast<const v4u*>(p + e) : v4u{0u, 0u, 0u, 0u};
+        for (int k = 0; k < N; ++k) {
+            if (chunk(k) * 8 >= D) continue;
+            const char* b = reinterpret_cast<const char*>(EVEN ? base + k * RS * st : base);
+            const unsigned off = (unsigned)(EVEN ? row(0) : row(k)) * s * 2u + (unsigned)chunk(k) * 16u;
+            r[k] = *reinterpret_cast<const v4u*>(b + off);
         }
     }
-    __device__ __forceinline__ void store(uint16_t* tile) const {
+    // at(row): pointer to the first element of a row that may be read, whatever becomes of it
+    template <typename At>
+    __device__ __forceinline__ void load_each(At at, int D) {
 #pragma unroll
-        for (int c = 0; c < N; ++c) {
-            const int i = threadIdx.x + c * kXThreads, row = i / CPR, e = (i - row * CPR) * 8;
-            *reinterpret_cast<v4u*>(tile + row * LD + e) = r[c];
-        }
+        for (int k = 0; k < N; ++k)
+            if (chunk(k) * 8 < D) r[k] = *reinterpret_cast<const v4u*>(at(row(k)) + chunk(k) * 8);
+    }
+    __device__ __forceinline__ void store(uint16_t* tile, int D) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (chunk(k) * 8 < D) *reinterpret_cast<v4u*>(tile + tile_at<DP>(row(k), chunk(k))) = r[k];
+    }
+    // rows without a bit in `live` become zeros
+    __device__ __forceinline__ void store_live(uint16_t* tile, int D, uint64_t live) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (chunk(k) * 8 < D)
+                *reinterpret_cast<v4u*>(tile + tile_at<DP>(row(k), chunk(k))) = (live >> row(k)) & 1 ? r[k] : v4u{0u, 0u, 0u, 0u};
     }
 };
+
+// zeros in tiles whose rows are longer than the head; followed by a barrier
+template <int ELEMS>
+__device__ __forceinline__ void clear_tiles(uint16_t* t) {
+    for (int i = threadIdx.x * 8; i < ELEMS; i += kXThreads * 8) *reinterpret_cast<v4u*>(t + i) = v4u{0u, 0u, 0u, 0u};
+}
 
 // Which keys of a batch element count: those below its length whose mask byte is not zero.
 struct XKeys {
@@ -123,14 +159,93 @@ struct XKeys {
     __device__ __forceinline__ const uint8_t* row(int b) const { return mask == nullptr ? nullptr : mask + b * mask_stride; }
 };
 
-// Work item of a workgroup such that consecutive items run on the same XCD (workgroups go to the 8 XCDs in turn): the row
-// blocks of a unit then share its K and V in one L2. The grid is 8 * ceil(items / 8); false: nothing to do.
-__device__ __forceinline__ bool xcd_item(unsigned items, unsigned& item) {
-    const unsigned per = (items + 7) / 8;
-    item = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
-    return (blockIdx.x >> 3) < per && item < items;
+// K and V in tiles of 64 keys: two buffers, the next tile in registers meanwhile.
+template <int DP>
+struct KVTiles {
+    static constexpr int ELEMS = kXTile * DP;
+    Stage<DP, kXTile> k, v;
+    const uint16_t *kp, *vp;
+    int64_t kst, vst;
+    const uint8_t* mask;
+    int len, D;
+    uint8_t byte;
+    __device__ __forceinline__ void load(int t) {
+        const int key0 = t * kXTile, lane = threadIdx.x & 63;
+        const uint16_t *kb = kp + key0 * kst, *vb = vp + key0 * vst;
+        const int last = len - 1 - key0;  // 0 or more: the tile exists
+        byte = 1;
+        if (mask != nullptr) byte = mask[key0 + (lane < last ? lane : last)];
+        if (last >= kXTile - 1) {
+            k.load(kb, kst, D);
+            v.load(vb, vst, D);
+        } else {
+            k.load_each([&](int r) { return kb + (r < last ? r : last) * kst; }, D);
+            v.load_each([&](int r) { return vb + (r < last ? r : last) * vst; }, D);
+        }
+    }
+    // writes the tile and the bias of its scores (0, or -infinity where a key does not count); returns the keys that count
+    __device__ __forceinline__ uint64_t store(int t, uint16_t* kt, uint16_t* vt, float* bias) const {
+        const int lane = threadIdx.x & 63;
+        const bool counts = t * kXTile + lane < len && byte != 0;
+        const uint64_t live = __builtin_amdgcn_ballot_w64(counts);
+        if (live == ~(uint64_t)0) {
+            k.store(kt, D);
+            v.store(vt, D);
+        } else {
+            k.store_live(kt, D, live);
+            v.store_live(vt, D, live);
+            if (threadIdx.x < kXTile) bias[threadIdx.x] = counts ? 0.f : -__builtin_inff();
+        }
+        return live;
+    }
+};
+// the start of a tile's scores: the bias of rows 32 u .. 32 u + 31
+__device__ __forceinline__ v16f bias16(const float* bias, int u, int half) {
+    v16f s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const v4f w = *reinterpret_cast<const v4f*>(bias + u * 32 + i * 8 + half * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i * 4 + j] = w[j];
+    }
+    return s;
 }
-inline unsigned xcd_grid(unsigned items) { return 8u * ((items + 7) / 8); }
+
+// Which block (128 rows or keys of a unit) a workgroup works on, and which part of its walk. The blocks that fill the card
+// whole times (`full`, a multiple of the workgroups that run at once) are walked by one workgroup each; those left (`tail`),
+// which would leave most of it idle for another whole turn, are divided over `splits` workgroups each. Workgroups go to the 8
+// XCDs in turn: consecutive blocks are given to the same XCD, whose L2 then holds the K and V (or Q and dO) that they share.
+struct XSchedule {
+    unsigned full, tail;
+    int splits;
+    __device__ __forceinline__ bool item(unsigned& block, int& split, int& of) const {
+        const unsigned id = blockIdx.x;
+        of = 1;
+        split = 0;
+        if (id < full) {
+            block = (id & 7u) * (full >> 3) + (id >> 3);
+            return true;
+        }
+        const unsigned j = id - full, n = tail * splits, per = (n + 7) / 8, k = (j & 7u) * per + (j >> 3);
+        if ((j >> 3) >= per || k >= n) return false;
+        split = (int)(k / tail);
+        block = full + k - split * tail;
+        of = splits;
+        return true;
+    }
+    unsigned grid() const { return full + 8u * ((tail * splits + 7) / 8); }
+    int64_t parts() const { return splits > 1 ? (int64_t)tail * splits : 0; }  // blocks of partial results
+};
+// `slots`: workgroups that run at once; a divided walk is four tiles or more
+inline XSchedule schedule(int64_t blocks, int64_t length, int slots) {
+    XSchedule s;
+    s.full = (unsigned)(blocks / slots * slots);
+    s.tail = (unsigned)(blocks - s.full);
+    const int64_t most = ((length + kXTile - 1) / kXTile + 3) / 4, want = s.tail ? slots / s.tail : 1;
+    s.splits = (int)(want < most ? want : most);
+    if (s.splits < 1) s.splits = 1;
+    return s;
+}
 
 // One 32 x D result of a wave (columns = rows of the output, results = its elements) to memory in whole 16-byte chunks,
 // through `buf` (32 rows of DP + 8 elements, the wave's own). at(row): pointer to the output row or NULL.
@@ -168,6 +283,7 @@ inline int x_tensor(const char* who, const char* name, const void* p, const int6
         if (s[i] % 8) return fail(Q8_ERR_ALIGN, "%s: strides of %s must be multiples of 8 elements", who, name);
         e += (__int128)(n[i] - 1) * s[i];
     }
+    if (t > 1 && s[2] >= (1 << 25)) return fail(Q8_ERR_SHAPE, "%s: token stride of %s (below 2^25 elements)", who, name);
     if (e > (INT64_MAX >> 4)) return fail(Q8_ERR_SHAPE, "%s: strides of %s", who, name);
     if (!aligned16(p)) return fail(Q8_ERR_ALIGN, "%s: %s must be 16-byte aligned", who, name);
     return Q8_OK;
