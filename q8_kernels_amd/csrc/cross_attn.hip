@@ -51,7 +51,6 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
-    if (t0 < t1) kv.load(t0);
     v4u qf[KS];
     {
         const int g = row < a.R ? row / a.M : 0, m = row - g * a.M;
@@ -59,6 +58,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = (row < a.R && s * 16 + half * 8 < a.D) ? *reinterpret_cast<const v4u*>(p + s * 16) : v4u{0u, 0u, 0u, 0u};
     }
+    // (after Q: the wait for the first tile then covers Q too, and none is left for the loop)
+    if (t0 < t1) kv.load(t0);
     if (a.D < DP) {
         clear_tiles<4 * ELEMS>(tiles_lds);
         __syncthreads();
@@ -70,10 +71,13 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     float m = -3.0e38f, l = 0.f;  // in units of log2; the sum over this lane's half of the keys
     uint64_t live = ~(uint64_t)0;
     if (t0 < t1) live = kv.store(t0, tiles_lds, tiles_lds + 2 * ELEMS, bias[0]);
+    wait_loads();
     __syncthreads();
 
+    LaneOffsets<DP> at(lane);
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
+        at.fresh();
         const uint16_t *kl = tiles_lds + BUF * ELEMS, *vl = tiles_lds + (2 + BUF) * ELEMS;
         const bool more = t + 1 < t1;
         if (more) kv.load(t + 1);
@@ -83,14 +87,15 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
             for (int u = 0; u < 2; ++u) {
                 s[u] = splat16(0.f);
 #pragma unroll
-                for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, lane), qf[e], s[u]);
+                for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s[u]);
             }
+            order_reads_ahead<2 * KS, 1, 4>();
         } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 s[u] = bias16(bias[BUF], u, half);
 #pragma unroll
-                for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, lane), qf[e], s[u]);
+                for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s[u]);
             }
         }
         float top = s[0][0];
@@ -120,7 +125,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(s[u], k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(vl, u * 32 + k * 16, d, lane), p, acc[d]);
+                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(vl, u * 32 + k * 16, d, at), p, acc[d]);
             }
         }
         if (more) live = kv.store(t + 1, tiles_lds + (1 - BUF) * ELEMS, tiles_lds + (3 - BUF) * ELEMS, bias[1 - BUF]);

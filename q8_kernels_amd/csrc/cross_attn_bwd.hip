@@ -55,7 +55,6 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
-    if (t0 < t1) kv.load(t0);
     v4u qf[KS], gf[KS];
     float delta = 0.f, lse = __builtin_inff();
     {
@@ -84,6 +83,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
             if (split == 0 && half == 0) a.delta[at] = delta;
         }
     }
+    if (t0 < t1) kv.load(t0);
     if (a.D < DP) {
         clear_tiles<4 * ELEMS>(tiles_lds);
         __syncthreads();
@@ -94,10 +94,13 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
     uint64_t live = ~(uint64_t)0;
     if (t0 < t1) live = kv.store(t0, tiles_lds, tiles_lds + 2 * ELEMS, bias[0]);
+    wait_loads();
     __syncthreads();
 
+    LaneOffsets<DP> at(lane);
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
+        at.fresh();
         const uint16_t *kl = tiles_lds + BUF * ELEMS, *vl = tiles_lds + (2 + BUF) * ELEMS;
         const bool more = t + 1 < t1;
         if (more) kv.load(t + 1);
@@ -107,21 +110,21 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
             if (live == ~(uint64_t)0) {
                 s = splat16(0.f);
 #pragma unroll
-                for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, lane), qf[e], s);
+                for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s);
             } else {
                 s = bias16(bias[BUF], u, half);
 #pragma unroll
-                for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, lane), qf[e], s);
+                for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s);
             }
 #pragma unroll
-            for (int e = 0; e < KS; ++e) dp = mfma16<DT>(lds_rows<DP>(vl, u * 32, e, lane), gf[e], dp);
+            for (int e = 0; e < KS; ++e) dp = mfma16<DT>(lds_rows<DP>(vl, u * 32, e, at), gf[e], dp);
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse));
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(dp, k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(kl, u * 32 + k * 16, d, lane), p, acc[d]);
+                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(kl, u * 32 + k * 16, d, at), p, acc[d]);
             }
         }
         if (more) live = kv.store(t + 1, tiles_lds + (1 - BUF) * ELEMS, tiles_lds + (3 - BUF) * ELEMS, bias[1 - BUF]);
@@ -173,7 +176,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     const int len = a.keys.length(b);
     const uint8_t* mask = a.keys.row(b);
     const bool counts = key < len && (mask == nullptr || mask[key]);
-    const int tiles = (a.R + TR - 1) / TR, per = (tiles + of - 1) / of;
+    // tiles of one head's rows each: the last of a head may be short
+    const int head_tiles = (a.M + TR - 1) / TR, tiles = a.G * head_tiles, per = (tiles + of - 1) / of;
     const int t0 = split * per;
     int t1 = t0 + per < tiles ? t0 + per : tiles;
     if (kb * 128 >= len) t1 = t0;  // no key of this workgroup counts: zeros
@@ -181,45 +185,36 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     Stage<DP, TR> qs, gs;
     float row_lse = 0.f, row_delta = 0.f;
     const uint16_t *qp = a.q.p + b * a.q.sb + (int64_t)hk * a.G * a.q.sh, *gp = a.g.p + b * a.g.sb + (int64_t)hk * a.G * a.g.sh;
+    int loaded = 0;  // rows of the tile on its way
     auto load = [&](int t) {
-        const int n0 = t * TR, g0 = n0 / a.M, m0 = n0 - g0 * a.M;
-        if (m0 + TR <= a.M) {  // all rows of one head
-            qs.load(qp + g0 * a.q.sh + m0 * a.q.st, a.q.st, a.D);
-            gs.load(gp + g0 * a.g.sh + m0 * a.g.st, a.g.st, a.D);
+        const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
+        const uint16_t *q = qp + g * a.q.sh + m * a.q.st, *d = gp + g * a.g.sh + m * a.g.st;
+        loaded = a.M - m;
+        if (loaded >= TR) {
+            qs.load(q, a.q.st, a.D);
+            gs.load(d, a.g.st, a.D);
         } else {
-            auto at = [&](const uint16_t* p, const XTensor& x) {
-                return [&, p](int r) {
-                    const int n = n0 + r < a.R ? n0 + r : a.R - 1, g = n / a.M;
-                    return p + g * x.sh + (n - g * a.M) * x.st;
-                };
-            };
-            qs.load_each(at(qp, a.q), a.D);
-            gs.load_each(at(gp, a.g), a.D);
+            qs.load_upto(q, a.q.st, a.D, loaded - 1);
+            gs.load_upto(d, a.g.st, a.D, loaded - 1);
         }
-        const int n = n0 + (int)threadIdx.x;
-        if (threadIdx.x < TR) {
-            row_lse = -__builtin_inff();
-            row_delta = 0.f;
-            if (n < a.R) {
-                row_lse = -a.lse[(int64_t)unit * a.R + n];
-                row_delta = -a.delta[(int64_t)unit * a.R + n];
-            }
-        }
+        const int n = (int)threadIdx.x & (TR - 1);
+        const int64_t at = (int64_t)unit * a.R + g * a.M + m + (n < loaded ? n : loaded - 1);
+        row_lse = a.lse[at];
+        row_delta = a.delta[at];
     };
-    auto store = [&](int t, int buf) {
+    auto store = [&](int buf) {
         uint16_t *q = tiles_lds + buf * ELEMS, *g = tiles_lds + (2 + buf) * ELEMS;
-        const int left = a.R - t * TR;
-        if (left >= TR) {
+        if (loaded >= TR) {
             qs.store(q, a.D);
             gs.store(g, a.D);
         } else {
-            const uint64_t live = ((uint64_t)1 << left) - 1;
+            const uint64_t live = ((uint64_t)1 << loaded) - 1;
             qs.store_live(q, a.D, live);
             gs.store_live(g, a.D, live);
         }
         if (threadIdx.x < TR) {
-            lt[buf][threadIdx.x] = row_lse;
-            dt[buf][threadIdx.x] = row_delta;
+            lt[buf][threadIdx.x] = (int)threadIdx.x < loaded ? -row_lse : -__builtin_inff();
+            dt[buf][threadIdx.x] = (int)threadIdx.x < loaded ? -row_delta : 0.f;
         }
     };
     if (t0 < t1) load(t0);
@@ -246,10 +241,13 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     v16f dk[DTL], dv[DTL];
 #pragma unroll
     for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
-    if (t0 < t1) store(t0, 0);
+    if (t0 < t1) store(0);
+    wait_loads();
     __syncthreads();
+    LaneOffsets<DP> at(lane);
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
+        at.fresh();
         const uint16_t *ql = tiles_lds + BUF * ELEMS, *gl = tiles_lds + (2 + BUF) * ELEMS;
         const bool more = t + 1 < t1;
         if (more) load(t + 1);
@@ -257,13 +255,13 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
         for (int u = 0; u < TR / 32; ++u) {
             v16f s = splat16(0.f), dp = bias16(dt[BUF], u, half);
 #pragma unroll
-            for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(ql, u * 32, e, lane), kf[e], s);
+            for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(ql, u * 32, e, at), kf[e], s);
 #pragma unroll
             for (int e = 0; e < KS; ++e) {
                 v4u v;
-                if constexpr (V_IN_LDS) v = lds_rows<DP>(vl, wave * 32, e, lane);
+                if constexpr (V_IN_LDS) v = lds_rows<DP>(vl, wave * 32, e, at);
                 else v = vf[e];
-                dp = mfma16<DT>(lds_rows<DP>(gl, u * 32, e, lane), v, dp);
+                dp = mfma16<DT>(lds_rows<DP>(gl, u * 32, e, at), v, dp);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -275,7 +273,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(s, k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) dv[d] = mfma16<DT>(lds_cols<DP>(gl, u * 32 + k * 16, d, lane), p, dv[d]);
+                for (int d = 0; d < DTL; ++d) dv[d] = mfma16<DT>(lds_cols<DP>(gl, u * 32 + k * 16, d, at), p, dv[d]);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] *= s[i];
@@ -283,10 +281,10 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(dp, k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(lds_cols<DP>(ql, u * 32 + k * 16, d, lane), p, dk[d]);
+                for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(lds_cols<DP>(ql, u * 32 + k * 16, d, at), p, dk[d]);
             }
         }
-        if (more) store(t + 1, 1 - BUF);
+        if (more) store(1 - BUF);
         __syncthreads();
     };
     for (int t = t0; t < t1; t += 2) {
@@ -314,15 +312,15 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
         return;
     }
     static_assert(kXWaves * 32 * (DP + 8) <= 4 * ELEMS + (V_IN_LDS ? 128 * DP : 0), "the output tiles fit the tile buffers");
-    auto at = [&](const XOut& x) {
+    auto to = [&](const XOut& x) {
         uint16_t* p = x.p + b * x.sb + hk * x.sh;
         return [&, p](int r) -> uint16_t* { return key0 + r < a.N ? p + (key0 + r) * x.st : nullptr; };
     };
     uint16_t* buf = tiles_lds + wave * 32 * (DP + 8);
-    store_tile<DT, DP>(dk, a.scale, buf, a.D, lane, at(a.dk));
+    store_tile<DT, DP>(dk, a.scale, buf, a.D, lane, to(a.dk));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    store_tile<DT, DP>(dv, 1.0f, buf, a.D, lane, at(a.dv));
+    store_tile<DT, DP>(dv, 1.0f, buf, a.D, lane, to(a.dv));
 }
 
 // Adds the parts of dQ (WIDTH = 1) or of dK and dV (WIDTH = 2): one thread for 4 elements of a row.
@@ -370,7 +368,7 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     p.dq_blocks = (p.rows + 127) / 128;
     p.kv_blocks = ((int64_t)N + 127) / 128;
     p.dq = schedule(p.units * p.dq_blocks, N, kBwdSlots);
-    p.kv = schedule(p.units * p.kv_blocks, p.rows, kBwdSlots);
+    p.kv = schedule(p.units * p.kv_blocks, (int64_t)(H / Hkv) * ((M + kXTile - 1) / kXTile) * kXTile, kBwdSlots);
     const int64_t dq = p.dq.parts() * 128 * D, kv = p.kv.parts() * 256 * D;
     p.parts = dq > kv ? dq : kv;  // one after the other in the same place
     return p;

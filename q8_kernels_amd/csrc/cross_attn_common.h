@@ -72,22 +72,56 @@ __device__ __forceinline__ int tile_at(int r, int c) {
     const int f = DP == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : DP == 64 ? ((r & 2) << 1) | ((r >> 2) & 3) : (r >> 2) & 3;
     return r * DP + ((c ^ f) << 3);
 }
+// A lane's byte offsets in a tile, for its chunk of elements 0 .. 15 (rows) and columns 0 .. 31 (cols). The other operands
+// are an XOR of a constant away (an addition where f leaves the bits alone), which is cheaper than keeping 16 addresses in
+// registers: fresh() keeps the compiler from doing that.
+template <int DP>
+struct LaneOffsets {
+    unsigned rows, cols;
+    __device__ __forceinline__ explicit LaneOffsets(int lane) {
+        rows = (unsigned)tile_at<DP>(lane & 31, lane >> 5) * 2u;
+        cols = (unsigned)tile_at<DP>(((lane >> 5) << 2) + ((lane & 15) >> 2), ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 2u + ((lane & 1) << 3);
+    }
+    __device__ __forceinline__ void fresh() {
+        asm volatile("" : "+v"(rows));
+        asm volatile("" : "+v"(cols));
+    }
+};
 // A operand: rows row0 + l % 32 (row0 a multiple of 32), elements 16 s + 8 (l / 32) .. + 7
 template <int DP>
-__device__ __forceinline__ v4u lds_rows(const uint16_t* tile, int row0, int s, int lane) {
-    return *reinterpret_cast<const v4u*>(tile + row0 * DP + tile_at<DP>(lane & 31, 2 * s + (lane >> 5)));
+__device__ __forceinline__ v4u lds_rows(const uint16_t* tile, int row0, int s, const LaneOffsets<DP>& at) {
+    const unsigned o = DP == 96 ? (at.rows ^ ((s & 1) << 5)) + ((s >> 1) << 6) : at.rows ^ (s << 5);
+    return *reinterpret_cast<const v4u*>(reinterpret_cast<const char*>(tile + row0 * DP) + o);
 }
 // A operand of the transposed tile: column 32 d + l % 32 over the 16 rows from row0 (a multiple of 16), in the order of a
-// score column's results
+// score column's results: 4 rows, and the 4 rows 8 further, where f differs in its second bit
 template <int DP>
-__device__ __forceinline__ v4u lds_cols(const uint16_t* tile, int row0, int d, int lane) {
-    const int r = ((lane >> 5) << 2) + ((lane & 15) >> 2), c = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), e = (lane & 1) << 2;
-    const uint16_t *p = tile + row0 * DP + tile_at<DP>(r, c) + e, *q = tile + row0 * DP + tile_at<DP>(r + 8, c) + e;
-    const v4s16 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s16*)(p));
-    const v4s16 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s16*)(q));
+__device__ __forceinline__ v4u lds_cols(const uint16_t* tile, int row0, int d, const LaneOffsets<DP>& at) {
+    const unsigned o = DP == 96 ? at.cols + (d << 6) : at.cols ^ (d << 6);
+    const char* p = reinterpret_cast<const char*>(tile + row0 * DP);
+    const v4s16 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s16*)(p + o));
+    const v4s16 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s16*)(p + 16 * DP + (o ^ 32u)));
     const v2i x = __builtin_bit_cast(v2i, a), y = __builtin_bit_cast(v2i, b);
     return v4u{(unsigned)x[0], (unsigned)x[1], (unsigned)y[0], (unsigned)y[1]};
 }
+
+// Instruction order of a product loop: LDS operand reads run AHEAD of the matrix instructions that use them (left alone, the
+// compiler puts each read right before its use and every matrix instruction waits out the LDS latency).
+// COUNT matrix instructions, each preceded by READS reads of LDS.
+template <int COUNT, int READS, int AHEAD>
+__device__ __forceinline__ void order_reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < COUNT - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
+// Waits for every load so far. In front of a loop whose first loads were requested under a condition: the compiler, which
+// cannot see that the conditions agree, would otherwise wait for ALL loads, the next tile's among them, in every turn.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // The B operand that results 8 s .. 8 s + 7 of a score column make
 template <int DT>
@@ -118,12 +152,15 @@ struct Stage {
             r[k] = *reinterpret_cast<const v4u*>(b + off);
         }
     }
-    // at(row): pointer to the first element of a row that may be read, whatever becomes of it
-    template <typename At>
-    __device__ __forceinline__ void load_each(At at, int D) {
+    // the same with rows 0 .. last there: the others are row `last` again
+    __device__ __forceinline__ void load_upto(const uint16_t* base, int64_t st, int D, int last) {
+        const unsigned s = (unsigned)st;
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (chunk(k) * 8 < D) r[k] = *reinterpret_cast<const v4u*>(at(row(k)) + chunk(k) * 8);
+        for (int k = 0; k < N; ++k) {
+            if (chunk(k) * 8 >= D) continue;
+            const int n = row(k) < last ? row(k) : last;
+            r[k] = *reinterpret_cast<const v4u*>(reinterpret_cast<const char*>(base) + ((unsigned)n * s * 2u + (unsigned)chunk(k) * 16u));
+        }
     }
     __device__ __forceinline__ void store(uint16_t* tile, int D) const {
 #pragma unroll
@@ -173,20 +210,20 @@ struct KVTiles {
         const int key0 = t * kXTile, lane = threadIdx.x & 63;
         const uint16_t *kb = kp + key0 * kst, *vb = vp + key0 * vst;
         const int last = len - 1 - key0;  // 0 or more: the tile exists
-        byte = 1;
-        if (mask != nullptr) byte = mask[key0 + (lane < last ? lane : last)];
+        // (without a mask some byte of K: a load that depends on a branch would be waited for at once)
+        byte = *(mask != nullptr ? mask + key0 + (lane < last ? lane : last) : reinterpret_cast<const uint8_t*>(kb));
         if (last >= kXTile - 1) {
             k.load(kb, kst, D);
             v.load(vb, vst, D);
         } else {
-            k.load_each([&](int r) { return kb + (r < last ? r : last) * kst; }, D);
-            v.load_each([&](int r) { return vb + (r < last ? r : last) * vst; }, D);
+            k.load_upto(kb, kst, D, last);
+            v.load_upto(vb, vst, D, last);
         }
     }
     // writes the tile and the bias of its scores (0, or -infinity where a key does not count); returns the keys that count
     __device__ __forceinline__ uint64_t store(int t, uint16_t* kt, uint16_t* vt, float* bias) const {
         const int lane = threadIdx.x & 63;
-        const bool counts = t * kXTile + lane < len && byte != 0;
+        const bool counts = t * kXTile + lane < len && (mask == nullptr || byte != 0);
         const uint64_t live = __builtin_amdgcn_ballot_w64(counts);
         if (live == ~(uint64_t)0) {
             k.store(kt, D);
