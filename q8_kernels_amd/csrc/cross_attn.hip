@@ -30,14 +30,14 @@ struct XFwd {
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32, ELEMS = kXTile * DP;
-    __shared__ __align__(16) uint16_t tiles_lds[4 * ELEMS];  // K, K, V, V
-    __shared__ __align__(16) float bias[2][kXTile];
+    __shared__ __align__(16) uint16_t k0[ELEMS], k1[ELEMS], v0[ELEMS], v1[ELEMS];
+    __shared__ __align__(16) float bias0[kXTile], bias1[kXTile];
     unsigned block;
     int split, of;
     if (!a.plan.item(block, split, of)) return;
     const int unit = block / a.row_blocks, rb = block - unit * a.row_blocks;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
 
     KVTiles<DP> kv;
@@ -48,6 +48,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
     kv.kst = a.k.st;
     kv.vst = a.v.st;
+    kv.wave = wave;
     const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
@@ -58,19 +59,12 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = (row < a.R && s * 16 + half * 8 < a.D) ? *reinterpret_cast<const v4u*>(p + s * 16) : v4u{0u, 0u, 0u, 0u};
     }
-    // (after Q: the wait for the first tile then covers Q too, and none is left for the loop)
-    if (t0 < t1) kv.load(t0);
-    if (a.D < DP) {
-        clear_tiles<4 * ELEMS>(tiles_lds);
-        __syncthreads();
-    }
+    if (t0 < t1) kv.first(t0, k0, v0, bias0);
 
     v16f acc[DTL];
 #pragma unroll
     for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
     float m = -3.0e38f, l = 0.f;  // in units of log2; the sum over this lane's half of the keys
-    uint64_t live = ~(uint64_t)0;
-    if (t0 < t1) live = kv.store(t0, tiles_lds, tiles_lds + 2 * ELEMS, bias[0]);
     wait_loads();
     __syncthreads();
 
@@ -78,11 +72,11 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
-        const uint16_t *kl = tiles_lds + BUF * ELEMS, *vl = tiles_lds + (2 + BUF) * ELEMS;
+        const uint16_t *kl = BUF ? k1 : k0, *vl = BUF ? v1 : v0;
         const bool more = t + 1 < t1;
-        if (more) kv.load(t + 1);
+        kv.begin(t, more, BUF ? k0 : k1, BUF ? v0 : v1, BUF ? bias0 : bias1);
         v16f s[2];
-        if (live == ~(uint64_t)0) {
+        if (kv.live[0] == ~(uint64_t)0) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 s[u] = splat16(0.f);
@@ -93,7 +87,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
         } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                s[u] = bias16(bias[BUF], u, half);
+                s[u] = bias16(BUF ? bias1 : bias0, u, half);
 #pragma unroll
                 for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s[u]);
             }
@@ -128,7 +122,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
                 for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(vl, u * 32 + k * 16, d, at), p, acc[d]);
             }
         }
-        if (more) live = kv.store(t + 1, tiles_lds + (1 - BUF) * ELEMS, tiles_lds + (3 - BUF) * ELEMS, bias[1 - BUF]);
+        kv.end(t, more);
         __syncthreads();
     };
     for (int t = t0; t < t1; t += 2) {
@@ -158,8 +152,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
         a.lse[(int64_t)unit * a.R + row] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     // (the tile buffers are free: every wave has passed the last barrier of the loop)
-    static_assert(kXWaves * 32 * (DP + 8) <= 4 * ELEMS, "the output tiles fit the tile buffers");
-    store_tile<DT, DP>(acc, inv, tiles_lds + wave * 32 * (DP + 8), a.D, lane, [&](int r) -> uint16_t* {
+    store_tile<DT, DP>(acc, inv, (wave < 2 ? wave == 0 ? k0 : k1 : wave == 2 ? v0 : v1), a.D, lane, [&](int r) -> uint16_t* {
         const int n = row0 + r;
         if (n >= a.R) return nullptr;
         const int g = n / a.M;
@@ -195,8 +188,8 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
-// two workgroups on every CU (three with heads of 64 or less, whose registers allow it)
-static int fwd_slots(int D) { return D <= 64 ? 768 : 512; }
+// workgroups that run at once: as many on each of the 256 CUs as registers (128, 158 and 218 a lane) and LDS allow
+static int fwd_slots(int D) { return D <= 64 ? 1024 : D <= 96 ? 768 : 512; }
 
 }  // namespace q8
 

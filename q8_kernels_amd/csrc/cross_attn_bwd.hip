@@ -34,14 +34,14 @@ struct XBwd {
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32, ELEMS = kXTile * DP;
-    __shared__ __align__(16) uint16_t tiles_lds[4 * ELEMS];  // K, K, V, V
-    __shared__ __align__(16) float bias[2][kXTile];
+    __shared__ __align__(16) uint16_t k0[ELEMS], k1[ELEMS], v0[ELEMS], v1[ELEMS];
+    __shared__ __align__(16) float bias0[kXTile], bias1[kXTile];
     unsigned block;
     int split, of;
     if (!a.plan.item(block, split, of)) return;
     const int unit = block / a.blocks, rb = block - unit * a.blocks;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
 
     KVTiles<DP> kv;
@@ -52,6 +52,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
     kv.kst = a.k.st;
     kv.vst = a.v.st;
+    kv.wave = wave;
     const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
@@ -83,17 +84,11 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
             if (split == 0 && half == 0) a.delta[at] = delta;
         }
     }
-    if (t0 < t1) kv.load(t0);
-    if (a.D < DP) {
-        clear_tiles<4 * ELEMS>(tiles_lds);
-        __syncthreads();
-    }
+    if (t0 < t1) kv.first(t0, k0, v0, bias0);
 
     v16f acc[DTL];
 #pragma unroll
     for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
-    uint64_t live = ~(uint64_t)0;
-    if (t0 < t1) live = kv.store(t0, tiles_lds, tiles_lds + 2 * ELEMS, bias[0]);
     wait_loads();
     __syncthreads();
 
@@ -101,18 +96,18 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
-        const uint16_t *kl = tiles_lds + BUF * ELEMS, *vl = tiles_lds + (2 + BUF) * ELEMS;
+        const uint16_t *kl = BUF ? k1 : k0, *vl = BUF ? v1 : v0;
         const bool more = t + 1 < t1;
-        if (more) kv.load(t + 1);
+        kv.begin(t, more, BUF ? k0 : k1, BUF ? v0 : v1, BUF ? bias0 : bias1);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             v16f s, dp = splat16(-delta);
-            if (live == ~(uint64_t)0) {
+            if (kv.live[0] == ~(uint64_t)0) {
                 s = splat16(0.f);
 #pragma unroll
                 for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s);
             } else {
-                s = bias16(bias[BUF], u, half);
+                s = bias16(BUF ? bias1 : bias0, u, half);
 #pragma unroll
                 for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s);
             }
@@ -127,7 +122,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
                 for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(kl, u * 32 + k * 16, d, at), p, acc[d]);
             }
         }
-        if (more) live = kv.store(t + 1, tiles_lds + (1 - BUF) * ELEMS, tiles_lds + (3 - BUF) * ELEMS, bias[1 - BUF]);
+        kv.end(t, more);
         __syncthreads();
     };
     for (int t = t0; t < t1; t += 2) {
@@ -147,8 +142,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
         }
         return;
     }
-    static_assert(kXWaves * 32 * (DP + 8) <= 4 * ELEMS, "the output tiles fit the tile buffers");
-    store_tile<DT, DP>(acc, a.scale, tiles_lds + wave * 32 * (DP + 8), a.D, lane, [&](int r) -> uint16_t* {
+    store_tile<DT, DP>(acc, a.scale, (wave < 2 ? wave == 0 ? k0 : k1 : wave == 2 ? v0 : v1), a.D, lane, [&](int r) -> uint16_t* {
         const int n = row0 + r;
         if (n >= a.R) return nullptr;
         const int g = n / a.M;
@@ -163,14 +157,14 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32;
     constexpr bool V_IN_LDS = DP > 96;
     constexpr int TR = V_IN_LDS ? 32 : 64, ELEMS = TR * DP;
-    __shared__ __align__(16) uint16_t tiles_lds[4 * ELEMS + (V_IN_LDS ? 128 * DP : 0)];  // Q, Q, dO, dO, V
-    __shared__ __align__(16) float lt[2][TR], dt[2][TR];  // -lse and -delta of the tile's rows
+    __shared__ __align__(16) uint16_t q0[ELEMS], q1[ELEMS], g0[ELEMS], g1[ELEMS], vl[V_IN_LDS ? 128 * DP : 8];
+    __shared__ __align__(16) float lse0[TR], lse1[TR], delta0[TR], delta1[TR];  // -lse and -delta of the tile's rows
     unsigned block;
     int split, of;
     if (!a.plan.item(block, split, of)) return;
     const int unit = block / a.blocks, kb = block - unit * a.blocks;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int key0 = kb * 128 + wave * 32, key = key0 + (lane & 31);
 
     const int len = a.keys.length(b);
@@ -182,49 +176,30 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     int t1 = t0 + per < tiles ? t0 + per : tiles;
     if (kb * 128 >= len) t1 = t0;  // no key of this workgroup counts: zeros
 
-    Stage<DP, TR> qs, gs;
+    // rows go to LDS by copies, their log-sums and deltas through a register each
     float row_lse = 0.f, row_delta = 0.f;
+    int rows = 0;
     const uint16_t *qp = a.q.p + b * a.q.sb + (int64_t)hk * a.G * a.q.sh, *gp = a.g.p + b * a.g.sb + (int64_t)hk * a.G * a.g.sh;
-    int loaded = 0;  // rows of the tile on its way
-    auto load = [&](int t) {
+    auto start = [&](int t, uint16_t* qt, uint16_t* gt) {
         const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
-        const uint16_t *q = qp + g * a.q.sh + m * a.q.st, *d = gp + g * a.g.sh + m * a.g.st;
-        loaded = a.M - m;
-        if (loaded >= TR) {
-            qs.load(q, a.q.st, a.D);
-            gs.load(d, a.g.st, a.D);
-        } else {
-            qs.load_upto(q, a.q.st, a.D, loaded - 1);
-            gs.load_upto(d, a.g.st, a.D, loaded - 1);
-        }
+        rows = a.M - m;
+        const uint64_t live = rows >= TR ? ~(uint64_t)0 : ((uint64_t)1 << rows) - 1;
+        Copy<DP, TR>::start(qp + g * a.q.sh + m * a.q.st, a.q.st, a.D, live, qt, wave);
+        Copy<DP, TR>::start(gp + g * a.g.sh + m * a.g.st, a.g.st, a.D, live, gt, wave);
         const int n = (int)threadIdx.x & (TR - 1);
-        const int64_t at = (int64_t)unit * a.R + g * a.M + m + (n < loaded ? n : loaded - 1);
+        const int64_t at = (int64_t)unit * a.R + g * a.M + m + (n < rows ? n : rows - 1);
         row_lse = a.lse[at];
         row_delta = a.delta[at];
     };
-    auto store = [&](int buf) {
-        uint16_t *q = tiles_lds + buf * ELEMS, *g = tiles_lds + (2 + buf) * ELEMS;
-        if (loaded >= TR) {
-            qs.store(q, a.D);
-            gs.store(g, a.D);
-        } else {
-            const uint64_t live = ((uint64_t)1 << loaded) - 1;
-            qs.store_live(q, a.D, live);
-            gs.store_live(g, a.D, live);
-        }
+    auto finish = [&](float* lt, float* dt) {
+        wait_loads();
         if (threadIdx.x < TR) {
-            lt[buf][threadIdx.x] = (int)threadIdx.x < loaded ? -row_lse : -__builtin_inff();
-            dt[buf][threadIdx.x] = (int)threadIdx.x < loaded ? -row_delta : 0.f;
+            lt[threadIdx.x] = (int)threadIdx.x < rows ? -row_lse : -__builtin_inff();
+            dt[threadIdx.x] = (int)threadIdx.x < rows ? -row_delta : 0.f;
         }
     };
-    if (t0 < t1) load(t0);
 
     v4u kf[KS], vf[V_IN_LDS ? 1 : KS];
-    uint16_t* vl = tiles_lds + 4 * ELEMS;
-    if (a.D < DP) {
-        clear_tiles<4 * ELEMS + (V_IN_LDS ? 128 * DP : 0)>(tiles_lds);
-        __syncthreads();
-    }
     {
         const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh + key * a.k.st + half * 8;
         const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh + key * a.v.st + half * 8;
@@ -237,23 +212,27 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
             else vf[s] = v;
         }
     }
+    if (t0 < t1) {
+        start(t0, q0, g0);
+        finish(lse0, delta0);
+    }
 
     v16f dk[DTL], dv[DTL];
 #pragma unroll
     for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
-    if (t0 < t1) store(0);
     wait_loads();
     __syncthreads();
     LaneOffsets<DP> at(lane);
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
-        const uint16_t *ql = tiles_lds + BUF * ELEMS, *gl = tiles_lds + (2 + BUF) * ELEMS;
+        const uint16_t *ql = BUF ? q1 : q0, *gl = BUF ? g1 : g0;
+        const float *lt = BUF ? lse1 : lse0, *dt = BUF ? delta1 : delta0;
         const bool more = t + 1 < t1;
-        if (more) load(t + 1);
+        if (more) start(t + 1, BUF ? q0 : q1, BUF ? g0 : g1);
 #pragma unroll
         for (int u = 0; u < TR / 32; ++u) {
-            v16f s = splat16(0.f), dp = bias16(dt[BUF], u, half);
+            v16f s = splat16(0.f), dp = bias16(dt, u, half);
 #pragma unroll
             for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(ql, u * 32, e, at), kf[e], s);
 #pragma unroll
@@ -265,7 +244,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const v4f w = *reinterpret_cast<const v4f*>(&lt[BUF][u * 32 + i * 8 + half * 4]);
+                const v4f w = *reinterpret_cast<const v4f*>(&lt[u * 32 + i * 8 + half * 4]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[i * 4 + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * 4 + j], a.c, w[j]));
             }
@@ -284,7 +263,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
                 for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(lds_cols<DP>(ql, u * 32 + k * 16, d, at), p, dk[d]);
             }
         }
-        if (more) store(1 - BUF);
+        if (more) finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
         __syncthreads();
     };
     for (int t = t0; t < t1; t += 2) {
@@ -311,12 +290,11 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
         }
         return;
     }
-    static_assert(kXWaves * 32 * (DP + 8) <= 4 * ELEMS + (V_IN_LDS ? 128 * DP : 0), "the output tiles fit the tile buffers");
     auto to = [&](const XOut& x) {
         uint16_t* p = x.p + b * x.sb + hk * x.sh;
         return [&, p](int r) -> uint16_t* { return key0 + r < a.N ? p + (key0 + r) * x.st : nullptr; };
     };
-    uint16_t* buf = tiles_lds + wave * 32 * (DP + 8);
+    uint16_t* buf = wave < 2 ? wave == 0 ? q0 : q1 : wave == 2 ? g0 : g1;
     store_tile<DT, DP>(dk, a.scale, buf, a.D, lane, to(a.dk));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -354,8 +332,9 @@ __global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(s[0] * f, s[1] * f), (int)pack2<DT>(s[2] * f, s[3] * f)};
 }
 
-// two workgroups on every CU
-constexpr int kBwdSlots = 512;
+// workgroups that run at once: as many on each of the 256 CUs as registers allow
+static int dq_slots(int D) { return D <= 32 ? 1024 : D <= 64 ? 768 : 512; }
+static int kv_slots(int D) { return D <= 32 ? 1024 : 512; }
 
 struct XPlan {
     int64_t units, rows, dq_blocks, kv_blocks, parts;  // blocks of a unit; floats of partial results
@@ -367,8 +346,8 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     p.rows = (int64_t)(H / Hkv) * M;
     p.dq_blocks = (p.rows + 127) / 128;
     p.kv_blocks = ((int64_t)N + 127) / 128;
-    p.dq = schedule(p.units * p.dq_blocks, N, kBwdSlots);
-    p.kv = schedule(p.units * p.kv_blocks, (int64_t)(H / Hkv) * ((M + kXTile - 1) / kXTile) * kXTile, kBwdSlots);
+    p.dq = schedule(p.units * p.dq_blocks, N, dq_slots(D));
+    p.kv = schedule(p.units * p.kv_blocks, (int64_t)(H / Hkv) * ((M + kXTile - 1) / kXTile) * kXTile, kv_slots(D));
     const int64_t dq = p.dq.parts() * 128 * D, kv = p.kv.parts() * 256 * D;
     p.parts = dq > kv ? dq : kv;  // one after the other in the same place
     return p;

@@ -66,12 +66,13 @@ __device__ __forceinline__ v16f splat16(float v) {
     return r;
 }
 
+template <int DP>
+__device__ __forceinline__ int tile_f(int r) {
+    return DP == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : DP == 64 ? ((r & 2) << 1) | ((r >> 2) & 3) : (r >> 2) & 3;
+}
 // element offset of chunk c of row r
 template <int DP>
-__device__ __forceinline__ int tile_at(int r, int c) {
-    const int f = DP == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : DP == 64 ? ((r & 2) << 1) | ((r >> 2) & 3) : (r >> 2) & 3;
-    return r * DP + ((c ^ f) << 3);
-}
+__device__ __forceinline__ int tile_at(int r, int c) { return r * DP + ((c ^ tile_f<DP>(r)) << 3); }
 // A lane's byte offsets in a tile, for its chunk of elements 0 .. 15 (rows) and columns 0 .. 31 (cols). The other operands
 // are an XOR of a constant away (an addition where f leaves the bits alone), which is cheaper than keeping 16 addresses in
 // registers: fresh() keeps the compiler from doing that.
@@ -119,8 +120,7 @@ __device__ __forceinline__ void order_reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 }
 
-// Waits for every load so far. In front of a loop whose first loads were requested under a condition: the compiler, which
-// cannot see that the conditions agree, would otherwise wait for ALL loads, the next tile's among them, in every turn.
+// Waits for every load and copy so far.
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // The B operand that results 8 s .. 8 s + 7 of a score column make
@@ -130,57 +130,42 @@ __device__ __forceinline__ v4u pack_step(const v16f& v, int s) {
                pack2<DT>(v[8 * s + 6], v[8 * s + 7])};
 }
 
-// TR rows of a tensor on their way to LDS: requested early, written later. A thread's chunks (16 bytes) are chunk `ch` of rows
-// row + k RS, or, where a row's chunks do not divide the workgroup (DP = 96), each on its own. Chunks past the head size are
-// neither read nor written: clear_tiles has zeroed them once.
+__device__ const uint4 x_zeros = {0, 0, 0, 0};
+
+// TR rows of a tensor into an LDS tile, by copies that do not pass through registers (a wave's copy fills 64 consecutive
+// 16-byte places; the chunk that belongs into a place is chosen by the lane's source address). They are done after wait_loads.
 template <int DP, int TR>
-struct Stage {
+struct Copy {
     static constexpr int CPR = DP / 8, N = TR * CPR / kXThreads, RS = kXThreads / CPR;
-    static constexpr bool EVEN = kXThreads % CPR == 0;
+    static constexpr bool EVEN = kXThreads % CPR == 0;  // then a thread's places are in rows RS apart (a multiple of 16: one f)
     static_assert(TR * CPR % kXThreads == 0, "whole chunks for every thread");
-    v4u r[N];
     static __device__ __forceinline__ int row(int k) { return EVEN ? (int)threadIdx.x / CPR + k * RS : ((int)threadIdx.x + k * kXThreads) / CPR; }
-    static __device__ __forceinline__ int chunk(int k) { return EVEN ? (int)threadIdx.x % CPR : ((int)threadIdx.x + k * kXThreads) % CPR; }
-    // rows base + row * st (st below 2^25: a tile's offsets fit 32 bits), all of them there
-    __device__ __forceinline__ void load(const uint16_t* base, int64_t st, int D) {
+    static __device__ __forceinline__ int chunk(int k) {
+        const int place = EVEN ? (int)threadIdx.x % CPR : ((int)threadIdx.x + k * kXThreads) % CPR;
+        return place ^ tile_f<DP>(EVEN ? row(0) : row(k));
+    }
+    static __device__ __forceinline__ void one(const void* p, uint16_t* tile, int k, int wave) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                         (__attribute__((address_space(3))) void*)(tile + (k * kXWaves + wave) * 512), 16, 0, 0);
+    }
+    // rows base + row * st; those without a bit in `live` become zeros and are not read, nor is anything past the head size
+    // (st below 2^25: a tile's offsets fit 32 bits). wave: uniform.
+    static __device__ __forceinline__ void start(const uint16_t* base, int64_t st, int D, uint64_t live, uint16_t* tile, int wave) {
         const unsigned s = (unsigned)st;
+        const bool whole = live == ~(uint64_t)0 && D == DP;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            if (chunk(k) * 8 >= D) continue;
             const char* b = reinterpret_cast<const char*>(EVEN ? base + k * RS * st : base);
             const unsigned off = (unsigned)(EVEN ? row(0) : row(k)) * s * 2u + (unsigned)chunk(k) * 16u;
-            r[k] = *reinterpret_cast<const v4u*>(b + off);
+            if (whole) {
+                one(b + off, tile, k, wave);
+            } else {
+                const bool in = ((live >> row(k)) & 1) && chunk(k) * 8 < D;
+                one(in ? b + off : reinterpret_cast<const char*>(&x_zeros), tile, k, wave);
+            }
         }
-    }
-    // the same with rows 0 .. last there: the others are row `last` again
-    __device__ __forceinline__ void load_upto(const uint16_t* base, int64_t st, int D, int last) {
-        const unsigned s = (unsigned)st;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            if (chunk(k) * 8 >= D) continue;
-            const int n = row(k) < last ? row(k) : last;
-            r[k] = *reinterpret_cast<const v4u*>(reinterpret_cast<const char*>(base) + ((unsigned)n * s * 2u + (unsigned)chunk(k) * 16u));
-        }
-    }
-    __device__ __forceinline__ void store(uint16_t* tile, int D) const {
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (chunk(k) * 8 < D) *reinterpret_cast<v4u*>(tile + tile_at<DP>(row(k), chunk(k))) = r[k];
-    }
-    // rows without a bit in `live` become zeros
-    __device__ __forceinline__ void store_live(uint16_t* tile, int D, uint64_t live) const {
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (chunk(k) * 8 < D)
-                *reinterpret_cast<v4u*>(tile + tile_at<DP>(row(k), chunk(k))) = (live >> row(k)) & 1 ? r[k] : v4u{0u, 0u, 0u, 0u};
     }
 };
-
-// zeros in tiles whose rows are longer than the head; followed by a barrier
-template <int ELEMS>
-__device__ __forceinline__ void clear_tiles(uint16_t* t) {
-    for (int i = threadIdx.x * 8; i < ELEMS; i += kXThreads * 8) *reinterpret_cast<v4u*>(t + i) = v4u{0u, 0u, 0u, 0u};
-}
 
 // Which keys of a batch element count: those below its length whose mask byte is not zero.
 struct XKeys {
@@ -196,44 +181,55 @@ struct XKeys {
     __device__ __forceinline__ const uint8_t* row(int b) const { return mask == nullptr ? nullptr : mask + b * mask_stride; }
 };
 
-// K and V in tiles of 64 keys: two buffers, the next tile in registers meanwhile.
+// K and V in tiles of 64 keys, in two buffers: while one tile is worked on, the next one's copies run, and the mask bytes of
+// the one after that are on their way, for the copies have to know which keys count. The buffers are arrays of their own: the
+// compiler waits for all copies before a read of LDS that it cannot tell from their targets.
 template <int DP>
 struct KVTiles {
     static constexpr int ELEMS = kXTile * DP;
-    Stage<DP, kXTile> k, v;
     const uint16_t *kp, *vp;
     int64_t kst, vst;
     const uint8_t* mask;
-    int len, D;
+    int len, D, wave;
     uint8_t byte;
-    __device__ __forceinline__ void load(int t) {
-        const int key0 = t * kXTile, lane = threadIdx.x & 63;
-        const uint16_t *kb = kp + key0 * kst, *vb = vp + key0 * vst;
-        const int last = len - 1 - key0;  // 0 or more: the tile exists
-        // (without a mask some byte of K: a load that depends on a branch would be waited for at once)
-        byte = *(mask != nullptr ? mask + key0 + (lane < last ? lane : last) : reinterpret_cast<const uint8_t*>(kb));
-        if (last >= kXTile - 1) {
-            k.load(kb, kst, D);
-            v.load(vb, vst, D);
-        } else {
-            k.load_upto(kb, kst, D, last);
-            v.load_upto(vb, vst, D, last);
-        }
+    uint64_t live[2];  // of the present tile and of the next one
+    // requests the mask bytes of tile t (any t: of an existing key)
+    __device__ __forceinline__ void ask(int t) {
+        const int key = t * kXTile + (int)(threadIdx.x & 63), last = len - 1;
+        // (without a mask some byte of K: a load under a condition would be waited for at its end)
+        byte = *(mask != nullptr ? mask + (key < last ? key : last) : reinterpret_cast<const uint8_t*>(kp));
     }
-    // writes the tile and the bias of its scores (0, or -infinity where a key does not count); returns the keys that count
-    __device__ __forceinline__ uint64_t store(int t, uint16_t* kt, uint16_t* vt, float* bias) const {
-        const int lane = threadIdx.x & 63;
-        const bool counts = t * kXTile + lane < len && (mask == nullptr || byte != 0);
-        const uint64_t live = __builtin_amdgcn_ballot_w64(counts);
-        if (live == ~(uint64_t)0) {
-            k.store(kt, D);
-            v.store(vt, D);
-        } else {
-            k.store_live(kt, D, live);
-            v.store_live(vt, D, live);
-            if (threadIdx.x < kXTile) bias[threadIdx.x] = counts ? 0.f : -__builtin_inff();
-        }
-        return live;
+    // which keys of tile t count, from its bytes
+    __device__ __forceinline__ uint64_t counted(int t) const {
+        return __builtin_amdgcn_ballot_w64(t * kXTile + (int)(threadIdx.x & 63) < len && (mask == nullptr || byte != 0));
+    }
+    // starts the copies of tile t, whose keys `alive` count, and writes the bias of its scores
+    __device__ __forceinline__ void start(int t, uint64_t alive, uint16_t* kt, uint16_t* vt, float* bias) const {
+        Copy<DP, kXTile>::start(kp + t * kXTile * kst, kst, D, alive, kt, wave);
+        Copy<DP, kXTile>::start(vp + t * kXTile * vst, vst, D, alive, vt, wave);
+        if (alive != ~(uint64_t)0 && threadIdx.x < kXTile) bias[threadIdx.x] = (alive >> threadIdx.x) & 1 ? 0.f : -__builtin_inff();
+    }
+    // the first tile, whole and in place after the barrier
+    __device__ __forceinline__ void first(int t, uint16_t* kt, uint16_t* vt, float* bias) {
+        ask(t);
+        wait_loads();
+        live[0] = counted(t);
+        start(t, live[0], kt, vt, bias);
+        ask(t + 1);
+        wait_loads();
+        live[1] = counted(t + 1);
+    }
+    // at the start of tile t, into the other buffer / before the barrier at its end
+    __device__ __forceinline__ void begin(int t, bool more, uint16_t* kt, uint16_t* vt, float* bias) {
+        if (!more) return;
+        start(t + 1, live[1], kt, vt, bias);
+        ask(t + 2);
+    }
+    __device__ __forceinline__ void end(int t, bool more) {
+        if (!more) return;
+        wait_loads();
+        live[0] = live[1];
+        live[1] = counted(t + 2);
     }
 };
 // the start of a tile's scores: the bias of rows 32 u .. 32 u + 31
@@ -285,24 +281,23 @@ inline XSchedule schedule(int64_t blocks, int64_t length, int slots) {
 }
 
 // One 32 x D result of a wave (columns = rows of the output, results = its elements) to memory in whole 16-byte chunks,
-// through `buf` (32 rows of DP + 8 elements, the wave's own). at(row): pointer to the output row or NULL.
+// through `buf`, 32 rows of a tile of the wave's own. at(row): pointer to the output row or NULL.
 template <int DT, int DP, typename At>
 __device__ __forceinline__ void store_tile(const v16f (&acc)[DP / 32], float scale, uint16_t* buf, int D, int lane, At at) {
-    constexpr int LB = DP + 8, CPR = DP / 8;
-    uint16_t* mine = buf + (lane & 31) * LB + ((lane >> 5) << 2);
+    constexpr int CPR = DP / 8;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<v2i*>(mine + t * 32 + i * 8) = v2i{(int)pack2<DT>(acc[t][4 * i] * scale, acc[t][4 * i + 1] * scale),
-                                                                 (int)pack2<DT>(acc[t][4 * i + 2] * scale, acc[t][4 * i + 3] * scale)};
+            *reinterpret_cast<v2i*>(buf + tile_at<DP>(lane & 31, t * 4 + i) + ((lane >> 5) << 2)) =
+                v2i{(int)pack2<DT>(acc[t][4 * i] * scale, acc[t][4 * i + 1] * scale), (int)pack2<DT>(acc[t][4 * i + 2] * scale, acc[t][4 * i + 3] * scale)};
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int c = 0; c < 32 * CPR / 64; ++c) {
         const int i = lane + c * 64, row = i / CPR, e = (i - row * CPR) * 8;
         uint16_t* p = at(row);
-        if (p != nullptr && e < D) *reinterpret_cast<v4u*>(p + e) = *reinterpret_cast<const v4u*>(buf + row * LB + e);
+        if (p != nullptr && e < D) *reinterpret_cast<v4u*>(p + e) = *reinterpret_cast<const v4u*>(buf + tile_at<DP>(row, e / 8));
     }
 }
 
