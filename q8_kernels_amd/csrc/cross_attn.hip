@@ -27,77 +27,59 @@ struct XFwd {
     float *part, *pm, *pl;  // divided blocks: [splits, tail, 128, D], [splits, tail, 128] twice
 };
 
+// One wave's rows: Q^T as operands, the running state of their softmax.
 template <int DT, int DP>
-__global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
-    constexpr int KS = DP / 16, DTL = DP / 32, ELEMS = kXTile * DP;
-    __shared__ __align__(16) uint16_t k0[ELEMS], k1[ELEMS], v0[ELEMS], v1[ELEMS];
-    __shared__ __align__(16) float bias0[kXTile], bias1[kXTile];
-    unsigned block;
-    int split, of;
-    if (!a.plan.item(block, split, of)) return;
-    const int unit = block / a.row_blocks, rb = block - unit * a.row_blocks;
-    const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
-
-    KVTiles<DP> kv;
-    kv.len = a.keys.length(b);
-    kv.mask = a.keys.row(b);
-    kv.D = a.D;
-    kv.kp = a.k.p + b * a.k.sb + hk * a.k.sh;
-    kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
-    kv.kst = a.k.st;
-    kv.vst = a.v.st;
-    kv.wave = wave;
-    const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
-    const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
-
+struct Rows32 {
+    static constexpr int KS = DP / 16, DTL = DP / 32;
     v4u qf[KS];
-    {
-        const int g = row < a.R ? row / a.M : 0, m = row - g * a.M;
-        const uint16_t* p = a.q.p + b * a.q.sb + (int64_t)(hk * a.G + g) * a.q.sh + m * a.q.st + half * 8;
+    v16f acc[DTL];
+    float m, l;  // m in units of log2; l: the sum over this lane's half of the keys
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
+        m = -3.0e38f;
+        l = 0.f;
+    }
+    __device__ __forceinline__ void load(const XFwd& a, int b, int hk, int row, int half) {
+        const int g = row < a.R ? row / a.M : 0, i = row - g * a.M;
+        const uint16_t* p = a.q.p + b * a.q.sb + (int64_t)(hk * a.G + g) * a.q.sh + i * a.q.st + half * 8;
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = (row < a.R && s * 16 + half * 8 < a.D) ? *reinterpret_cast<const v4u*>(p + s * 16) : v4u{0u, 0u, 0u, 0u};
     }
-    if (t0 < t1) kv.first(t0, k0, v0, bias0);
-
-    v16f acc[DTL];
-#pragma unroll
-    for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
-    float m = -3.0e38f, l = 0.f;  // in units of log2; the sum over this lane's half of the keys
-    wait_loads();
-    __syncthreads();
-
-    LaneOffsets<DP> at(lane);
-    auto step = [&](int t, auto buffer) {
-        constexpr int BUF = decltype(buffer)::value;
-        at.fresh();
-        const uint16_t *kl = BUF ? k1 : k0, *vl = BUF ? v1 : v0;
-        const bool more = t + 1 < t1;
-        kv.begin(t, more, BUF ? k0 : k1, BUF ? v0 : v1, BUF ? bias0 : bias1);
+    // One tile of 64 keys: whole (all of them count) or with a bias of 0 and -infinity. copies(i, n): what goes to memory
+    // beside group i of the n that form the scores.
+    template <typename Copy>
+    __device__ __forceinline__ void tile(const uint16_t* kl, const uint16_t* vl, bool whole, const float* bias, float c, const LaneOffsets<DP>& at, int half,
+                                         Copy copies) {
+        Operands<DP, 4> ops;
         v16f s[2];
-        if (kv.live[0] == ~(uint64_t)0) {
+        auto scores = [&](auto masked) {
+            ops.rows(0, kl, 0, 0, at);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                s[u] = splat16(0.f);
+            for (int i = 0; i < 2 * ops.RN; ++i) {
+                const int u = i / ops.RN, g = i % ops.RN;
+                if (i + 1 < 2 * ops.RN) ops.rows((i + 1) & 1, kl, (i + 1) / ops.RN * 32, (i + 1) % ops.RN, at);
+                else ops.cols(0, vl, 0, 0, at);
+                copies(i, 2 * ops.RN);
+                if (g == 0) {
+                    if constexpr (masked) s[u] = bias16(bias, u, half);
+                    else s[u] = splat16(0.f);
+                }
+                fence();
 #pragma unroll
-                for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s[u]);
+                for (int j = 0; j < ops.RG; ++j) s[u] = mfma16<DT>(ops.f[i & 1][j], qf[g * ops.RG + j], s[u]);
+                fence();
             }
-            order_reads_ahead<2 * KS, 1, 4>();
-        } else {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                s[u] = bias16(BUF ? bias1 : bias0, u, half);
-#pragma unroll
-                for (int e = 0; e < KS; ++e) s[u] = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s[u]);
-            }
-        }
+        };
+        if (whole) scores(std::false_type{});
+        else scores(std::true_type{});
         float top = s[0][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = max_ieee(top, s[0][i]);
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = max_ieee(top, s[1][i]);
-        top = half_pair_max(top) * a.c;
+        top = half_pair_max(top) * c;
         const bool grown = top > m + 8.f;
         if (__builtin_amdgcn_ballot_w64(grown) != 0) {
             const float next = grown ? top : m, f = __builtin_amdgcn_exp2f(m - next);
@@ -108,64 +90,124 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[d][i] *= f;
         }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        auto weights = [&](int u) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], a.c, -m));
+                s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -m));
                 l += s[u][i];
             }
+        };
+        weights(0);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const v4u p = pack_step<DT>(s[u], k);
+        for (int i = 0; i < 4; ++i) {
+            const v4u p = pack_step<DT>(s[i / 2], i % 2);
+            if (i < 3) ops.cols((i + 1) & 1, vl, (i + 1) * 16, 0, at);
+            fence();
+            if (i == 0) weights(1);  // beside the matrix instructions of the first half
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(vl, u * 32 + k * 16, d, at), p, acc[d]);
+            for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(ops.f[i & 1][d], p, acc[d]);
+            if (i == 0) {
+#pragma unroll
+                for (int d = 0; d < DTL; ++d) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, 48 / DTL, 0);
+                }
             }
+            fence();
         }
-        kv.end(t, more);
+    }
+    // the sum over all keys
+    __device__ __forceinline__ void join_halves() {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    // log-sum and O, through 32 rows of LDS of the wave's own
+    __device__ __forceinline__ void finish(const XFwd& a, int unit, int b, int hk, int row0, int lane, uint16_t* buf) const {
+        const int row = row0 + (lane & 31);
+        if (a.lse != nullptr && row < a.R && lane < 32) a.lse[(int64_t)unit * a.R + row] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
+        store_tile<DT, DP>(acc, l == 0.f ? 0.f : 1.0f / l, buf, a.D, lane, [&](int r) -> uint16_t* {
+            const int n = row0 + r;
+            if (n >= a.R) return nullptr;
+            const int g = n / a.M;
+            return a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (n - g * a.M) * a.o.st;
+        });
+    }
+};
+
+template <int DT, int DP>
+__global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
+    constexpr int ELEMS = kXTile * DP;
+    __shared__ __align__(16) uint16_t k0[ELEMS], k1[ELEMS], v0[ELEMS], v1[ELEMS];
+    __shared__ __align__(16) float bias0[kXTile], bias1[kXTile];
+    unsigned block;
+    int split, of;
+    if (!a.plan.item(block, split, of)) return;
+    const int unit = block / a.row_blocks, rb = block - unit * a.row_blocks;
+    const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int row0 = rb * kXRows + wave * 32, row = row0 + (lane & 31);
+
+    Rows32<DT, DP> rows;
+    rows.load(a, b, hk, row, half);
+    KVTiles<DP> kv;
+    kv.len = a.keys.length(b);
+    kv.mask = a.keys.row(b);
+    kv.copies.D = a.D;
+    kv.copies.wave = wave;
+    kv.kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+    kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+    kv.kst = a.k.st;
+    kv.vst = a.v.st;
+    const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
+    const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+    if (t0 < t1) kv.first(t0, k0, v0, bias0);
+    rows.clear();
+    wait_loads();
+    __syncthreads();
+
+    LaneOffsets<DP> at(lane);
+    auto step = [&](int t, auto buffer) {
+        constexpr int BUF = decltype(buffer)::value;
+        at.fresh();
+        // (past the last tile of this workgroup the copies are of a tile that nobody reads, or empty)
+        kv.bias_of(kv.live[1], BUF ? bias0 : bias1);
+        kv.ask(t + 2);
+        const XTile knext = kv.k_tile(t + 1), vnext = kv.v_tile(t + 1);
+        rows.tile(BUF ? k1 : k0, BUF ? v1 : v0, kv.live[0] == ~(uint64_t)0, BUF ? bias1 : bias0, a.c, at, half,
+                  [&](int i, int n) { kv.copies.group(i, n, knext, vnext, ~kv.live[1], BUF ? k0 : k1, BUF ? v0 : v1); });
+        kv.end(t);
         __syncthreads();
     };
     for (int t = t0; t < t1; t += 2) {
         step(t, std::integral_constant<int, 0>{});
         if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
     }
-    {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-        l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
+    rows.join_halves();
     if (of > 1) {
         if (row < a.R) {
-            const int64_t at = ((int64_t)split * a.plan.tail + (block - a.plan.full)) * 128 + wave * 32 + (lane & 31);
-            if (half == 0) { a.pm[at] = m; a.pl[at] = l; }
-            float* p = a.part + at * a.D;
+            const int64_t to = ((int64_t)split * a.plan.tail + (block - a.plan.full)) * kXRows + wave * 32 + (lane & 31);
+            if (half == 0) { a.pm[to] = rows.m; a.pl[to] = rows.l; }
+            float* p = a.part + to * a.D;
 #pragma unroll
-            for (int d = 0; d < DTL; ++d)
+            for (int d = 0; d < rows.DTL; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int e = d * 32 + i * 8 + half * 4;
-                    if (e < a.D) *reinterpret_cast<v4f*>(p + e) = v4f{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                    if (e < a.D) *reinterpret_cast<v4f*>(p + e) = v4f{rows.acc[d][4 * i], rows.acc[d][4 * i + 1], rows.acc[d][4 * i + 2], rows.acc[d][4 * i + 3]};
                 }
         }
         return;
     }
-    if (a.lse != nullptr && row < a.R && half == 0)
-        a.lse[(int64_t)unit * a.R + row] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
     // (the tile buffers are free: every wave has passed the last barrier of the loop)
-    store_tile<DT, DP>(acc, inv, (wave < 2 ? wave == 0 ? k0 : k1 : wave == 2 ? v0 : v1), a.D, lane, [&](int r) -> uint16_t* {
-        const int n = row0 + r;
-        if (n >= a.R) return nullptr;
-        const int g = n / a.M;
-        return a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (n - g * a.M) * a.o.st;
-    });
+    rows.finish(a, unit, b, hk, row0, lane, (wave < 2 ? k0 : k1) + (wave & 1) * 32 * DP);
 }
 
 // Joins the parts of a row: weights exp2(m_i - max m). 32 lanes a row, 4 elements a lane.
 template <int DT>
 __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
-    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), all = (int64_t)a.plan.tail * 128;
-    const unsigned block = a.plan.full + (unsigned)(n >> 7);
-    const int unit = block / a.row_blocks, r = (block - unit * a.row_blocks) * 128 + (int)(n & 127);
+    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), all = (int64_t)a.plan.tail * kXRows;
+    const unsigned tail = (unsigned)(n / kXRows), block = a.plan.full + tail;
+    const int unit = block / a.row_blocks, r = (block - unit * a.row_blocks) * kXRows + (int)(n - (int64_t)tail * kXRows);
     if (n >= all || r >= a.R) return;
     const int e = (threadIdx.x & 31) * 4;
     float m = -3.0e38f, l = 0.f;
@@ -188,8 +230,10 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
-// workgroups that run at once: as many on each of the 256 CUs as registers (128, 158 and 218 a lane) and LDS allow
-static int fwd_slots(int D) { return D <= 64 ? 1024 : D <= 96 ? 768 : 512; }
+static XSchedule fwd_plan(int64_t units, int64_t rows, int N, int D) {
+    // workgroups that run at once on the 256 CUs, by the registers of a lane
+    return schedule(units * ((rows + kXRows - 1) / kXRows), N, D <= 32 ? 1024 : D <= 64 ? 768 : 512);
+}
 
 }  // namespace q8
 
@@ -197,8 +241,8 @@ using namespace q8;
 
 extern "C" int64_t q8_cross_attn_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
     if (int e = x_sizes("q8_cross_attn_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
-    const int64_t units = B * Hkv, rows = (int64_t)(H / Hkv) * M, blocks = units * ((rows + 127) / 128);
-    return schedule(blocks, N, fwd_slots(D)).parts() * 128 * (D + 2) * (int64_t)sizeof(float);
+    const int64_t rows = (int64_t)(H / Hkv) * M;
+    return fwd_plan(B * Hkv, rows, N, D).parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
@@ -231,16 +275,15 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
     a.M = M;
     a.D = D;
     a.R = a.G * M;
-    a.row_blocks = (a.R + 127) / 128;
-    const int64_t blocks = B * Hkv * a.row_blocks;
-    if (blocks > 0x7ffff000) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
-    a.plan = schedule(blocks, N, fwd_slots(D));
+    a.row_blocks = (a.R + kXRows - 1) / kXRows;
+    if (B * Hkv * a.row_blocks > 0x7ffff000) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
+    a.plan = fwd_plan(B * Hkv, a.R, N, D);
     if (a.plan.parts()) {
         const int64_t need = q8_cross_attn_workspace(B, H, Hkv, M, N, D);
         if (workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
         if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
         if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
-        const int64_t n = a.plan.parts() * 128;
+        const int64_t n = a.plan.parts() * kXRows;
         a.part = static_cast<float*>(workspace);
         a.pm = a.part + n * D;
         a.pl = a.pm + n;
@@ -258,7 +301,7 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
 #undef X_FWD
     if (int e = launch_status(who)) return e;
     if (a.plan.parts()) {
-        const unsigned n = a.plan.tail * 16;
+        const unsigned n = a.plan.tail * (kXRows / 8);
         if (dt == Q8_BF16) cross_attn_join_kernel<Q8_BF16><<<n, 256, 0, st>>>(a);
         else cross_attn_join_kernel<Q8_F16><<<n, 256, 0, st>>>(a);
         return launch_status(who);

@@ -42,17 +42,17 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     const int unit = block / a.blocks, rb = block - unit * a.blocks;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
+    const int row0 = (rb * kXWaves + wave) * 32, row = row0 + (lane & 31);
 
     KVTiles<DP> kv;
     kv.len = a.keys.length(b);
     kv.mask = a.keys.row(b);
-    kv.D = a.D;
+    kv.copies.D = a.D;
     kv.kp = a.k.p + b * a.k.sb + hk * a.k.sh;
     kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
     kv.kst = a.k.st;
     kv.vst = a.v.st;
-    kv.wave = wave;
+    kv.copies.wave = wave;
     const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
@@ -93,36 +93,63 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     __syncthreads();
 
     LaneOffsets<DP> at(lane);
+    Operands<DP, 4> ops;
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
         const uint16_t *kl = BUF ? k1 : k0, *vl = BUF ? v1 : v0;
-        const bool more = t + 1 < t1;
-        kv.begin(t, more, BUF ? k0 : k1, BUF ? v0 : v1, BUF ? bias0 : bias1);
+        uint16_t *kn = BUF ? k0 : k1, *vn = BUF ? v0 : v1;
+        // (past the last tile of this workgroup the copies are of a tile that nobody reads, or empty)
+        kv.bias_of(kv.live[1], BUF ? bias0 : bias1);
+        kv.ask(t + 2);
+        const XTile knext = kv.k_tile(t + 1), vnext = kv.v_tile(t + 1);
+        constexpr int PARTS = 4 * ops.RN;  // groups that form scores and dP in a tile: the next tile's copies go with them
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             v16f s, dp = splat16(-delta);
-            if (kv.live[0] == ~(uint64_t)0) {
-                s = splat16(0.f);
+            auto scores = [&](auto masked) {
+                if constexpr (masked) s = bias16(BUF ? bias1 : bias0, u, half);
+                else s = splat16(0.f);
+                if (u == 0) ops.rows(0, kl, 0, 0, at);
 #pragma unroll
-                for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s);
-            } else {
-                s = bias16(BUF ? bias1 : bias0, u, half);
+                for (int g = 0; g < ops.RN; ++g) {
+                    if (g + 1 < ops.RN) ops.rows((g + 1) & 1, kl, u * 32, g + 1, at);
+                    else ops.rows((g + 1) & 1, vl, u * 32, 0, at);
+                    kv.copies.group(u * 2 * ops.RN + g, PARTS, knext, vnext, ~kv.live[1], kn, vn);
+                    fence();
 #pragma unroll
-                for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(kl, u * 32, e, at), qf[e], s);
+                    for (int j = 0; j < ops.RG; ++j) s = mfma16<DT>(ops.f[g & 1][j], qf[g * ops.RG + j], s);
+                    fence();
+                }
+            };
+            if (kv.live[0] == ~(uint64_t)0) scores(std::false_type{});
+            else scores(std::true_type{});
+#pragma unroll
+            for (int g = 0; g < ops.RN; ++g) {
+                const int now = (ops.RN + g) & 1;
+                if (g + 1 < ops.RN) ops.rows(now ^ 1, vl, u * 32, g + 1, at);
+                else ops.cols(now ^ 1, kl, u * 32, 0, at);
+                kv.copies.group((u * 2 + 1) * ops.RN + g, PARTS, knext, vnext, ~kv.live[1], kn, vn);
+                fence();
+#pragma unroll
+                for (int j = 0; j < ops.RG; ++j) dp = mfma16<DT>(ops.f[now][j], gf[g * ops.RG + j], dp);
+                fence();
             }
-#pragma unroll
-            for (int e = 0; e < KS; ++e) dp = mfma16<DT>(lds_rows<DP>(vl, u * 32, e, at), gf[e], dp);
+            // (2 RN groups so far: the columns are in place 0)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse));
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(dp, k);
+                if (k == 0) ops.cols(1, kl, u * 32 + 16, 0, at);
+                else if (u == 0) ops.rows(0, kl, 32, 0, at);
+                fence();
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(lds_cols<DP>(kl, u * 32 + k * 16, d, at), p, acc[d]);
+                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(ops.f[k][d], p, acc[d]);
+                fence();
             }
         }
-        kv.end(t, more);
+        kv.end(t);
         __syncthreads();
     };
     for (int t = t0; t < t1; t += 2) {
@@ -131,7 +158,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     }
     if (of > 1) {
         if (row < a.R) {
-            float* p = a.part + (((int64_t)split * a.plan.tail + (block - a.plan.full)) * 128 + wave * 32 + (lane & 31)) * a.D;
+            float* p = a.part + (((int64_t)split * a.plan.tail + (block - a.plan.full)) * kXRows + wave * 32 + (lane & 31)) * a.D;
 #pragma unroll
             for (int d = 0; d < DTL; ++d)
 #pragma unroll
@@ -142,7 +169,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
         }
         return;
     }
-    store_tile<DT, DP>(acc, a.scale, (wave < 2 ? wave == 0 ? k0 : k1 : wave == 2 ? v0 : v1), a.D, lane, [&](int r) -> uint16_t* {
+    store_tile<DT, DP>(acc, a.scale, (wave < 2 ? k0 : k1) + (wave & 1) * 32 * DP, a.D, lane, [&](int r) -> uint16_t* {
         const int n = row0 + r;
         if (n >= a.R) return nullptr;
         const int g = n / a.M;
@@ -150,14 +177,15 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     });
 }
 
-// A head of more than 96 leaves no registers for V beside K and the two sums (two waves a SIMD have 256 each): V stays in LDS
-// and the rows are walked in tiles of 32.
+// A head of more than 96 leaves no registers for V beside K and the two sums (two waves a SIMD have 256 each): V stays in
+// LDS, the rows are walked in tiles of 32, and the order of the instructions is the compiler's (keeping the groups apart costs
+// registers that have to be spilled).
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32;
     constexpr bool V_IN_LDS = DP > 96;
     constexpr int TR = V_IN_LDS ? 32 : 64, ELEMS = TR * DP;
-    __shared__ __align__(16) uint16_t q0[ELEMS], q1[ELEMS], g0[ELEMS], g1[ELEMS], vl[V_IN_LDS ? 128 * DP : 8];
+    __shared__ __align__(16) uint16_t q0[ELEMS], q1[ELEMS], g0[ELEMS], g1[ELEMS], vl[V_IN_LDS ? kXRows * DP : 8];
     __shared__ __align__(16) float lse0[TR], lse1[TR], delta0[TR], delta1[TR];  // -lse and -delta of the tile's rows
     unsigned block;
     int split, of;
@@ -165,7 +193,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     const int unit = block / a.blocks, kb = block - unit * a.blocks;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int key0 = kb * 128 + wave * 32, key = key0 + (lane & 31);
+    const int key0 = (kb * kXWaves + wave) * 32, key = key0 + (lane & 31);
 
     const int len = a.keys.length(b);
     const uint8_t* mask = a.keys.row(b);
@@ -174,22 +202,31 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     const int head_tiles = (a.M + TR - 1) / TR, tiles = a.G * head_tiles, per = (tiles + of - 1) / of;
     const int t0 = split * per;
     int t1 = t0 + per < tiles ? t0 + per : tiles;
-    if (kb * 128 >= len) t1 = t0;  // no key of this workgroup counts: zeros
+    if (kb * kXRows >= len) t1 = t0;  // no key of this workgroup counts: zeros
 
     // rows go to LDS by copies, their log-sums and deltas through a register each
     float row_lse = 0.f, row_delta = 0.f;
     int rows = 0;
     const uint16_t *qp = a.q.p + b * a.q.sb + (int64_t)hk * a.G * a.q.sh, *gp = a.g.p + b * a.g.sb + (int64_t)hk * a.G * a.g.sh;
-    auto start = [&](int t, uint16_t* qt, uint16_t* gt) {
+    Copies<DP, TR> copies;
+    copies.wave = wave;
+    copies.D = a.D;
+    // the tile that is next (t past the end: empty)
+    auto aim = [&](int t) {
         const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
-        rows = a.M - m;
-        const uint64_t live = rows >= TR ? ~(uint64_t)0 : ((uint64_t)1 << rows) - 1;
-        Copy<DP, TR>::start(qp + g * a.q.sh + m * a.q.st, a.q.st, a.D, live, qt, wave);
-        Copy<DP, TR>::start(gp + g * a.g.sh + m * a.g.st, a.g.st, a.D, live, gt, wave);
+        rows = t < t1 ? a.M - m : 0;
         const int n = (int)threadIdx.x & (TR - 1);
-        const int64_t at = (int64_t)unit * a.R + g * a.M + m + (n < rows ? n : rows - 1);
+        const int64_t at = (int64_t)unit * a.R + (rows ? g * a.M + m + (n < rows ? n : rows - 1) : 0);
         row_lse = a.lse[at];
         row_delta = a.delta[at];
+    };
+    auto q_tile = [&](int t) {
+        const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
+        return XTile(qp + g * a.q.sh + m * a.q.st, a.q.st, rows, a.D, TR);
+    };
+    auto g_tile = [&](int t) {
+        const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
+        return XTile(gp + g * a.g.sh + m * a.g.st, a.g.st, rows, a.D, TR);
     };
     auto finish = [&](float* lt, float* dt) {
         wait_loads();
@@ -213,7 +250,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
         }
     }
     if (t0 < t1) {
-        start(t0, q0, g0);
+        aim(t0);
+        copies.group(0, 1, q_tile(t0), g_tile(t0), 0, q0, g0);
         finish(lse0, delta0);
     }
 
@@ -223,47 +261,89 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     wait_loads();
     __syncthreads();
     LaneOffsets<DP> at(lane);
+    Operands<DP, V_IN_LDS ? 2 : 4> ops;
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
         const uint16_t *ql = BUF ? q1 : q0, *gl = BUF ? g1 : g0;
         const float *lt = BUF ? lse1 : lse0, *dt = BUF ? delta1 : delta0;
-        const bool more = t + 1 < t1;
-        if (more) start(t + 1, BUF ? q0 : q1, BUF ? g0 : g1);
+        uint16_t *qnext = BUF ? q0 : q1, *gnext = BUF ? g0 : g1;
+        aim(t + 1);
+        const XTile qtile = q_tile(t + 1), gtile = g_tile(t + 1);
+        constexpr int PARTS = TR / 16 * ops.RN;
+        auto keep = [] { if constexpr (!V_IN_LDS) fence(); };
 #pragma unroll
         for (int u = 0; u < TR / 32; ++u) {
             v16f s = splat16(0.f), dp = bias16(dt, u, half);
+            int w = 0;  // the place of the operands that are next
+            if (u == 0) ops.rows(0, ql, 0, 0, at);
 #pragma unroll
-            for (int e = 0; e < KS; ++e) s = mfma16<DT>(lds_rows<DP>(ql, u * 32, e, at), kf[e], s);
+            for (int g = 0; g < ops.RN; ++g, w ^= 1) {
+                if (g + 1 < ops.RN) ops.rows(w ^ 1, ql, u * 32, g + 1, at);
+                else ops.rows(w ^ 1, gl, u * 32, 0, at);
+                copies.group(u * 2 * ops.RN + g, PARTS, qtile, gtile, 0, qnext, gnext);
+                keep();
 #pragma unroll
-            for (int e = 0; e < KS; ++e) {
-                v4u v;
-                if constexpr (V_IN_LDS) v = lds_rows<DP>(vl, wave * 32, e, at);
-                else v = vf[e];
-                dp = mfma16<DT>(lds_rows<DP>(gl, u * 32, e, at), v, dp);
+                for (int j = 0; j < ops.RG; ++j) s = mfma16<DT>(ops.f[w][j], kf[g * ops.RG + j], s);
+                keep();
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const v4f w = *reinterpret_cast<const v4f*>(&lt[u * 32 + i * 8 + half * 4]);
+            for (int g = 0; g < ops.RN; ++g, w ^= 1) {
+                v4u v[ops.RG];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[i * 4 + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * 4 + j], a.c, w[j]));
+                for (int j = 0; j < ops.RG; ++j) {
+                    if constexpr (V_IN_LDS) v[j] = lds_rows<DP>(vl, wave * 32, g * ops.RG + j, at);
+                    else v[j] = vf[g * ops.RG + j];
+                }
+                if (g + 1 < ops.RN) ops.rows(w ^ 1, gl, u * 32, g + 1, at);
+                else ops.cols(w ^ 1, gl, u * 32, 0, at);
+                copies.group((u * 2 + 1) * ops.RN + g, PARTS, qtile, gtile, 0, qnext, gnext);
+                keep();
+#pragma unroll
+                for (int j = 0; j < ops.RG; ++j) dp = mfma16<DT>(ops.f[w][j], v[j], dp);
+                // P, a part of it beside each group
+#pragma unroll
+                for (int i = g * 4 / ops.RN; i < (g + 1) * 4 / ops.RN; ++i) {
+                    const v4f x = *reinterpret_cast<const v4f*>(&lt[u * 32 + i * 8 + half * 4]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[i * 4 + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * 4 + j], a.c, x[j]));
+                }
+                keep();
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(s, k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) dv[d] = mfma16<DT>(lds_cols<DP>(gl, u * 32 + k * 16, d, at), p, dv[d]);
-            }
+                for (int c = 0; c < ops.CN; ++c, w ^= 1) {
+                    if (c + 1 < ops.CN) ops.cols(w ^ 1, gl, u * 32 + k * 16, c + 1, at);
+                    else if (k == 0) ops.cols(w ^ 1, gl, u * 32 + 16, 0, at);
+                    else ops.cols(w ^ 1, ql, u * 32, 0, at);
+                    keep();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+                    for (int d = 0; d < ops.CG; ++d) dv[c * ops.CG + d] = mfma16<DT>(ops.f[w][d], p, dv[c * ops.CG + d]);
+                    if (k == 0 && c == 0) {  // dS, beside them (P's second half is still needed as it is)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+                    }
+                    keep();
+                }
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(dp, k);
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(lds_cols<DP>(ql, u * 32 + k * 16, d, at), p, dk[d]);
+                for (int c = 0; c < ops.CN; ++c, w ^= 1) {
+                    if (c + 1 < ops.CN) ops.cols(w ^ 1, ql, u * 32 + k * 16, c + 1, at);
+                    else if (k == 0) ops.cols(w ^ 1, ql, u * 32 + 16, 0, at);
+                    else if (u + 1 < TR / 32) ops.rows(w ^ 1, ql, 32, 0, at);
+                    keep();
+#pragma unroll
+                    for (int d = 0; d < ops.CG; ++d) dk[c * ops.CG + d] = mfma16<DT>(ops.f[w][d], p, dk[c * ops.CG + d]);
+                    keep();
+                }
             }
         }
-        if (more) finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
+        finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
         __syncthreads();
     };
     for (int t = t0; t < t1; t += 2) {
@@ -276,7 +356,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     }
     if (of > 1) {
         if (key < a.N) {
-            float* p = a.part + (((int64_t)split * a.plan.tail + (block - a.plan.full)) * 128 + wave * 32 + (lane & 31)) * 2 * a.D;
+            float* p = a.part + (((int64_t)split * a.plan.tail + (block - a.plan.full)) * kXRows + wave * 32 + (lane & 31)) * 2 * a.D;
 #pragma unroll
             for (int d = 0; d < DTL; ++d)
 #pragma unroll
@@ -294,7 +374,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
         uint16_t* p = x.p + b * x.sb + hk * x.sh;
         return [&, p](int r) -> uint16_t* { return key0 + r < a.N ? p + (key0 + r) * x.st : nullptr; };
     };
-    uint16_t* buf = wave < 2 ? wave == 0 ? q0 : q1 : wave == 2 ? g0 : g1;
+    // (32 rows for each wave: its own rows of V, or half a tile)
+    uint16_t* buf = V_IN_LDS ? vl + wave * 32 * DP : (wave < 2 ? q0 : q1) + (wave & 1) * 32 * DP;
     store_tile<DT, DP>(dk, a.scale, buf, a.D, lane, to(a.dk));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -304,11 +385,11 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
 // Adds the parts of dQ (WIDTH = 1) or of dK and dV (WIDTH = 2): one thread for 4 elements of a row.
 template <int DT, int WIDTH>
 __global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
-    const int64_t rows = (int64_t)a.plan.tail * 128;
+    const int64_t rows = (int64_t)a.plan.tail * kXRows;
     const int quads = WIDTH * a.D / 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = i / quads;
-    const unsigned block = a.plan.full + (unsigned)(n >> 7);
-    const int unit = block / a.blocks, r = (block - unit * a.blocks) * 128 + (int)(n & 127);
+    const unsigned tail = (unsigned)(n / kXRows), block = a.plan.full + tail;
+    const int unit = block / a.blocks, r = (block - unit * a.blocks) * kXRows + (int)(n - (int64_t)tail * kXRows);
     if (n >= rows || r >= (WIDTH == 1 ? a.R : a.N)) return;
     int e = (int)(i - n * quads) * 4;
     v4f s = {0.f, 0.f, 0.f, 0.f};
@@ -332,10 +413,6 @@ __global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(s[0] * f, s[1] * f), (int)pack2<DT>(s[2] * f, s[3] * f)};
 }
 
-// workgroups that run at once: as many on each of the 256 CUs as registers allow
-static int dq_slots(int D) { return D <= 32 ? 1024 : D <= 64 ? 768 : 512; }
-static int kv_slots(int D) { return D <= 32 ? 1024 : 512; }
-
 struct XPlan {
     int64_t units, rows, dq_blocks, kv_blocks, parts;  // blocks of a unit; floats of partial results
     XSchedule dq, kv;
@@ -344,11 +421,12 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     XPlan p{};
     p.units = B * Hkv;
     p.rows = (int64_t)(H / Hkv) * M;
-    p.dq_blocks = (p.rows + 127) / 128;
-    p.kv_blocks = ((int64_t)N + 127) / 128;
-    p.dq = schedule(p.units * p.dq_blocks, N, dq_slots(D));
-    p.kv = schedule(p.units * p.kv_blocks, (int64_t)(H / Hkv) * ((M + kXTile - 1) / kXTile) * kXTile, kv_slots(D));
-    const int64_t dq = p.dq.parts() * 128 * D, kv = p.kv.parts() * 256 * D;
+    p.dq_blocks = (p.rows + kXRows - 1) / kXRows;
+    p.kv_blocks = ((int64_t)N + kXRows - 1) / kXRows;
+    // workgroups that run at once on the 256 CUs, by the registers of a lane
+    p.dq = schedule(p.units * p.dq_blocks, N, D <= 32 ? 1024 : 512);
+    p.kv = schedule(p.units * p.kv_blocks, (int64_t)(H / Hkv) * ((M + kXTile - 1) / kXTile) * kXTile, D <= 32 ? 1024 : 512);
+    const int64_t dq = p.dq.parts() * kXRows * D, kv = p.kv.parts() * kXRows * 2 * D;
     p.parts = dq > kv ? dq : kv;  // one after the other in the same place
     return p;
 }

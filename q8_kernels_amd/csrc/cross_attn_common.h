@@ -23,7 +23,7 @@
 
 namespace q8 {
 
-constexpr int kXThreads = 256, kXWaves = 4, kXTile = 64;  // a workgroup; rows of a staged tile
+constexpr int kXThreads = 256, kXWaves = 4, kXTile = 64, kXRows = 128;  // a workgroup; rows of a staged tile; rows (keys) a workgroup owns, 32 a wave
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef short v4s16 __attribute__((ext_vector_type(4)));
@@ -106,22 +106,38 @@ __device__ __forceinline__ v4u lds_cols(const uint16_t* tile, int row0, int d, c
     return v4u{(unsigned)x[0], (unsigned)x[1], (unsigned)y[0], (unsigned)y[1]};
 }
 
-// Instruction order of a product loop: LDS operand reads run AHEAD of the matrix instructions that use them (left alone, the
-// compiler puts each read right before its use and every matrix instruction waits out the LDS latency).
-// COUNT matrix instructions, each preceded by READS reads of LDS.
-template <int COUNT, int READS, int AHEAD>
-__device__ __forceinline__ void order_reads_ahead() {
-    __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+// Operands of a group of matrix instructions (at most G), read one group ahead of their use: left alone, the compiler reads
+// each right before its instruction, which then waits out the LDS latency. fence() keeps the groups apart.
+template <int DP, int G>
+struct Operands {
+    static constexpr int KS = DP / 16, DTL = DP / 32;
+    static constexpr int RG = KS <= G ? KS : KS % G == 0 ? G : 3, CG = DTL <= G ? DTL : DTL % G == 0 ? G : 1;  // instructions of a group
+    static constexpr int RN = KS / RG, CN = DTL / CG;  // groups of a product over the head, and of one over 16 rows
+    static_assert(RG * RN == KS && CG * CN == DTL, "whole groups");
+    v4u f[2][RG > CG ? RG : CG];
+    __device__ __forceinline__ void rows(int to, const uint16_t* tile, int row0, int group, const LaneOffsets<DP>& at) {
 #pragma unroll
-    for (int i = 0; i < COUNT - AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        for (int j = 0; j < RG; ++j) f[to][j] = lds_rows<DP>(tile, row0, group * RG + j, at);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
-}
+    __device__ __forceinline__ void cols(int to, const uint16_t* tile, int row0, int group, const LaneOffsets<DP>& at) {
+#pragma unroll
+        for (int j = 0; j < CG; ++j) f[to][j] = lds_cols<DP>(tile, row0, group * CG + j, at);
+    }
+};
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
-// Waits for every load and copy so far.
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// Waits until at most LEFT (below 16) of the loads and copies so far are under way.
+template <int LEFT = 0>
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70 | LEFT); }
+
+// A barrier that leaves copies under way (__syncthreads waits for all of them): LDS accesses before it are done, and the
+// compiler moves none across it.
+__device__ __forceinline__ void barrier() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 // The B operand that results 8 s .. 8 s + 7 of a score column make
 template <int DT>
@@ -130,40 +146,58 @@ __device__ __forceinline__ v4u pack_step(const v16f& v, int s) {
                pack2<DT>(v[8 * s + 6], v[8 * s + 7])};
 }
 
-__device__ const uint4 x_zeros = {0, 0, 0, 0};
-
-// TR rows of a tensor into an LDS tile, by copies that do not pass through registers (a wave's copy fills 64 consecutive
-// 16-byte places; the chunk that belongs into a place is chosen by the lane's source address). They are done after wait_loads.
-template <int DP, int TR>
-struct Copy {
-    static constexpr int CPR = DP / 8, N = TR * CPR / kXThreads, RS = kXThreads / CPR;
-    static constexpr bool EVEN = kXThreads % CPR == 0;  // then a thread's places are in rows RS apart (a multiple of 16: one f)
-    static_assert(TR * CPR % kXThreads == 0, "whole chunks for every thread");
-    static __device__ __forceinline__ int row(int k) { return EVEN ? (int)threadIdx.x / CPR + k * RS : ((int)threadIdx.x + k * kXThreads) / CPR; }
-    static __device__ __forceinline__ int chunk(int k) {
-        const int place = EVEN ? (int)threadIdx.x % CPR : ((int)threadIdx.x + k * kXThreads) % CPR;
-        return place ^ tile_f<DP>(EVEN ? row(0) : row(k));
+// Copies of TR rows to an LDS tile that do not pass through registers: one fills 64 consecutive 16-byte places with the rows
+// from 64 / CPR * idx on; the chunk that belongs into a place is chosen by the lane's source offset. They are buffer loads:
+// what lies outside the tile's bytes (rows past the end, and the offsets given to chunks past the head size and to rows that
+// do not count) comes as zeros and is not read. So a copy is one instruction whatever the tile, without a branch, which
+// would make the compiler wait for every LDS read under way at its end. They are done after wait_loads.
+//
+// Two tensors (K and V, or Q and dO) go together: a wave's share of both is COPIES instructions, which are spread over the
+// work on the tile before, because a burst of them stops the wave until the memory path has taken them.
+struct XTile {
+    __amdgpu_buffer_rsrc_t bytes;
+    unsigned st2;  // bytes between rows
+    __device__ __forceinline__ XTile(const uint16_t* base, int64_t st, int rows, int D, int most = kXTile) {
+        const int n = rows < most ? rows : most;
+        st2 = (unsigned)st * 2u;  // (st below 2^24: a tile stays below 2^31 bytes)
+        bytes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, n > 0 ? (int)((unsigned)(n - 1) * st2 + (unsigned)D * 2u) : 0, 0x00020000);
     }
-    static __device__ __forceinline__ void one(const void* p, uint16_t* tile, int k, int wave) {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
-                                         (__attribute__((address_space(3))) void*)(tile + (k * kXWaves + wave) * 512), 16, 0, 0);
-    }
-    // rows base + row * st; those without a bit in `live` become zeros and are not read, nor is anything past the head size
-    // (st below 2^25: a tile's offsets fit 32 bits). wave: uniform.
-    static __device__ __forceinline__ void start(const uint16_t* base, int64_t st, int D, uint64_t live, uint16_t* tile, int wave) {
-        const unsigned s = (unsigned)st;
-        const bool whole = live == ~(uint64_t)0 && D == DP;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const char* b = reinterpret_cast<const char*>(EVEN ? base + k * RS * st : base);
-            const unsigned off = (unsigned)(EVEN ? row(0) : row(k)) * s * 2u + (unsigned)chunk(k) * 16u;
-            if (whole) {
-                one(b + off, tile, k, wave);
-            } else {
-                const bool in = ((live >> row(k)) & 1) && chunk(k) * 8 < D;
-                one(in ? b + off : reinterpret_cast<const char*>(&x_zeros), tile, k, wave);
-            }
+};
+template <int DP, int TR = kXTile>
+struct Copies {
+    static constexpr int CPR = DP / 8, ALONE = TR * CPR / 64, COPIES = 2 * ALONE / kXWaves;
+    static constexpr bool EVEN = 64 % CPR == 0;  // a copy is whole rows
+    static_assert(2 * ALONE % kXWaves == 0, "whole copies for every wave");
+    int wave, D;
+    // copy idx (0 .. ALONE - 1) of a tile; rows with a bit in `dead` become zeros
+    __device__ __forceinline__ void one(const XTile& x, int idx, uint64_t dead, uint16_t* tile) const {
+        const int lane = threadIdx.x & 63;
+        const int row = EVEN ? lane / CPR : (idx * 64 + lane) / CPR;  // EVEN: of the copy
+        // (idx is wave + a multiple of 4, and f looks at rows modulo 16: the lane's part is the same for all its copies)
+        const int f = EVEN ? tile_f<DP>((wave & 3) * (64 / CPR) + row) : tile_f<DP>(row);
+        const int chunk = (EVEN ? lane % CPR : (idx * 64 + lane) % CPR) ^ f;
+        unsigned off = (unsigned)row * x.st2 + (chunk * 8 < D ? (unsigned)chunk * 16u : 0x80000000u);
+        const int row0 = EVEN ? idx * (64 / CPR) : 0;
+        off += (unsigned)row0 * x.st2;
+        if constexpr (EVEN) {
+            const int word = row0 < 32 ? (int)dead : (int)(dead >> 32);  // a copy's rows lie in one half of the tile
+            off |= (unsigned)__builtin_amdgcn_sbfe(word, (unsigned)((row0 & 31) + row), 1u);
+        } else {
+            off |= (dead >> row) & 1 ? ~0u : 0u;
         }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(x.bytes, (__attribute__((address_space(3))) void*)(tile + idx * 512), 16, (int)off, 0, 0, 0);
+    }
+    // share i of the wave's COPIES
+    __device__ __forceinline__ void share(int i, const XTile& x, const XTile& y, uint64_t dead, uint16_t* xt, uint16_t* yt) const {
+        const int idx = wave + i * kXWaves;
+        if (idx < ALONE) one(x, idx, dead, xt);
+        else one(y, idx - ALONE, dead, yt);
+    }
+    // the shares that go with group g of `of`
+    __device__ __forceinline__ void group(int g, int of, const XTile& x, const XTile& y, uint64_t dead, uint16_t* xt, uint16_t* yt) const {
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i)
+            if (i * of / COPIES == g) share(i, x, y, dead, xt, yt);
     }
 };
 
@@ -187,15 +221,16 @@ struct XKeys {
 template <int DP>
 struct KVTiles {
     static constexpr int ELEMS = kXTile * DP;
+    Copies<DP> copies;
     const uint16_t *kp, *vp;
     int64_t kst, vst;
     const uint8_t* mask;
-    int len, D, wave;
+    int len;
     uint8_t byte;
     uint64_t live[2];  // of the present tile and of the next one
     // requests the mask bytes of tile t (any t: of an existing key)
     __device__ __forceinline__ void ask(int t) {
-        const int key = t * kXTile + (int)(threadIdx.x & 63), last = len - 1;
+        const int key = t * kXTile + (int)(threadIdx.x & 63), last = len - 1;  // (t0 < t1: len is 1 or more)
         // (without a mask some byte of K: a load under a condition would be waited for at its end)
         byte = *(mask != nullptr ? mask + (key < last ? key : last) : reinterpret_cast<const uint8_t*>(kp));
     }
@@ -203,30 +238,25 @@ struct KVTiles {
     __device__ __forceinline__ uint64_t counted(int t) const {
         return __builtin_amdgcn_ballot_w64(t * kXTile + (int)(threadIdx.x & 63) < len && (mask == nullptr || byte != 0));
     }
-    // starts the copies of tile t, whose keys `alive` count, and writes the bias of its scores
-    __device__ __forceinline__ void start(int t, uint64_t alive, uint16_t* kt, uint16_t* vt, float* bias) const {
-        Copy<DP, kXTile>::start(kp + t * kXTile * kst, kst, D, alive, kt, wave);
-        Copy<DP, kXTile>::start(vp + t * kXTile * vst, vst, D, alive, vt, wave);
+    // tile t of K and of V (any t: past the end they are empty)
+    __device__ __forceinline__ XTile k_tile(int t) const { return XTile(kp + (int64_t)t * kXTile * kst, kst, len - t * kXTile, copies.D); }
+    __device__ __forceinline__ XTile v_tile(int t) const { return XTile(vp + (int64_t)t * kXTile * vst, vst, len - t * kXTile, copies.D); }
+    // the bias of a tile's scores
+    static __device__ __forceinline__ void bias_of(uint64_t alive, float* bias) {
         if (alive != ~(uint64_t)0 && threadIdx.x < kXTile) bias[threadIdx.x] = (alive >> threadIdx.x) & 1 ? 0.f : -__builtin_inff();
     }
     // the first tile, whole and in place after the barrier
     __device__ __forceinline__ void first(int t, uint16_t* kt, uint16_t* vt, float* bias) {
-        ask(t);
-        wait_loads();
+        if (mask != nullptr) ask(t);  // (without a mask nothing is waited for)
         live[0] = counted(t);
-        start(t, live[0], kt, vt, bias);
+        copies.group(0, 1, k_tile(t), v_tile(t), ~live[0], kt, vt);
+        bias_of(live[0], bias);
         ask(t + 1);
         wait_loads();
         live[1] = counted(t + 1);
     }
-    // at the start of tile t, into the other buffer / before the barrier at its end
-    __device__ __forceinline__ void begin(int t, bool more, uint16_t* kt, uint16_t* vt, float* bias) {
-        if (!more) return;
-        start(t + 1, live[1], kt, vt, bias);
-        ask(t + 2);
-    }
-    __device__ __forceinline__ void end(int t, bool more) {
-        if (!more) return;
+    // before the barrier at the end of tile t
+    __device__ __forceinline__ void end(int t) {
         wait_loads();
         live[0] = live[1];
         live[1] = counted(t + 2);
@@ -315,7 +345,7 @@ inline int x_tensor(const char* who, const char* name, const void* p, const int6
         if (s[i] % 8) return fail(Q8_ERR_ALIGN, "%s: strides of %s must be multiples of 8 elements", who, name);
         e += (__int128)(n[i] - 1) * s[i];
     }
-    if (t > 1 && s[2] >= (1 << 25)) return fail(Q8_ERR_SHAPE, "%s: token stride of %s (below 2^25 elements)", who, name);
+    if (t > 1 && s[2] >= (1 << 24)) return fail(Q8_ERR_SHAPE, "%s: token stride of %s (below 2^24 elements)", who, name);
     if (e > (INT64_MAX >> 4)) return fail(Q8_ERR_SHAPE, "%s: strides of %s", who, name);
     if (!aligned16(p)) return fail(Q8_ERR_ALIGN, "%s: %s must be 16-byte aligned", who, name);
     return Q8_OK;

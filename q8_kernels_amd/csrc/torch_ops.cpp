@@ -243,7 +243,7 @@ std::array<Tensor, 2> apply_rotary(const Tensor& q, const OptTensor& key, const 
 
 // t itself where its rows are 16-byte chunks that the kernels can address, else a contiguous copy
 Tensor chunks(const Tensor& t) {
-    bool fine = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    bool fine = t.stride(3) == 1 && (t.size(2) <= 1 || t.stride(2) < (1 << 24)) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     for (int i = 0; i < 3; ++i) fine = fine && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
     return fine ? t : t.clone(at::MemoryFormat::Contiguous);
 }
