@@ -121,16 +121,12 @@ struct Rows32 {
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
         l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
-    // log-sum and O, through 32 rows of LDS of the wave's own
-    __device__ __forceinline__ void finish(const XFwd& a, int unit, int b, int hk, int row0, int lane, uint16_t* buf) const {
-        const int row = row0 + (lane & 31);
+    // log-sum and O
+    __device__ __forceinline__ void finish(const XFwd& a, int unit, int b, int hk, int row, int lane) const {
         if (a.lse != nullptr && row < a.R && lane < 32) a.lse[(int64_t)unit * a.R + row] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
-        store_tile<DT, DP>(acc, l == 0.f ? 0.f : 1.0f / l, buf, a.D, lane, [&](int r) -> uint16_t* {
-            const int n = row0 + r;
-            if (n >= a.R) return nullptr;
-            const int g = n / a.M;
-            return a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (n - g * a.M) * a.o.st;
-        });
+        const int g = row < a.R ? row / a.M : 0;
+        uint16_t* p = row < a.R ? a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (row - g * a.M) * a.o.st : nullptr;
+        store_rows<DT, DP>(acc, l == 0.f ? 0.f : 1.0f / l, p, a.D, lane);
     }
 };
 
@@ -198,8 +194,62 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
         }
         return;
     }
-    // (the tile buffers are free: every wave has passed the last barrier of the loop)
-    rows.finish(a, unit, b, hk, row0, lane, (wave < 2 ? k0 : k1) + (wave & 1) * 32 * DP);
+    rows.finish(a, unit, b, hk, row, lane);
+}
+
+// Few keys (two tiles at most): all of K and V stay in LDS, and a workgroup walks over the rows of its unit instead, each wave
+// by itself, without a barrier; the next 32 rows of Q are on their way meanwhile. The kernel above would fill LDS again for
+// every 128 rows (2 x 32 heads of 64, 6144 x 128 keys: 30 us here, 38 to 48 us there; with room for four tiles, and so two
+// workgroups on a CU instead of three, 6144 x 256 took 47 us here and 48 us there).
+constexpr int kFewTiles = 2;
+template <int DT, int DP>
+__global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd a, int parts) {
+    constexpr int ELEMS = kXTile * DP, KS = DP / 16;
+    __shared__ __align__(16) uint16_t k[kFewTiles * ELEMS], v[kFewTiles * ELEMS];
+    __shared__ __align__(16) float bias[kFewTiles * kXTile];
+    const int unit = blockIdx.x / parts, part = blockIdx.x - unit * parts;
+    const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int step = parts * kXRows;
+    int row = part * kXRows + wave * 32 + (lane & 31);
+
+    Rows32<DT, DP> rows;
+    rows.load(a, b, hk, row, half);
+    KVTiles<DP> kv;
+    kv.len = a.keys.length(b);
+    kv.mask = a.keys.row(b);
+    kv.copies.D = a.D;
+    kv.copies.wave = wave;
+    kv.kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+    kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+    kv.kst = a.k.st;
+    kv.vst = a.v.st;
+    const int tiles = (kv.len + kXTile - 1) / kXTile;  // at most kFewTiles
+#pragma unroll
+    for (int t = 0; t < kFewTiles; ++t) {
+        if (t >= tiles) break;
+        if (kv.mask != nullptr) kv.ask(t);
+        const uint64_t live = kv.counted(t);
+        kv.copies.group(0, 1, kv.k_tile(t), kv.v_tile(t), ~live, k + t * ELEMS, v + t * ELEMS);
+        if (threadIdx.x < kXTile) bias[t * kXTile + threadIdx.x] = (live >> threadIdx.x) & 1 ? 0.f : -__builtin_inff();
+    }
+    wait_loads();
+    __syncthreads();
+
+    LaneOffsets<DP> at(lane);
+    for (int row0 = part * kXRows + wave * 32; row0 < a.R; row0 += step, row += step) {
+        Rows32<DT, DP> ahead;
+        ahead.load(a, b, hk, row + step, half);
+        rows.clear();
+        for (int t = 0; t < tiles; ++t) {
+            at.fresh();
+            rows.tile(k + t * ELEMS, v + t * ELEMS, kv.mask == nullptr && (t + 1) * kXTile <= kv.len, bias + t * kXTile, a.c, at, half, [](int, int) {});
+        }
+        rows.join_halves();
+        rows.finish(a, unit, b, hk, row, lane);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) rows.qf[s] = ahead.qf[s];
+    }
 }
 
 // Joins the parts of a row: weights exp2(m_i - max m). 32 lanes a row, 4 elements a lane.
@@ -230,6 +280,12 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
+// The kernel for few keys, for heads of 64 or less, wants work for its 768 workgroups (three on each CU): 128 rows each.
+constexpr int kFewBlocks = 768;
+static bool few_keys(int64_t units, int64_t rows, int N, int D) {
+    return D <= 64 && N <= kFewTiles * kXTile && units * rows >= kFewBlocks * kXRows && rows >= 4 * kXRows;
+}
+
 static XSchedule fwd_plan(int64_t units, int64_t rows, int N, int D) {
     // workgroups that run at once on the 256 CUs, by the registers of a lane
     return schedule(units * ((rows + kXRows - 1) / kXRows), N, D <= 32 ? 1024 : D <= 64 ? 768 : 512);
@@ -242,6 +298,7 @@ using namespace q8;
 extern "C" int64_t q8_cross_attn_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
     if (int e = x_sizes("q8_cross_attn_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
     const int64_t rows = (int64_t)(H / Hkv) * M;
+    if (few_keys(B * Hkv, rows, N, D)) return 0;
     return fwd_plan(B * Hkv, rows, N, D).parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
 }
 
@@ -277,6 +334,20 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
     a.R = a.G * M;
     a.row_blocks = (a.R + kXRows - 1) / kXRows;
     if (B * Hkv * a.row_blocks > 0x7ffff000) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (few_keys(B * Hkv, a.R, N, D)) {
+        const int64_t units = B * Hkv, want = (kFewBlocks + units - 1) / units, parts = want < a.row_blocks ? want : a.row_blocks;
+        if (units * parts > 0x7fffffff) return fail(Q8_ERR_SHAPE, "%s: too many heads", who);
+        const unsigned grid = (unsigned)(units * parts);
+#define X_FEW(DT)                                                                                        \
+    do {                                                                                                 \
+        if (D <= 32) cross_attn_few_keys_kernel<DT, 32><<<grid, kXThreads, 0, st>>>(a, (int)parts);      \
+        else cross_attn_few_keys_kernel<DT, 64><<<grid, kXThreads, 0, st>>>(a, (int)parts);              \
+    } while (0)
+        if (dt == Q8_BF16) X_FEW(Q8_BF16); else X_FEW(Q8_F16);
+#undef X_FEW
+        return launch_status(who);
+    }
     a.plan = fwd_plan(B * Hkv, a.R, N, D);
     if (a.plan.parts()) {
         const int64_t need = q8_cross_attn_workspace(B, H, Hkv, M, N, D);
@@ -288,7 +359,6 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
         a.pm = a.part + n * D;
         a.pl = a.pm + n;
     }
-    hipStream_t st = static_cast<hipStream_t>(stream);
     const unsigned grid = a.plan.grid();
 #define X_FWD(DT)                                                                       \
     switch (padded_head(D)) {                                                           \

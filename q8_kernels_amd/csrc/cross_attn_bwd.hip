@@ -32,7 +32,7 @@ struct XBwd {
 };
 
 template <int DT, int DP>
-__global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
+__global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_kernel(XBwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32, ELEMS = kXTile * DP;
     __shared__ __align__(16) uint16_t k0[ELEMS], k1[ELEMS], v0[ELEMS], v1[ELEMS];
     __shared__ __align__(16) float bias0[kXTile], bias1[kXTile];
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
     __syncthreads();
 
     LaneOffsets<DP> at(lane);
-    Operands<DP, 4> ops;
+    Operands<DP, 2> ops;
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
@@ -138,16 +138,22 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
             // (2 RN groups so far: the columns are in place 0)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse));
+            int w = 0;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const v4u p = pack_step<DT>(dp, k);
-                if (k == 0) ops.cols(1, kl, u * 32 + 16, 0, at);
-                else if (u == 0) ops.rows(0, kl, 32, 0, at);
-                fence();
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(ops.f[k][d], p, acc[d]);
-                fence();
+                for (int c = 0; c < ops.CN; ++c, w ^= 1) {
+                    if (c + 1 < ops.CN) ops.cols(w ^ 1, kl, u * 32 + k * 16, c + 1, at);
+                    else if (k == 0) ops.cols(w ^ 1, kl, u * 32 + 16, 0, at);
+                    else if (u == 0) ops.rows(w ^ 1, kl, 32, 0, at);
+                    fence();
+#pragma unroll
+                    for (int d = 0; d < ops.CG; ++d) acc[c * ops.CG + d] = mfma16<DT>(ops.f[w][d], p, acc[c * ops.CG + d]);
+                    fence();
+                }
             }
+            // (an even number of groups: the next rows are in place 0)
         }
         kv.end(t);
         __syncthreads();
@@ -169,12 +175,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dq_kernel(XBwd a) {
         }
         return;
     }
-    store_tile<DT, DP>(acc, a.scale, (wave < 2 ? k0 : k1) + (wave & 1) * 32 * DP, a.D, lane, [&](int r) -> uint16_t* {
-        const int n = row0 + r;
-        if (n >= a.R) return nullptr;
-        const int g = n / a.M;
-        return a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (n - g * a.M) * a.dq.st;
-    });
+    const int g = row < a.R ? row / a.M : 0;
+    store_rows<DT, DP>(acc, a.scale, row < a.R ? a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (row - g * a.M) * a.dq.st : nullptr, a.D, lane);
 }
 
 // A head of more than 96 leaves no registers for V beside K and the two sums (two waves a SIMD have 256 each): V stays in
@@ -370,16 +372,9 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
         }
         return;
     }
-    auto to = [&](const XOut& x) {
-        uint16_t* p = x.p + b * x.sb + hk * x.sh;
-        return [&, p](int r) -> uint16_t* { return key0 + r < a.N ? p + (key0 + r) * x.st : nullptr; };
-    };
-    // (32 rows for each wave: its own rows of V, or half a tile)
-    uint16_t* buf = V_IN_LDS ? vl + wave * 32 * DP : (wave < 2 ? q0 : q1) + (wave & 1) * 32 * DP;
-    store_tile<DT, DP>(dk, a.scale, buf, a.D, lane, to(a.dk));
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    store_tile<DT, DP>(dv, 1.0f, buf, a.D, lane, to(a.dv));
+    const bool there = key < a.N;
+    store_rows<DT, DP>(dk, a.scale, there ? a.dk.p + b * a.dk.sb + hk * a.dk.sh + key * a.dk.st : nullptr, a.D, lane);
+    store_rows<DT, DP>(dv, 1.0f, there ? a.dv.p + b * a.dv.sb + hk * a.dv.sh + key * a.dv.st : nullptr, a.D, lane);
 }
 
 // Adds the parts of dQ (WIDTH = 1) or of dK and dV (WIDTH = 2): one thread for 4 elements of a row.
@@ -424,7 +419,7 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     p.dq_blocks = (p.rows + kXRows - 1) / kXRows;
     p.kv_blocks = ((int64_t)N + kXRows - 1) / kXRows;
     // workgroups that run at once on the 256 CUs, by the registers of a lane
-    p.dq = schedule(p.units * p.dq_blocks, N, D <= 32 ? 1024 : 512);
+    p.dq = schedule(p.units * p.dq_blocks, N, D <= 32 ? 1024 : D <= 64 ? 768 : 512);
     p.kv = schedule(p.units * p.kv_blocks, (int64_t)(H / Hkv) * ((M + kXTile - 1) / kXTile) * kXTile, D <= 32 ? 1024 : 512);
     const int64_t dq = p.dq.parts() * kXRows * D, kv = p.kv.parts() * kXRows * 2 * D;
     p.parts = dq > kv ? dq : kv;  // one after the other in the same place

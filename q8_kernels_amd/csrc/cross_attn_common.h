@@ -310,25 +310,27 @@ inline XSchedule schedule(int64_t blocks, int64_t length, int slots) {
     return s;
 }
 
-// One 32 x D result of a wave (columns = rows of the output, results = its elements) to memory in whole 16-byte chunks,
-// through `buf`, 32 rows of a tile of the wave's own. at(row): pointer to the output row or NULL.
-template <int DT, int DP, typename At>
-__device__ __forceinline__ void store_tile(const v16f (&acc)[DP / 32], float scale, uint16_t* buf, int D, int lane, At at) {
-    constexpr int CPR = DP / 8;
+// One 32 x D result of a wave (columns = rows of the output, results = its elements) to memory. Lanes l and l + 32 hold 4
+// elements each of the same 8: two half exchanges make 16 consecutive bytes of either, 8 elements of group i in the low lane
+// and those of group i + 1 in the high one. p: the lane's output row (of column l % 32), NULL where there is none.
+template <int DT, int DP>
+__device__ __forceinline__ void store_rows(const v16f (&acc)[DP / 32], float scale, uint16_t* p, int D, int lane) {
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<v2i*>(buf + tile_at<DP>(lane & 31, t * 4 + i) + ((lane >> 5) << 2)) =
-                v2i{(int)pack2<DT>(acc[t][4 * i] * scale, acc[t][4 * i + 1] * scale), (int)pack2<DT>(acc[t][4 * i + 2] * scale, acc[t][4 * i + 3] * scale)};
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+        for (int i = 0; i < 4; i += 2) {
+            uint32_t w[2][2];
 #pragma unroll
-    for (int c = 0; c < 32 * CPR / 64; ++c) {
-        const int i = lane + c * 64, row = i / CPR, e = (i - row * CPR) * 8;
-        uint16_t* p = at(row);
-        if (p != nullptr && e < D) *reinterpret_cast<v4u*>(p + e) = *reinterpret_cast<const v4u*>(buf + tile_at<DP>(row, e / 8));
-    }
+            for (int k = 0; k < 2; ++k) {
+                const int r = 4 * (i + k);
+                w[k][0] = pack2<DT>(acc[t][r] * scale, acc[t][r + 1] * scale);
+                w[k][1] = pack2<DT>(acc[t][r + 2] * scale, acc[t][r + 3] * scale);
+            }
+            const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+            const int e = t * 32 + (i + (lane >> 5)) * 8;
+            if (p != nullptr && e < D) *reinterpret_cast<v4u*>(p + e) = v4u{x[0], y[0], x[1], y[1]};
+        }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------
