@@ -34,43 +34,168 @@ struct RotArgs {
     int per_block;            // tokens of a workgroup
 };
 
-template <int DT>
-__device__ __forceinline__ float rot_get(const void* p, int64_t e) {
-    if constexpr (DT == Q8_F32) return static_cast<const float*>(p)[e];
-    const uint32_t h = static_cast<const uint16_t*>(p)[e];
-    return DT == Q8_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
-}
-template <int DT>
-__device__ __forceinline__ void rot_put(void* p, int64_t e, float v) {
-    if constexpr (DT == Q8_F32) static_cast<float*>(p)[e] = v;
-    else static_cast<uint16_t*>(p)[e] = DT == Q8_BF16 ? (uint16_t)(pack2_bf16(v, 0.f) & 0xffffu) : __builtin_bit_cast(uint16_t, (_Float16)v);
-}
-template <int DT>
-__device__ __forceinline__ void rot_store8(void* p, int64_t e, const float (&v)[8]) {
-    if constexpr (DT == Q8_F32) {
-        v4f* s = reinterpret_cast<v4f*>(static_cast<float*>(p) + e);
-        s[0] = v4f{v[0], v[1], v[2], v[3]};
-        s[1] = v4f{v[4], v[5], v[6], v[7]};
-    } else {
-        v4u w;
+// A work item's elements as they are in memory: VEC = 8: 16 bytes (32 of fp32) from one place, or from two for the pairs of the
+// half layout; VEC = 1: one element each.
+template <int DT, int VEC>
+struct RotPart {
+    static constexpr int N = VEC == 1 ? 1 : DT == Q8_F32 ? 8 : 4;
+    uint32_t r[N];
+    __device__ __forceinline__ void load(const void* p, int64_t e) {
+        if constexpr (VEC == 1) {
+            r[0] = DT == Q8_F32 ? static_cast<const uint32_t*>(p)[e] : static_cast<const uint16_t*>(p)[e];
+        } else {
+            const v4u* s = reinterpret_cast<const v4u*>(static_cast<const char*>(p) + e * (DT == Q8_F32 ? 4 : 2));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = DT == Q8_BF16 ? pack2_bf16(v[2 * i], v[2 * i + 1])
-                                 : __builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) << 16);
-        *reinterpret_cast<v4u*>(static_cast<uint16_t*>(p) + e) = w;
+            for (int q = 0; q < N / 4; ++q) {
+                const v4u w = s[q];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) r[q * 4 + k] = w[k];
+            }
+        }
     }
-}
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (DT == Q8_F32) return __uint_as_float(r[i]);
+        const uint32_t h = VEC == 1 ? r[0] : (i & 1) ? r[i >> 1] >> 16 : r[i >> 1] & 0xffffu;
+        return DT == Q8_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+    }
+    __device__ __forceinline__ void set(const float (&v)[VEC]) {
+        if constexpr (VEC == 1) {
+            r[0] = DT == Q8_F32 ? __float_as_uint(v[0]) : DT == Q8_BF16 ? pack2_bf16(v[0], 0.f) & 0xffffu : __builtin_bit_cast(uint16_t, (_Float16)v[0]);
+        } else if constexpr (DT == Q8_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                r[i] = DT == Q8_BF16 ? pack2_bf16(v[2 * i], v[2 * i + 1])
+                                     : __builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) << 16);
+        }
+    }
+    __device__ __forceinline__ void store(void* p, int64_t e) const {
+        if constexpr (VEC == 1) {
+            if constexpr (DT == Q8_F32) static_cast<uint32_t*>(p)[e] = r[0];
+            else static_cast<uint16_t*>(p)[e] = (uint16_t)r[0];
+        } else {
+            v4u* s = reinterpret_cast<v4u*>(static_cast<char*>(p) + e * (DT == Q8_F32 ? 4 : 2));
+#pragma unroll
+            for (int q = 0; q < N / 4; ++q) s[q] = v4u{r[q * 4], r[q * 4 + 1], r[q * 4 + 2], r[q * 4 + 3]};
+        }
+    }
+};
 
 // One work item of a head: VEC = 8: 8 pairs (half) / 4 pairs (interleaved) or 8 copied elements, in 16-byte accesses;
-// VEC = 1: one pair or one copied element. Threads with the same threadIdx / items share a head.
+// VEC = 1: one pair or one copied element. Threads with the same threadIdx / items share a head; a thread has BATCH items
+// under way at once, the first of them requested before the angles are formed.
 template <int DT, bool HALF, int VEC>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
+    constexpr int BATCH = 4, PAIRS = VEC == 1 ? 1 : (HALF ? 8 : 4);  // pairs of an item
+    constexpr bool TWO = HALF || VEC == 1;                          // a pair's elements come from two places
     __shared__ float2 cs[kRotAngles];
     const int64_t token0 = (int64_t)blockIdx.x * a.per_block;
     const int here = (int)(a.all_tokens - token0 < a.per_block ? a.all_tokens - token0 : a.per_block);
+    const int64_t b0 = token0 / a.tokens, t0 = token0 - b0 * a.tokens;
+    // batch element and token of the workgroup's token tok (of fewer than 64)
+    auto place = [&](int tok, int64_t& b, int64_t& t) {
+        b = b0;
+        t = t0 + tok;
+        if (a.tokens >= 64) {
+            if (t >= a.tokens) { t -= a.tokens; ++b; }
+        } else {
+            const unsigned n = (unsigned)t / (unsigned)a.tokens;
+            b += n;
+            t -= (int64_t)n * a.tokens;
+        }
+    };
+    const int rot_items = a.pairs / PAIRS, items = rot_items + (a.dim - 2 * a.pairs) / VEC;
+    const int lanes = kRotThreads / items > 0 ? kRotThreads / items : 1;  // heads in flight
+    const int dtok = lanes / a.heads, dhead = lanes - dtok * a.heads;
+
+    struct Item {
+        RotPart<DT, VEC> u, v;
+        void* out;
+        int64_t to;
+        int tok;
+    } x[BATCH];
+    int item = items <= kRotThreads ? (int)threadIdx.x % items : (int)threadIdx.x;
+    const int lane = items <= kRotThreads ? (int)threadIdx.x / items : 0;
+    int tok = here, head = 0;  // a thread without a head, or with no item, has no token
+    auto begin = [&] {
+        if (lane < lanes && item < items) {
+            tok = lane / a.heads;
+            head = lane - tok * a.heads;
+        } else {
+            tok = here;
+        }
+    };
+    // element offsets of the item's first and second place in a head
+    auto places = [&](int& eu, int& ev) {
+        if (item >= rot_items) eu = ev = 2 * a.pairs + (item - rot_items) * VEC;
+        else if (VEC == 1) { eu = HALF ? item : 2 * item; ev = HALF ? item + a.pairs : 2 * item + 1; }
+        else { eu = item * 8; ev = HALF ? a.pairs + item * 8 : eu; }
+    };
+    auto request = [&] {
+        int eu, ev;
+        places(eu, ev);
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            x[k].tok = tok;
+            if (tok < here) {
+                int64_t b, t;
+                place(tok, b, t);
+                const bool is_q = head < a.q_heads;
+                const int h = is_q ? head : head - a.q_heads;
+                const RotTensor& y = is_q ? a.q : a.k;
+                const int64_t in = b * y.ib + h * y.ih + t * y.it;
+                x[k].out = y.out;
+                x[k].to = b * y.ob + h * y.oh + t * y.ot;
+                x[k].u.load(y.in, in + eu);
+                if (TWO && item < rot_items) x[k].v.load(y.in, in + ev);
+            }
+            tok += dtok;
+            head += dhead;
+            if (head >= a.heads) { head -= a.heads; ++tok; }
+        }
+    };
+    auto finish = [&] {
+        int eu, ev;
+        places(eu, ev);
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            if (x[k].tok >= here) continue;
+            if (item < rot_items) {
+                const float2* w = cs + x[k].tok * a.pairs + item * PAIRS;
+                if constexpr (TWO) {
+                    float ou[VEC], ov[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float u = x[k].u.get(i), v = x[k].v.get(i);
+                        ou[i] = u * w[i].x - v * w[i].y;
+                        ov[i] = v * w[i].x + u * w[i].y;
+                    }
+                    x[k].u.set(ou);
+                    x[k].v.set(ov);
+                    x[k].v.store(x[k].out, x[k].to + ev);
+                } else {
+                    float o[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC / 2; ++i) {
+                        const float u = x[k].u.get(2 * i), v = x[k].u.get(2 * i + 1);
+                        o[2 * i] = u * w[i].x - v * w[i].y;
+                        o[2 * i + 1] = v * w[i].x + u * w[i].y;
+                    }
+                    x[k].u.set(o);
+                }
+            }
+            x[k].u.store(x[k].out, x[k].to + eu);
+        }
+    };
+
+    begin();
+    request();
     for (int i = threadIdx.x; i < here * a.pairs; i += kRotThreads) {
-        const int tok = i / a.pairs, pr = i - tok * a.pairs;
-        const int64_t g = token0 + tok, b = g / a.tokens, t = g - b * a.tokens;
+        const int n = i / a.pairs, pr = i - n * a.pairs;
+        int64_t b, t;
+        place(n, b, t);
         int64_t p = t;
         if (a.positions != nullptr) {
             const int64_t at = b * a.pos_stride + t;
@@ -85,63 +210,14 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
         cs[i] = make_float2(c * a.factor, s * a.factor * a.sign);
     }
     __syncthreads();
-    constexpr int PAIRS = VEC == 1 ? 1 : (HALF ? 8 : 4);  // pairs of an item
-    const int rot_items = a.pairs / PAIRS, items = rot_items + (a.dim - 2 * a.pairs) / VEC;
-    const int lanes = kRotThreads / items > 0 ? kRotThreads / items : 1;  // heads in flight
-    const int item0 = items <= kRotThreads ? (int)threadIdx.x % items : (int)threadIdx.x;
-    const int lane = items <= kRotThreads ? (int)threadIdx.x / items : 0;
-    if (lane >= lanes) return;
-    for (int item = item0; item < items; item += kRotThreads) {  // (one turn unless a head has more items than there are threads)
-        int tok = lane / a.heads, head = lane - tok * a.heads;
-        const int dtok = lanes / a.heads, dhead = lanes - dtok * a.heads;
-        while (tok < here) {
-            const int64_t g = token0 + tok, b = g / a.tokens, t = g - b * a.tokens;
-            const bool is_q = head < a.q_heads;
-            const int h = is_q ? head : head - a.q_heads;
-            const RotTensor& x = is_q ? a.q : a.k;
-            const int64_t in = b * x.ib + h * x.ih + t * x.it, out = b * x.ob + h * x.oh + t * x.ot;
-            if (item < rot_items) {
-                const float2* w = cs + tok * a.pairs + item * PAIRS;
-                if constexpr (VEC == 1) {
-                    const int eu = HALF ? item : 2 * item, ev = HALF ? item + a.pairs : 2 * item + 1;
-                    const float u = rot_get<DT>(x.in, in + eu), v = rot_get<DT>(x.in, in + ev);
-                    rot_put<DT>(x.out, out + eu, u * w[0].x - v * w[0].y);
-                    rot_put<DT>(x.out, out + ev, v * w[0].x + u * w[0].y);
-                } else if constexpr (HALF) {
-                    float u[8], v[8], ou[8], ov[8];
-                    load8<DT>(x.in, in + item * 8, u);
-                    load8<DT>(x.in, in + a.pairs + item * 8, v);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        ou[i] = u[i] * w[i].x - v[i] * w[i].y;
-                        ov[i] = v[i] * w[i].x + u[i] * w[i].y;
-                    }
-                    rot_store8<DT>(x.out, out + item * 8, ou);
-                    rot_store8<DT>(x.out, out + a.pairs + item * 8, ov);
-                } else {
-                    float u[8], o[8];
-                    load8<DT>(x.in, in + item * 8, u);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[2 * i] = u[2 * i] * w[i].x - u[2 * i + 1] * w[i].y;
-                        o[2 * i + 1] = u[2 * i + 1] * w[i].x + u[2 * i] * w[i].y;
-                    }
-                    rot_store8<DT>(x.out, out + item * 8, o);
-                }
-            } else {
-                const int e = 2 * a.pairs + (item - rot_items) * VEC;
-                if constexpr (VEC == 1) {
-                    rot_put<DT>(x.out, out + e, rot_get<DT>(x.in, in + e));
-                } else {
-                    float u[8];
-                    load8<DT>(x.in, in + e, u);
-                    rot_store8<DT>(x.out, out + e, u);
-                }
-            }
-            tok += dtok;
-            head += dhead;
-            if (head >= a.heads) { head -= a.heads; ++tok; }
+    for (;;) {
+        finish();
+        if (tok >= here) {  // the next item, where a head has more of them than there are threads
+            item += kRotThreads;
+            if (item >= items) break;
+            begin();
         }
+        request();
     }
 }
 
@@ -206,10 +282,11 @@ extern "C" int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, c
     a.pairs = rotary_dim / 2;
     a.tokens = tokens;
     a.all_tokens = all;
-    // tokens of a workgroup: about 2048 items of 8 elements, while 1024 workgroups remain and the angles fit
+    // tokens of a workgroup (63 at most): about 2048 items of 8 elements, while 1024 workgroups remain and the angles fit
     const int64_t per_token = (int64_t)a.heads * ((dim + 7) / 8);
     int64_t per = 2048 / per_token;
     if (per > all / 1024) per = all / 1024;
+    if (per > 63) per = 63;
     if (per > kRotAngles / a.pairs) per = kRotAngles / a.pairs;
     a.per_block = per < 1 ? 1 : (int)per;
     const int64_t blocks = (all + a.per_block - 1) / a.per_block;
