@@ -162,22 +162,28 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     __syncthreads();
 
     LaneOffsets<DP> at(lane);
-    auto step = [&](int t, auto buffer) {
+    auto step = [&](int t, auto buffer, auto with_rows) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
         // (past the last tile of this workgroup the copies are of a tile that nobody reads, or empty)
         kv.bias_of(kv.live[1], BUF ? bias0 : bias1);
         kv.ask(t + 2);
         const XTile knext = kv.k_tile(t + 1), vnext = kv.v_tile(t + 1);
-        rows.tile(BUF ? k1 : k0, BUF ? v1 : v0, kv.live[0] == ~(uint64_t)0, BUF ? bias1 : bias0, a.c, at, half,
-                  [&](int i, int n) { kv.copies.group(i, n, knext, vnext, ~kv.live[1], BUF ? k0 : k1, BUF ? v0 : v1); });
+        auto copies = [&](int i, int n) { kv.copies.group(i, n, knext, vnext, ~kv.live[1], BUF ? k0 : k1, BUF ? v0 : v1); };
+        if constexpr (with_rows) rows.tile(BUF ? k1 : k0, BUF ? v1 : v0, kv.live[0] == ~(uint64_t)0, BUF ? bias1 : bias0, a.c, at, half, copies);
+        else copies(0, 1);
         kv.end(t);
         __syncthreads();
     };
-    for (int t = t0; t < t1; t += 2) {
-        step(t, std::integral_constant<int, 0>{});
-        if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
-    }
+    auto walk = [&](auto with_rows) {
+        for (int t = t0; t < t1; t += 2) {
+            step(t, std::integral_constant<int, 0>{}, with_rows);
+            if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{}, with_rows);
+        }
+    };
+    // a wave without rows only copies (it meets the same barriers: they count waves)
+    if (row0 < a.R) walk(std::true_type{});
+    else walk(std::false_type{});
     rows.join_halves();
     if (of > 1) {
         if (row < a.R) {
@@ -197,16 +203,15 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     rows.finish(a, unit, b, hk, row, lane);
 }
 
-// Few keys (two tiles at most): all of K and V stay in LDS, and a workgroup walks over the rows of its unit instead, each wave
+// Few keys (NT tiles at most): all of K and V stay in LDS, and a workgroup walks over the rows of its unit instead, each wave
 // by itself, without a barrier; the next 32 rows of Q are on their way meanwhile. The kernel above would fill LDS again for
-// every 128 rows (2 x 32 heads of 64, 6144 x 128 keys: 30 us here, 38 to 48 us there; with room for four tiles, and so two
-// workgroups on a CU instead of three, 6144 x 256 took 47 us here and 48 us there).
-constexpr int kFewTiles = 2;
-template <int DT, int DP>
+// every 128 rows. 2 x 32 heads of 64, ragged lengths: 6144 x 128 keys (NT = 2, three workgroups on a CU) 30 us here and 38 to
+// 48 us there, 6144 x 256 keys (NT = 4, two workgroups) 47 us here and 57 us there.
+template <int DT, int DP, int NT>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd a, int parts) {
     constexpr int ELEMS = kXTile * DP, KS = DP / 16;
-    __shared__ __align__(16) uint16_t k[kFewTiles * ELEMS], v[kFewTiles * ELEMS];
-    __shared__ __align__(16) float bias[kFewTiles * kXTile];
+    __shared__ __align__(16) uint16_t k[NT * ELEMS], v[NT * ELEMS];
+    __shared__ __align__(16) float bias[NT * kXTile];
     const int unit = blockIdx.x / parts, part = blockIdx.x - unit * parts;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
@@ -224,9 +229,9 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd 
     kv.vp = a.v.p + b * a.v.sb + hk * a.v.sh;
     kv.kst = a.k.st;
     kv.vst = a.v.st;
-    const int tiles = (kv.len + kXTile - 1) / kXTile;  // at most kFewTiles
+    const int tiles = (kv.len + kXTile - 1) / kXTile;  // at most NT
 #pragma unroll
-    for (int t = 0; t < kFewTiles; ++t) {
+    for (int t = 0; t < NT; ++t) {
         if (t >= tiles) break;
         if (kv.mask != nullptr) kv.ask(t);
         const uint64_t live = kv.counted(t);
@@ -261,15 +266,32 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     if (n >= all || r >= a.R) return;
     const int e = (threadIdx.x & 31) * 4;
     float m = -3.0e38f, l = 0.f;
-    for (int i = 0; i < a.plan.splits; ++i) m = fmaxf(m, a.pm[i * all + n]);
     v4f o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.plan.splits; ++i) {
-        const float w = __builtin_amdgcn_exp2f(a.pm[i * all + n] - m);
-        l += w * a.pl[i * all + n];
-        if (e < a.D) {
-            const v4f p = *reinterpret_cast<const v4f*>(a.part + (i * all + n) * a.D + e);
+    // 8 parts at a time, their loads all under way together
+    for (int i0 = 0; i0 < a.plan.splits; i0 += 8) {
+        float pm[8], pl[8];
+        v4f po[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] += w * p[j];
+        for (int i = 0; i < 8; ++i) {
+            const int64_t at = (i0 + i < a.plan.splits ? i0 + i : i0) * all + n;
+            pm[i] = i0 + i < a.plan.splits ? a.pm[at] : -3.0e38f;
+            pl[i] = i0 + i < a.plan.splits ? a.pl[at] : 0.f;
+            po[i] = e < a.D ? *reinterpret_cast<const v4f*>(a.part + at * a.D + e) : v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max_ieee(top, pm[i]);
+        const float f = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float w = i0 + i < a.plan.splits ? __builtin_amdgcn_exp2f(pm[i] - m) : 0.f;
+            l += w * pl[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += w * po[i][j];
         }
     }
     if (a.lse != nullptr && e == 0) a.lse[(int64_t)unit * a.R + r] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
@@ -280,15 +302,15 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
-// The kernel for few keys, for heads of 64 or less, wants work for its 768 workgroups (three on each CU): 128 rows each.
-constexpr int kFewBlocks = 768;
+// The kernel for few keys, for heads of 64 or less, wants rows for all the workgroups that run at once.
+static int few_blocks(int N) { return N <= 2 * kXTile ? 768 : 512; }
 static bool few_keys(int64_t units, int64_t rows, int N, int D) {
-    return D <= 64 && N <= kFewTiles * kXTile && units * rows >= kFewBlocks * kXRows && rows >= 4 * kXRows;
+    return D <= 64 && N <= 4 * kXTile && units * rows >= few_blocks(N) * kXRows && rows >= 4 * kXRows;
 }
 
-static XSchedule fwd_plan(int64_t units, int64_t rows, int N, int D) {
+static XSchedule fwd_plan(int64_t units, int64_t rows, int N, int D, bool ragged) {
     // workgroups that run at once on the 256 CUs, by the registers of a lane
-    return schedule(units * ((rows + kXRows - 1) / kXRows), N, D <= 32 ? 1024 : D <= 64 ? 768 : 512);
+    return schedule(units * ((rows + kXRows - 1) / kXRows), N, D <= 32 ? 1024 : D <= 64 ? 768 : 512, ragged ? 2 : 1);
 }
 
 }  // namespace q8
@@ -299,7 +321,7 @@ extern "C" int64_t q8_cross_attn_workspace(int64_t B, int H, int Hkv, int M, int
     if (int e = x_sizes("q8_cross_attn_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
     const int64_t rows = (int64_t)(H / Hkv) * M;
     if (few_keys(B * Hkv, rows, N, D)) return 0;
-    return fwd_plan(B * Hkv, rows, N, D).parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
+    return fwd_plan(B * Hkv, rows, N, D, true).parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
@@ -336,21 +358,25 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
     if (B * Hkv * a.row_blocks > 0x7ffff000) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (few_keys(B * Hkv, a.R, N, D)) {
-        const int64_t units = B * Hkv, want = (kFewBlocks + units - 1) / units, parts = want < a.row_blocks ? want : a.row_blocks;
+        const int64_t units = B * Hkv, want = (few_blocks(N) + units - 1) / units, parts = want < a.row_blocks ? want : a.row_blocks;
         if (units * parts > 0x7fffffff) return fail(Q8_ERR_SHAPE, "%s: too many heads", who);
         const unsigned grid = (unsigned)(units * parts);
-#define X_FEW(DT)                                                                                        \
-    do {                                                                                                 \
-        if (D <= 32) cross_attn_few_keys_kernel<DT, 32><<<grid, kXThreads, 0, st>>>(a, (int)parts);      \
-        else cross_attn_few_keys_kernel<DT, 64><<<grid, kXThreads, 0, st>>>(a, (int)parts);              \
+#define X_FEW(DT, NT)                                                                                        \
+    do {                                                                                                     \
+        if (D <= 32) cross_attn_few_keys_kernel<DT, 32, NT><<<grid, kXThreads, 0, st>>>(a, (int)parts);      \
+        else cross_attn_few_keys_kernel<DT, 64, NT><<<grid, kXThreads, 0, st>>>(a, (int)parts);              \
     } while (0)
-        if (dt == Q8_BF16) X_FEW(Q8_BF16); else X_FEW(Q8_F16);
+        if (N <= 2 * kXTile) {
+            if (dt == Q8_BF16) X_FEW(Q8_BF16, 2); else X_FEW(Q8_F16, 2);
+        } else {
+            if (dt == Q8_BF16) X_FEW(Q8_BF16, 4); else X_FEW(Q8_F16, 4);
+        }
 #undef X_FEW
         return launch_status(who);
     }
-    a.plan = fwd_plan(B * Hkv, a.R, N, D);
+    a.plan = fwd_plan(B * Hkv, a.R, N, D, kv_lens != nullptr);
     if (a.plan.parts()) {
-        const int64_t need = q8_cross_attn_workspace(B, H, Hkv, M, N, D);
+        const int64_t need = a.plan.parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
         if (workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
         if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
         if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);

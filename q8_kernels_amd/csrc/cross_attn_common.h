@@ -299,12 +299,13 @@ struct XSchedule {
     unsigned grid() const { return full + 8u * ((tail * splits + 7) / 8); }
     int64_t parts() const { return splits > 1 ? (int64_t)tail * splits : 0; }  // blocks of partial results
 };
-// `slots`: workgroups that run at once; a divided walk is four tiles or more
-inline XSchedule schedule(int64_t blocks, int64_t length, int slots) {
+// `slots`: workgroups that run at once; a divided walk is four tiles or more. `turns`: how many times the workgroups of the
+// divided blocks may fill the card: with lengths that differ, pieces half as long even them out.
+inline XSchedule schedule(int64_t blocks, int64_t length, int slots, int turns = 1) {
     XSchedule s;
     s.full = (unsigned)(blocks / slots * slots);
     s.tail = (unsigned)(blocks - s.full);
-    const int64_t most = ((length + kXTile - 1) / kXTile + 3) / 4, want = s.tail ? slots / s.tail : 1;
+    const int64_t most = ((length + kXTile - 1) / kXTile + 3) / 4, want = s.tail ? (int64_t)slots * turns / s.tail : 1;
     s.splits = (int)(want < most ? want : most);
     if (s.splits < 1) s.splits = 1;
     return s;

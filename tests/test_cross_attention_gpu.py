@@ -328,3 +328,18 @@ def test_refusals(dev):
     (dq,) = torch.autograd.grad(attend(x, k, v), x, torch.ones_like(q), create_graph=True)
     with pytest.raises(RuntimeError):
         dq.float().sum().backward()
+
+
+@pytest.mark.parametrize("b,h,hk,m,n,d,dtype", [(2, 32, 32, 1700, 128, 64, torch.bfloat16), (3, 16, 4, 2311, 77, 64, torch.float16), (1, 48, 48, 2100, 256, 64, torch.bfloat16),
+                                                (2, 24, 24, 2050, 200, 40, torch.float16), (4, 16, 8, 1601, 1, 32, torch.bfloat16), (2, 40, 5, 1300, 129, 24, torch.bfloat16)])
+def test_few_keys_and_many_rows(dev, b, h, hk, m, n, d, dtype):
+    gen = torch.Generator(device=dev).manual_seed(n)
+    q, k, v = make(dev, b, h, hk, m, n, d, dtype, seed=n)
+    check(q, k, v, seed=1)
+    lens = torch.randint(0, n + 1, (b,), generator=gen, device=dev, dtype=torch.int32)
+    lens[0] = 0 if b > 1 else n
+    mask = torch.rand((b, n), generator=gen, device=dev) < 0.6
+    check(q, k, v, lens=lens, seed=2, grads=False)
+    out = check(q, k, v, lens=lens, mask=mask, seed=3, grads=False)
+    dead = ~(mask & (torch.arange(n, device=dev) < lens[:, None]))[:, None, :, None].expand(k.shape)
+    assert torch.equal(out, attend(q, k.masked_fill(dead, float("nan")), v.masked_fill(dead, float("inf")), None, lens, mask))
