@@ -185,22 +185,23 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     if (row0 < a.R) walk(std::true_type{});
     else walk(std::false_type{});
     rows.join_halves();
+    const XFwd& z = arguments_again<XFwd>();
     if (of > 1) {
-        if (row < a.R) {
-            const int64_t to = ((int64_t)split * a.plan.tail + (block - a.plan.full)) * kXRows + wave * 32 + (lane & 31);
-            if (half == 0) { a.pm[to] = rows.m; a.pl[to] = rows.l; }
-            float* p = a.part + to * a.D;
+        if (row < z.R) {
+            const int64_t to = ((int64_t)split * z.plan.tail + (block - z.plan.full)) * kXRows + wave * 32 + (lane & 31);
+            if (half == 0) { z.pm[to] = rows.m; z.pl[to] = rows.l; }
+            float* p = z.part + to * z.D;
 #pragma unroll
             for (int d = 0; d < rows.DTL; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int e = d * 32 + i * 8 + half * 4;
-                    if (e < a.D) *reinterpret_cast<v4f*>(p + e) = v4f{rows.acc[d][4 * i], rows.acc[d][4 * i + 1], rows.acc[d][4 * i + 2], rows.acc[d][4 * i + 3]};
+                    if (e < z.D) *reinterpret_cast<v4f*>(p + e) = v4f{rows.acc[d][4 * i], rows.acc[d][4 * i + 1], rows.acc[d][4 * i + 2], rows.acc[d][4 * i + 3]};
                 }
         }
         return;
     }
-    rows.finish(a, unit, b, hk, row, lane);
+    rows.finish(z, unit, b, hk, row, lane);
 }
 
 // Few keys (NT tiles at most): all of K and V stay in LDS, and a workgroup walks over the rows of its unit instead, each wave

@@ -162,21 +162,22 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
         step(t, std::integral_constant<int, 0>{});
         if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
     }
+    const XBwd& z = arguments_again<XBwd>();
     if (of > 1) {
-        if (row < a.R) {
-            float* p = a.part + (((int64_t)split * a.plan.tail + (block - a.plan.full)) * kXRows + wave * 32 + (lane & 31)) * a.D;
+        if (row < z.R) {
+            float* p = z.part + (((int64_t)split * z.plan.tail + (block - z.plan.full)) * kXRows + wave * 32 + (lane & 31)) * z.D;
 #pragma unroll
             for (int d = 0; d < DTL; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int e = d * 32 + i * 8 + half * 4;
-                    if (e < a.D) *reinterpret_cast<v4f*>(p + e) = v4f{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                    if (e < z.D) *reinterpret_cast<v4f*>(p + e) = v4f{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
                 }
         }
         return;
     }
-    const int g = row < a.R ? row / a.M : 0;
-    store_rows<DT, DP>(acc, a.scale, row < a.R ? a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (row - g * a.M) * a.dq.st : nullptr, a.D, lane);
+    const int g = row < z.R ? row / z.M : 0;
+    store_rows<DT, DP>(acc, z.scale, row < z.R ? z.dq.p + b * z.dq.sb + (int64_t)(hk * z.G + g) * z.dq.sh + (row - g * z.M) * z.dq.st : nullptr, z.D, lane);
 }
 
 // A head of more than 96 leaves no registers for V beside K and the two sums (two waves a SIMD have 256 each): V stays in
@@ -356,25 +357,26 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
 #pragma unroll
         for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
     }
+    const XBwd& z = arguments_again<XBwd>();
     if (of > 1) {
-        if (key < a.N) {
-            float* p = a.part + (((int64_t)split * a.plan.tail + (block - a.plan.full)) * kXRows + wave * 32 + (lane & 31)) * 2 * a.D;
+        if (key < z.N) {
+            float* p = z.part + (((int64_t)split * z.plan.tail + (block - z.plan.full)) * kXRows + wave * 32 + (lane & 31)) * 2 * z.D;
 #pragma unroll
             for (int d = 0; d < DTL; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int e = d * 32 + i * 8 + half * 4;
-                    if (e < a.D) {
+                    if (e < z.D) {
                         *reinterpret_cast<v4f*>(p + e) = v4f{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
-                        *reinterpret_cast<v4f*>(p + a.D + e) = v4f{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
+                        *reinterpret_cast<v4f*>(p + z.D + e) = v4f{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
                     }
                 }
         }
         return;
     }
-    const bool there = key < a.N;
-    store_rows<DT, DP>(dk, a.scale, there ? a.dk.p + b * a.dk.sb + hk * a.dk.sh + key * a.dk.st : nullptr, a.D, lane);
-    store_rows<DT, DP>(dv, 1.0f, there ? a.dv.p + b * a.dv.sb + hk * a.dv.sh + key * a.dv.st : nullptr, a.D, lane);
+    const bool there = key < z.N;
+    store_rows<DT, DP>(dk, z.scale, there ? z.dk.p + b * z.dk.sb + hk * z.dk.sh + key * z.dk.st : nullptr, z.D, lane);
+    store_rows<DT, DP>(dv, 1.0f, there ? z.dv.p + b * z.dv.sb + hk * z.dv.sh + key * z.dv.st : nullptr, z.D, lane);
 }
 
 // Adds the parts of dQ (WIDTH = 1) or of dK and dV (WIDTH = 2): one thread for 4 elements of a row.

@@ -124,6 +124,14 @@ struct Operands {
         for (int j = 0; j < CG; ++j) f[to][j] = lds_cols<DP>(tile, row0, group * CG + j, at);
     }
 };
+// The kernel's arguments (its first parameter) read again from memory: what is only needed behind a loop then takes no scalar
+// registers in it (they are spilled into vector registers otherwise, and read back in every turn).
+template <typename Args>
+__device__ __forceinline__ const Args& arguments_again() {
+    auto p = (const __attribute__((address_space(4))) Args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Args*)p;
+}
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
 // Waits until at most LEFT (below 16) of the loads and copies so far are under way.
