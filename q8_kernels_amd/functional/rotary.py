@@ -44,7 +44,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
         if not high_turns > low_turns:
             raise ValueError("rotary_frequencies: high_turns must be above low_turns")
         keep = ((trained_positions * f / (2 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
-        f = f * keep + f / stretch * (1.0 - keep)
+        f = torch.where(keep < 1.0, f / stretch + keep * (f - f / stretch), f)
         factor = 0.1 * math.log(stretch) + 1.0
     elif scaling not in (None, "ntk"):
         raise ValueError("rotary_frequencies: scaling %r" % (scaling,))

@@ -1,7 +1,8 @@
 """Multi-head attention over Q8Linear projections (reference: q8_kernels/modules/attention.py:15-106).
 
 attn_type 'q8_kernels' runs the fp8 flash-attention kernel, 'torch' (the reference's default) runs
-torch SDPA in `non_mm_precision`."""
+torch SDPA in `non_mm_precision`, '16bit' the differentiable 16-bit attention kernels (functional.cross_attention;
+`non_mm_precision` bfloat16 or float16): what fine-tunes adapters in the projections without torch's attention."""
 from typing import Optional
 
 import torch
@@ -129,6 +130,7 @@ class Attention(nn.Module):
             if isinstance(x, tuple):  # already (int8 codes, row scales)
                 return [layer(x[0], x[1], out_dtype=mm_out_dtype) for layer in layers]
             if (self.fuse_prologue and len(layers) > 1 and x.is_cuda and Q8F.fused.can_fuse_hadamard_quantize(x)
+                    and all(type(layer) is Q8Linear for layer in layers)     # (an adapter's layer needs the values)
                     and not (torch.is_grad_enabled() and x.requires_grad)):  # the shared codes carry no gradient
                 xq, xs = Q8F.fused.hadamard_quantize(x)
                 return [layer(xq, xs, out_dtype=mm_out_dtype) for layer in layers]
@@ -221,6 +223,13 @@ class Attention(nn.Module):
                 attention_mask = add[:, None, None, :].expand(-1, self.num_heads, -1, -1).to(query.dtype)
             hidden_states = torch.nn.functional.scaled_dot_product_attention(
                 query, key, value, attn_mask=attention_mask, dropout_p=0.0, is_causal=False)
+        elif attn_type == "16bit":
+            query, key, value = (t.to(non_mm_precision) for t in (query, key, value))
+            # [batch] valid lengths, or a [batch, keys] mask whose keys with a zero do not count (holes stay holes)
+            lens, mask = attention_mask, None
+            if attention_mask is not None:
+                lens, mask = (None, attention_mask != 0) if attention_mask.ndim > 1 else (attention_mask.to(torch.int32), None)
+            hidden_states = Q8F.cross_attention.cross_attention(query, key, value, kv_lens=lens, key_mask=mask)
         else:
             raise ValueError(f"Invalid attention type: {attn_type}")
 
