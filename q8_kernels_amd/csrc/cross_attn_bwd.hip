@@ -1,6 +1,8 @@
 // 16-bit cross attention, backward. With P = exp2(c S - lse) formed again from Q, K and the forward's log-sums:
 //   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta),  delta = rowsum(dO O),  dQ = scale dS K,  dK = scale dS^T Q
 //
+// Up to 128 keys (or 256, with many rows) a kernel of its own holds all of them, see there. Otherwise:
+//
 // Two kernels, so that every sum has one owner and a fixed order (no atomics), at the price of forming S and dP twice (seven
 // products instead of five; partial sums of dQ per key tile would move more time's worth of bytes than the two products
 // cost). The first owns 128 query rows and walks over the keys: it forms delta, writes it for the second, and dQ. The second
@@ -11,12 +13,19 @@
 // and V are zeros; in the second a key is a column of every product, whose garbage stays in its column, and its gradient is
 // written as zeros. A row without keys has lse = +infinity, which makes its P zero everywhere.
 //
+// delta is formed from the rounded O, whose error is that of every score's gradient in the row: with many keys it is lost
+// beside the rounding of dS, but with 2 it leaves dQ 2.3 roundings off, with 8 still 1.6 (from the root of 2 that dS and the
+// result cost). So up to kXExact keys, which one wave or one score tile holds, the dS of a row are summed before they are
+// rounded: the true ones add up to zero, so the sum is that error, and it is taken off.
+//
 // Few workgroups: the walk is divided over several of them, their fp32 sums are added by a third kernel in order.
 #include "cross_attn_common.h"
 
 #include <type_traits>
 
 namespace q8 {
+
+constexpr int kXExact = 32;
 
 struct XBwd {
     XTensor q, k, v, o, g;
@@ -55,6 +64,7 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
     kv.copies.wave = wave;
     const int tiles = (kv.len + kXTile - 1) / kXTile, per = (tiles + of - 1) / of;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+    const bool few = kv.len > 0 && kv.len <= kXExact;
 
     v4u qf[KS], gf[KS];
     float delta = 0.f, lse = __builtin_inff();
@@ -81,7 +91,7 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
         if (ok) {
             const int64_t at = (int64_t)unit * a.R + row;
             lse = a.lse[at];
-            if (split == 0 && half == 0) a.delta[at] = delta;
+            if (split == 0 && half == 0 && !few) a.delta[at] = delta;
         }
     }
     if (t0 < t1) kv.first(t0, k0, v0, bias0);
@@ -137,7 +147,21 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
             }
             // (2 RN groups so far: the columns are in place 0)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse));
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse));
+            if constexpr (BUF == 0) {
+                if (u == 0 && few) {  // all keys are here: what their dS adds up to is the error of delta
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum += dp[i] * s[i];
+                    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+                    sum = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dp[i] -= sum;
+                    if (const XBwd& z = arguments_again<XBwd>(); row < z.R && half == 0) z.delta[(int64_t)unit * z.R + row] = delta + sum;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
             int w = 0;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -379,6 +403,247 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     store_rows<DT, DP>(dv, 1.0f, there ? z.dv.p + b * z.dv.sb + hk * z.dv.sh + key * z.dv.st : nullptr, z.D, lane);
 }
 
+// Few keys (32 W of them at most) and many rows: all gradients in one pass over the rows, five products instead of seven, and
+// Q, dO and O read once. A wave owns 32 keys, as above; dS of a tile of 64 rows goes to LDS as [key][row], from where (turned
+// while it is read, like K) it is an operand of dQ^T = K^T dS^T. A wave forms one 32 x 32 block of dQ^T over a part of the keys;
+// where more waves share a block, the others' sums go through LDS to the first. delta comes from the same tile's O and dO.
+// A workgroup walks over a part of its unit's tiles; the parts' dK and dV are added by the kernel below. D up to 64: beyond, the
+// registers and LDS of one workgroup leave no second wave on a SIMD. bf16, 2 x 32 heads of 64, 6144 rows, 256 keys: 100 us and 7
+// for the parts (200 MB at 2.0 TB/s; 40 MFMA of a wave and tile would take 30 us, exp2 and the roundings of P and dS about as
+// long, and between the two barriers of a tile they overlap only in part).
+template <int DT, int DP, int W>
+__global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd a, int parts) {
+    constexpr int KS = DP / 16, DTL = DP / 32, TR = kXTile, ELEMS = TR * DP, CPR = DP / 8;
+    constexpr int NB = 2 * DTL, KG = W / NB, STEPS = W * 2 / KG;  // blocks of dQ^T, waves that share one, 16-key steps of each
+    constexpr int CHUNKS = TR * CPR / (W * 64) > 0 ? TR * CPR / (W * 64) : 1;  // of dO and O, for delta
+    __shared__ __align__(16) uint16_t q0[ELEMS], q1[ELEMS], g0[ELEMS], g1[ELEMS], kt[W * 32 * DP], ds[W * 32 * TR];
+    __shared__ __align__(16) float lse0[TR], lse1[TR], delta0[TR], delta1[TR];  // -lse and -delta of the tile's rows
+    __shared__ __align__(16) float sums[KG > 1 ? (KG - 1) * NB * 1024 : 4];
+    const int unit = blockIdx.x / parts, part = blockIdx.x - unit * parts;
+    const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int key = wave * 32 + (lane & 31);
+    const int len = a.keys.length(b);
+    const uint8_t* mask = a.keys.row(b);
+    const bool counts = key < len && (mask == nullptr || mask[key]);
+    const uint32_t keep = counts ? ~0u : 0u;
+    const bool idle = __builtin_amdgcn_ballot_w64(counts) == 0;  // no key of this wave counts
+    const int head_tiles = (a.M + TR - 1) / TR, tiles = a.G * head_tiles, per = (tiles + parts - 1) / parts;
+    const int t0 = part * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+
+    v4u kf[KS], vf[KS];
+    {
+        const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh + key * a.k.st + half * 8;
+        const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh + key * a.v.st + half * 8;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const bool in = counts && s * 16 + half * 8 < a.D;
+            kf[s] = in ? *reinterpret_cast<const v4u*>(kp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            vf[s] = in ? *reinterpret_cast<const v4u*>(vp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            *reinterpret_cast<v4u*>(kt + wave * 32 * DP + tile_at<DP>(lane & 31, 2 * s + half)) = kf[s];
+        }
+    }
+    if (idle) {  // its part of dS stays zero
+        for (int i = lane; i < 32 * TR / 8; i += 64) *reinterpret_cast<v4u*>(ds + wave * 32 * TR + i * 8) = v4u{0u, 0u, 0u, 0u};
+    }
+
+    Copies<DP, TR, W> copies;
+    copies.wave = wave;
+    copies.D = a.D;
+    int rows = 0;
+    float row_lse = 0.f;
+    v4u dor[CHUNKS], orr[CHUNKS];
+    const uint16_t *qp = a.q.p + b * a.q.sb + (int64_t)hk * a.G * a.q.sh, *gp = a.g.p + b * a.g.sb + (int64_t)hk * a.G * a.g.sh;
+    const uint16_t* op = a.o.p + b * a.o.sb + (int64_t)hk * a.G * a.o.sh;
+    const int chunk = (int)threadIdx.x % CPR, crow = (int)threadIdx.x / CPR;  // of delta: rows crow + k W 64 / CPR
+    // the tile that is next (t past the end: empty)
+    auto aim = [&](int t) {
+        const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
+        rows = t < t1 ? a.M - m : 0;
+        if (rows > TR) rows = TR;
+        const int last = rows - 1;
+        const int n = (int)threadIdx.x & (TR - 1);
+        row_lse = a.lse[(int64_t)unit * a.R + (rows ? g * a.M + m + (n < rows ? n : last) : 0)];
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            const int r = crow + k * (W * 64 / CPR), i = m + (r < last ? r : last);
+            const bool in = rows > 0 && chunk * 8 < a.D;
+            dor[k] = in ? *reinterpret_cast<const v4u*>(gp + g * a.g.sh + i * a.g.st + chunk * 8) : v4u{0u, 0u, 0u, 0u};
+            orr[k] = in ? *reinterpret_cast<const v4u*>(op + g * a.o.sh + i * a.o.st + chunk * 8) : v4u{0u, 0u, 0u, 0u};
+        }
+    };
+    auto tile_of = [&](const uint16_t* p, const XTensor& x, int t) {
+        const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
+        return XTile(p + g * x.sh + m * x.st, x.st, rows, a.D);
+    };
+    auto finish = [&](float* lt, float* dt) {
+        wait_loads();
+        if (threadIdx.x < TR) lt[threadIdx.x] = (int)threadIdx.x < rows ? -row_lse : -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            float d = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                d += unpack<DT>(dor[k][i] & 0xffffu) * unpack<DT>(orr[k][i] & 0xffffu);
+                d += unpack<DT>(dor[k][i] >> 16) * unpack<DT>(orr[k][i] >> 16);
+            }
+            d = group_sum<CPR>(d);
+            const int r = crow + k * (W * 64 / CPR);
+            if (chunk == 0 && r < TR) dt[r] = r < rows ? -d : 0.f;
+        }
+    };
+
+    v16f dk[DTL], dv[DTL];
+#pragma unroll
+    for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
+    if (t0 < t1) {
+        aim(t0);
+        copies.group(0, 1, tile_of(qp, a.q, t0), tile_of(gp, a.g, t0), 0, q0, g0);
+        finish(lse0, delta0);
+    }
+    wait_loads();
+    __syncthreads();
+
+    LaneOffsets<DP> at(lane);
+    LaneOffsets<TR> ds_at(lane);
+    Operands<DP, 4> ops;
+    static_assert(ops.RN == 1 && ops.CN == 1, "one group each");
+    auto step = [&](int t, auto buffer, auto exact) {
+        constexpr int BUF = decltype(buffer)::value;
+        at.fresh();
+        const uint16_t *ql = BUF ? q1 : q0, *gl = BUF ? g1 : g0;
+        const float *lt = BUF ? lse1 : lse0, *dt = BUF ? delta1 : delta0;
+        uint16_t *qnext = BUF ? q0 : q1, *gnext = BUF ? g0 : g1;
+        const int g = t / head_tiles, m = (t - g * head_tiles) * TR, here = rows;
+        aim(t + 1);
+        copies.group(0, 1, tile_of(qp, a.q, t + 1), tile_of(gp, a.g, t + 1), 0, qnext, gnext);
+        if (!idle) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                v16f s = splat16(0.f), dp = bias16(dt, u, half);
+                if (u == 0) ops.rows(0, ql, 0, 0, at);
+                ops.rows(1, gl, u * 32, 0, at);
+                fence();
+#pragma unroll
+                for (int j = 0; j < KS; ++j) s = mfma16<DT>(ops.f[0][j], kf[j], s);
+                fence();
+                ops.cols(0, gl, u * 32, 0, at);
+                fence();
+#pragma unroll
+                for (int j = 0; j < KS; ++j) dp = mfma16<DT>(ops.f[1][j], vf[j], dp);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // P, beside them
+                    const v4f x = *reinterpret_cast<const v4f*>(&lt[u * 32 + i * 8 + half * 4]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[i * 4 + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * 4 + j], a.c, x[j]));
+                }
+                fence();
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const v4u p = pack_step<DT>(s, k);
+                    if (k == 0) ops.cols(1, gl, u * 32 + 16, 0, at);
+                    else ops.cols(0, ql, u * 32, 0, at);
+                    fence();
+#pragma unroll
+                    for (int d = 0; d < DTL; ++d) dv[d] = mfma16<DT>(ops.f[k][d], p, dv[d]);
+                    if (k == 0) {  // dS, beside them
+                        if constexpr (exact) {  // all keys are in this wave: what their dS adds up to is the error of delta
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                dp[i] -= group_sum<32>(__uint_as_float(__float_as_uint(dp[i] * s[i]) & keep));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+                    }
+                    fence();
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    v4u p = pack_step<DT>(dp, k);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[i] &= keep;  // a key that does not count may hold anything here
+                    // rows u * 32 + 8 (2 k) + 4 half .. + 3 and the 4 rows 8 further, of this lane's key
+                    *reinterpret_cast<v2i*>(ds + wave * 32 * TR + tile_at<TR>(lane & 31, u * 4 + 2 * k) + half * 4) = v2i{(int)p[0], (int)p[1]};
+                    *reinterpret_cast<v2i*>(ds + wave * 32 * TR + tile_at<TR>(lane & 31, u * 4 + 2 * k + 1) + half * 4) = v2i{(int)p[2], (int)p[3]};
+                    if (k == 0) ops.cols(1, ql, u * 32 + 16, 0, at);
+                    else if (u == 0) ops.rows(0, ql, 32, 0, at);
+                    fence();
+#pragma unroll
+                    for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(ops.f[k][d], p, dk[d]);
+                    fence();
+                }
+            }
+        }
+        barrier();
+        // dQ^T: this wave's block of rows and elements, over its part of the keys
+        const int block = wave % NB, kg = wave / NB, rb = block & 1, db = block >> 1;
+        v16f dq = splat16(0.f);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            const int key0 = (kg * STEPS + i) * 16;
+            dq = mfma16<DT>(lds_cols<DP>(kt, key0, db, at), lds_cols<TR>(ds, key0, rb, ds_at), dq);
+        }
+        if constexpr (KG > 1) {
+            if (kg > 0) {
+                float* to = sums + ((kg - 1) * NB + block) * 1024 + lane * 4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<v4f*>(to + i * 256) = v4f{dq[4 * i], dq[4 * i + 1], dq[4 * i + 2], dq[4 * i + 3]};
+            }
+            barrier();
+            if (kg == 0) {
+#pragma unroll
+                for (int o = 0; o < KG - 1; ++o) {
+                    const float* from = sums + (o * NB + block) * 1024 + lane * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const v4f x = *reinterpret_cast<const v4f*>(from + i * 256);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) dq[4 * i + j] += x[j];
+                    }
+                }
+            }
+        }
+        if (kg == 0) {
+            const int r = rb * 32 + (lane & 31);
+            uint16_t* p = a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (int64_t)(m + r) * a.dq.st + db * 32;
+            store_rows<DT, 32>({dq}, a.scale, r < here ? p : nullptr, a.D - db * 32, lane);
+        }
+        finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
+        __syncthreads();
+    };
+    auto walk = [&](auto exact) {
+        for (int t = t0; t < t1; t += 2) {
+            step(t, std::integral_constant<int, 0>{}, exact);
+            if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{}, exact);
+        }
+    };
+    if (len <= kXExact) walk(std::true_type{});
+    else walk(std::false_type{});
+    if (!counts) {  // a key that does not count has no gradient, whatever its column holds
+#pragma unroll
+        for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
+    }
+    const XBwd& z = arguments_again<XBwd>();
+    if (key >= z.N) return;
+    if (parts > 1) {
+        const int kb = wave / kXWaves;  // the block of 128 keys that the kernel below counts in
+        float* p = z.part + (((int64_t)part * z.plan.tail + (unsigned)(unit * z.blocks + kb)) * kXRows + (wave & 3) * 32 + (lane & 31)) * 2 * z.D;
+#pragma unroll
+        for (int d = 0; d < DTL; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = d * 32 + i * 8 + half * 4;
+                if (e < z.D) {
+                    *reinterpret_cast<v4f*>(p + e) = v4f{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
+                    *reinterpret_cast<v4f*>(p + z.D + e) = v4f{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
+                }
+            }
+        return;
+    }
+    store_rows<DT, DP>(dk, z.scale, z.dk.p + b * z.dk.sb + hk * z.dk.sh + key * z.dk.st, z.D, lane);
+    store_rows<DT, DP>(dv, 1.0f, z.dv.p + b * z.dv.sb + hk * z.dv.sh + key * z.dv.st, z.D, lane);
+}
+
 // Adds the parts of dQ (WIDTH = 1) or of dK and dV (WIDTH = 2): one thread for 4 elements of a row.
 template <int DT, int WIDTH>
 __global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
@@ -412,6 +677,7 @@ __global__ __launch_bounds__(256) void cross_attn_add_kernel(XBwd a) {
 
 struct XPlan {
     int64_t units, rows, dq_blocks, kv_blocks, parts;  // blocks of a unit; floats of partial results
+    int few;  // waves of the kernel for few keys, 0: not taken
     XSchedule dq, kv;
 };
 static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
@@ -420,14 +686,29 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     p.rows = (int64_t)(H / Hkv) * M;
     p.dq_blocks = (p.rows + kXRows - 1) / kXRows;
     p.kv_blocks = ((int64_t)N + kXRows - 1) / kXRows;
+    const int64_t tiles = (int64_t)(H / Hkv) * (((int64_t)M + kXTile - 1) / kXTile);
+    // The kernel for few keys, a workgroup for up to four tiles: one of 8 waves on a CU, or two of 4 (LDS). bf16 times, this kernel
+    // against the other two (B x H x M x N x D): 2 x 32 x 6144 x 256 x 64 115 against 146 us, x 128 65 against 97, 32 x 2048 x 128
+    // 25.4 against 33.5, 16 x 1024 x 64 18.3 against 19.2, 16 x 32 x 256 x 128 28 against 45. With 129 to 256 keys it takes 1024
+    // tiles to be faster: 8 x 8192 x 256 38 against 48, 16 x 2048 x 256 (512 tiles) 32.2 against 31.5, 8 x 512 x 256 24.6 against 22.5.
+    const int64_t at_once = N > kXRows ? 256 : 512;
+    if (D <= 64 && p.units > 0 && M > 0 && N > 0 && (N <= kXRows || (N <= 2 * kXRows && p.units * tiles >= 4 * at_once)) && p.units <= 0x3fffffff) {
+        const int64_t most = (tiles + 3) / 4, want = (at_once + p.units - 1) / p.units;
+        p.few = N > kXRows ? 8 : 4;
+        p.kv.full = 0;
+        p.kv.tail = (unsigned)(p.units * p.kv_blocks);
+        p.kv.splits = (int)(want < most ? want : most);
+        p.parts = p.kv.parts() * kXRows * 2 * D;
+        return p;
+    }
     // workgroups that run at once on the 256 CUs, by the registers of a lane
     p.dq = schedule(p.units * p.dq_blocks, N, D <= 32 ? 1024 : D <= 64 ? 768 : 512);
-    p.kv = schedule(p.units * p.kv_blocks, (int64_t)(H / Hkv) * ((M + kXTile - 1) / kXTile) * kXTile, D <= 32 ? 1024 : 512);
+    p.kv = schedule(p.units * p.kv_blocks, tiles * kXTile, D <= 32 ? 1024 : 512);
     const int64_t dq = p.dq.parts() * kXRows * D, kv = p.kv.parts() * kXRows * 2 * D;
     p.parts = dq > kv ? dq : kv;  // one after the other in the same place
     return p;
 }
-static int64_t delta_floats(const XPlan& p) { return (p.units * p.rows + 3) / 4 * 4; }
+static int64_t delta_floats(const XPlan& p) { return p.few ? 0 : (p.units * p.rows + 3) / 4 * 4; }
 
 }  // namespace q8
 
@@ -507,7 +788,24 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
         case 96: NAME<DT, 96><<<grid, kXThreads, 0, st>>>(a); break;          \
         default: NAME<DT, 128><<<grid, kXThreads, 0, st>>>(a);                \
     }
-    if (M) {
+    if (p.few) {
+        a.blocks = (int)p.kv_blocks;
+        a.plan = p.kv;
+        const unsigned grid = (unsigned)(p.units * p.kv.splits);
+#define X_FEW(DT, W)                                                                                                           \
+    do {                                                                                                                       \
+        if (D <= 32) cross_attn_bwd_few_keys_kernel<DT, 32, W><<<grid, W * 64, 0, st>>>(a, p.kv.splits);                       \
+        else cross_attn_bwd_few_keys_kernel<DT, 64, W><<<grid, W * 64, 0, st>>>(a, p.kv.splits);                               \
+    } while (0)
+        if (p.few == 4) {
+            if (dt == Q8_BF16) X_FEW(Q8_BF16, 4); else X_FEW(Q8_F16, 4);
+        } else {
+            if (dt == Q8_BF16) X_FEW(Q8_BF16, 8); else X_FEW(Q8_F16, 8);
+        }
+#undef X_FEW
+        if (int e = launch_status(who)) return e;
+    }
+    if (M && !p.few) {
         a.blocks = (int)p.dq_blocks;
         a.plan = p.dq;
         const unsigned grid = a.plan.grid();
@@ -523,9 +821,11 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
     if (N) {
         a.blocks = (int)p.kv_blocks;
         a.plan = p.kv;
-        const unsigned grid = a.plan.grid();
-        if (dt == Q8_BF16) { X_BWD(cross_attn_dkdv_kernel, Q8_BF16) } else { X_BWD(cross_attn_dkdv_kernel, Q8_F16) }
-        if (int e = launch_status(who)) return e;
+        if (!p.few) {
+            const unsigned grid = a.plan.grid();
+            if (dt == Q8_BF16) { X_BWD(cross_attn_dkdv_kernel, Q8_BF16) } else { X_BWD(cross_attn_dkdv_kernel, Q8_F16) }
+            if (int e = launch_status(who)) return e;
+        }
         if (a.plan.parts()) {
             const unsigned n = a.plan.tail * (D / 4);
             if (dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 2><<<n, 256, 0, st>>>(a);

@@ -141,6 +141,7 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70
 // A barrier that leaves copies under way (__syncthreads waits for all of them): LDS accesses before it are done, and the
 // compiler moves none across it.
 __device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -171,11 +172,11 @@ struct XTile {
         bytes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, n > 0 ? (int)((unsigned)(n - 1) * st2 + (unsigned)D * 2u) : 0, 0x00020000);
     }
 };
-template <int DP, int TR = kXTile>
+template <int DP, int TR = kXTile, int W = kXWaves>
 struct Copies {
-    static constexpr int CPR = DP / 8, ALONE = TR * CPR / 64, COPIES = 2 * ALONE / kXWaves;
+    static constexpr int CPR = DP / 8, ALONE = TR * CPR / 64, COPIES = 2 * ALONE / W;
     static constexpr bool EVEN = 64 % CPR == 0;  // a copy is whole rows
-    static_assert(2 * ALONE % kXWaves == 0, "whole copies for every wave");
+    static_assert(2 * ALONE % W == 0, "whole copies for every wave");
     int wave, D;
     // copy idx (0 .. ALONE - 1) of a tile; rows with a bit in `dead` become zeros
     __device__ __forceinline__ void one(const XTile& x, int idx, uint64_t dead, uint16_t* tile) const {
@@ -197,7 +198,7 @@ struct Copies {
     }
     // share i of the wave's COPIES
     __device__ __forceinline__ void share(int i, const XTile& x, const XTile& y, uint64_t dead, uint16_t* xt, uint16_t* yt) const {
-        const int idx = wave + i * kXWaves;
+        const int idx = wave + i * W;
         if (idx < ALONE) one(x, idx, dead, xt);
         else one(y, idx - ALONE, dead, yt);
     }

@@ -7,7 +7,9 @@ the row sum) + N 2^-24; the probabilities entering a product round by u. With p 
   o:  (u + 2 es) sum_j p |v_j| + t sum_j |v_j| + half a step of o                           =: eo
   dv: (u + 2 es) sum_i p |g_i| + t sum_i |g_i| + half a step
   ds: |ds| (u + 2 es) + p (D 2^-23 sum|g v| + sum_d |g| eo + D 2^-23 sum|g o|) + t          =: eds
-  dq: scale (sum_j eds |k_j| + N 2^-24 sum_j |ds k_j|) + half a step;  dk with the sums over the rows"""
+  dq: scale (sum_j eds |k_j| + N 2^-24 sum_j |ds k_j|) + half a step;  dk with the sums over the rows
+Where at most 32 keys can count, delta is corrected by what the ds of its row add up to, which leaves the errors of that sum,
+sum_j (es |ds_j| + p_j D 2^-23 sum|g v_j|), and 2 es of the correction itself, in the place of sum_d |g| eo + D 2^-23 sum|g o|."""
 import pytest
 import torch
 
@@ -18,7 +20,7 @@ attend = Q8F.cross_attention.cross_attention
 TYPES = [torch.bfloat16, torch.float16]
 
 
-def reference(q, k, v, g, scale, valid):
+def reference(q, k, v, g, scale, valid, exact=False):
     """((o, dq, dk, dv), their tolerances) in float64; valid bool [B, N]"""
     b, h, m, d = q.shape
     hk, n = k.shape[1], k.shape[2]
@@ -43,7 +45,11 @@ def reference(q, k, v, g, scale, valid):
     edv = (p * (u + es)).transpose(2, 3) @ g6.abs() + t * g6.abs().sum(2, keepdim=True)
     dp = g6 @ v6.transpose(2, 3)
     ds = p * (dp - (g6 * o).sum(-1, keepdim=True))
-    eds = ds.abs() * (u + es) + p * (d * 2.0 ** -23 * (g6.abs() @ v6.abs().transpose(2, 3)) + (g6.abs() * (eo + d * 2.0 ** -23 * o.abs())).sum(-1, keepdim=True)) + t
+    edp = d * 2.0 ** -23 * (g6.abs() @ v6.abs().transpose(2, 3))
+    edelta = (g6.abs() * (eo + d * 2.0 ** -23 * o.abs())).sum(-1, keepdim=True)
+    if exact:
+        edelta = (es * ds.abs() + p * edp).sum(-1, keepdim=True) + edelta * (es * (p > 0)).amax(-1, keepdim=True)
+    eds = ds.abs() * (u + es) + p * (edp + edelta) + t
     dq, dk = scale * (ds @ k6), scale * (ds.transpose(2, 3) @ q6)
     edq = scale * (eds @ k6.abs() + n * 2.0 ** -24 * (ds.abs() @ k6.abs()))
     edk = scale * (eds.transpose(2, 3) @ q6.abs() + q6.shape[2] * 2.0 ** -24 * (ds.abs().transpose(2, 3) @ q6.abs()))
@@ -59,7 +65,7 @@ def close(got, want, tol, what):
     assert (off <= tol).all(), "%s: off by %g where %g is allowed" % (what, (off - tol).max() + tol[off > tol].min(), tol[off > tol].min())
 
 
-def check(q, k, v, scale=None, lens=None, mask=None, seed=0, grads=True):
+def check(q, k, v, scale=None, lens=None, mask=None, seed=0, grads=True, exact=False):
     b, n = k.shape[0], k.shape[2]
     valid = torch.ones(b, n, dtype=torch.bool, device=q.device)
     if lens is not None:
@@ -68,7 +74,7 @@ def check(q, k, v, scale=None, lens=None, mask=None, seed=0, grads=True):
         valid = valid & mask
     gen = torch.Generator(device=q.device).manual_seed(seed)
     g = torch.randn(q.shape, generator=gen, device=q.device).to(q.dtype)
-    want, tol = reference(q, k, v, g, scale if scale is not None else q.shape[-1] ** -0.5, valid)
+    want, tol = reference(q, k, v, g, scale if scale is not None else q.shape[-1] ** -0.5, valid, exact)
     out = attend(q, k, v, scale, lens, mask)
     assert out.dtype == q.dtype
     close(out, want[0], tol[0], "o")
@@ -343,3 +349,13 @@ def test_few_keys_and_many_rows(dev, b, h, hk, m, n, d, dtype):
     out = check(q, k, v, lens=lens, mask=mask, seed=3, grads=False)
     dead = ~(mask & (torch.arange(n, device=dev) < lens[:, None]))[:, None, :, None].expand(k.shape)
     assert torch.equal(out, attend(q, k.masked_fill(dead, float("nan")), v.masked_fill(dead, float("inf")), None, lens, mask))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,n,lens", [(64, 2, None), (64, 32, None), (24, 100, [1, 2, 32]), (64, 200, [5, 0, 31]), (64, 700, [2, 3, 32]), (128, 2, None), (128, 8, None),
+                                      (96, 65, [7, 32, 1]), (128, 900, [16, 2, 9])])
+def test_gradients_of_few_counted_keys(dev, dtype, d, n, lens):
+    q, k, v = make(dev, 3, 4, 2, 133, n, d, dtype, seed=n)
+    lens = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev)
+    check(q, k, v, lens=lens, seed=5, exact=True)
+    check(q, k, v, lens=lens, mask=torch.arange(n, device=dev).expand(3, n) % 3 != 1, seed=6, exact=True)
