@@ -368,7 +368,7 @@ inline int x_sizes(const char* who, int dt, int64_t B, int H, int Hkv, int M, in
     if (B < 0 || H < 1 || Hkv < 1 || M < 0 || N < 0) return fail(Q8_ERR_SHAPE, "%s: B %lld, heads %d and %d, M %d, N %d", who, (long long)B, H, Hkv, M, N);
     if (H % Hkv) return fail(Q8_ERR_SHAPE, "%s: %d query heads on %d key heads (a multiple is needed)", who, H, Hkv);
     if (D < 8 || D > 128 || D % 8) return fail(Q8_ERR_SHAPE, "%s: head dim %d (a multiple of 8 up to 128)", who, D);
-    if (!(scale > 0.f) || scale > 3e38f) return fail(Q8_ERR_SHAPE, "%s: softmax scale %g (positive and finite)", who, (double)scale);
+    if (!(scale > 0.f) || scale > 1e38f) return fail(Q8_ERR_SHAPE, "%s: softmax scale %g (positive and finite)", who, (double)scale);
     // rows, units and the fp32 scratch stay in 32-bit counts
     if ((int64_t)(H / Hkv) * M > 0x3fffffff || N > 0x3fffffff || (B && (int64_t)Hkv > 0x3fffffff / B) ||
         (B && M && (int64_t)H > ((int64_t)1 << 40) / B / M))

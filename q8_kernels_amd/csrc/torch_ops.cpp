@@ -7,7 +7,9 @@
 // Host code only, compiled against torch; the kernels are reached through the C ABI (include/q8_hip.h).
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -47,6 +49,22 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 q8_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void require_gpu(const Tensor& t, const char* name) { TORCH_CHECK(t.is_cuda(), name, " must be a CUDA (HIP) tensor"); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// A leaf whose eager graph still lives keeps the stream that graph was built on for its gradients. If that is the default
+// stream, a backward captured on another one would make it wait inside the capture, which ends the process from the engine's
+// thread: refused here, before anything is recorded.
+void no_eager_graph(const Tensor& x, std::initializer_list<const Tensor*> inputs, const char* who) {
+    const hipStream_t stream = c10::hip::getCurrentHIPStream(x.device().index()).stream();
+    if (stream == nullptr) return;  // the default stream is never captured
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    for (const Tensor* t : inputs) {
+        if (!wants_grad(*t) || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto own = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!own || own->id() != 0, who, ": an eager graph of the same leaf still lives on the default stream; drop its results before capturing a backward");
+    }
+}
 
 // gradients of gradients are not formed: where the caller records this backward, using its results again raises
 variable_list once(variable_list grads) {
@@ -146,7 +164,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
     const Tensor w = or_none(weight), b = or_none(bias);
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) return LayerNorm::apply(x, given(w), given(b), eps);
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) {
+        require_gpu(x, "x");
+        no_eager_graph(x, {&x, &w, &b}, "layer_norm");
+        return LayerNorm::apply(x, given(w), given(b), eps);
+    }
     return norm_forward(x, w, b, eps, false)[0];
 }
 
@@ -232,7 +254,10 @@ struct Rotary : torch::autograd::Function<Rotary> {
 
 std::array<Tensor, 2> apply_rotary(const Tensor& q, const OptTensor& key, const OptTensor& positions, const Tensor& inv_freq, bool half, double factor) {
     const Tensor k = or_none(key), p = or_none(positions);
+    TORCH_CHECK(!at::GradMode::is_enabled() || !inv_freq.requires_grad(), "rotary: no gradient of inv_freq is formed");
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k))) {
+        require_gpu(q, "q and k");
+        no_eager_graph(q, {&q, &k}, "rotary");
         auto out = Rotary::apply(q, given(k), given(p), inv_freq, half, factor);
         return {out[0], out.size() > 1 ? out[1] : Tensor()};
     }
@@ -339,7 +364,11 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, std::o
                        const OptTensor& key_mask) {
     const double scale = softmax_scale.has_value() ? *softmax_scale : q.dim() && q.size(-1) ? 1.0 / std::sqrt((double)q.size(-1)) : 1.0;
     const Tensor lens = or_none(kv_lens), mask = or_none(key_mask);
-    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v))) return CrossAttention::apply(q, k, v, scale, given(lens), given(mask));
+    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v))) {
+        require_gpu(q, "q, k and v");
+        no_eager_graph(q, {&q, &k, &v}, "cross_attention");
+        return CrossAttention::apply(q, k, v, scale, given(lens), given(mask));
+    }
     return attn_forward(q, k, v, scale, lens, mask, false)[0];
 }
 

@@ -169,3 +169,63 @@ def test_attention_module_runs_the_16_bit_kernels(dev, monkeypatch):
     assert torch.nn.functional.cosine_similarity(a.float().flatten(), t.float().flatten(), dim=0) > 0.999
     with pytest.raises(ValueError):
         attn(x, attn_type="other", mm_out_dtype=BF16)
+
+
+def leaves_and_step(dev):
+    """The three operators in a row, on leaves of their own, and their gradients."""
+    gen = torch.Generator(device=dev).manual_seed(3)
+    rnd = lambda *s: torch.randn(s, generator=gen, device=dev)  # noqa: E731
+    x, q = rnd(2, 70, 256).to(BF16), rnd(2, 4, 70, 64).to(BF16)
+    w, v = 1 + 0.1 * rnd(256), rnd(2, 4, 70, 64).to(BF16)
+    grad, f = rnd(2, 4, 70, 64).to(BF16), rotary_frequencies(64)[0].to(dev)
+
+    def step(x, q, v, w):
+        k = Q8F.layer_norm.layer_norm(x, w).view(2, 70, 4, 64).transpose(1, 2)
+        rq, rk = apply_rotary(q, k, None, f)
+        return Q8F.cross_attention.cross_attention(rq, rk, v)
+
+    return [t.requires_grad_() for t in (x, q, v, w)], grad, step
+
+
+@pytest.mark.gpu
+def test_captured_training_step(dev):
+    leaves, grad, step = leaves_and_step(dev)
+
+    def eager():
+        o = step(*leaves)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, grad)
+
+    eager()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = step(*leaves)
+        out = (o.detach(),) + torch.autograd.grad(o, leaves, grad)
+    del o
+    for turn in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.mul_(0.75).add_(0.01 * turn)
+        graph.replay()
+        want = eager()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+def test_capture_beside_an_eager_graph_is_refused(dev):
+    (x, q, v, w), _, step = leaves_and_step(dev)
+    f = rotary_frequencies(64)[0].to(dev)
+    alive = step(x, q, v, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: Q8F.layer_norm.layer_norm(x), lambda: Q8F.layer_norm.layer_norm(x.detach(), w), lambda: apply_rotary(q, None, None, f),
+                     lambda: Q8F.cross_attention.cross_attention(q.detach(), q.detach(), v)):
+            with pytest.raises(RuntimeError, match="eager graph"):
+                call()
+        with torch.no_grad():
+            o = step(x, q, v, w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, alive.detach())
+    with pytest.raises(RuntimeError, match="inv_freq"):
+        apply_rotary(q, None, None, f.clone().requires_grad_())
