@@ -692,7 +692,7 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     // 25.4 against 33.5, 16 x 1024 x 64 18.3 against 19.2, 16 x 32 x 256 x 128 28 against 45. With 129 to 256 keys it takes 1024
     // tiles to be faster: 8 x 8192 x 256 38 against 48, 16 x 2048 x 256 (512 tiles) 32.2 against 31.5, 8 x 512 x 256 24.6 against 22.5.
     const int64_t at_once = N > kXRows ? 256 : 512;
-    if (D <= 64 && p.units > 0 && M > 0 && N > 0 && (N <= kXRows || (N <= 2 * kXRows && p.units * tiles >= 4 * at_once)) && p.units <= 0x3fffffff) {
+    if (D <= 64 && p.units > 0 && M > 0 && N > 0 && (N <= kXRows || (N <= 2 * kXRows && p.units * tiles >= 4 * at_once)) && p.units <= kXMostBlocks / 2) {
         const int64_t most = (tiles + 3) / 4, want = (at_once + p.units - 1) / p.units;
         p.few = N > kXRows ? 8 : 4;
         p.kv.full = 0;
@@ -750,7 +750,7 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
     if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
     if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
     const XPlan p = plan(B, H, Hkv, M, N, D);
-    if (p.units * p.dq_blocks > 0x7ffff000 || p.units * p.kv_blocks > 0x7ffff000) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
+    if (p.units * p.dq_blocks > kXMostBlocks || p.units * p.kv_blocks > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
     XBwd a{};
     auto in = [&](const void* x, const int64_t* s, int n) {
         const int64_t* t = n ? s : none;

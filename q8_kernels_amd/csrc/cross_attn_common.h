@@ -24,6 +24,7 @@
 namespace q8 {
 
 constexpr int kXThreads = 256, kXWaves = 4, kXTile = 64, kXRows = 128;  // a workgroup; rows of a staged tile; rows (keys) a workgroup owns, 32 a wave
+constexpr int64_t kXMostBlocks = 0xff0000;  // workgroups of a launch: below 2^32 threads, with room for the divided walks
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef short v4s16 __attribute__((ext_vector_type(4)));

@@ -372,7 +372,9 @@ extern "C" int q8_layernorm(const void* x, int dt, int64_t x_row_stride, const v
     if (!(eps >= 0.f)) return fail(Q8_ERR_SHAPE, "q8_layernorm: eps %g", (double)eps);
     const bool vec = dim % 8 == 0 && (rows == 1 || x_row_stride % 8 == 0) && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
     const int t = ln_threads_of(dim), groups = (t < 256 ? 256 : t) / t;
-    const dim3 grid((unsigned)((rows + groups - 1) / groups));
+    const int64_t blocks = (rows + groups - 1) / groups;
+    if (blocks > most_blocks(t < 256 ? 256 : t)) return fail(Q8_ERR_SHAPE, "q8_layernorm: too many rows (%lld of %d elements)", (long long)rows, dim);
+    const dim3 grid((unsigned)blocks);
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define LN_FWD(DT, VEC) \
     layernorm_kernel<DT, VEC, T, CH><<<grid, ln_threads<T>(), 0, s>>>(x, x_row_stride, w, b, w_dtype == Q8_F32, y, mean, rstd, rows, dim, eps)

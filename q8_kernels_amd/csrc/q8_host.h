@@ -22,6 +22,9 @@ inline int fail(int code, const char* fmt, ...) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Workgroups of one launch: its threads are counted in 32 bits.
+inline int64_t most_blocks(int threads) { return 0xffffffffll / threads; }
+
 inline int launch_status(const char* what) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(Q8_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));

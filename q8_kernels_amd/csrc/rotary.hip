@@ -290,7 +290,7 @@ extern "C" int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, c
     if (per > kRotAngles / a.pairs) per = kRotAngles / a.pairs;
     a.per_block = per < 1 ? 1 : (int)per;
     const int64_t blocks = (all + a.per_block - 1) / a.per_block;
-    if (blocks > 0x7fffffff) return fail(Q8_ERR_SHAPE, "q8_rotary: too many tokens");
+    if (blocks > most_blocks(kRotThreads)) return fail(Q8_ERR_SHAPE, "q8_rotary: too many tokens");
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define ROT(DT)                                                                                             \
     do {                                                                                                    \

@@ -82,11 +82,16 @@ def test_refusals_of_the_c_entry_points():
     assert need > 0 and att(n=100000) == -1 and att(n=100000, ws=16, size=16) == -3
     assert L.q8_cross_attn_workspace(2, 8, 3, 8, 8, 64) == -3 and L.q8_cross_attn_backward_workspace(2, 8, 8, 8, 8, 60) == -3
 
-    def bwd(g=16, lse=16, dq=16, dk=16, ws=16, size=1 << 40, dt=B16, d=64, n=8, qs=ok):
-        return L.q8_cross_attn_backward(g, ok, 16, qs, 16, ok, 16, ok, 16, ok, lse, dq, ok, dk, ok, 16, ok, None, None, 0, dt, 0.1, 2, 8, 8, 8, n, d, ws, size, None)
+    def bwd(g=16, lse=16, dq=16, dk=16, ws=16, size=1 << 40, dt=B16, d=64, n=300, qs=ok, b=2, h=8):
+        return L.q8_cross_attn_backward(g, ok, 16, qs, 16, ok, 16, ok, 16, ok, lse, dq, ok, dk, ok, 16, ok, None, None, 0, dt, 0.1, b, h, h, 8, n, d, ws, size, None)
 
     assert bwd(g=None) == -1 and bwd(lse=None) == -1 and bwd(dq=None) == -1 and bwd(dk=None) == -1 and bwd(ws=None) == -1
     assert bwd(size=16) == -3 and bwd(d=12) == -3 and bwd(dt=F32) == -2 and bwd(ws=20) == -4 and bwd(qs=odd) == -4
+    # more workgroups than a launch takes (2^32 threads)
+    assert ln(rows=(1 << 31) - 1) == -3 and ln(rows=1 << 25, dim=8000, st=8000) == -3 and ln(rows=1 << 23, dim=9000, st=9000) == -3
+    assert rot(h=1, b=1, t=1 << 34, d=8, r=8) == -3
+    assert att(b=1 << 20, h=16, hk=16, m=1) == -3 and att(b=1 << 16, h=1 << 12, hk=1, n=300) == -3
+    assert bwd(b=1 << 20, h=16) == -3 and bwd(b=1 << 20, h=16, n=8) == -3
 
 
 @pytest.mark.gpu
