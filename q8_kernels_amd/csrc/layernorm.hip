@@ -4,7 +4,7 @@
 //   with u_j = g_j w_j:  dx_j = rstd (u_j - mean(u) - h_j mean(u h)),  dw_j = sum_rows g_j h_j,  db_j = sum_rows g_j
 //
 // HBM-bound: the forward reads x and writes y, the backward reads x and g and writes dx, all of them once. A row therefore
-// stays in the registers of the T threads that own it (T = 16, 64, 256 or 1024, at most 32 elements each) between the
+// stays in the registers of the T threads that own it (16 to 1024, at most 32 elements each) between the
 // passes over it: the variance is the mean of the squared distances from the finished mean, not E x^2 - mu^2, which
 // cancels. All sums are fp32. Rows whose length or address does not allow 16-byte accesses take element accesses instead
 // (VEC = 1), strided by T so that a wave still covers consecutive addresses.
@@ -12,7 +12,12 @@
 // The parameters' gradients are sums over rows. A workgroup of the backward walks over rows and keeps the sums of its
 // columns in registers, adds the groups of threads that hold the same columns in LDS, one after the other, and writes one
 // row of partial sums to the workspace; a second kernel adds those in a fixed order. No atomics: the same inputs give the
-// same bits. The number of workgroups (ln_blocks) trades rows in flight against the partial sums' traffic.
+// same bits. The number of workgroups (ln_blocks) trades rows in flight against the partial sums' traffic. Rows of more than
+// 16384 elements (8192 where accesses are by element) leave no registers for the sums: a kernel of its own reads x and g once
+// more for them (1000 x 30000: 61 us; with spilled registers in one kernel 172).
+//
+// bf16, 12288 x 2048: forward 19 us (5.3 TB/s, of data partly in the last-level cache), backward 37 us with the parameters' sums
+// (5.5 of them; 4.1 TB/s of what it has to move). What bounds it: HBM, and at the smallest sizes the launches.
 #include "q8_common.h"
 #include "q8_host.h"
 
@@ -132,7 +137,7 @@ __device__ __forceinline__ void row_sums(float (&v)[NV], float (*red)[NV][16], i
     for (int k = 0; k < NV; ++k) v[k] = group_sum<(T < 64 ? T : 64)>(v[k]);
     if constexpr (T > 64) {
         constexpr int W = T / 64;
-        const int wave = threadIdx.x >> 6;
+        const int wave = threadIdx.x >> 6, first = threadIdx.x / T * W;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) red[slot][k][wave] = v[k];
@@ -140,13 +145,17 @@ __device__ __forceinline__ void row_sums(float (&v)[NV], float (*red)[NV][16], i
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            float s = red[slot][k][0];
+            float s = red[slot][k][first];
 #pragma unroll
-            for (int i = 1; i < W; ++i) s += red[slot][k][i];
+            for (int i = 1; i < W; ++i) s += red[slot][k][first + i];
             v[k] = s;
         }
     }
 }
+
+// Whether the backward's threads have registers for the parameters' gradients beside the row (128 each with 1024 threads).
+template <int VEC, int T, int CH>
+constexpr bool ln_fused() { return T < 1024 || CH == 1 || (CH == 2 && VEC == 8); }
 
 template <int T>
 constexpr int ln_threads() { return T < 256 ? 256 : T; }
@@ -192,15 +201,15 @@ __global__ __launch_bounds__(ln_threads<T>()) void layernorm_kernel(const void* 
 }
 
 // partials: [gridDim.x][2][dim] fp32 (sums of g h, sums of g), or NULL when no parameter needs a gradient.
-// dx NULL: not wanted. The next row is requested before the present one's sums are formed (not with 1024 threads, whose
-// register budget of 128 does not hold both).
+// dx NULL: not wanted. The next row is requested before the present one's sums are formed, where the registers
+// hold both (1000 x 16384 fp32, 1024 threads with 16 elements: 56 us without, 78 with).
 template <int DT, int VEC, int T, int CH>
 __global__ __launch_bounds__(ln_threads<T>()) void layernorm_backward_kernel(const void* __restrict__ g, int64_t g_stride, const void* __restrict__ x,
                                                                            int64_t x_stride, const void* __restrict__ w, int w_f32,
                                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                            void* __restrict__ dx, float* __restrict__ partials, int64_t rows, int dim) {
     constexpr int N = 8 * CH, G = ln_threads<T>() / T;
-    constexpr bool AHEAD = T < 1024;
+    constexpr bool FUSED = ln_fused<VEC, T, CH>(), AHEAD = T < 1024 || CH == 1;
     using Part = RowPart<DT, VEC, T, CH>;
     __shared__ float red[2][2][16];
     __shared__ float cols[G > 1 ? 2 * T * N : 1];
@@ -241,14 +250,16 @@ __global__ __launch_bounds__(ln_threads<T>()) void layernorm_backward_kernel(con
             const float gv = gr.get(i), h = (xr.get(i) - mu) * rs, u = gv * wv[i];
             s[0] += u;
             s[1] += u * h;
-            dw[i] += gv * h;
-            db[i] += gv;
+            if constexpr (FUSED) {
+                dw[i] += gv * h;
+                db[i] += gv;
+            }
         }
         row_sums<T, 2>(s, red, (int)(it & 1));
         if (row_ok && dx != nullptr) {
             const float mu_u = s[0] * inv_dim, mu_uh = s[1] * inv_dim;
             float o[N];
-#pragma unroll
+    #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float h = (xr.get(i) - mu) * rs;
                 o[i] = rs * (gr.get(i) * wv[i] - mu_u - h * mu_uh);
@@ -257,7 +268,7 @@ __global__ __launch_bounds__(ln_threads<T>()) void layernorm_backward_kernel(con
         }
         if constexpr (AHEAD) { xr = xn; gr = gn; mu = mn; rs = rn; }
     }
-    if (partials == nullptr) return;
+    if (!FUSED || partials == nullptr) return;
     if constexpr (G > 1) {
         for (int k = 0; k < G; ++k) {
             if (grp == k) {
@@ -280,6 +291,66 @@ __global__ __launch_bounds__(ln_threads<T>()) void layernorm_backward_kernel(con
         const int e = Part::index(i, t);
         if (e < dim) { out[e] = dw[i]; out[dim + e] = db[i]; }
     }
+}
+
+// VEC consecutive elements in fp32
+template <int DT, int VEC>
+__device__ __forceinline__ void load_columns(const void* p, int64_t at, float (&v)[VEC == 8 ? 8 : 1]) {
+    if constexpr (VEC == 1) {
+        if constexpr (DT == Q8_F32) v[0] = static_cast<const float*>(p)[at];
+        else v[0] = DT == Q8_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p)[at]) : f16_bits_to_f32(static_cast<const uint16_t*>(p)[at]);
+    } else if constexpr (DT == Q8_F32) {
+        const v4f a = *reinterpret_cast<const v4f*>(static_cast<const float*>(p) + at), b = *reinterpret_cast<const v4f*>(static_cast<const float*>(p) + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[i + 4] = b[i]; }
+    } else {
+        const v4u a = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = DT == Q8_BF16 ? bf16_bits_to_f32(a[i] & 0xffffu) : f16_bits_to_f32(a[i] & 0xffffu);
+            v[2 * i + 1] = DT == Q8_BF16 ? bf16_bits_to_f32(a[i] >> 16) : f16_bits_to_f32(a[i] >> 16);
+        }
+    }
+}
+
+// The partial sums of a part of the rows alone, for rows too long for the kernel above: a thread holds VEC columns.
+template <int DT, int VEC>
+__global__ __launch_bounds__(256) void layernorm_columns_kernel(const void* __restrict__ g, int64_t g_stride, const void* __restrict__ x, int64_t x_stride,
+                                                                const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                                float* __restrict__ partials, int64_t rows, int dim) {
+    constexpr int BATCH = 4, N = VEC == 8 ? 8 : 1;
+    const int col = (blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (col >= dim) return;
+    const int64_t per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
+    float dw[N], db[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) { dw[i] = 0.f; db[i] = 0.f; }
+    for (int64_t r = r0; r < r1; r += BATCH) {
+        float xv[BATCH][N], gv[BATCH][N], mu[BATCH], rs[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const bool ok = r + k < r1;
+            const int64_t row = ok ? r + k : r;
+            load_columns<DT, VEC>(x, row * x_stride + col, xv[k]);
+            load_columns<DT, VEC>(g, row * g_stride + col, gv[k]);
+            mu[k] = mean[row];
+            rs[k] = ok ? rstd[row] : 0.f;
+            if (!ok) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) xv[k][i] = gv[k][i] = mu[k] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                dw[i] += gv[k][i] * ((xv[k][i] - mu[k]) * rs[k]);
+                db[i] += gv[k][i];
+            }
+    }
+    float* out = partials + (int64_t)blockIdx.y * 2 * dim + col;
+#pragma unroll
+    for (int i = 0; i < N; ++i) { out[i] = dw[i]; out[dim + i] = db[i]; }
 }
 
 __device__ __forceinline__ void store_any(void* p, int dt, int64_t e, float v) {
@@ -307,14 +378,30 @@ __global__ __launch_bounds__(1024) void layernorm_params_kernel(const float* __r
     if (out != nullptr) store_any(out, dt, col < dim ? col : col - dim, s);
 }
 
-// threads per row for a length: at most 32 elements each
-static int ln_threads_of(int dim) { return dim <= 128 ? 16 : dim <= 2048 ? 64 : dim <= 8192 ? 256 : 1024; }
+// The threads of a row, as LN_BY_DIM below chooses them with the chunks of 8 elements that each holds. The forward takes few
+// threads with up to 32 elements; the backward holds six times as many registers an element, so it takes more threads with 8
+// or 16, which leaves two waves or more on a SIMD. us of forward / backward with the parameters' sums, bf16 unless fp32 is said:
+//   12288 x 2048: 64 threads 20.1 / 37.1, 128 19.1 / 37.1, 256 22.3 / 37.9     4099 x 1155 fp32: 64 14.1 / 43.9, 128 11.0 / 23.6
+//   8192 x 4096:  256 24.6 / 49.0, 512 28.1 / 46.7                             4000 x 3001: 256 of 32 42.9 / 77.0, 512 of 8 22.9 / 27.8
+//   4096 x 8192:  256 26.8 / 66.1 (256 workgroups: 54), 1024 32.2 / 48.6       2000 x 5001: 256 30.3 / 53.0, 512 28.5 / 34.4, 1024 of 8 - / 39.7
+//   65536 x 128:  16 8.8 / 21.3, 64 22.5 / 34.6                                16000 x 601: 64 of 32 32.6 / 73.1, of 16 18.0 / 27.4
+static int ln_fwd_threads(int dim) { return dim <= 128 ? 16 : dim <= 1024 ? 64 : dim <= 2048 ? 128 : dim <= 8192 ? 256 : 1024; }
+static int ln_threads_of(int dim, bool vec) { return dim <= 128 ? 16 : dim <= 1024 ? 64 : dim <= 2048 ? 128 : dim <= 4096 ? 512 : dim <= 8192 && !vec ? 512 : 1024; }
 
-// Workgroups of the backward: four rows or more for each group of threads, at most 512 (256 of 1024 threads).
-static int64_t ln_blocks(int64_t rows, int dim) {
-    const int t = ln_threads_of(dim), groups = (t < 256 ? 256 : t) / t;
-    const int64_t most = t == 1024 ? 256 : 512, b = (rows + 4 * groups - 1) / (4 * groups);
+// Workgroups of the backward: two rows or more for each group of threads (300 x 2048: 9.8 us, with four 11.4), and few enough
+// that the partial sums stay small beside the rows: 512 (12288 x 2048: 256 39.7 us, 512 37.1, 1024 43.7), 256 of 1024 threads
+// (4096 x 8192: 512 92 us with 256 threads, 256 54), 128 of the longest rows (2000 x 16384: 59 us).
+static int64_t ln_blocks(int64_t rows, int dim, bool vec) {
+    const int t = ln_threads_of(dim, vec), groups = (t < 256 ? 256 : t) / t;
+    const int64_t most = t < 1024 ? 512 : dim <= 8192 ? 256 : 128, b = (rows + 2 * groups - 1) / (2 * groups);
     return b < 1 ? 1 : b < most ? b : most;
+}
+// Parts of the rows for the kernel that forms the partial sums alone: 32 rows or more, at most 128.
+static int64_t ln_parts(int64_t rows) { return rows <= 32 ? 1 : rows < 4096 ? (rows + 31) / 32 : 128; }
+// workspace for either kind of access: the call may be of an unaligned tensor (which needs no more for long rows)
+static int64_t ln_partials(int64_t rows, int dim) {
+    const int64_t a = ln_blocks(rows, dim, true), b = ln_blocks(rows, dim, false);
+    return (a > b ? a : b) * 2 * dim * (int64_t)sizeof(float);
 }
 
 static int ln_check(const char* who, int dt, int w_dtype, bool has_param, int64_t rows, int dim) {
@@ -336,27 +423,28 @@ static bool elem_aligned(const void* p, int dt) { return (reinterpret_cast<uintp
 
 using namespace q8;
 
-#define LN_BY_DIM(DT, VEC, ...)                                                             \
-    do {                                                                                    \
-        if (dim <= 128) { constexpr int T = 16, CH = 1; __VA_ARGS__(DT, VEC); }             \
-        else if (dim <= 512) { constexpr int T = 64, CH = 1; __VA_ARGS__(DT, VEC); }        \
-        else if (VEC == 8 && dim <= 1024) { constexpr int T = 64, CH = 2; __VA_ARGS__(DT, VEC); } \
-        else if (dim <= 2048) { constexpr int T = 64, CH = 4; __VA_ARGS__(DT, VEC); }       \
-        else if (VEC == 8 && dim <= 4096) { constexpr int T = 256, CH = 2; __VA_ARGS__(DT, VEC); } \
-        else if (dim <= 8192) { constexpr int T = 256, CH = 4; __VA_ARGS__(DT, VEC); }      \
-        else { constexpr int T = 1024, CH = 4; __VA_ARGS__(DT, VEC); }                      \
+#define LN_BY_DIM(DT, VEC, FWD, ...)                                                                        \
+    do {                                                                                                    \
+        if (dim <= 128) { constexpr int T = 16, CH = 1; __VA_ARGS__(DT, VEC); }                             \
+        else if (dim <= 512) { constexpr int T = 64, CH = 1; __VA_ARGS__(DT, VEC); }                        \
+        else if (dim <= 1024) { constexpr int T = 64, CH = 2; __VA_ARGS__(DT, VEC); }                       \
+        else if (dim <= 2048) { constexpr int T = 128, CH = 2; __VA_ARGS__(DT, VEC); }                      \
+        else if (dim <= 4096) { constexpr int T = FWD ? 256 : 512, CH = 512 / T; __VA_ARGS__(DT, VEC); }    \
+        else if (dim <= 8192) { constexpr int T = FWD ? 256 : VEC == 8 ? 1024 : 512, CH = 1024 / T; __VA_ARGS__(DT, VEC); } \
+        else if (dim <= 16384) { constexpr int T = 1024, CH = 2; __VA_ARGS__(DT, VEC); }                    \
+        else { constexpr int T = 1024, CH = 4; __VA_ARGS__(DT, VEC); }                                      \
     } while (0)
-#define LN_BY_TYPE(vec, ...)                                    \
-    do {                                                        \
-        if (vec) {                                              \
-            if (dt == Q8_BF16) LN_BY_DIM(Q8_BF16, 8, __VA_ARGS__);      \
-            else if (dt == Q8_F16) LN_BY_DIM(Q8_F16, 8, __VA_ARGS__);   \
-            else LN_BY_DIM(Q8_F32, 8, __VA_ARGS__);             \
-        } else {                                                \
-            if (dt == Q8_BF16) LN_BY_DIM(Q8_BF16, 1, __VA_ARGS__);      \
-            else if (dt == Q8_F16) LN_BY_DIM(Q8_F16, 1, __VA_ARGS__);   \
-            else LN_BY_DIM(Q8_F32, 1, __VA_ARGS__);             \
-        }                                                       \
+#define LN_BY_TYPE(vec, FWD, ...)                                    \
+    do {                                                             \
+        if (vec) {                                                   \
+            if (dt == Q8_BF16) LN_BY_DIM(Q8_BF16, 8, FWD, __VA_ARGS__);      \
+            else if (dt == Q8_F16) LN_BY_DIM(Q8_F16, 8, FWD, __VA_ARGS__);   \
+            else LN_BY_DIM(Q8_F32, 8, FWD, __VA_ARGS__);             \
+        } else {                                                     \
+            if (dt == Q8_BF16) LN_BY_DIM(Q8_BF16, 1, FWD, __VA_ARGS__);      \
+            else if (dt == Q8_F16) LN_BY_DIM(Q8_F16, 1, FWD, __VA_ARGS__);   \
+            else LN_BY_DIM(Q8_F32, 1, FWD, __VA_ARGS__);             \
+        }                                                            \
     } while (0)
 
 extern "C" int q8_layernorm(const void* x, int dt, int64_t x_row_stride, const void* w, const void* b, int w_dtype, void* y, float* mean,
@@ -371,21 +459,21 @@ extern "C" int q8_layernorm(const void* x, int dt, int64_t x_row_stride, const v
         return fail(Q8_ERR_ALIGN, "q8_layernorm: pointer not aligned to its element type");
     if (!(eps >= 0.f)) return fail(Q8_ERR_SHAPE, "q8_layernorm: eps %g", (double)eps);
     const bool vec = dim % 8 == 0 && (rows == 1 || x_row_stride % 8 == 0) && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
-    const int t = ln_threads_of(dim), groups = (t < 256 ? 256 : t) / t;
+    const int t = ln_fwd_threads(dim), groups = (t < 256 ? 256 : t) / t;
     const int64_t blocks = (rows + groups - 1) / groups;
     if (blocks > most_blocks(t < 256 ? 256 : t)) return fail(Q8_ERR_SHAPE, "q8_layernorm: too many rows (%lld of %d elements)", (long long)rows, dim);
     const dim3 grid((unsigned)blocks);
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define LN_FWD(DT, VEC) \
     layernorm_kernel<DT, VEC, T, CH><<<grid, ln_threads<T>(), 0, s>>>(x, x_row_stride, w, b, w_dtype == Q8_F32, y, mean, rstd, rows, dim, eps)
-    LN_BY_TYPE(vec, LN_FWD);
+    LN_BY_TYPE(vec, true, LN_FWD);
 #undef LN_FWD
     return launch_status("q8_layernorm");
 }
 
 extern "C" int64_t q8_layernorm_backward_workspace(int64_t rows, int dim) {
     if (rows < 0 || dim < 1 || dim > kLnMaxDim) return fail(Q8_ERR_SHAPE, "q8_layernorm_backward_workspace: rows %lld, dim %d", (long long)rows, dim);
-    return ln_blocks(rows, dim) * 2 * dim * (int64_t)sizeof(float);
+    return ln_partials(rows, dim);
 }
 
 extern "C" int q8_layernorm_backward(const void* grad, int64_t grad_row_stride, const void* x, int dt, int64_t x_row_stride, const void* w, int w_dtype,
@@ -401,22 +489,31 @@ extern "C" int q8_layernorm_backward(const void* grad, int64_t grad_row_stride, 
     if (!elem_aligned(grad, dt) || !elem_aligned(x, dt) || !elem_aligned(dx, dt) || (w && !elem_aligned(w, wd)) || (dw && !elem_aligned(dw, wd)) ||
         (db && !elem_aligned(db, wd)) || !elem_aligned(mean, Q8_F32) || !elem_aligned(rstd, Q8_F32) || (params && !elem_aligned(workspace, Q8_F32)))
         return fail(Q8_ERR_ALIGN, "q8_layernorm_backward: pointer not aligned to its element type");
-    if (params && workspace_bytes < q8_layernorm_backward_workspace(rows, dim))
+    if (params && workspace_bytes < ln_partials(rows, dim))
         return fail(Q8_ERR_SHAPE, "q8_layernorm_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                    (long long)q8_layernorm_backward_workspace(rows, dim));
+                    (long long)ln_partials(rows, dim));
     const bool vec = dim % 8 == 0 && (rows <= 1 || (x_row_stride % 8 == 0 && grad_row_stride % 8 == 0)) && aligned16(x) && aligned16(grad) &&
                      aligned16(dx) && aligned16(w);
-    const int blocks = (int)ln_blocks(rows, dim);
+    const bool fused = dim <= (vec ? 16384 : 8192);
+    const int parts = (int)(fused ? ln_blocks(rows, dim, vec) : ln_parts(rows));
+    const int blocks = fused ? parts : (int)(rows < 512 ? rows : 512);
     float* partials = params ? static_cast<float*>(workspace) : nullptr;
     hipStream_t s = static_cast<hipStream_t>(stream);
-#define LN_BWD(DT, VEC)                                                                                                                  \
-    layernorm_backward_kernel<DT, VEC, T, CH><<<blocks, ln_threads<T>(), 0, s>>>(grad, grad_row_stride, x, x_row_stride, w, w_dtype == Q8_F32, mean, rstd, \
-                                                                                 dx, partials, rows, dim)
-    LN_BY_TYPE(vec, LN_BWD);
+#define LN_BWD(DT, VEC)                                                                                                                                    \
+    do {                                                                                                                                                   \
+        constexpr bool fused = ln_fused<VEC, T, CH>();                                                                                                     \
+        if (fused || (dx && rows))                                                                                                                         \
+            layernorm_backward_kernel<DT, VEC, T, CH><<<blocks, ln_threads<T>(), 0, s>>>(grad, grad_row_stride, x, x_row_stride, w, w_dtype == Q8_F32, mean, \
+                                                                                         rstd, dx, partials, rows, dim);                                  \
+        if (!fused && params)                                                                                                                              \
+            layernorm_columns_kernel<DT, VEC><<<dim3((unsigned)((dim + 256 * VEC - 1) / (256 * VEC)), (unsigned)parts), 256, 0, s>>>(                       \
+                grad, grad_row_stride, x, x_row_stride, mean, rstd, partials, rows, dim);                                                                  \
+    } while (0)
+    LN_BY_TYPE(vec, false, LN_BWD);
 #undef LN_BWD
     if (int e = launch_status("q8_layernorm_backward")) return e;
     if (params) {
-        layernorm_params_kernel<<<(2 * dim + 31) / 32, 1024, 0, s>>>(partials, blocks, dw, db, wd, dim);
+        layernorm_params_kernel<<<(2 * dim + 31) / 32, 1024, 0, s>>>(partials, parts, dw, db, wd, dim);
         return launch_status("q8_layernorm_backward");
     }
     return Q8_OK;

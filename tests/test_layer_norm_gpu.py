@@ -86,6 +86,23 @@ def test_many_rows(dev, rows, dim):
     check(*make(dev, rows, dim, torch.bfloat16, torch.float32, seed=rows))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim", [(1201, 2041), (1030, 4001), (611, 6144), (601, 6151), (530, 9001), (290, 16384), (517, 20000), (131, 30001)])
+def test_many_long_rows(dev, dtype, rows, dim):
+    check(*make(dev, rows, dim, dtype, torch.float32, seed=rows))
+
+
+def test_long_rows_and_no_rows_or_one_gradient(dev):
+    x, w, b, g = make(dev, 70, 20000, torch.bfloat16, torch.float32, seed=10)
+    y, mean, rstd = _C.layer_norm(x, w, b)
+    full = _C.layer_norm_backward(g, x, w, b, mean, rstd)
+    for i in range(3):
+        one = _C.layer_norm_backward(g, x, w, b, mean, rstd, [j == i for j in range(3)])
+        assert all((one[j] is None) if j != i else torch.equal(one[j], full[j]) for j in range(3))
+    none = _C.layer_norm_backward(g[:0], x[:0], w, b, mean[:0], rstd[:0])
+    assert none[0].shape == (0, 20000) and (none[1] == 0).all() and (none[2] == 0).all()
+
+
 def test_large_mean_does_not_cancel(dev):
     x, w, b, g = make(dev, 20, 512, torch.float32, torch.float32, seed=8)
     check(x * 1e-2 + 100.0, w, b, g)
