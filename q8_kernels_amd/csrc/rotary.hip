@@ -7,7 +7,8 @@
 // HBM-bound: every head is read and written once. The angles are formed here instead of being read from a table: p * f_i
 // in fp64, whose whole turns are dropped there before the fp32 sine and cosine of the rest, so a far position is as exact as
 // its fp64 angle, and no table limits the positions. A workgroup forms the R / 2 angles of
-// its tokens once, in LDS, and all heads of those tokens use them.
+// its tokens once, in LDS, and all heads of those tokens use them. bf16, 2 x 6144 tokens, 32 + 32 heads of 64: 41 us for 201 MB
+// (4.9 TB/s; a copy of them reaches 5.1), 16 single tokens of 32 + 8 heads 4.3 us, which is the launch.
 #include "q8_common.h"
 #include "q8_host.h"
 
@@ -34,28 +35,29 @@ struct RotArgs {
     int per_block;            // tokens of a workgroup
 };
 
-// A work item's elements as they are in memory: VEC = 8: 16 bytes (32 of fp32) from one place, or from two for the pairs of the
-// half layout; VEC = 1: one element each.
+// A work item's elements as they are in memory: VEC of them from one place, or from two for the pairs of the half layout, in
+// accesses of 16 bytes (8 bytes for 4 16-bit elements, an element for VEC = 1).
 template <int DT, int VEC>
 struct RotPart {
-    static constexpr int N = VEC == 1 ? 1 : DT == Q8_F32 ? 8 : 4;
+    static constexpr int N = VEC == 1 ? 1 : DT == Q8_F32 ? VEC : VEC / 2, CHUNK = N < 4 ? N : 4;
+    typedef uint32_t Words __attribute__((ext_vector_type(CHUNK > 1 ? CHUNK : 2)));
     uint32_t r[N];
     __device__ __forceinline__ void load(const void* p, int64_t e) {
         if constexpr (VEC == 1) {
             r[0] = DT == Q8_F32 ? static_cast<const uint32_t*>(p)[e] : static_cast<const uint16_t*>(p)[e];
         } else {
-            const v4u* s = reinterpret_cast<const v4u*>(static_cast<const char*>(p) + e * (DT == Q8_F32 ? 4 : 2));
+            const Words* s = reinterpret_cast<const Words*>(static_cast<const char*>(p) + e * (DT == Q8_F32 ? 4 : 2));
 #pragma unroll
-            for (int q = 0; q < N / 4; ++q) {
-                const v4u w = s[q];
+            for (int q = 0; q < N / CHUNK; ++q) {
+                const Words w = s[q];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) r[q * 4 + k] = w[k];
+                for (int i = 0; i < CHUNK; ++i) r[q * CHUNK + i] = w[i];
             }
         }
     }
     __device__ __forceinline__ float get(int i) const {
         if constexpr (DT == Q8_F32) return __uint_as_float(r[i]);
-        const uint32_t h = VEC == 1 ? r[0] : (i & 1) ? r[i >> 1] >> 16 : r[i >> 1] & 0xffffu;
+        const uint32_t h = VEC == 1 ? r[0] : i & 1 ? r[i >> 1] >> 16 : r[i >> 1] & 0xffffu;
         return DT == Q8_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
     }
     __device__ __forceinline__ void set(const float (&v)[VEC]) {
@@ -63,10 +65,10 @@ struct RotPart {
             r[0] = DT == Q8_F32 ? __float_as_uint(v[0]) : DT == Q8_BF16 ? pack2_bf16(v[0], 0.f) & 0xffffu : __builtin_bit_cast(uint16_t, (_Float16)v[0]);
         } else if constexpr (DT == Q8_F32) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(v[i]);
+            for (int i = 0; i < VEC; ++i) r[i] = __float_as_uint(v[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < N; ++i)
                 r[i] = DT == Q8_BF16 ? pack2_bf16(v[2 * i], v[2 * i + 1])
                                      : __builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) << 16);
         }
@@ -76,19 +78,24 @@ struct RotPart {
             if constexpr (DT == Q8_F32) static_cast<uint32_t*>(p)[e] = r[0];
             else static_cast<uint16_t*>(p)[e] = (uint16_t)r[0];
         } else {
-            v4u* s = reinterpret_cast<v4u*>(static_cast<char*>(p) + e * (DT == Q8_F32 ? 4 : 2));
+            Words* s = reinterpret_cast<Words*>(static_cast<char*>(p) + e * (DT == Q8_F32 ? 4 : 2));
 #pragma unroll
-            for (int q = 0; q < N / 4; ++q) s[q] = v4u{r[q * 4], r[q * 4 + 1], r[q * 4 + 2], r[q * 4 + 3]};
+            for (int q = 0; q < N / CHUNK; ++q) {
+                Words w;
+#pragma unroll
+                for (int i = 0; i < CHUNK; ++i) w[i] = r[q * CHUNK + i];
+                s[q] = w;
+            }
         }
     }
 };
 
-// One work item of a head: VEC = 8: 8 pairs (half) / 4 pairs (interleaved) or 8 copied elements, in 16-byte accesses;
-// VEC = 1: one pair or one copied element. Threads with the same threadIdx / items share a head; a thread has BATCH items
+// One work item of a head: VEC pairs (half) / VEC / 2 pairs (interleaved) or VEC copied elements; VEC = 1: one pair or one copied
+// element. Threads with the same threadIdx / items share a head; a thread has BATCH items
 // under way at once, the first of them requested before the angles are formed.
 template <int DT, bool HALF, int VEC>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
-    constexpr int BATCH = 4, PAIRS = VEC == 1 ? 1 : (HALF ? 8 : 4);  // pairs of an item
+    constexpr int BATCH = 4, PAIRS = VEC == 1 ? 1 : (HALF ? VEC : VEC / 2);  // pairs of an item
     constexpr bool TWO = HALF || VEC == 1;                          // a pair's elements come from two places
     __shared__ float2 cs[kRotAngles];
     const int64_t token0 = (int64_t)blockIdx.x * a.per_block;
@@ -131,7 +138,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
     auto places = [&](int& eu, int& ev) {
         if (item >= rot_items) eu = ev = 2 * a.pairs + (item - rot_items) * VEC;
         else if (VEC == 1) { eu = HALF ? item : 2 * item; ev = HALF ? item + a.pairs : 2 * item + 1; }
-        else { eu = item * 8; ev = HALF ? a.pairs + item * 8 : eu; }
+        else { eu = item * VEC; ev = HALF ? a.pairs + item * VEC : eu; }
     };
     auto request = [&] {
         int eu, ev;
@@ -255,8 +262,10 @@ extern "C" int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, c
         return fail(Q8_ERR_SHAPE, "q8_rotary: row stride %lld of the positions", (long long)pos_row_stride);
     RotArgs a{};
     const int size = elem_size(dt), half = half_layout != 0;
-    const int need = 8;  // elements of a 16- or 32-byte access
-    bool vec = dim % 8 == 0 && rotary_dim % (half ? 16 : 8) == 0;
+    // The elements of an item: 8, or 4 where the pairs' second halves or the strides are not multiples of 8 (fp16, 10183 tokens of
+    // 10 heads of 48, 24 elements of them turned in the half layout: 10.4 us, by single elements 20.7), else one.
+    auto fits = [&](int n) { return dim % n == 0 && rotary_dim % (half ? 2 * n : n) == 0; };
+    int vec = fits(8) ? 8 : fits(4) ? 4 : 1;
     const struct { const void* in; void* out; const int64_t *is, *os; int heads; RotTensor* to; } side[2] = {
         {q, q_out, q_strides, q_out_strides, q_heads, &a.q}, {k, k_out, k_strides, k_out_strides, k_heads, &a.k}};
     for (const auto& s : side) {
@@ -265,8 +274,14 @@ extern "C" int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, c
             return fail(Q8_ERR_SHAPE, "q8_rotary: strides (0 or more, offsets below 2^59)");
         if ((reinterpret_cast<uintptr_t>(s.in) | reinterpret_cast<uintptr_t>(s.out)) & (uintptr_t)(size - 1)) return fail(Q8_ERR_ALIGN, "q8_rotary: tensor not aligned to its element type");
         *s.to = RotTensor{s.in, s.out, s.is[0], s.is[1], s.is[2], s.os[0], s.os[1], s.os[2]};
-        vec = vec && aligned16(s.in) && aligned16(s.out);
-        for (int i = 0; i < 3; ++i) vec = vec && s.is[i] % need == 0 && s.os[i] % need == 0;
+        const auto goes = [&](int n) {
+            const uintptr_t bytes = n * size < 16 ? n * size : 16;
+            bool ok = ((reinterpret_cast<uintptr_t>(s.in) | reinterpret_cast<uintptr_t>(s.out)) & (bytes - 1)) == 0;
+            for (int i = 0; i < 3; ++i) ok = ok && s.is[i] % n == 0 && s.os[i] % n == 0;
+            return ok;
+        };
+        if (vec == 8 && !goes(8)) vec = fits(4) ? 4 : 1;
+        if (vec == 4 && !goes(4)) vec = 1;
     }
     if ((reinterpret_cast<uintptr_t>(inv_freq) & 7) || (positions && (reinterpret_cast<uintptr_t>(positions) & (uintptr_t)(pos_bits / 8 - 1))))
         return fail(Q8_ERR_ALIGN, "q8_rotary: positions or frequencies not aligned");
@@ -282,7 +297,8 @@ extern "C" int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, c
     a.pairs = rotary_dim / 2;
     a.tokens = tokens;
     a.all_tokens = all;
-    // tokens of a workgroup (63 at most): about 2048 items of 8 elements, while 1024 workgroups remain and the angles fit
+    // tokens of a workgroup (63 at most): about 2048 items of 8 elements (2 x 6144 tokens of 64 heads of 64: 34.4 us; 1024 items
+    // 34.0, 4096 35.0), while 1024 workgroups remain (4099 tokens of 10 heads: 6.5 us; 256 workgroups 6.1) and the angles fit
     const int64_t per_token = (int64_t)a.heads * ((dim + 7) / 8);
     int64_t per = 2048 / per_token;
     if (per > all / 1024) per = all / 1024;
@@ -292,16 +308,21 @@ extern "C" int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, c
     const int64_t blocks = (all + a.per_block - 1) / a.per_block;
     if (blocks > most_blocks(kRotThreads)) return fail(Q8_ERR_SHAPE, "q8_rotary: too many tokens");
     hipStream_t s = static_cast<hipStream_t>(stream);
+#define ROT_VEC(DT, HALF)                                                                                   \
+    do {                                                                                                    \
+        if (vec == 8) rotary_kernel<DT, HALF, 8><<<(unsigned)blocks, kRotThreads, 0, s>>>(a);               \
+        else if (vec == 4) rotary_kernel<DT, HALF, 4><<<(unsigned)blocks, kRotThreads, 0, s>>>(a);          \
+        else rotary_kernel<DT, HALF, 1><<<(unsigned)blocks, kRotThreads, 0, s>>>(a);                        \
+    } while (0)
 #define ROT(DT)                                                                                             \
     do {                                                                                                    \
-        if (vec && half) rotary_kernel<DT, true, 8><<<(unsigned)blocks, kRotThreads, 0, s>>>(a);            \
-        else if (vec) rotary_kernel<DT, false, 8><<<(unsigned)blocks, kRotThreads, 0, s>>>(a);              \
-        else if (half) rotary_kernel<DT, true, 1><<<(unsigned)blocks, kRotThreads, 0, s>>>(a);              \
-        else rotary_kernel<DT, false, 1><<<(unsigned)blocks, kRotThreads, 0, s>>>(a);                       \
+        if (half) ROT_VEC(DT, true);                                                                        \
+        else ROT_VEC(DT, false);                                                                            \
     } while (0)
     if (dt == Q8_BF16) ROT(Q8_BF16);
     else if (dt == Q8_F16) ROT(Q8_F16);
     else ROT(Q8_F32);
 #undef ROT
+#undef ROT_VEC
     return launch_status("q8_rotary");
 }
