@@ -258,37 +258,39 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd 
     }
 }
 
-// Joins the parts of a row: weights exp2(m_i - max m). 32 lanes a row, 4 elements a lane.
-template <int DT>
+// Joins the parts of a row: weights exp2(m_i - max m). D / 4 threads a row, 4 elements each, BATCH parts at a time, their loads
+// all under way together. Two parts of 2 x 23732 rows of 64: 7.8 us (30 MB; with batches
+// of 8 for them too 14 us), 16 parts of 8 x 1024 rows of 128 5.8 us.
+template <int DT, int BATCH>
 __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
-    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), all = (int64_t)a.plan.tail * kXRows;
-    const unsigned tail = (unsigned)(n / kXRows), block = a.plan.full + tail;
-    const int unit = block / a.row_blocks, r = (block - unit * a.row_blocks) * kXRows + (int)(n - (int64_t)tail * kXRows);
+    const unsigned lanes = (unsigned)a.D / 4, id = blockIdx.x * 256 + threadIdx.x, n = id / lanes, all = a.plan.tail * kXRows;
+    const unsigned tail = n / kXRows, block = a.plan.full + tail;
+    const int unit = block / a.row_blocks, r = (int)(block - unit * a.row_blocks) * kXRows + (int)(n - tail * kXRows);
     if (n >= all || r >= a.R) return;
-    const int e = (threadIdx.x & 31) * 4;
+    const int e = (int)(id - n * lanes) * 4;
     float m = -3.0e38f, l = 0.f;
     v4f o = {0.f, 0.f, 0.f, 0.f};
-    // 8 parts at a time, their loads all under way together
-    for (int i0 = 0; i0 < a.plan.splits; i0 += 8) {
-        float pm[8], pl[8];
-        v4f po[8];
+    for (int i0 = 0; i0 < a.plan.splits; i0 += BATCH) {
+        float pm[BATCH], pl[BATCH];
+        v4f po[BATCH];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int64_t at = (i0 + i < a.plan.splits ? i0 + i : i0) * all + n;
-            pm[i] = i0 + i < a.plan.splits ? a.pm[at] : -3.0e38f;
-            pl[i] = i0 + i < a.plan.splits ? a.pl[at] : 0.f;
-            po[i] = e < a.D ? *reinterpret_cast<const v4f*>(a.part + at * a.D + e) : v4f{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < BATCH; ++i) {
+            const bool in = i0 + i < a.plan.splits;
+            const int64_t at = (int64_t)(in ? i0 + i : i0) * all + n;
+            pm[i] = in ? a.pm[at] : -3.0e38f;
+            pl[i] = in ? a.pl[at] : 0.f;
+            po[i] = *reinterpret_cast<const v4f*>(a.part + at * a.D + e);
         }
         float top = m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max_ieee(top, pm[i]);
+        for (int i = 0; i < BATCH; ++i) top = max_ieee(top, pm[i]);
         const float f = __builtin_amdgcn_exp2f(m - top);
         m = top;
         l *= f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] *= f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < BATCH; ++i) {
             const float w = i0 + i < a.plan.splits ? __builtin_amdgcn_exp2f(pm[i] - m) : 0.f;
             l += w * pl[i];
 #pragma unroll
@@ -296,10 +298,9 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
         }
     }
     if (a.lse != nullptr && e == 0) a.lse[(int64_t)unit * a.R + r] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
-    if (e >= a.D) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     const int g = r / a.M, b = unit / a.Hkv, hk = unit - b * a.Hkv;
-    uint16_t* p = a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (r - g * a.M) * a.o.st;
+    uint16_t* p = a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (int64_t)(r - g * a.M) * a.o.st;
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
@@ -398,9 +399,10 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
 #undef X_FWD
     if (int e = launch_status(who)) return e;
     if (a.plan.parts()) {
-        const unsigned n = a.plan.tail * (kXRows / 8);
-        if (dt == Q8_BF16) cross_attn_join_kernel<Q8_BF16><<<n, 256, 0, st>>>(a);
-        else cross_attn_join_kernel<Q8_F16><<<n, 256, 0, st>>>(a);
+        const unsigned n = a.plan.tail * (D / 8);  // 128 rows of D / 4 threads
+        const bool two = a.plan.splits == 2;
+        if (dt == Q8_BF16) { if (two) cross_attn_join_kernel<Q8_BF16, 2><<<n, 256, 0, st>>>(a); else cross_attn_join_kernel<Q8_BF16, 8><<<n, 256, 0, st>>>(a); }
+        else { if (two) cross_attn_join_kernel<Q8_F16, 2><<<n, 256, 0, st>>>(a); else cross_attn_join_kernel<Q8_F16, 8><<<n, 256, 0, st>>>(a); }
         return launch_status(who);
     }
     return Q8_OK;
