@@ -360,7 +360,7 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
     if (B * Hkv * a.row_blocks > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (few_keys(B * Hkv, a.R, N, D)) {
-        const int64_t units = B * Hkv, want = (few_blocks(N) + units - 1) / units, parts = want < a.row_blocks ? want : a.row_blocks;
+        const int64_t units = B * Hkv, parts = walk_parts(units, a.row_blocks, few_blocks(N), 1);
         if (units * parts > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many heads", who);
         const unsigned grid = (unsigned)(units * parts);
 #define X_FEW(DT, NT)                                                                                        \

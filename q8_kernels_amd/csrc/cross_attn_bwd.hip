@@ -403,19 +403,25 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     store_rows<DT, DP>(dv, 1.0f, there ? z.dv.p + b * z.dv.sb + hk * z.dv.sh + key * z.dv.st : nullptr, z.D, lane);
 }
 
-// Few keys (32 W of them at most) and many rows: all gradients in one pass over the rows, five products instead of seven, and
-// Q, dO and O read once. A wave owns 32 keys, as above; dS of a tile of 64 rows goes to LDS as [key][row], from where (turned
-// while it is read, like K) it is an operand of dQ^T = K^T dS^T. A wave forms one 32 x 32 block of dQ^T over a part of the keys;
-// where more waves share a block, the others' sums go through LDS to the first. delta comes from the same tile's O and dO.
-// A workgroup walks over a part of its unit's tiles; the parts' dK and dV are added by the kernel below. D up to 64: beyond, the
-// registers and LDS of one workgroup leave no second wave on a SIMD. bf16, 2 x 32 heads of 64, 6144 rows, 256 keys: 100 us and 7
-// for the parts (200 MB at 2.0 TB/s; 40 MFMA of a wave and tile would take 30 us, exp2 and the roundings of P and dS about as
-// long, and between the two barriers of a tile they overlap only in part).
+// Few keys (32 W of them at most): all gradients in one pass over the rows, five products instead of seven, and Q, dO and O read
+// once. A wave owns 32 keys, as above; dS of a tile of TR rows goes to LDS as [key][row], from where (turned while it is read,
+// like K) it is an operand of dQ^T = K^T dS^T. A wave forms one 32 x 32 block of dQ^T over a part of the keys; where more waves
+// share a block, the others' sums go through LDS to the first. delta comes from the same tile's O and dO. A workgroup walks over
+// a part of its unit's tiles; the parts' dK and dV are added by the kernel below.
+//
+// Heads of more than 64 have tiles of 32 rows, K's operands from LDS, O and dO for delta only asked for behind the products and
+// the compiler's order of instructions: what two waves on a SIMD have registers for (43 spilled ones otherwise; 2 x 32 heads of
+// 128, 6144 rows, 128 keys: 166 us, with 9 spilled ones 138).
+//
+// bf16, 2 x 32 heads of 64, 6144 rows, 256 keys: 100 us and 7 for the parts (200 MB at 2.0 TB/s; 40 MFMA of a wave and tile would
+// take 30 us, exp2 and the roundings of P and dS about as long, and between the two barriers of a tile they overlap only in part).
 template <int DT, int DP, int W>
 __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd a, int parts) {
-    constexpr int KS = DP / 16, DTL = DP / 32, TR = kXTile, ELEMS = TR * DP, CPR = DP / 8;
-    constexpr int NB = 2 * DTL, KG = W / NB, STEPS = W * 2 / KG;  // blocks of dQ^T, waves that share one, 16-key steps of each
-    constexpr int CHUNKS = TR * CPR / (W * 64) > 0 ? TR * CPR / (W * 64) : 1;  // of dO and O, for delta
+    constexpr bool LONG = DP > 64;
+    constexpr int KS = DP / 16, DTL = DP / 32, TR = !LONG || (DP == 96 && W == 8) ? 64 : 32, ELEMS = TR * DP;
+    constexpr int RB = TR / 32, NB = RB * DTL, KG = W / NB, STEPS = W * 2 / KG;  // blocks of dQ^T, waves that share one, 16-key steps of each
+    constexpr int CL = DP == 32 ? 4 : DP == 64 ? 8 : 16;  // lanes that share a row of dO and O, for delta
+    constexpr int CHUNKS = TR * CL / (W * 64) > 0 ? TR * CL / (W * 64) : 1;
     __shared__ __align__(16) uint16_t q0[ELEMS], q1[ELEMS], g0[ELEMS], g1[ELEMS], kt[W * 32 * DP], ds[W * 32 * TR];
     __shared__ __align__(16) float lse0[TR], lse1[TR], delta0[TR], delta1[TR];  // -lse and -delta of the tile's rows
     __shared__ __align__(16) float sums[KG > 1 ? (KG - 1) * NB * 1024 : 4];
@@ -431,16 +437,17 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     const int head_tiles = (a.M + TR - 1) / TR, tiles = a.G * head_tiles, per = (tiles + parts - 1) / parts;
     const int t0 = part * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
-    v4u kf[KS], vf[KS];
+    v4u kf[LONG ? 1 : KS], vf[KS];
     {
         const uint16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh + key * a.k.st + half * 8;
         const uint16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh + key * a.v.st + half * 8;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const bool in = counts && s * 16 + half * 8 < a.D;
-            kf[s] = in ? *reinterpret_cast<const v4u*>(kp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            const v4u x = in ? *reinterpret_cast<const v4u*>(kp + s * 16) : v4u{0u, 0u, 0u, 0u};
+            if constexpr (!LONG) kf[s] = x;
             vf[s] = in ? *reinterpret_cast<const v4u*>(vp + s * 16) : v4u{0u, 0u, 0u, 0u};
-            *reinterpret_cast<v4u*>(kt + wave * 32 * DP + tile_at<DP>(lane & 31, 2 * s + half)) = kf[s];
+            *reinterpret_cast<v4u*>(kt + wave * 32 * DP + tile_at<DP>(lane & 31, 2 * s + half)) = x;
         }
     }
     if (idle) {  // its part of dS stays zero
@@ -455,18 +462,21 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     v4u dor[CHUNKS], orr[CHUNKS];
     const uint16_t *qp = a.q.p + b * a.q.sb + (int64_t)hk * a.G * a.q.sh, *gp = a.g.p + b * a.g.sb + (int64_t)hk * a.G * a.g.sh;
     const uint16_t* op = a.o.p + b * a.o.sb + (int64_t)hk * a.G * a.o.sh;
-    const int chunk = (int)threadIdx.x % CPR, crow = (int)threadIdx.x / CPR;  // of delta: rows crow + k W 64 / CPR
+    const int chunk = (int)threadIdx.x % CL, crow = (int)threadIdx.x / CL;  // of delta: rows crow + k W 64 / CL
     // the tile that is next (t past the end: empty)
     auto aim = [&](int t) {
         const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
         rows = t < t1 ? a.M - m : 0;
         if (rows > TR) rows = TR;
-        const int last = rows - 1;
-        const int n = (int)threadIdx.x & (TR - 1);
+        const int last = rows - 1, n = (int)threadIdx.x & (TR - 1);
         row_lse = a.lse[(int64_t)unit * a.R + (rows ? g * a.M + m + (n < rows ? n : last) : 0)];
+    };
+    // what its delta is formed of
+    auto ask = [&](int t) {
+        const int g = t / head_tiles, m = (t - g * head_tiles) * TR, last = rows - 1;
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
-            const int r = crow + k * (W * 64 / CPR), i = m + (r < last ? r : last);
+            const int r = crow + k * (W * 64 / CL), i = m + (r < last ? r : last);
             const bool in = rows > 0 && chunk * 8 < a.D;
             dor[k] = in ? *reinterpret_cast<const v4u*>(gp + g * a.g.sh + i * a.g.st + chunk * 8) : v4u{0u, 0u, 0u, 0u};
             orr[k] = in ? *reinterpret_cast<const v4u*>(op + g * a.o.sh + i * a.o.st + chunk * 8) : v4u{0u, 0u, 0u, 0u};
@@ -474,7 +484,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     };
     auto tile_of = [&](const uint16_t* p, const XTensor& x, int t) {
         const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
-        return XTile(p + g * x.sh + m * x.st, x.st, rows, a.D);
+        return XTile(p + g * x.sh + m * x.st, x.st, rows, a.D, TR);
     };
     auto finish = [&](float* lt, float* dt) {
         wait_loads();
@@ -487,8 +497,8 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
                 d += unpack<DT>(dor[k][i] & 0xffffu) * unpack<DT>(orr[k][i] & 0xffffu);
                 d += unpack<DT>(dor[k][i] >> 16) * unpack<DT>(orr[k][i] >> 16);
             }
-            d = group_sum<CPR>(d);
-            const int r = crow + k * (W * 64 / CPR);
+            d = group_sum<CL>(d);
+            const int r = crow + k * (W * 64 / CL);
             if (chunk == 0 && r < TR) dt[r] = r < rows ? -d : 0.f;
         }
     };
@@ -498,6 +508,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
     if (t0 < t1) {
         aim(t0);
+        ask(t0);
         copies.group(0, 1, tile_of(qp, a.q, t0), tile_of(gp, a.g, t0), 0, q0, g0);
         finish(lse0, delta0);
     }
@@ -506,8 +517,8 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
 
     LaneOffsets<DP> at(lane);
     LaneOffsets<TR> ds_at(lane);
-    Operands<DP, 4> ops;
-    static_assert(ops.RN == 1 && ops.CN == 1, "one group each");
+    Operands<DP, LONG ? 2 : 4> ops;
+    auto keep_apart = [] { if constexpr (!LONG) fence(); };
     auto step = [&](int t, auto buffer, auto exact) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
@@ -516,46 +527,67 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
         uint16_t *qnext = BUF ? q0 : q1, *gnext = BUF ? g0 : g1;
         const int g = t / head_tiles, m = (t - g * head_tiles) * TR, here = rows;
         aim(t + 1);
+        if constexpr (!LONG) ask(t + 1);
         copies.group(0, 1, tile_of(qp, a.q, t + 1), tile_of(gp, a.g, t + 1), 0, qnext, gnext);
         if (!idle) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < RB; ++u) {
                 v16f s = splat16(0.f), dp = bias16(dt, u, half);
+                int w = 0;  // the place of the operands that are next
                 if (u == 0) ops.rows(0, ql, 0, 0, at);
-                ops.rows(1, gl, u * 32, 0, at);
-                fence();
 #pragma unroll
-                for (int j = 0; j < KS; ++j) s = mfma16<DT>(ops.f[0][j], kf[j], s);
-                fence();
-                ops.cols(0, gl, u * 32, 0, at);
-                fence();
+                for (int i = 0; i < ops.RN; ++i, w ^= 1) {
+                    v4u k[ops.RG];
 #pragma unroll
-                for (int j = 0; j < KS; ++j) dp = mfma16<DT>(ops.f[1][j], vf[j], dp);
+                    for (int j = 0; j < ops.RG; ++j) {
+                        if constexpr (LONG) k[j] = lds_rows<DP>(kt, wave * 32, i * ops.RG + j, at);
+                        else k[j] = kf[i * ops.RG + j];
+                    }
+                    if (i + 1 < ops.RN) ops.rows(w ^ 1, ql, u * 32, i + 1, at);
+                    else ops.rows(w ^ 1, gl, u * 32, 0, at);
+                    keep_apart();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {  // P, beside them
-                    const v4f x = *reinterpret_cast<const v4f*>(&lt[u * 32 + i * 8 + half * 4]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[i * 4 + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * 4 + j], a.c, x[j]));
+                    for (int j = 0; j < ops.RG; ++j) s = mfma16<DT>(ops.f[w][j], k[j], s);
+                    keep_apart();
                 }
-                fence();
+#pragma unroll
+                for (int i = 0; i < ops.RN; ++i, w ^= 1) {
+                    if (i + 1 < ops.RN) ops.rows(w ^ 1, gl, u * 32, i + 1, at);
+                    else ops.cols(w ^ 1, gl, u * 32, 0, at);
+                    keep_apart();
+#pragma unroll
+                    for (int j = 0; j < ops.RG; ++j) dp = mfma16<DT>(ops.f[w][j], vf[i * ops.RG + j], dp);
+                    // P, a part of it beside each group
+#pragma unroll
+                    for (int q = i * 4 / ops.RN; q < (i + 1) * 4 / ops.RN; ++q) {
+                        const v4f x = *reinterpret_cast<const v4f*>(&lt[u * 32 + q * 8 + half * 4]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[q * 4 + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q * 4 + j], a.c, x[j]));
+                    }
+                    keep_apart();
+                }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const v4u p = pack_step<DT>(s, k);
-                    if (k == 0) ops.cols(1, gl, u * 32 + 16, 0, at);
-                    else ops.cols(0, ql, u * 32, 0, at);
-                    fence();
 #pragma unroll
-                    for (int d = 0; d < DTL; ++d) dv[d] = mfma16<DT>(ops.f[k][d], p, dv[d]);
-                    if (k == 0) {  // dS, beside them
-                        if constexpr (exact) {  // all keys are in this wave: what their dS adds up to is the error of delta
+                    for (int c = 0; c < ops.CN; ++c, w ^= 1) {
+                        if (c + 1 < ops.CN) ops.cols(w ^ 1, gl, u * 32 + k * 16, c + 1, at);
+                        else if (k == 0) ops.cols(w ^ 1, gl, u * 32 + 16, 0, at);
+                        else ops.cols(w ^ 1, ql, u * 32, 0, at);
+                        keep_apart();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                dp[i] -= group_sum<32>(__uint_as_float(__float_as_uint(dp[i] * s[i]) & keep));
+                        for (int d = 0; d < ops.CG; ++d) dv[c * ops.CG + d] = mfma16<DT>(ops.f[w][d], p, dv[c * ops.CG + d]);
+                        if (k == 0 && c == 0) {  // dS, beside them (P's second half is still needed as it is)
+                            if constexpr (exact) {  // all keys are in this wave: what their dS adds up to is the error of delta
+#pragma unroll
+                                for (int i = 0; i < 16; ++i)
+                                    dp[i] -= group_sum<32>(__uint_as_float(__float_as_uint(dp[i] * s[i]) & keep));
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
                         }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+                        keep_apart();
                     }
-                    fence();
                 }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -565,26 +597,33 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
                     // rows u * 32 + 8 (2 k) + 4 half .. + 3 and the 4 rows 8 further, of this lane's key
                     *reinterpret_cast<v2i*>(ds + wave * 32 * TR + tile_at<TR>(lane & 31, u * 4 + 2 * k) + half * 4) = v2i{(int)p[0], (int)p[1]};
                     *reinterpret_cast<v2i*>(ds + wave * 32 * TR + tile_at<TR>(lane & 31, u * 4 + 2 * k + 1) + half * 4) = v2i{(int)p[2], (int)p[3]};
-                    if (k == 0) ops.cols(1, ql, u * 32 + 16, 0, at);
-                    else if (u == 0) ops.rows(0, ql, 32, 0, at);
-                    fence();
 #pragma unroll
-                    for (int d = 0; d < DTL; ++d) dk[d] = mfma16<DT>(ops.f[k][d], p, dk[d]);
-                    fence();
+                    for (int c = 0; c < ops.CN; ++c, w ^= 1) {
+                        if (c + 1 < ops.CN) ops.cols(w ^ 1, ql, u * 32 + k * 16, c + 1, at);
+                        else if (k == 0) ops.cols(w ^ 1, ql, u * 32 + 16, 0, at);
+                        else if (u + 1 < RB) ops.rows(w ^ 1, ql, 32, 0, at);
+                        keep_apart();
+#pragma unroll
+                        for (int d = 0; d < ops.CG; ++d) dk[c * ops.CG + d] = mfma16<DT>(ops.f[w][d], p, dk[c * ops.CG + d]);
+                        keep_apart();
+                    }
                 }
+                // (an even number of groups: the next rows are in place 0)
             }
         }
+        if constexpr (LONG) ask(t + 1);  // (here: before, there are no registers for it)
         barrier();
         // dQ^T: this wave's block of rows and elements, over its part of the keys
-        const int block = wave % NB, kg = wave / NB, rb = block & 1, db = block >> 1;
+        const int block = wave % NB, kg = wave / NB, rb = block % RB, db = block / RB;  // (kg = KG: a wave without one)
         v16f dq = splat16(0.f);
+        if (kg < KG)
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
             const int key0 = (kg * STEPS + i) * 16;
             dq = mfma16<DT>(lds_cols<DP>(kt, key0, db, at), lds_cols<TR>(ds, key0, rb, ds_at), dq);
         }
         if constexpr (KG > 1) {
-            if (kg > 0) {
+            if (kg > 0 && kg < KG) {
                 float* to = sums + ((kg - 1) * NB + block) * 1024 + lane * 4;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) *reinterpret_cast<v4f*>(to + i * 256) = v4f{dq[4 * i], dq[4 * i + 1], dq[4 * i + 2], dq[4 * i + 3]};
@@ -687,17 +726,19 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     p.dq_blocks = (p.rows + kXRows - 1) / kXRows;
     p.kv_blocks = ((int64_t)N + kXRows - 1) / kXRows;
     const int64_t tiles = (int64_t)(H / Hkv) * (((int64_t)M + kXTile - 1) / kXTile);
-    // The kernel for few keys, a workgroup for up to four tiles: one of 8 waves on a CU, or two of 4 (LDS). bf16 times, this kernel
-    // against the other two (B x H x M x N x D): 2 x 32 x 6144 x 256 x 64 115 against 146 us, x 128 65 against 97, 32 x 2048 x 128
-    // 25.4 against 33.5, 16 x 1024 x 64 18.3 against 19.2, 16 x 32 x 256 x 128 28 against 45. With 129 to 256 keys it takes 1024
-    // tiles to be faster: 8 x 8192 x 256 38 against 48, 16 x 2048 x 256 (512 tiles) 32.2 against 31.5, 8 x 512 x 256 24.6 against 22.5.
-    const int64_t at_once = N > kXRows ? 256 : 512;
-    if (D <= 64 && p.units > 0 && M > 0 && N > 0 && (N <= kXRows || (N <= 2 * kXRows && p.units * tiles >= 4 * at_once)) && p.units <= kXMostBlocks / 2) {
-        const int64_t most = (tiles + 3) / 4, want = (at_once + p.units - 1) / p.units;
+    // The kernel for few keys, a workgroup for four tiles of 64 rows or more: one of 8 waves on a CU, or two of 4 (LDS). bf16 times,
+    // this kernel against the other two (B x H x M x N x D), us:
+    //   2 x 32 x 6144 x 256 x 64   110, 146     2 x 32 x 6144 x 128 x 64   65, 97     2 x 32 x 6144 x 128 x 128   138, 229
+    //   2 x 32 x 6144 x 256 x 128  208, 292     2 x 32 x 6144 x 256 x 96  150, 211    11 x 4 x 8 x 2836 x 16 x 128  314, 424
+    //   1 x 32 x 2048 x 128 x 64   25, 34       1 x 16 x 1024 x 64 x 64    18, 19     16 x 32 x 256 x 128 x 64     28, 45
+    // With 129 to 256 keys it takes 1024 tiles to be faster: 8 x 8192 x 256 x 64 38 against 48, but 16 x 2048 x 256 x 64 (512
+    // tiles) 32.2 against 31.5, 8 x 512 x 256 x 64 24.6 against 22.5, 16 x 2048 x 256 x 128 51.3 against 51.0.
+    const int at_once = N > kXRows ? 256 : 512;
+    if (p.units > 0 && M > 0 && N > 0 && (N <= kXRows || (N <= 2 * kXRows && p.units * tiles >= 4 * at_once)) && p.units <= kXMostBlocks / 2) {
         p.few = N > kXRows ? 8 : 4;
         p.kv.full = 0;
         p.kv.tail = (unsigned)(p.units * p.kv_blocks);
-        p.kv.splits = (int)(want < most ? want : most);
+        p.kv.splits = walk_parts(p.units, tiles, at_once, 4);
         p.parts = p.kv.parts() * kXRows * 2 * D;
         return p;
     }
@@ -794,8 +835,12 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
         const unsigned grid = (unsigned)(p.units * p.kv.splits);
 #define X_FEW(DT, W)                                                                                                           \
     do {                                                                                                                       \
-        if (D <= 32) cross_attn_bwd_few_keys_kernel<DT, 32, W><<<grid, W * 64, 0, st>>>(a, p.kv.splits);                       \
-        else cross_attn_bwd_few_keys_kernel<DT, 64, W><<<grid, W * 64, 0, st>>>(a, p.kv.splits);                               \
+        switch (padded_head(D)) {                                                                                              \
+            case 32: cross_attn_bwd_few_keys_kernel<DT, 32, W><<<grid, W * 64, 0, st>>>(a, p.kv.splits); break;                \
+            case 64: cross_attn_bwd_few_keys_kernel<DT, 64, W><<<grid, W * 64, 0, st>>>(a, p.kv.splits); break;                \
+            case 96: cross_attn_bwd_few_keys_kernel<DT, 96, W><<<grid, W * 64, 0, st>>>(a, p.kv.splits); break;                \
+            default: cross_attn_bwd_few_keys_kernel<DT, 128, W><<<grid, W * 64, 0, st>>>(a, p.kv.splits);                      \
+        }                                                                                                                      \
     } while (0)
         if (p.few == 4) {
             if (dt == Q8_BF16) X_FEW(Q8_BF16, 4); else X_FEW(Q8_F16, 4);

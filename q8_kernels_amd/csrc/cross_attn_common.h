@@ -321,6 +321,21 @@ inline XSchedule schedule(int64_t blocks, int64_t length, int slots, int turns =
     return s;
 }
 
+// Into how many parts each of `units` walks of `steps` goes, `least` steps each or more, when `slots` workgroups run at once: the
+// number with which the last one ends first, a workgroup costing about two steps beside its walk. (44 walks of 360 tiles on 512
+// slots, backward with 16 keys of 128: 11 parts 314 us; 12, whose last 16 workgroups wait for a free place, 476.)
+inline int walk_parts(int64_t units, int64_t steps, int slots, int least) {
+    const int64_t most = steps > least ? (steps + least - 1) / least : 1;
+    int64_t best = 1, cost = INT64_MAX;
+    for (int turns = 1; turns <= 8; ++turns) {  // the most parts that take so many turns of the card, or one
+        int64_t n = (int64_t)slots * turns / units;
+        n = n < 1 ? 1 : n < most ? n : most;
+        const int64_t c = (units * n + slots - 1) / slots * ((steps + n - 1) / n + 2);
+        if (c < cost) { best = n; cost = c; }
+    }
+    return (int)best;
+}
+
 // One 32 x D result of a wave (columns = rows of the output, results = its elements) to memory. Lanes l and l + 32 hold 4
 // elements each of the same 8: two half exchanges make 16 consecutive bytes of either, 8 elements of group i in the low lane
 // and those of group i + 1 in the high one. p: the lane's output row (of column l % 32), NULL where there is none.

@@ -359,3 +359,22 @@ def test_gradients_of_few_counted_keys(dev, dtype, d, n, lens):
     lens = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev)
     check(q, k, v, lens=lens, seed=5, exact=True)
     check(q, k, v, lens=lens, mask=torch.arange(n, device=dev).expand(3, n) % 3 != 1, seed=6, exact=True)
+
+
+@pytest.mark.parametrize("b,h,hk,m,n,d,dtype", [(2, 16, 16, 2100, 256, 128, torch.bfloat16), (1, 20, 10, 1300, 128, 128, torch.float16), (3, 16, 4, 700, 100, 96, torch.bfloat16),
+                                                (2, 32, 32, 1100, 200, 80, torch.float16), (2, 32, 8, 1025, 256, 96, torch.bfloat16), (1, 6, 2, 77, 33, 104, torch.float16),
+                                                (2, 16, 16, 2050, 255, 64, torch.bfloat16), (1, 4, 4, 33, 65, 128, torch.bfloat16)])
+def test_gradients_of_few_keys(dev, b, h, hk, m, n, d, dtype):
+    gen = torch.Generator(device=dev).manual_seed(n)
+    q, k, v = make(dev, b, h, hk, m, n, d, dtype, seed=n + 1)
+    check(q, k, v, seed=1)
+    lens = torch.randint(33, n + 1, (b,), generator=gen, device=dev, dtype=torch.int32)
+    mask = torch.rand((b, n), generator=gen, device=dev) < 0.7
+    check(q, k, v, lens=lens, mask=mask, seed=2)
+    # what stands in keys that do not count is not looked at
+    dead = ~(mask & (torch.arange(n, device=dev) < lens[:, None]))[:, None, :, None].expand(k.shape)
+    g = torch.randn_like(q)
+    o, lse = _C.cross_attention(q, k, v, 0.1, lens, mask)
+    a = _C.cross_attention_backward(g, q, k, v, o, lse, 0.1, lens, mask)
+    c = _C.cross_attention_backward(g, q, k.masked_fill(dead, float("inf")), v.masked_fill(dead, float("nan")), o, lse, 0.1, lens, mask)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
