@@ -472,7 +472,7 @@ extern "C" int q8_layernorm(const void* x, int dt, int64_t x_row_stride, const v
 }
 
 extern "C" int64_t q8_layernorm_backward_workspace(int64_t rows, int dim) {
-    if (rows < 0 || dim < 1 || dim > kLnMaxDim) return fail(Q8_ERR_SHAPE, "q8_layernorm_backward_workspace: rows %lld, dim %d", (long long)rows, dim);
+    if (rows < 0 || rows > (int64_t)0x7fffffff || dim < 1 || dim > kLnMaxDim) return fail(Q8_ERR_SHAPE, "q8_layernorm_backward_workspace: rows %lld, dim %d", (long long)rows, dim);
     return ln_partials(rows, dim);
 }
 

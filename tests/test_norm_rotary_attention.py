@@ -50,7 +50,7 @@ def test_refusals_of_the_c_entry_points():
     assert ln(dt=E4) == -2 and ln(w=16, wd=F16) == -2
     assert ln(dim=0) == -3 and ln(dim=32769) == -3 and ln(rows=-1) == -3 and ln(rows=1 << 32) == -3 and ln(st=63) == -3 and ln(eps=-1.0) == -3
     assert ln(x=17) == -4 and ln(w=18) == -4
-    assert L.q8_layernorm_backward_workspace(100, 64) > 0 and L.q8_layernorm_backward_workspace(-1, 64) == -3
+    assert L.q8_layernorm_backward_workspace(100, 64) > 0 and L.q8_layernorm_backward_workspace(-1, 64) == -3 and L.q8_layernorm_backward_workspace((1 << 63) - 1, 64) == -3
     lb = lambda g=16, x=16, dt=B16, w=None, m=16, r=16, dx=16, dw=None, db=None, ws=None, size=0, rows=4, dim=64: (  # noqa: E731
         L.q8_layernorm_backward(g, dim, x, dt, dim, w, F32, m, r, dx, dw, db, ws, size, rows, dim, None))
     assert lb(dx=None) == 0 and lb(rows=0, g=None, x=None, m=None, r=None) == 0
