@@ -99,7 +99,8 @@ int norm_params(const Tensor& x, Tensor& w, Tensor& b, const char* who) {
     return !type || *type == at::kFloat ? Q8_F32 : type_of(x);
 }
 
-std::array<Tensor, 3> norm_forward(const Tensor& x, Tensor w, Tensor b, double eps, bool stats) {
+// stats: NULL, or what the mean and the reciprocal deviation of every row go to: two tensors, or one of both
+Tensor norm_forward(const Tensor& x, Tensor w, Tensor b, double eps, std::array<Tensor, 2>* stats, bool together = false) {
     require_gpu(x, "x");
     const int dt = type_of(x);
     TORCH_CHECK(dt >= 0, "layer_norm: x must be bfloat16, float16 or float32, got ", x.scalar_type());
@@ -108,26 +109,28 @@ std::array<Tensor, 3> norm_forward(const Tensor& x, Tensor w, Tensor b, double e
     const int wd = norm_params(x, w, b, "layer_norm");
     const c10::DeviceGuard guard(x.device());
     const Tensor r = as_rows(x);
-    Tensor y = at::empty(x.sizes(), x.options()), mean, rstd;
-    if (stats) {
-        mean = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
-        rstd = at::empty(mean.sizes(), mean.options());
+    Tensor y = at::empty(x.sizes(), x.options());
+    float *mean = nullptr, *rstd = nullptr;
+    if (stats && together) {
+        (*stats)[0] = at::empty({2, r.size(0)}, x.options().dtype(at::kFloat));
+        mean = (float*)ptr((*stats)[0]);
+        rstd = mean + r.size(0);
+    } else if (stats) {
+        for (Tensor& t : *stats) t = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+        mean = (float*)ptr((*stats)[0]);
+        rstd = (float*)ptr((*stats)[1]);
     }
-    check(q8_layernorm(ptr(r), dt, r.stride(0), ptr(w), ptr(b), wd, ptr(y), (float*)ptr(mean), (float*)ptr(rstd), r.size(0), (int)r.size(1), (float)eps,
-                       stream_of(x)));
-    return {y, mean, rstd};
+    check(q8_layernorm(ptr(r), dt, r.stride(0), ptr(w), ptr(b), wd, ptr(y), mean, rstd, r.size(0), (int)r.size(1), (float)eps, stream_of(x)));
+    return y;
 }
 
-std::array<Tensor, 3> norm_backward(const Tensor& grad, const Tensor& x, Tensor w, Tensor b, const Tensor& mean, const Tensor& rstd,
+std::array<Tensor, 3> norm_backward(const Tensor& grad, const Tensor& x, Tensor w, Tensor b, const float* mean, const float* rstd,
                                     std::array<bool, 3> needs) {
     const char* who = "layer_norm_backward";
     require_gpu(x, "x");
     TORCH_CHECK(type_of(x) >= 0 && x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 32768, who, ": x is not one that the forward takes");
     TORCH_CHECK(grad.sizes() == x.sizes() && grad.scalar_type() == x.scalar_type() && grad.device() == x.device(), who, ": grad must match x");
     const int wd = norm_params(x, w, b, who);
-    for (const Tensor* t : {&mean, &rstd})
-        TORCH_CHECK(t->scalar_type() == at::kFloat && t->sizes() == x.sizes().slice(0, x.dim() - 1) && t->device() == x.device() && t->is_contiguous(),
-                    who, ": mean and rstd must be the forward's");
     const c10::DeviceGuard guard(x.device());
     const Tensor r = as_rows(x), g = as_rows(grad);
     Tensor dx, dw, db, work;
@@ -140,7 +143,7 @@ std::array<Tensor, 3> norm_backward(const Tensor& grad, const Tensor& x, Tensor 
         check(size);
         work = at::empty({size}, x.options().dtype(at::kByte));
     }
-    check(q8_layernorm_backward(ptr(g), g.stride(0), ptr(r), type_of(x), r.stride(0), ptr(w), wd, (const float*)ptr(mean), (const float*)ptr(rstd), ptr(dx),
+    check(q8_layernorm_backward(ptr(g), g.stride(0), ptr(r), type_of(x), r.stride(0), ptr(w), wd, mean, rstd, ptr(dx),
                                 ptr(dw), ptr(db), ptr(work), size, r.size(0), (int)r.size(1), stream_of(x)));
     return {dx, dw, db};
 }
@@ -148,15 +151,17 @@ std::array<Tensor, 3> norm_backward(const Tensor& grad, const Tensor& x, Tensor 
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
         const Tensor w = or_none(weight), b = or_none(bias);
-        auto out = norm_forward(x, w, b, eps, true);
-        ctx->save_for_backward({x, w, b, out[1], out[2]});
-        return out[0];
+        std::array<Tensor, 2> stats;
+        Tensor y = norm_forward(x, w, b, eps, &stats, true);
+        ctx->save_for_backward({x, w, b, stats[0]});
+        return y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const auto s = ctx->get_saved_variables();
         // (needs_input_grad counts the tensors that were given)
         const bool w = s[1].defined(), b = s[2].defined();
-        auto d = norm_backward(grads[0], s[0], s[1], s[2], s[3], s[4],
+        const float* mean = (const float*)ptr(s[3]);
+        auto d = norm_backward(grads[0], s[0], s[1], s[2], mean, mean + s[3].size(1),
                                {ctx->needs_input_grad(0), w && ctx->needs_input_grad(1), b && ctx->needs_input_grad(w ? 2 : 1)});
         return once({d[0], d[1], d[2], Tensor()});
     }
@@ -169,7 +174,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
         no_eager_graph(x, {&x, &w, &b}, "layer_norm");
         return LayerNorm::apply(x, given(w), given(b), eps);
     }
-    return norm_forward(x, w, b, eps, false)[0];
+    return norm_forward(x, w, b, eps, nullptr);
 }
 
 // ---- rotary positions --------------------------------------------------------------------------------------------
@@ -386,12 +391,16 @@ PYBIND11_MODULE(_torch_ops, m) {
     });
     m.def("layer_norm", &layer_norm);
     m.def("layer_norm_forward", [](const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, bool stats) {
-        auto r = norm_forward(x, or_none(w), or_none(b), eps, stats);
-        return std::vector<OptTensor>{r[0], given(r[1]), given(r[2])};
+        std::array<Tensor, 2> s;
+        Tensor y = norm_forward(x, or_none(w), or_none(b), eps, stats ? &s : nullptr);
+        return std::vector<OptTensor>{y, given(s[0]), given(s[1])};
     });
     m.def("layer_norm_backward", [](const Tensor& g, const Tensor& x, const OptTensor& w, const OptTensor& b, const Tensor& mean, const Tensor& rstd,
                                     std::array<bool, 3> needs) {
-        auto r = norm_backward(g, x, or_none(w), or_none(b), mean, rstd, needs);
+        for (const Tensor* t : {&mean, &rstd})
+            TORCH_CHECK(x.dim() >= 1 && t->scalar_type() == at::kFloat && t->sizes() == x.sizes().slice(0, x.dim() - 1) && t->device() == x.device() &&
+                            t->is_contiguous(), "layer_norm_backward: mean and rstd must be the forward's");
+        auto r = norm_backward(g, x, or_none(w), or_none(b), (const float*)ptr(mean), (const float*)ptr(rstd), needs);
         return std::vector<OptTensor>{given(r[0]), given(r[1]), given(r[2])};
     });
     m.def("apply_rotary", [](const Tensor& q, const OptTensor& k, const OptTensor& p, const Tensor& f, bool half, double factor) {
