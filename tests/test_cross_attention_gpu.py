@@ -378,3 +378,21 @@ def test_gradients_of_few_keys(dev, b, h, hk, m, n, d, dtype):
     a = _C.cross_attention_backward(g, q, k, v, o, lse, 0.1, lens, mask)
     c = _C.cross_attention_backward(g, q, k.masked_fill(dead, float("inf")), v.masked_fill(dead, float("nan")), o, lse, 0.1, lens, mask)
     assert all(torch.equal(x, y) for x, y in zip(a, c))
+
+
+@pytest.mark.parametrize("n", [90, 300])
+def test_rows_beyond_32_bits(dev, n):
+    """Queries, outputs and their gradients 2^23 elements apart, one after the other in a buffer of 5e9 bytes: the same bits as side by side."""
+    q, k, v = make(dev, 1, 2, 2, 300, n, 64, torch.bfloat16, seed=24)
+    g = torch.randn_like(q)
+    o, lse = _C.cross_attention(q, k, v, 0.1)
+    want = _C.cross_attention_backward(g, q, k, v, o, lse, 0.1)
+    far = torch.empty(300 * 2 ** 23, dtype=torch.bfloat16, device=dev).as_strided((1, 2, 300, 64), (0, 64, 2 ** 23, 1))
+    for i in range(3):
+        side = [q, o, g]
+        far.copy_(side[i])
+        side[i] = far
+        if i == 0:
+            assert all(torch.equal(a, b) for a, b in zip(_C.cross_attention(far, k, v, 0.1), (o, lse)))
+        got = _C.cross_attention_backward(side[2], side[0], k, v, side[1], lse, 0.1)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -234,3 +234,36 @@ def test_capture_beside_an_eager_graph_is_refused(dev):
     assert torch.equal(o, alive.detach())
     with pytest.raises(RuntimeError, match="inv_freq"):
         apply_rotary(q, None, None, f.clone().requires_grad_())
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """The same training step on two streams, calls of both under way together, against one after the other."""
+    leaves, grad, step = leaves_and_step(dev)
+    other = [(0.5 * t.detach() + 0.25).requires_grad_() for t in leaves]
+
+    def run(x):
+        o = step(*x)
+        return (o.detach(),) + torch.autograd.grad(o, x, grad)
+
+    want = [run(leaves), run(other)]
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [[], []]
+    for _ in range(20):
+        for i, x in enumerate((leaves, other)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(x))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for r in got[i] for a, b in zip(r, want[i]))
+
+
+@pytest.mark.gpu
+def test_norm_and_rotary_rows_beyond_32_bits(dev):
+    far = torch.empty(300 * 2 ** 23, dtype=BF16, device=dev).as_strided((300, 512), (2 ** 23, 1))
+    x = torch.randn(300, 512, device=dev).to(BF16)
+    far.copy_(x)
+    assert torch.equal(Q8F.layer_norm.layer_norm(far), Q8F.layer_norm.layer_norm(x))
+    q, f = far.view(1, 300, 8, 64).transpose(1, 2), rotary_frequencies(64)[0].to(dev)
+    assert torch.equal(apply_rotary(q, None, None, f), apply_rotary(x.view(1, 300, 8, 64).transpose(1, 2), None, None, f))
