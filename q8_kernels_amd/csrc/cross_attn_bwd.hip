@@ -622,7 +622,19 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
             const int key0 = (kg * STEPS + i) * 16;
             dq = mfma16<DT>(lds_cols<DP>(kt, key0, db, at), lds_cols<TR>(ds, key0, rb, ds_at), dq);
         }
-        if constexpr (KG > 1) {
+        auto store = [&] {
+            const int r = rb * 32 + (lane & 31);
+            uint16_t* p = a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (int64_t)(m + r) * a.dq.st + db * 32;
+            store_rows<DT, 32>({dq}, a.scale, r < here ? p : nullptr, a.D - db * 32, lane);
+        };
+        // Behind the barrier the next tile is whole and dS has been read. (The sums have been when their writers come back to them:
+        // the barrier in front of the product lies between.)
+        if constexpr (KG == 1) {
+            if (kg == 0) store();
+            finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
+            barrier();
+        } else {
+            finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
             if (kg > 0 && kg < KG) {
                 float* to = sums + ((kg - 1) * NB + block) * 1024 + lane * 4;
 #pragma unroll
@@ -640,15 +652,9 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
                         for (int j = 0; j < 4; ++j) dq[4 * i + j] += x[j];
                     }
                 }
+                store();
             }
         }
-        if (kg == 0) {
-            const int r = rb * 32 + (lane & 31);
-            uint16_t* p = a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (int64_t)(m + r) * a.dq.st + db * 32;
-            store_rows<DT, 32>({dq}, a.scale, r < here ? p : nullptr, a.D - db * 32, lane);
-        }
-        finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
-        __syncthreads();
     };
     auto walk = [&](auto exact) {
         for (int t = t0; t < t1; t += 2) {
