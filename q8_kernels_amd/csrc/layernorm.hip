@@ -16,8 +16,8 @@
 // 16384 elements (8192 where accesses are by element) leave no registers for the sums: a kernel of its own reads x and g once
 // more for them (1000 x 30000: 61 us; with spilled registers in one kernel 172).
 //
-// bf16, 12288 x 2048: forward 19 us (5.3 TB/s, of data partly in the last-level cache), backward 37 us with the parameters' sums
-// (5.5 of them; 4.1 TB/s of what it has to move). What bounds it: HBM, and at the smallest sizes the launches.
+// bf16, 12288 x 2048: forward 19 us (5.3 TB/s, of data partly in the last-level cache), backward 36 us with the parameters' sums
+// (4 of them; 4.2 TB/s of what it has to move). What bounds it: HBM, and at the smallest sizes the launches.
 #include "q8_common.h"
 #include "q8_host.h"
 
@@ -366,7 +366,16 @@ __global__ __launch_bounds__(1024) void layernorm_params_kernel(const float* __r
     const int col = blockIdx.x * 32 + c;  // 0 .. 2 dim - 1: dw's columns, then db's
     float s = 0.f;
     if (col < 2 * dim) {
-        for (int r = k; r < blocks; r += 32) s += partials[(int64_t)r * 2 * dim + col];
+        const float* p = partials + (int64_t)k * 2 * dim + col;
+        int r = k;
+        for (; r + 7 * 32 < blocks; r += 8 * 32, p += (int64_t)8 * 32 * 2 * dim) {  // 8 loads under way at once
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = p[(int64_t)i * 32 * 2 * dim];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
+        for (; r < blocks; r += 32, p += (int64_t)32 * 2 * dim) s += *p;
     }
     part[k][c] = s;
     __syncthreads();
