@@ -130,6 +130,9 @@ struct Rows32 {
     }
 };
 
+// bf16, us: 2 x 16 heads of 128 on 4, 4096 x 4096 275 to 290 (950 to 1000 TFLOP/s; the matrix instructions alone 131 at 2.1 GHz, a
+// rate that their own load does not leave the clock at), 2 x 16 of 64 on 4, 4096 x 4096 176; 8 single tokens, 32 heads of 128 on 8,
+// 8192 keys 32 to 37 (4.1 to 4.7 TB/s of keys and values: HBM).
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     constexpr int ELEMS = kXTile * DP;
@@ -304,15 +307,15 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
-// The kernel for few keys, for heads of 64 or less, wants rows for all the workgroups that run at once.
+// The kernel for few keys, for heads of 64 or less (longer ones leave no registers for the next rows), and how many of its
+// workgroups run at once. us, this kernel and the general one: 16 heads, 1024 x 128 6.2, 6.6; 4 x 16, 512 x 128 6.7, 7.1; 32 x 32,
+// 64 x 64 8.8, 10.7; 64 x 32 on 8, 1 x 100 5.9, 6.8; the other way round only 16 x 16, 300 x 128 11.4, 11.0.
+static bool few_keys(int N, int D) { return D <= 64 && N <= 4 * kXTile; }
 static int few_blocks(int N) { return N <= 2 * kXTile ? 768 : 512; }
-static bool few_keys(int64_t units, int64_t rows, int N, int D) {
-    return D <= 64 && N <= 4 * kXTile && units * rows >= few_blocks(N) * kXRows && rows >= 4 * kXRows;
-}
 
-static XSchedule fwd_plan(int64_t units, int64_t rows, int N, int D, bool ragged) {
-    // workgroups that run at once on the 256 CUs, by the registers of a lane
-    return schedule(units * ((rows + kXRows - 1) / kXRows), N, D <= 32 ? 1024 : D <= 64 ? 768 : 512, ragged ? 2 : 1);
+static XSchedule fwd_plan(int64_t units, int64_t rows, int N, int D) {
+    // workgroups that run at once, by the registers of a lane
+    return schedule(units * ((rows + kXRows - 1) / kXRows), N, D <= 32 ? 1024 : D <= 64 ? 768 : 512, (double)(rows < kXRows ? rows : kXRows) * D);
 }
 
 }  // namespace q8
@@ -322,8 +325,8 @@ using namespace q8;
 extern "C" int64_t q8_cross_attn_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
     if (int e = x_sizes("q8_cross_attn_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
     const int64_t rows = (int64_t)(H / Hkv) * M;
-    if (few_keys(B * Hkv, rows, N, D)) return 0;
-    return fwd_plan(B * Hkv, rows, N, D, true).parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
+    if (few_keys(N, D)) return 0;
+    return fwd_plan(B * Hkv, rows, N, D).parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
@@ -359,7 +362,7 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
     a.row_blocks = (a.R + kXRows - 1) / kXRows;
     if (B * Hkv * a.row_blocks > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (few_keys(B * Hkv, a.R, N, D)) {
+    if (few_keys(N, D)) {
         const int64_t units = B * Hkv, parts = walk_parts(units, a.row_blocks, few_blocks(N), 1);
         if (units * parts > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many heads", who);
         const unsigned grid = (unsigned)(units * parts);
@@ -376,7 +379,7 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
 #undef X_FEW
         return launch_status(who);
     }
-    a.plan = fwd_plan(B * Hkv, a.R, N, D, kv_lens != nullptr);
+    a.plan = fwd_plan(B * Hkv, a.R, N, D);
     if (a.plan.parts()) {
         const int64_t need = a.plan.parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
         if (workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);

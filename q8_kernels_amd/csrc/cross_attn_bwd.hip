@@ -40,6 +40,8 @@ struct XBwd {
     float* part;         // divided blocks: [splits, tail, 128, D], or [splits, tail, 128, 2 D] (dK, dV)
 };
 
+// bf16, 2 x 16 heads of 128 on 4, 4096 x 4096: 370 us (three products, 1110 TFLOP/s); operands in groups of 2: with groups of 4, as
+// in the forward, 394.
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_kernel(XBwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32, ELEMS = kXTile * DP;
@@ -206,7 +208,8 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
 
 // A head of more than 96 leaves no registers for V beside K and the two sums (two waves a SIMD have 256 each): V stays in
 // LDS, the rows are walked in tiles of 32, and the order of the instructions is the compiler's (keeping the groups apart costs
-// registers that have to be spilled).
+// registers that have to be spilled). bf16, 2 x 16 heads of 128 on 4, 4096 x 4096: 495 us (four products, 1110 TFLOP/s; 784 with V
+// in registers, staged through registers and spilled).
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32;
@@ -413,8 +416,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
 // the compiler's order of instructions: what two waves on a SIMD have registers for (43 spilled ones otherwise; 2 x 32 heads of
 // 128, 6144 rows, 128 keys: 166 us, with 9 spilled ones 138).
 //
-// bf16, 2 x 32 heads of 64, 6144 rows, 256 keys: 100 us and 7 for the parts (200 MB at 2.0 TB/s; 40 MFMA of a wave and tile would
-// take 30 us, exp2 and the roundings of P and dS about as long, and between the two barriers of a tile they overlap only in part).
+// bf16, 2 x 32 heads of 64, 6144 rows, 256 keys: 97 us and 7 for the parts (200 MB at 2.1 TB/s; the matrix pipes are busy 29 % of
+// the time, the vector units 33 %, LDS 32 %: between the two barriers of a tile the two waves of a SIMD are in the same phase).
 template <int DT, int DP, int W>
 __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd a, int parts) {
     constexpr bool LONG = DP > 64;
@@ -734,8 +737,8 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     const int64_t tiles = (int64_t)(H / Hkv) * (((int64_t)M + kXTile - 1) / kXTile);
     // The kernel for few keys, a workgroup for four tiles of 64 rows or more: one of 8 waves on a CU, or two of 4 (LDS). bf16 times,
     // this kernel against the other two (B x H x M x N x D), us:
-    //   2 x 32 x 6144 x 256 x 64   110, 146     2 x 32 x 6144 x 128 x 64   65, 97     2 x 32 x 6144 x 128 x 128   138, 229
-    //   2 x 32 x 6144 x 256 x 128  208, 292     2 x 32 x 6144 x 256 x 96  150, 211    11 x 4 x 8 x 2836 x 16 x 128  314, 424
+    //   2 x 32 x 6144 x 256 x 64   111, 146     2 x 32 x 6144 x 128 x 64   65, 97     2 x 32 x 6144 x 128 x 128   138, 229
+    //   2 x 32 x 6144 x 256 x 128  201, 292     2 x 32 x 6144 x 256 x 96  150, 211    11 x 4 x 8 x 2836 x 16 x 128  314, 424
     //   1 x 32 x 2048 x 128 x 64   25, 34       1 x 16 x 1024 x 64 x 64    18, 19     16 x 32 x 256 x 128 x 64     28, 45
     // With 129 to 256 keys it takes 1024 tiles to be faster: 8 x 8192 x 256 x 64 38 against 48, but 16 x 2048 x 256 x 64 (512
     // tiles) 32.2 against 31.5, 8 x 512 x 256 x 64 24.6 against 22.5, 16 x 2048 x 256 x 128 51.3 against 51.0.
@@ -748,9 +751,11 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
         p.parts = p.kv.parts() * kXRows * 2 * D;
         return p;
     }
-    // workgroups that run at once on the 256 CUs, by the registers of a lane
-    p.dq = schedule(p.units * p.dq_blocks, N, D <= 32 ? 1024 : D <= 64 ? 768 : 512);
-    p.kv = schedule(p.units * p.kv_blocks, tiles * kXTile, D <= 32 ? 1024 : 512);
+    // Workgroups that run at once on the 256 CUs, by the registers of a lane. A tile takes these kernels 1.3 and 1.7 times what it
+    // takes the forward, which is what the floats of a part (for dK and dV twice as many) are weighed with: 8 heads of 128,
+    // 1024 x 1024 58 us with dK and dV in 4 parts, 71 in one.
+    p.dq = schedule(p.units * p.dq_blocks, N, D <= 32 ? 1024 : D <= 64 ? 768 : 512, 0.75 * (p.rows < kXRows ? p.rows : kXRows) * D);
+    p.kv = schedule(p.units * p.kv_blocks, tiles * kXTile, D <= 32 ? 1024 : 512, (double)(N < kXRows ? N : kXRows) * D);
     const int64_t dq = p.dq.parts() * kXRows * D, kv = p.kv.parts() * kXRows * 2 * D;
     p.parts = dq > kv ? dq : kv;  // one after the other in the same place
     return p;

@@ -309,18 +309,30 @@ struct XSchedule {
     unsigned grid() const { return full + 8u * ((tail * splits + 7) / 8); }
     int64_t parts() const { return splits > 1 ? (int64_t)tail * splits : 0; }  // blocks of partial results
 };
-// `slots`: workgroups that run at once; a divided walk is four tiles or more. `turns`: how many times the workgroups of the
-// divided blocks may fill the card: with lengths that differ, pieces half as long even them out.
-inline XSchedule schedule(int64_t blocks, int64_t length, int slots, int turns = 1) {
+// `slots`: workgroups that run at once on the 256 CUs; `length`: of a walk; `floats`: of a block's partial result. The blocks left
+// are divided (into parts of four tiles or more) with the number that ends first by this estimate, in tiles: a workgroup takes one
+// tile's time longer than its walk; a CU with one workgroup on it works a tile off faster than one with all its slots taken (half
+// the slots: 0.6 of the time); parts are written, read and joined: 6 tiles' time for 128 x 128 floats of every slot, and 2 for the
+// launch. Forward, us: 3 x 16 heads of 128, 700 x 700 (288 blocks) 22 whole, 41 in three parts; 8 x 16 heads of 64, 512 x 2048 (512
+// blocks) 46 whole, 62 in two; 8 single tokens, 8192 keys (64 blocks) 35 in 8 parts, 37 in 16, 43 in 32.
+inline XSchedule schedule(int64_t blocks, int64_t length, int slots, double floats) {
     XSchedule s;
     s.full = (unsigned)(blocks / slots * slots);
     s.tail = (unsigned)(blocks - s.full);
-    const int64_t most = ((length + kXTile - 1) / kXTile + 3) / 4, want = s.tail ? (int64_t)slots * turns / s.tail : 1;
-    s.splits = (int)(want < most ? want : most);
-    if (s.splits < 1) s.splits = 1;
+    s.splits = 1;
+    const int64_t tiles = (length + kXTile - 1) / kXTile, most = (tiles + 3) / 4;
+    double cost = 1e300;
+    for (int cus = 0; s.tail && cus <= 2 * slots; cus += 256) {  // whole, or the most parts that so many places take
+        int64_t n = cus / s.tail;
+        n = n < most ? n : most;
+        n = n < 1 ? 1 : n;
+        const double groups = (double)s.tail * n, load = (groups > 256 ? groups : 256) / slots;
+        const double turns = load <= 1 ? 0.25 + 0.75 * load : (double)(int64_t)((groups + slots - 1) / slots);
+        const double c = turns * ((double)((tiles + n - 1) / n) + 1) + (n > 1 ? 6 * groups / slots * floats / (kXRows * 128) + 2 : 0);
+        if (c < cost) { cost = c; s.splits = (int)n; }
+    }
     return s;
 }
-
 // Into how many parts each of `units` walks of `steps` goes, `least` steps each or more, when `slots` workgroups run at once: the
 // number with which the last one ends first, a workgroup costing about two steps beside its walk. (44 walks of 360 tiles on 512
 // slots, backward with 16 keys of 128: 11 parts 314 us; 12, whose last 16 workgroups wait for a free place, 476.)
