@@ -267,3 +267,66 @@ def test_norm_and_rotary_rows_beyond_32_bits(dev):
     assert torch.equal(Q8F.layer_norm.layer_norm(far), Q8F.layer_norm.layer_norm(x))
     q, f = far.view(1, 300, 8, 64).transpose(1, 2), rotary_frequencies(64)[0].to(dev)
     assert torch.equal(apply_rotary(q, None, None, f), apply_rotary(x.view(1, 300, 8, 64).transpose(1, 2), None, None, f))
+
+
+@pytest.mark.gpu
+def test_forms_of_the_calls(dev):
+    """Arguments that mean the same give the same bits: one and many dimensions, views, one tensor in two places, parts that need no gradient."""
+    gen = torch.Generator(device=dev).manual_seed(5)
+    rnd = lambda *s: torch.randn(s, generator=gen, device=dev)  # noqa: E731
+    norm, attend = Q8F.layer_norm.layer_norm, Q8F.cross_attention.cross_attention
+    x, w, b = rnd(3, 4, 5, 72).to(BF16), 1 + 0.1 * rnd(72), rnd(72)
+    flat = norm(x.reshape(60, 72), w, b)
+    assert torch.equal(norm(x, w, b).reshape(60, 72), flat) and torch.equal(norm(x[1, 2, 3], w, b), flat[33])
+    assert torch.equal(norm(x.transpose(0, 2), w, b).transpose(0, 2).reshape(60, 72), flat)
+    assert torch.equal(norm(x.reshape(60, 72), torch.stack((w, w), 1)[:, 0], b), flat)
+    one = x[0, 0, 0].clone().requires_grad_()
+    wg = w.clone().requires_grad_()
+    g = rnd(72).to(BF16)
+    d1, dw = torch.autograd.grad(norm(one, wg, b), (one, wg), g)
+    d2 = torch.autograd.grad(norm(x[0, 0, 0], wg, b), wg, g)[0]
+    assert d1.shape == (72,) and torch.equal(dw, d2)
+
+    q, k, v = (rnd(2, n, h, 64).to(BF16).transpose(1, 2) for n, h in ((40, 8), (70, 2), (70, 2)))
+    lens, mask, go = torch.tensor([70, 33], dtype=torch.int32, device=dev), rnd(2, 70) > -1, rnd(2, 8, 40, 64).to(BF16)
+    want = attend(q, k, v, None, lens, mask)
+    assert torch.equal(attend(q, k, v, 0.125, torch.stack((lens, lens), 1)[:, 0], mask.t().contiguous().t()), want)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    every = torch.autograd.grad(attend(*leaves, None, lens, mask), leaves, go)
+    for i in range(3):
+        args = [leaves[j] if j == i else leaves[j].detach() for j in range(3)]
+        assert torch.equal(torch.autograd.grad(attend(*args, None, lens, mask), leaves[i], go)[0], every[i])
+    both = torch.autograd.grad(attend(leaves[0], leaves[1], leaves[1], None, lens, mask), leaves[1], go)[0]
+    twice = [leaves[1].detach().requires_grad_() for _ in range(2)]
+    apart = torch.autograd.grad(attend(leaves[0], *twice, None, lens, mask), twice, go)
+    assert torch.equal(both, apart[0] + apart[1])
+    # a shared key head is the same as its copies, gradients summed
+    wide = [leaves[0]] + [t.detach().repeat_interleave(4, 1).requires_grad_() for t in leaves[1:]]
+    o = attend(*wide, None, lens, mask)
+    assert torch.equal(o, want)
+    copies = torch.autograd.grad(o, wide, go)
+    assert torch.equal(copies[0], every[0])
+    for a, c in zip(every[1:], copies[1:]):
+        c = c.double().view(2, 2, 4, 70, 64)
+        # each copy is rounded once, and the shared one too; P and dS are the same
+        assert ((a.double() - c.sum(2)).abs() <= 2.0 ** -8 * (a.double().abs() + c.abs().sum(2)) + 1e-5).all()
+
+    f, positions = rotary_frequencies(64)[0].to(dev), torch.randint(0, 9999, (2, 40), generator=gen, device=dev)
+    turned = apply_rotary(q, None, positions, f)
+    assert torch.equal(apply_rotary(q, None, positions.t().contiguous().t().int(), f), turned)
+    assert torch.equal(apply_rotary(q[:1], None, positions[:1], f), turned[:1]) and torch.equal(apply_rotary(q[:1], None, positions[0], f), turned[:1])
+    assert torch.equal(apply_rotary(q, q, positions, f)[1], turned)
+
+
+@pytest.mark.gpu
+def test_attention_module_self_attention_with_positions(dev):
+    from q8_kernels_amd.modules import Attention, Q8Linear
+    torch.manual_seed(1)
+    attn = Attention(256, 4, 64, bias=True, out_bias=True, qk_rms_norm=True, use_rope=True).to(dev)
+    for name in ("to_q", "to_k", "to_v", "to_out"):
+        setattr(attn, name, Q8Linear.from_linear(torch.nn.Linear(256, 256, device=dev, dtype=BF16)))
+    x = torch.randn(2, 60, 256, device=dev, dtype=BF16)
+    angle = torch.rand(2, 60, 128, device=dev).repeat_interleave(2, -1) * 6
+    with torch.no_grad():
+        a, t = (attn(x, freqs_cis=(angle.cos(), angle.sin()), mm_out_dtype=BF16, attn_type=kind) for kind in ("16bit", "torch"))
+    assert torch.nn.functional.cosine_similarity(a.float().flatten(), t.float().flatten(), dim=0) > 0.999
