@@ -307,11 +307,12 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
-// The kernel for few keys, for heads of 64 or less (longer ones leave no registers for the next rows), and how many of its
-// workgroups run at once. us, this kernel and the general one: 16 heads, 1024 x 128 6.2, 6.6; 4 x 16, 512 x 128 6.7, 7.1; 32 x 32,
-// 64 x 64 8.8, 10.7; 64 x 32 on 8, 1 x 100 5.9, 6.8; the other way round only 16 x 16, 300 x 128 11.4, 11.0.
-static bool few_keys(int N, int D) { return D <= 64 && N <= 4 * kXTile; }
-static int few_blocks(int N) { return N <= 2 * kXTile ? 768 : 512; }
+// The kernel for few keys: 256 for heads up to 64, 128 for longer ones (two workgroups on a CU, by LDS), and how many of its
+// workgroups run at once. us, this kernel and the general one, heads of 64: 16 heads, 1024 x 128 6.2, 6.6; 32 x 32, 64 x 64 8.8,
+// 10.7; 64 x 32 on 8, 1 x 100 5.9, 6.8; the other way round only 16 x 16, 300 x 128 11.4, 11.0. Of 128: 2 x 32, 6144 x 128 59, 71;
+// 32, 1 x 128 6.5, 7.2. Of 96: 2 x 32, 6144 x 128 42, 56; 32 x 32, 64 x 64 16.0, 15.5; 13 x 16 on 8, 3610 x 1 98, 93.
+static bool few_keys(int N, int D) { return N <= (D <= 64 ? 4 : 2) * kXTile; }
+static int few_blocks(int N, int D) { return D <= 64 && N <= 2 * kXTile ? 768 : 512; }
 
 static XSchedule fwd_plan(int64_t units, int64_t rows, int N, int D) {
     // workgroups that run at once, by the registers of a lane
@@ -363,13 +364,15 @@ extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void
     if (B * Hkv * a.row_blocks > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (few_keys(N, D)) {
-        const int64_t units = B * Hkv, parts = walk_parts(units, a.row_blocks, few_blocks(N), 1);
+        const int64_t units = B * Hkv, parts = walk_parts(units, a.row_blocks, few_blocks(N, D), 1);
         if (units * parts > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many heads", who);
         const unsigned grid = (unsigned)(units * parts);
 #define X_FEW(DT, NT)                                                                                        \
     do {                                                                                                     \
         if (D <= 32) cross_attn_few_keys_kernel<DT, 32, NT><<<grid, kXThreads, 0, st>>>(a, (int)parts);      \
-        else cross_attn_few_keys_kernel<DT, 64, NT><<<grid, kXThreads, 0, st>>>(a, (int)parts);              \
+        else if (D <= 64) cross_attn_few_keys_kernel<DT, 64, NT><<<grid, kXThreads, 0, st>>>(a, (int)parts); \
+        else if (D <= 96) cross_attn_few_keys_kernel<DT, 96, 2><<<grid, kXThreads, 0, st>>>(a, (int)parts);  \
+        else cross_attn_few_keys_kernel<DT, 128, 2><<<grid, kXThreads, 0, st>>>(a, (int)parts);              \
     } while (0)
         if (N <= 2 * kXTile) {
             if (dt == Q8_BF16) X_FEW(Q8_BF16, 2); else X_FEW(Q8_F16, 2);
