@@ -425,6 +425,10 @@ int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_
  * kv_lens: int32 [B], clamped to 0 .. N, or NULL = N; key_mask: one byte per key [B, N] with a row stride in bytes, 0 = does
  * not count, or NULL. Keys and values that do not count are not read into any result; their gradients are zeros.
  * lse: fp32 [B, H, M] (forward: NULL = not wanted). softmax_scale positive and finite.
+ * o_low int8 [B, H, M, D], contiguous, 16-byte aligned: what rounding o to dt left off, 8 further bits of its fp32 code (in units
+ * of 2^8 for BF16, 2^5 for F16). The backward forms rowsum(do o) from o and o_low: the rounding of o alone would be an error in
+ * every ds of its row. q8_cross_attn_train writes o, o_low and lse, q8_cross_attn_train_backward reads them;
+ * q8_cross_attn_backward does the forward's work once more to form o_low.
  * The workspaces hold partial sums (the forward's: 0 bytes where none are needed); a negative size is an error code. They are
  * written before they are read and may be reused as soon as the call's work on the stream is done.
  */
@@ -433,6 +437,17 @@ int q8_cross_attn(const void* q, const int64_t* q_strides, const void* k, const 
                   const int64_t* v_strides, void* o, const int64_t* o_strides, float* lse, const int32_t* kv_lens,
                   const uint8_t* key_mask, int64_t mask_row_stride, int dt, float softmax_scale, int64_t B, int H, int Hkv, int M,
                   int N, int D, void* workspace, int64_t workspace_bytes, q8_stream_t stream);
+int q8_cross_attn_train(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, void* o, const int64_t* o_strides, void* o_low, float* lse, const int32_t* kv_lens,
+                        const uint8_t* key_mask, int64_t mask_row_stride, int dt, float softmax_scale, int64_t B, int H, int Hkv,
+                        int M, int N, int D, void* workspace, int64_t workspace_bytes, q8_stream_t stream);
+int64_t q8_cross_attn_train_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D);
+int q8_cross_attn_train_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides,
+                                 const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* o,
+                                 const int64_t* o_strides, const void* o_low, const float* lse, void* dq, const int64_t* dq_strides,
+                                 void* dk, const int64_t* dk_strides, void* dv, const int64_t* dv_strides, const int32_t* kv_lens,
+                                 const uint8_t* key_mask, int64_t mask_row_stride, int dt, float softmax_scale, int64_t B, int H,
+                                 int Hkv, int M, int N, int D, void* workspace, int64_t workspace_bytes, q8_stream_t stream);
 int64_t q8_cross_attn_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D);
 int q8_cross_attn_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides, const void* k,
                            const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* o,

@@ -785,14 +785,16 @@ def rotary(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: Opti
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, kv_lens: Optional[torch.Tensor] = None,
-                    key_mask: Optional[torch.Tensor] = None, *, stats: bool = True) -> List[Optional[torch.Tensor]]:
+                    key_mask: Optional[torch.Tensor] = None, *, stats: bool = True, rest: bool = False) -> List[Optional[torch.Tensor]]:
     """[o (q's shape, type and memory order), lse (float32 [B, H, M], log2 of the sum of 2^(score * log2 e); +inf where no key
-    counts; None without stats)], see functional.cross_attention.cross_attention."""
-    return _lib.ops().cross_attention_forward(q, k, v, softmax_scale, kv_lens, key_mask, stats)
+    counts; None without stats)], and with rest o_low (int8 [B, H, M, D], contiguous: what the rounding of o left off, for
+    the backward); see functional.cross_attention.cross_attention."""
+    return _lib.ops().cross_attention_forward(q, k, v, softmax_scale, kv_lens, key_mask, stats, rest)
 
 
 def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                              softmax_scale: float, kv_lens: Optional[torch.Tensor] = None,
-                             key_mask: Optional[torch.Tensor] = None) -> List[torch.Tensor]:
-    """[dq, dk, dv] in the memory orders of q, k and v; o and lse as the forward gave them."""
-    return _lib.ops().cross_attention_backward(grad, q, k, v, o, lse, softmax_scale, kv_lens, key_mask)
+                             key_mask: Optional[torch.Tensor] = None, *, o_low: Optional[torch.Tensor] = None) -> List[torch.Tensor]:
+    """[dq, dk, dv] in the memory orders of q, k and v; o, lse and o_low as the forward gave them. Without o_low the forward's work
+    is done once more to form it (the same bits)."""
+    return _lib.ops().cross_attention_backward(grad, q, k, v, o, lse, softmax_scale, kv_lens, key_mask, o_low)

@@ -62,9 +62,13 @@ SIGNATURES = {
     "q8_rotary": (_i, [_vp, _i64p, _vp, _i64p, _i, _vp, _i64p, _vp, _i64p, _i, _i, _vp, _i, _i64, _vp, _i, _i, _f, _i, _i64, _i64, _i, _vp]),
     "q8_cross_attn_workspace": (_i64, [_i64, _i, _i, _i, _i, _i]),
     "q8_cross_attn": (_i, [_vp, _i64p] * 4 + [_vp, _vp, _vp, _i64, _i, _f, _i64, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
+    "q8_cross_attn_train": (_i, [_vp, _i64p] * 4 + [_vp, _vp, _vp, _vp, _i64, _i, _f, _i64, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
     "q8_cross_attn_backward_workspace": (_i64, [_i64, _i, _i, _i, _i, _i]),
+    "q8_cross_attn_train_backward_workspace": (_i64, [_i64, _i, _i, _i, _i, _i]),
     "q8_cross_attn_backward": (_i, [_vp, _i64p] * 5 + [_vp] + [_vp, _i64p] * 3 + [_vp, _vp, _i64, _i, _f, _i64, _i, _i, _i, _i, _i, _vp, _i64,
                                                                                   _vp]),
+    "q8_cross_attn_train_backward": (_i, [_vp, _i64p] * 5 + [_vp, _vp] + [_vp, _i64p] * 3 + [_vp, _vp, _i64, _i, _f, _i64, _i, _i, _i, _i, _i,
+                                                                                              _vp, _i64, _vp]),
     "q8_attn_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i64, _f, _i, _i, _vp]),
 }
 

@@ -7,6 +7,12 @@
 // product (as its operand has to be), relative to a maximum that trails the running one by at most 2^8, so the rounding is
 // a relative one. O is rescaled only when the maximum has grown beyond that.
 //
+// O is divided by the sum of the rounded P, so it is a mean of the values with weights that add up to one: with relative
+// roundings r_j it is off by sum_j r_j P_j (v_j - O), not by sum_j r_j P_j v_j, and what a training step forms from it,
+// delta = dO . O, by sum_j r_j dS_j. (The log-sum has the sum of the unrounded P, which the backward forms P from.) The
+// rounding of O itself would be an error of every score's gradient in the row, which where few keys count or a few take most
+// of the row is larger than the gradient's own rounding: 2 to 6 roundings. So a training step keeps 8 bits of what it left off.
+//
 // Row blocks that do not fill the card: their keys are divided over several workgroups, whose unnormalised results, maxima and
 // sums a second kernel joins.
 #include "cross_attn_common.h"
@@ -17,29 +23,30 @@ namespace q8 {
 
 struct XFwd {
     XTensor q, k, v;
-    XOut o;
+    XOut o;              // p NULL: not wanted
+    uint8_t* o_low;      // [units, R, D]: what the rounding of O to 16 bits left off. NULL: not wanted
     float* lse;          // [units, R]: log2 of the sum of exp2 (c s); +inf: no key counts. NULL: not wanted
     XKeys keys;
     float c;             // softmax scale * log2 e
     int Hkv, G, M, D, R;
     int row_blocks;         // of a unit
     XSchedule plan;
-    float *part, *pm, *pl;  // divided blocks: [splits, tail, 128, D], [splits, tail, 128] twice
+    float *part, *pm, *pw, *pl;  // divided blocks: [splits, tail, 128, D], [splits, tail, 128] three times
 };
 
-// One wave's rows: Q^T as operands, the running state of their softmax.
-template <int DT, int DP>
+// One wave's rows: Q^T as operands, the running state of their softmax. STATS: the log-sum is wanted.
+template <int DT, int DP, bool STATS>
 struct Rows32 {
     static constexpr int KS = DP / 16, DTL = DP / 32;
     v4u qf[KS];
     v16f acc[DTL];
-    float m, l;  // m in units of log2; l: the sum over this lane's half of the keys
+    float m, w, l;  // m in units of log2; w, l: the sums of P as it is rounded and as it was, over this lane's half of the keys
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int t = 0; t < DTL; ++t) acc[t] = splat16(0.f);
         m = -3.0e38f;
-        l = 0.f;
+        w = l = 0.f;
     }
     __device__ __forceinline__ void load(const XFwd& a, int b, int hk, int row, int half) {
         const int g = row < a.R ? row / a.M : 0, i = row - g * a.M;
@@ -84,7 +91,8 @@ struct Rows32 {
         if (__builtin_amdgcn_ballot_w64(grown) != 0) {
             const float next = grown ? top : m, f = __builtin_amdgcn_exp2f(m - next);
             m = next;
-            l *= f;
+            w *= f;
+            if constexpr (STATS) l *= f;
 #pragma unroll
             for (int d = 0; d < DTL; ++d)
 #pragma unroll
@@ -94,7 +102,7 @@ struct Rows32 {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -m));
-                l += s[u][i];
+                if constexpr (STATS) l += s[u][i];
             }
         };
         weights(0);
@@ -106,6 +114,8 @@ struct Rows32 {
             if (i == 0) weights(1);  // beside the matrix instructions of the first half
 #pragma unroll
             for (int d = 0; d < DTL; ++d) acc[d] = mfma16<DT>(ops.f[i & 1][d], p, acc[d]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w = add_pair<DT>(p[j], w);
             if (i == 0) {
 #pragma unroll
                 for (int d = 0; d < DTL; ++d) {
@@ -116,24 +126,33 @@ struct Rows32 {
             fence();
         }
     }
-    // the sum over all keys
+    // the sums over all keys
+    static __device__ __forceinline__ float both_halves(float x) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
     __device__ __forceinline__ void join_halves() {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-        l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        w = both_halves(w);
+        if constexpr (STATS) l = both_halves(l);
     }
     // log-sum and O
     __device__ __forceinline__ void finish(const XFwd& a, int unit, int b, int hk, int row, int lane) const {
-        if (a.lse != nullptr && row < a.R && lane < 32) a.lse[(int64_t)unit * a.R + row] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
-        const int g = row < a.R ? row / a.M : 0;
-        uint16_t* p = row < a.R ? a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (row - g * a.M) * a.o.st : nullptr;
-        store_rows<DT, DP>(acc, l == 0.f ? 0.f : 1.0f / l, p, a.D, lane);
+        const bool in = row < a.R;
+        const int64_t at = (int64_t)unit * a.R + row;
+        if constexpr (STATS) {
+            if (in && lane < 32) a.lse[at] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
+        }
+        const int g = in ? row / a.M : 0;
+        const float inv = w == 0.f ? 0.f : 1.0f / w;
+        if (a.o.p != nullptr) store_rows<DT, DP>(acc, inv, in ? a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (row - g * a.M) * a.o.st : nullptr, a.D, lane);
+        if (a.o_low != nullptr) store_rests<DT, DP>(acc, inv, in ? a.o_low + at * a.D : nullptr, a.D, lane);
     }
 };
 
 // bf16, us: 2 x 16 heads of 128 on 4, 4096 x 4096 275 to 290 (950 to 1000 TFLOP/s; the matrix instructions alone 131 at 2.1 GHz, a
 // rate that their own load does not leave the clock at), 2 x 16 of 64 on 4, 4096 x 4096 176; 8 single tokens, 32 heads of 128 on 8,
 // 8192 keys 32 to 37 (4.1 to 4.7 TB/s of keys and values: HBM).
-template <int DT, int DP>
+template <int DT, int DP, bool STATS>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     constexpr int ELEMS = kXTile * DP;
     __shared__ __align__(16) uint16_t k0[ELEMS], k1[ELEMS], v0[ELEMS], v1[ELEMS];
@@ -146,7 +165,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int row0 = rb * kXRows + wave * 32, row = row0 + (lane & 31);
 
-    Rows32<DT, DP> rows;
+    Rows32<DT, DP, STATS> rows;
     rows.load(a, b, hk, row, half);
     KVTiles<DP> kv;
     kv.len = a.keys.length(b);
@@ -192,7 +211,11 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     if (of > 1) {
         if (row < z.R) {
             const int64_t to = ((int64_t)split * z.plan.tail + (block - z.plan.full)) * kXRows + wave * 32 + (lane & 31);
-            if (half == 0) { z.pm[to] = rows.m; z.pl[to] = rows.l; }
+            if (half == 0) {
+                z.pm[to] = rows.m;
+                z.pw[to] = rows.w;
+                if constexpr (STATS) z.pl[to] = rows.l;
+            }
             float* p = z.part + to * z.D;
 #pragma unroll
             for (int d = 0; d < rows.DTL; ++d)
@@ -211,7 +234,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
 // by itself, without a barrier; the next 32 rows of Q are on their way meanwhile. The kernel above would fill LDS again for
 // every 128 rows. 2 x 32 heads of 64, ragged lengths: 6144 x 128 keys (NT = 2, three workgroups on a CU) 30 us here and 38 to
 // 48 us there, 6144 x 256 keys (NT = 4, two workgroups) 47 us here and 57 us there.
-template <int DT, int DP, int NT>
+template <int DT, int DP, int NT, bool STATS>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd a, int parts) {
     constexpr int ELEMS = kXTile * DP, KS = DP / 16;
     __shared__ __align__(16) uint16_t k[NT * ELEMS], v[NT * ELEMS];
@@ -222,7 +245,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd 
     const int step = parts * kXRows;
     int row = part * kXRows + wave * 32 + (lane & 31);
 
-    Rows32<DT, DP> rows;
+    Rows32<DT, DP, STATS> rows;
     rows.load(a, b, hk, row, half);
     KVTiles<DP> kv;
     kv.len = a.keys.length(b);
@@ -247,7 +270,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd 
 
     LaneOffsets<DP> at(lane);
     for (int row0 = part * kXRows + wave * 32; row0 < a.R; row0 += step, row += step) {
-        Rows32<DT, DP> ahead;
+        Rows32<DT, DP, STATS> ahead;
         ahead.load(a, b, hk, row + step, half);
         rows.clear();
         for (int t = 0; t < tiles; ++t) {
@@ -271,17 +294,19 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     const int unit = block / a.row_blocks, r = (int)(block - unit * a.row_blocks) * kXRows + (int)(n - tail * kXRows);
     if (n >= all || r >= a.R) return;
     const int e = (int)(id - n * lanes) * 4;
-    float m = -3.0e38f, l = 0.f;
+    float m = -3.0e38f, w = 0.f, l = 0.f;
     v4f o = {0.f, 0.f, 0.f, 0.f};
+    const float* pls = a.lse != nullptr ? a.pl : a.pw;  // (without a log-sum: anything)
     for (int i0 = 0; i0 < a.plan.splits; i0 += BATCH) {
-        float pm[BATCH], pl[BATCH];
+        float pm[BATCH], pw[BATCH], pl[BATCH];
         v4f po[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const bool in = i0 + i < a.plan.splits;
             const int64_t at = (int64_t)(in ? i0 + i : i0) * all + n;
             pm[i] = in ? a.pm[at] : -3.0e38f;
-            pl[i] = in ? a.pl[at] : 0.f;
+            pw[i] = in ? a.pw[at] : 0.f;
+            pl[i] = in ? pls[at] : 0.f;
             po[i] = *reinterpret_cast<const v4f*>(a.part + at * a.D + e);
         }
         float top = m;
@@ -289,22 +314,28 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
         for (int i = 0; i < BATCH; ++i) top = max_ieee(top, pm[i]);
         const float f = __builtin_amdgcn_exp2f(m - top);
         m = top;
+        w *= f;
         l *= f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] *= f;
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-            const float w = i0 + i < a.plan.splits ? __builtin_amdgcn_exp2f(pm[i] - m) : 0.f;
-            l += w * pl[i];
+            const float share = i0 + i < a.plan.splits ? __builtin_amdgcn_exp2f(pm[i] - m) : 0.f;
+            w += share * pw[i];
+            l += share * pl[i];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] += w * po[i][j];
+            for (int j = 0; j < 4; ++j) o[j] += share * po[i][j];
         }
     }
     if (a.lse != nullptr && e == 0) a.lse[(int64_t)unit * a.R + r] = l == 0.f ? __builtin_inff() : m + __builtin_log2f(l);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = w == 0.f ? 0.f : 1.0f / w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] *= inv;
     const int g = r / a.M, b = unit / a.Hkv, hk = unit - b * a.Hkv;
-    uint16_t* p = a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (int64_t)(r - g * a.M) * a.o.st;
-    *reinterpret_cast<v2i*>(p + e) = v2i{(int)pack2<DT>(o[0] * inv, o[1] * inv), (int)pack2<DT>(o[2] * inv, o[3] * inv)};
+    const uint32_t x = pack2<DT>(o[0], o[1]), y = pack2<DT>(o[2], o[3]);
+    if (a.o.p != nullptr) *reinterpret_cast<v2i*>(a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + (int64_t)(r - g * a.M) * a.o.st + e) = v2i{(int)x, (int)y};
+    if (a.o_low != nullptr)
+        *reinterpret_cast<uint32_t*>(a.o_low + ((int64_t)unit * a.R + r) * a.D + e) = rests_of<DT>(o[0], o[1], o[2], o[3], x, y);
 }
 
 // The kernel for few keys: 256 for heads up to 64, 128 for longer ones (two workgroups on a CU, by LDS), and how many of its
@@ -319,97 +350,130 @@ static XSchedule fwd_plan(int64_t units, int64_t rows, int N, int D) {
     return schedule(units * ((rows + kXRows - 1) / kXRows), N, D <= 32 ? 1024 : D <= 64 ? 768 : 512, (double)(rows < kXRows ? rows : kXRows) * D);
 }
 
+static int64_t part_bytes(const XSchedule& plan, int D) { return plan.parts() * kXRows * (D + 3) * (int64_t)sizeof(float); }
+
+int64_t cross_attn_forward_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
+    return few_keys(N, D) ? 0 : part_bytes(fwd_plan(B * Hkv, (int64_t)(H / Hkv) * M, N, D), D);
+}
+
+int cross_attn_forward(const char* who, const XForward& c) {
+    if (int e = x_sizes(who, c.dt, c.B, c.H, c.Hkv, c.M, c.N, c.D, c.softmax_scale)) return e;
+    const int N = c.N, D = c.D;
+    if (c.B == 0 || c.M == 0) return Q8_OK;
+    if (int e = x_tensor(who, "q", c.q, c.q_strides, c.B, c.H, c.M, D)) return e;
+    if (c.o != nullptr || c.o_low == nullptr)
+        if (int e = x_tensor(who, "o", c.o, c.o_strides, c.B, c.H, c.M, D)) return e;
+    if (N) {
+        if (int e = x_tensor(who, "k", c.k, c.k_strides, c.B, c.Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "v", c.v, c.v_strides, c.B, c.Hkv, N, D)) return e;
+    }
+    if (!aligned16(c.o_low)) return fail(Q8_ERR_ALIGN, "%s: o_low must be 16-byte aligned", who);
+    if ((reinterpret_cast<uintptr_t>(c.lse) & 3) || (reinterpret_cast<uintptr_t>(c.kv_lens) & 3)) return fail(Q8_ERR_ALIGN, "%s: lse or kv_lens not aligned", who);
+    if (c.key_mask && (c.mask_row_stride < 0 || (c.B > 1 && c.mask_row_stride > INT64_MAX / 2 / c.B))) return fail(Q8_ERR_SHAPE, "%s: row stride of the mask", who);
+    XFwd a{};
+    static const int64_t none[3] = {0, 0, 0};
+    const int64_t *ks = N ? c.k_strides : none, *vs = N ? c.v_strides : none, *os = c.o ? c.o_strides : none;
+    a.q = XTensor{static_cast<const uint16_t*>(c.q), c.q_strides[0], c.q_strides[1], c.q_strides[2]};
+    a.k = XTensor{static_cast<const uint16_t*>(c.k), ks[0], ks[1], ks[2]};
+    a.v = XTensor{static_cast<const uint16_t*>(c.v), vs[0], vs[1], vs[2]};
+    a.o = XOut{static_cast<uint16_t*>(c.o), os[0], os[1], os[2]};
+    a.o_low = static_cast<uint8_t*>(c.o_low);
+    a.lse = c.lse;
+    a.keys = XKeys{c.kv_lens, c.key_mask, c.mask_row_stride, N};
+    a.c = c.softmax_scale * kLog2e;
+    a.Hkv = c.Hkv;
+    a.G = c.H / c.Hkv;
+    a.M = c.M;
+    a.D = D;
+    a.R = a.G * c.M;
+    a.row_blocks = (a.R + kXRows - 1) / kXRows;
+    const int64_t units = c.B * c.Hkv;
+    if (units * a.row_blocks > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
+    const bool stats = c.lse != nullptr, bf16 = c.dt == Q8_BF16;
+    if (few_keys(N, D)) {
+        const int64_t parts = walk_parts(units, a.row_blocks, few_blocks(N, D), 1);
+        if (units * parts > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many heads", who);
+        const unsigned grid = (unsigned)(units * parts);
+#define X_FEW(DT, NT, STATS)                                                                                               \
+    do {                                                                                                                   \
+        if (D <= 32) cross_attn_few_keys_kernel<DT, 32, NT, STATS><<<grid, kXThreads, 0, c.stream>>>(a, (int)parts);       \
+        else if (D <= 64) cross_attn_few_keys_kernel<DT, 64, NT, STATS><<<grid, kXThreads, 0, c.stream>>>(a, (int)parts);  \
+        else if (D <= 96) cross_attn_few_keys_kernel<DT, 96, 2, STATS><<<grid, kXThreads, 0, c.stream>>>(a, (int)parts);   \
+        else cross_attn_few_keys_kernel<DT, 128, 2, STATS><<<grid, kXThreads, 0, c.stream>>>(a, (int)parts);               \
+    } while (0)
+#define X_FEW_TYPE(NT, STATS)                                                       \
+    do {                                                                            \
+        if (bf16) X_FEW(Q8_BF16, NT, STATS); else X_FEW(Q8_F16, NT, STATS);         \
+    } while (0)
+        if (N <= 2 * kXTile) {
+            if (stats) X_FEW_TYPE(2, true); else X_FEW_TYPE(2, false);
+        } else {
+            if (stats) X_FEW_TYPE(4, true); else X_FEW_TYPE(4, false);
+        }
+#undef X_FEW_TYPE
+#undef X_FEW
+        return launch_status(who);
+    }
+    a.plan = fwd_plan(units, a.R, N, D);
+    if (a.plan.parts()) {
+        const int64_t need = part_bytes(a.plan, D), n = a.plan.parts() * kXRows;
+        if (c.workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
+        if (c.workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)c.workspace_bytes, (long long)need);
+        if (!aligned16(c.workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+        a.part = static_cast<float*>(c.workspace);
+        a.pm = a.part + n * D;
+        a.pw = a.pm + n;
+        a.pl = a.pw + n;
+    }
+    const unsigned grid = a.plan.grid();
+#define X_FWD(DT, STATS)                                                                              \
+    switch (padded_head(D)) {                                                                         \
+        case 32: cross_attn_fwd_kernel<DT, 32, STATS><<<grid, kXThreads, 0, c.stream>>>(a); break;    \
+        case 64: cross_attn_fwd_kernel<DT, 64, STATS><<<grid, kXThreads, 0, c.stream>>>(a); break;    \
+        case 96: cross_attn_fwd_kernel<DT, 96, STATS><<<grid, kXThreads, 0, c.stream>>>(a); break;    \
+        default: cross_attn_fwd_kernel<DT, 128, STATS><<<grid, kXThreads, 0, c.stream>>>(a);          \
+    }
+    if (bf16) {
+        if (stats) { X_FWD(Q8_BF16, true) } else { X_FWD(Q8_BF16, false) }
+    } else {
+        if (stats) { X_FWD(Q8_F16, true) } else { X_FWD(Q8_F16, false) }
+    }
+#undef X_FWD
+    if (int e = launch_status(who)) return e;
+    if (a.plan.parts()) {
+        const unsigned n = a.plan.tail * (D / 8);  // 128 rows of D / 4 threads
+        const bool two = a.plan.splits == 2;
+        if (bf16) { if (two) cross_attn_join_kernel<Q8_BF16, 2><<<n, 256, 0, c.stream>>>(a); else cross_attn_join_kernel<Q8_BF16, 8><<<n, 256, 0, c.stream>>>(a); }
+        else { if (two) cross_attn_join_kernel<Q8_F16, 2><<<n, 256, 0, c.stream>>>(a); else cross_attn_join_kernel<Q8_F16, 8><<<n, 256, 0, c.stream>>>(a); }
+        return launch_status(who);
+    }
+    return Q8_OK;
+}
+
 }  // namespace q8
 
 using namespace q8;
 
 extern "C" int64_t q8_cross_attn_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
     if (int e = x_sizes("q8_cross_attn_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
-    const int64_t rows = (int64_t)(H / Hkv) * M;
-    if (few_keys(N, D)) return 0;
-    return fwd_plan(B * Hkv, rows, N, D).parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
+    return cross_attn_forward_workspace(B, H, Hkv, M, N, D);
 }
 
 extern "C" int q8_cross_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
                              void* o, const int64_t* o_strides, float* lse, const int32_t* kv_lens, const uint8_t* key_mask, int64_t mask_row_stride,
                              int dt, float softmax_scale, int64_t B, int H, int Hkv, int M, int N, int D, void* workspace, int64_t workspace_bytes,
                              q8_stream_t stream) {
-    const char* who = "q8_cross_attn";
+    return cross_attn_forward("q8_cross_attn", XForward{q, q_strides, k, k_strides, v, v_strides, o, o_strides, nullptr, lse, kv_lens, key_mask, mask_row_stride, dt,
+                                                        softmax_scale, B, H, Hkv, M, N, D, workspace, workspace_bytes, static_cast<hipStream_t>(stream)});
+}
+
+extern "C" int q8_cross_attn_train(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                   void* o, const int64_t* o_strides, void* o_low, float* lse, const int32_t* kv_lens, const uint8_t* key_mask,
+                                   int64_t mask_row_stride, int dt, float softmax_scale, int64_t B, int H, int Hkv, int M, int N, int D, void* workspace,
+                                   int64_t workspace_bytes, q8_stream_t stream) {
+    const char* who = "q8_cross_attn_train";
     if (int e = x_sizes(who, dt, B, H, Hkv, M, N, D, softmax_scale)) return e;
-    if (B == 0 || M == 0) return Q8_OK;
-    if (int e = x_tensor(who, "q", q, q_strides, B, H, M, D)) return e;
-    if (int e = x_tensor(who, "o", o, o_strides, B, H, M, D)) return e;
-    if (N) {
-        if (int e = x_tensor(who, "k", k, k_strides, B, Hkv, N, D)) return e;
-        if (int e = x_tensor(who, "v", v, v_strides, B, Hkv, N, D)) return e;
-    }
-    if ((reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(kv_lens) & 3)) return fail(Q8_ERR_ALIGN, "%s: lse or kv_lens not aligned", who);
-    if (key_mask && (mask_row_stride < 0 || (B > 1 && mask_row_stride > INT64_MAX / 2 / B))) return fail(Q8_ERR_SHAPE, "%s: row stride of the mask", who);
-    XFwd a{};
-    static const int64_t none[3] = {0, 0, 0};
-    const int64_t *ksr = N ? k_strides : none, *vsr = N ? v_strides : none;
-    a.q = XTensor{static_cast<const uint16_t*>(q), q_strides[0], q_strides[1], q_strides[2]};
-    a.k = XTensor{static_cast<const uint16_t*>(k), ksr[0], ksr[1], ksr[2]};
-    a.v = XTensor{static_cast<const uint16_t*>(v), vsr[0], vsr[1], vsr[2]};
-    a.o = XOut{static_cast<uint16_t*>(o), o_strides[0], o_strides[1], o_strides[2]};
-    a.lse = lse;
-    a.keys = XKeys{kv_lens, key_mask, mask_row_stride, N};
-    a.c = softmax_scale * kLog2e;
-    a.Hkv = Hkv;
-    a.G = H / Hkv;
-    a.M = M;
-    a.D = D;
-    a.R = a.G * M;
-    a.row_blocks = (a.R + kXRows - 1) / kXRows;
-    if (B * Hkv * a.row_blocks > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many rows", who);
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    if (few_keys(N, D)) {
-        const int64_t units = B * Hkv, parts = walk_parts(units, a.row_blocks, few_blocks(N, D), 1);
-        if (units * parts > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: too many heads", who);
-        const unsigned grid = (unsigned)(units * parts);
-#define X_FEW(DT, NT)                                                                                        \
-    do {                                                                                                     \
-        if (D <= 32) cross_attn_few_keys_kernel<DT, 32, NT><<<grid, kXThreads, 0, st>>>(a, (int)parts);      \
-        else if (D <= 64) cross_attn_few_keys_kernel<DT, 64, NT><<<grid, kXThreads, 0, st>>>(a, (int)parts); \
-        else if (D <= 96) cross_attn_few_keys_kernel<DT, 96, 2><<<grid, kXThreads, 0, st>>>(a, (int)parts);  \
-        else cross_attn_few_keys_kernel<DT, 128, 2><<<grid, kXThreads, 0, st>>>(a, (int)parts);              \
-    } while (0)
-        if (N <= 2 * kXTile) {
-            if (dt == Q8_BF16) X_FEW(Q8_BF16, 2); else X_FEW(Q8_F16, 2);
-        } else {
-            if (dt == Q8_BF16) X_FEW(Q8_BF16, 4); else X_FEW(Q8_F16, 4);
-        }
-#undef X_FEW
-        return launch_status(who);
-    }
-    a.plan = fwd_plan(B * Hkv, a.R, N, D);
-    if (a.plan.parts()) {
-        const int64_t need = a.plan.parts() * kXRows * (D + 2) * (int64_t)sizeof(float);
-        if (workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
-        if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
-        if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
-        const int64_t n = a.plan.parts() * kXRows;
-        a.part = static_cast<float*>(workspace);
-        a.pm = a.part + n * D;
-        a.pl = a.pm + n;
-    }
-    const unsigned grid = a.plan.grid();
-#define X_FWD(DT)                                                                       \
-    switch (padded_head(D)) {                                                           \
-        case 32: cross_attn_fwd_kernel<DT, 32><<<grid, kXThreads, 0, st>>>(a); break;   \
-        case 64: cross_attn_fwd_kernel<DT, 64><<<grid, kXThreads, 0, st>>>(a); break;   \
-        case 96: cross_attn_fwd_kernel<DT, 96><<<grid, kXThreads, 0, st>>>(a); break;   \
-        default: cross_attn_fwd_kernel<DT, 128><<<grid, kXThreads, 0, st>>>(a);         \
-    }
-    if (dt == Q8_BF16) { X_FWD(Q8_BF16) } else { X_FWD(Q8_F16) }
-#undef X_FWD
-    if (int e = launch_status(who)) return e;
-    if (a.plan.parts()) {
-        const unsigned n = a.plan.tail * (D / 8);  // 128 rows of D / 4 threads
-        const bool two = a.plan.splits == 2;
-        if (dt == Q8_BF16) { if (two) cross_attn_join_kernel<Q8_BF16, 2><<<n, 256, 0, st>>>(a); else cross_attn_join_kernel<Q8_BF16, 8><<<n, 256, 0, st>>>(a); }
-        else { if (two) cross_attn_join_kernel<Q8_F16, 2><<<n, 256, 0, st>>>(a); else cross_attn_join_kernel<Q8_F16, 8><<<n, 256, 0, st>>>(a); }
-        return launch_status(who);
-    }
-    return Q8_OK;
+    if (B && M && (o == nullptr || o_low == nullptr || lse == nullptr)) return fail(Q8_ERR_NULL, "%s: o, o_low and lse are needed", who);
+    return cross_attn_forward(who, XForward{q, q_strides, k, k_strides, v, v_strides, o, o_strides, o_low, lse, kv_lens, key_mask, mask_row_stride, dt,
+                                            softmax_scale, B, H, Hkv, M, N, D, workspace, workspace_bytes, static_cast<hipStream_t>(stream)});
 }

@@ -13,10 +13,12 @@
 // and V are zeros; in the second a key is a column of every product, whose garbage stays in its column, and its gradient is
 // written as zeros. A row without keys has lse = +infinity, which makes its P zero everywhere.
 //
-// delta is formed from the rounded O, whose error is that of every score's gradient in the row: with many keys it is lost
-// beside the rounding of dS, but with 2 it leaves dQ 2.3 roundings off, with 8 still 1.6 (from the root of 2 that dS and the
-// result cost). So up to kXExact keys, which one wave or one score tile holds, the dS of a row are summed before they are
-// rounded: the true ones add up to zero, so the sum is that error, and it is taken off.
+// delta's error is that of every score's gradient in the row. It is formed from the forward's O with 8 bits
+// more than its result has, normalised by the sum of the rounded P: what is left of the error is sum_j r_j dS_j with the
+// roundings r_j of the forward's P, beside the root of 2 roundings that dS and the result cost nothing with many keys and
+// at most a sixth with few (from the rounded O alone: 512 keys, scores of deviation 4 2.0 roundings, with a mean of 3 in V 6.1, 2
+// keys 2.3). Up to kXExact keys, which one wave or one score tile holds, that goes too: the dS of a row are summed before they
+// are rounded; the true ones add up to zero, so the sum is the error, and it is taken off.
 //
 // Few workgroups: the walk is divided over several of them, their fp32 sums are added by a third kernel in order.
 #include "cross_attn_common.h"
@@ -27,8 +29,20 @@ namespace q8 {
 
 constexpr int kXExact = 32;
 
+// d + sum of g o over 8 elements, o with its rest
+template <int DT>
+__device__ __forceinline__ float dot_sum(v4u g, v4u o, v2i low, float d) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        d += unpack<DT>(g[i] & 0xffffu) * with_rest<DT>(o[i] & 0xffffu, (uint32_t)low[i / 2], i % 2 * 2);
+        d += unpack<DT>(g[i] >> 16) * with_rest<DT>(o[i] >> 16, (uint32_t)low[i / 2], i % 2 * 2 + 1);
+    }
+    return d;
+}
+
 struct XBwd {
     XTensor q, k, v, o, g;
+    const uint8_t* o_low;   // [units, R, D]: what the rounding of O left off
     XOut dq, dk, dv;
     const float* lse;    // [units, R]
     float* delta;        // [units, R], workspace
@@ -76,17 +90,15 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
         const uint16_t* qp = a.q.p + b * a.q.sb + (int64_t)(hk * a.G + g) * a.q.sh + m * a.q.st + half * 8;
         const uint16_t* gp = a.g.p + b * a.g.sb + (int64_t)(hk * a.G + g) * a.g.sh + m * a.g.st + half * 8;
         const uint16_t* op = a.o.p + b * a.o.sb + (int64_t)(hk * a.G + g) * a.o.sh + m * a.o.st + half * 8;
+        const uint8_t* lp = a.o_low + ((int64_t)unit * a.R + row) * a.D + half * 8;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const bool in = ok && s * 16 + half * 8 < a.D;
             qf[s] = in ? *reinterpret_cast<const v4u*>(qp + s * 16) : v4u{0u, 0u, 0u, 0u};
             gf[s] = in ? *reinterpret_cast<const v4u*>(gp + s * 16) : v4u{0u, 0u, 0u, 0u};
             const v4u of = in ? *reinterpret_cast<const v4u*>(op + s * 16) : v4u{0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                delta += unpack<DT>(gf[s][i] & 0xffffu) * unpack<DT>(of[i] & 0xffffu);
-                delta += unpack<DT>(gf[s][i] >> 16) * unpack<DT>(of[i] >> 16);
-            }
+            const v2i lf = in ? *reinterpret_cast<const v2i*>(lp + s * 16) : v2i{0, 0};
+            delta = dot_sum<DT>(gf[s], of, lf, delta);
         }
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(delta), __float_as_uint(delta), false, false);
         delta = __uint_as_float(r[0]) + __uint_as_float(r[1]);
@@ -463,8 +475,10 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     int rows = 0;
     float row_lse = 0.f;
     v4u dor[CHUNKS], orr[CHUNKS];
+    v2i lowr[CHUNKS];
     const uint16_t *qp = a.q.p + b * a.q.sb + (int64_t)hk * a.G * a.q.sh, *gp = a.g.p + b * a.g.sb + (int64_t)hk * a.G * a.g.sh;
     const uint16_t* op = a.o.p + b * a.o.sb + (int64_t)hk * a.G * a.o.sh;
+    const uint8_t* lp = a.o_low + (int64_t)unit * a.R * a.D;
     const int chunk = (int)threadIdx.x % CL, crow = (int)threadIdx.x / CL;  // of delta: rows crow + k W 64 / CL
     // the tile that is next (t past the end: empty)
     auto aim = [&](int t) {
@@ -483,6 +497,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
             const bool in = rows > 0 && chunk * 8 < a.D;
             dor[k] = in ? *reinterpret_cast<const v4u*>(gp + g * a.g.sh + i * a.g.st + chunk * 8) : v4u{0u, 0u, 0u, 0u};
             orr[k] = in ? *reinterpret_cast<const v4u*>(op + g * a.o.sh + i * a.o.st + chunk * 8) : v4u{0u, 0u, 0u, 0u};
+            lowr[k] = in ? *reinterpret_cast<const v2i*>(lp + ((int64_t)g * a.M + i) * a.D + chunk * 8) : v2i{0, 0};
         }
     };
     auto tile_of = [&](const uint16_t* p, const XTensor& x, int t) {
@@ -494,13 +509,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
         if (threadIdx.x < TR) lt[threadIdx.x] = (int)threadIdx.x < rows ? -row_lse : -__builtin_inff();
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
-            float d = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                d += unpack<DT>(dor[k][i] & 0xffffu) * unpack<DT>(orr[k][i] & 0xffffu);
-                d += unpack<DT>(dor[k][i] >> 16) * unpack<DT>(orr[k][i] >> 16);
-            }
-            d = group_sum<CL>(d);
+            const float d = group_sum<CL>(dot_sum<DT>(dor[k], orr[k], lowr[k], 0.f));
             const int r = crow + k * (W * 64 / CL);
             if (chunk == 0 && r < TR) dt[r] = r < rows ? -d : 0.f;
         }
@@ -762,47 +771,70 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
 }
 static int64_t delta_floats(const XPlan& p) { return p.few ? 0 : (p.units * p.rows + 3) / 4 * 4; }
 
-}  // namespace q8
+struct XBackward {
+    const void* grad; const int64_t* grad_strides;
+    const void* q; const int64_t* q_strides;
+    const void* k; const int64_t* k_strides;
+    const void* v; const int64_t* v_strides;
+    const void* o; const int64_t* o_strides;
+    const void* o_low;  // NULL: formed here, by the forward once more
+    const float* lse;
+    void* dq; const int64_t* dq_strides;
+    void* dk; const int64_t* dk_strides;
+    void* dv; const int64_t* dv_strides;
+    const int32_t* kv_lens; const uint8_t* key_mask; int64_t mask_row_stride;
+    int dt; float softmax_scale;
+    int64_t B; int H, Hkv, M, N, D;
+    void* workspace; int64_t workspace_bytes;
+    hipStream_t stream;
+};
 
-using namespace q8;
-
-extern "C" int64_t q8_cross_attn_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
-    if (int e = x_sizes("q8_cross_attn_backward_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
-    const XPlan p = plan(B, H, Hkv, M, N, D);
-    return (delta_floats(p) + p.parts) * (int64_t)sizeof(float);
+static int64_t plan_bytes(const XPlan& p) { return (delta_floats(p) + p.parts) * (int64_t)sizeof(float); }
+static int64_t low_bytes(int64_t B, int H, int M, int D) { return (B * H * M * D + 15) / 16 * 16; }
+// with o_low formed here: it, and behind it what the forward and then the backward use
+static int64_t whole_bytes(int64_t B, int H, int Hkv, int M, int N, int D) {
+    const int64_t fwd = cross_attn_forward_workspace(B, H, Hkv, M, N, D), bwd = plan_bytes(plan(B, H, Hkv, M, N, D));
+    return low_bytes(B, H, M, D) + (fwd > bwd ? fwd : bwd);
 }
 
-extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides, const void* k,
-                                      const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* o, const int64_t* o_strides,
-                                      const float* lse, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
-                                      const int64_t* dv_strides, const int32_t* kv_lens, const uint8_t* key_mask, int64_t mask_row_stride, int dt,
-                                      float softmax_scale, int64_t B, int H, int Hkv, int M, int N, int D, void* workspace, int64_t workspace_bytes,
-                                      q8_stream_t stream) {
-    const char* who = "q8_cross_attn_backward";
-    if (int e = x_sizes(who, dt, B, H, Hkv, M, N, D, softmax_scale)) return e;
-    if (B == 0 || (M == 0 && N == 0)) return Q8_OK;
+static int cross_attn_backward(const char* who, const XBackward& c) {
+    if (int e = x_sizes(who, c.dt, c.B, c.H, c.Hkv, c.M, c.N, c.D, c.softmax_scale)) return e;
+    const int M = c.M, N = c.N, D = c.D;
+    if (c.B == 0 || (M == 0 && N == 0)) return Q8_OK;
     static const int64_t none[3] = {0, 0, 0};
     if (M) {
-        if (int e = x_tensor(who, "grad", grad, grad_strides, B, H, M, D)) return e;
-        if (int e = x_tensor(who, "q", q, q_strides, B, H, M, D)) return e;
-        if (int e = x_tensor(who, "o", o, o_strides, B, H, M, D)) return e;
-        if (int e = x_tensor(who, "dq", dq, dq_strides, B, H, M, D)) return e;
-        if (lse == nullptr) return fail(Q8_ERR_NULL, "%s: lse is NULL", who);
+        if (int e = x_tensor(who, "grad", c.grad, c.grad_strides, c.B, c.H, M, D)) return e;
+        if (int e = x_tensor(who, "q", c.q, c.q_strides, c.B, c.H, M, D)) return e;
+        if (int e = x_tensor(who, "o", c.o, c.o_strides, c.B, c.H, M, D)) return e;
+        if (int e = x_tensor(who, "dq", c.dq, c.dq_strides, c.B, c.H, M, D)) return e;
+        if (c.lse == nullptr) return fail(Q8_ERR_NULL, "%s: lse is NULL", who);
+        if (!aligned16(c.o_low)) return fail(Q8_ERR_ALIGN, "%s: o_low must be 16-byte aligned", who);
     }
     if (N) {
-        if (int e = x_tensor(who, "k", k, k_strides, B, Hkv, N, D)) return e;
-        if (int e = x_tensor(who, "v", v, v_strides, B, Hkv, N, D)) return e;
-        if (int e = x_tensor(who, "dk", dk, dk_strides, B, Hkv, N, D)) return e;
-        if (int e = x_tensor(who, "dv", dv, dv_strides, B, Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "k", c.k, c.k_strides, c.B, c.Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "v", c.v, c.v_strides, c.B, c.Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "dk", c.dk, c.dk_strides, c.B, c.Hkv, N, D)) return e;
+        if (int e = x_tensor(who, "dv", c.dv, c.dv_strides, c.B, c.Hkv, N, D)) return e;
     }
-    if ((reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(kv_lens) & 3)) return fail(Q8_ERR_ALIGN, "%s: lse or kv_lens not aligned", who);
-    if (key_mask && (mask_row_stride < 0 || (B > 1 && mask_row_stride > INT64_MAX / 2 / B))) return fail(Q8_ERR_SHAPE, "%s: row stride of the mask", who);
-    const int64_t need = q8_cross_attn_backward_workspace(B, H, Hkv, M, N, D);
-    if (need && workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
-    if (workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
-    if (!aligned16(workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
-    const XPlan p = plan(B, H, Hkv, M, N, D);
+    if ((reinterpret_cast<uintptr_t>(c.lse) & 3) || (reinterpret_cast<uintptr_t>(c.kv_lens) & 3)) return fail(Q8_ERR_ALIGN, "%s: lse or kv_lens not aligned", who);
+    if (c.key_mask && (c.mask_row_stride < 0 || (c.B > 1 && c.mask_row_stride > INT64_MAX / 2 / c.B))) return fail(Q8_ERR_SHAPE, "%s: row stride of the mask", who);
+    const XPlan p = plan(c.B, c.H, c.Hkv, M, N, D);
+    const bool form_low = c.o_low == nullptr && M;
+    const int64_t need = form_low ? whole_bytes(c.B, c.H, c.Hkv, M, N, D) : plan_bytes(p);
+    if (need && c.workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
+    if (c.workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)c.workspace_bytes, (long long)need);
+    if (!aligned16(c.workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
     if (p.units * p.dq_blocks > kXMostBlocks || p.units * p.kv_blocks > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
+    char* work = static_cast<char*>(c.workspace);
+    const void* o_low = c.o_low;
+    if (form_low) {
+        o_low = work;
+        work += low_bytes(c.B, c.H, M, D);
+        if (int e = cross_attn_forward(who, XForward{c.q, c.q_strides, c.k, c.k_strides, c.v, c.v_strides, nullptr, nullptr, c.workspace, nullptr, c.kv_lens, c.key_mask,
+                                                     c.mask_row_stride, c.dt, c.softmax_scale, c.B, c.H, c.Hkv, M, N, D, work,
+                                                     c.workspace_bytes - low_bytes(c.B, c.H, M, D), c.stream}))
+            return e;
+    }
     XBwd a{};
     auto in = [&](const void* x, const int64_t* s, int n) {
         const int64_t* t = n ? s : none;
@@ -812,27 +844,28 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
         const int64_t* t = n ? s : none;
         return XOut{static_cast<uint16_t*>(x), t[0], t[1], t[2]};
     };
-    a.q = in(q, q_strides, M);
-    a.o = in(o, o_strides, M);
-    a.g = in(grad, grad_strides, M);
-    a.k = in(k, k_strides, N);
-    a.v = in(v, v_strides, N);
-    a.dq = out(dq, dq_strides, M);
-    a.dk = out(dk, dk_strides, N);
-    a.dv = out(dv, dv_strides, N);
-    a.lse = lse;
-    a.delta = static_cast<float*>(workspace);
+    a.q = in(c.q, c.q_strides, M);
+    a.o = in(c.o, c.o_strides, M);
+    a.o_low = static_cast<const uint8_t*>(o_low);
+    a.g = in(c.grad, c.grad_strides, M);
+    a.k = in(c.k, c.k_strides, N);
+    a.v = in(c.v, c.v_strides, N);
+    a.dq = out(c.dq, c.dq_strides, M);
+    a.dk = out(c.dk, c.dk_strides, N);
+    a.dv = out(c.dv, c.dv_strides, N);
+    a.lse = c.lse;
+    a.delta = reinterpret_cast<float*>(work);
     a.part = a.delta + delta_floats(p);
-    a.keys = XKeys{kv_lens, key_mask, mask_row_stride, N};
-    a.c = softmax_scale * kLog2e;
-    a.scale = softmax_scale;
-    a.Hkv = Hkv;
-    a.G = H / Hkv;
+    a.keys = XKeys{c.kv_lens, c.key_mask, c.mask_row_stride, N};
+    a.c = c.softmax_scale * kLog2e;
+    a.scale = c.softmax_scale;
+    a.Hkv = c.Hkv;
+    a.G = c.H / c.Hkv;
     a.M = M;
     a.N = N;
     a.D = D;
     a.R = (int)p.rows;
-    hipStream_t st = static_cast<hipStream_t>(stream);
+    hipStream_t st = c.stream;
 #define X_BWD(NAME, DT)                                                       \
     switch (padded_head(D)) {                                                 \
         case 32: NAME<DT, 32><<<grid, kXThreads, 0, st>>>(a); break;          \
@@ -854,9 +887,9 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
         }                                                                                                                      \
     } while (0)
         if (p.few == 4) {
-            if (dt == Q8_BF16) X_FEW(Q8_BF16, 4); else X_FEW(Q8_F16, 4);
+            if (c.dt == Q8_BF16) X_FEW(Q8_BF16, 4); else X_FEW(Q8_F16, 4);
         } else {
-            if (dt == Q8_BF16) X_FEW(Q8_BF16, 8); else X_FEW(Q8_F16, 8);
+            if (c.dt == Q8_BF16) X_FEW(Q8_BF16, 8); else X_FEW(Q8_F16, 8);
         }
 #undef X_FEW
         if (int e = launch_status(who)) return e;
@@ -865,11 +898,11 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
         a.blocks = (int)p.dq_blocks;
         a.plan = p.dq;
         const unsigned grid = a.plan.grid();
-        if (dt == Q8_BF16) { X_BWD(cross_attn_dq_kernel, Q8_BF16) } else { X_BWD(cross_attn_dq_kernel, Q8_F16) }
+        if (c.dt == Q8_BF16) { X_BWD(cross_attn_dq_kernel, Q8_BF16) } else { X_BWD(cross_attn_dq_kernel, Q8_F16) }
         if (int e = launch_status(who)) return e;
         if (a.plan.parts()) {
             const unsigned n = a.plan.tail * (D / 8);  // 128 rows of D / 4 threads
-            if (dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 1><<<n, 256, 0, st>>>(a);
+            if (c.dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 1><<<n, 256, 0, st>>>(a);
             else cross_attn_add_kernel<Q8_F16, 1><<<n, 256, 0, st>>>(a);
             if (int e = launch_status(who)) return e;
         }
@@ -879,16 +912,56 @@ extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_stri
         a.plan = p.kv;
         if (!p.few) {
             const unsigned grid = a.plan.grid();
-            if (dt == Q8_BF16) { X_BWD(cross_attn_dkdv_kernel, Q8_BF16) } else { X_BWD(cross_attn_dkdv_kernel, Q8_F16) }
+            if (c.dt == Q8_BF16) { X_BWD(cross_attn_dkdv_kernel, Q8_BF16) } else { X_BWD(cross_attn_dkdv_kernel, Q8_F16) }
             if (int e = launch_status(who)) return e;
         }
         if (a.plan.parts()) {
             const unsigned n = a.plan.tail * (D / 4);
-            if (dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 2><<<n, 256, 0, st>>>(a);
+            if (c.dt == Q8_BF16) cross_attn_add_kernel<Q8_BF16, 2><<<n, 256, 0, st>>>(a);
             else cross_attn_add_kernel<Q8_F16, 2><<<n, 256, 0, st>>>(a);
             if (int e = launch_status(who)) return e;
         }
     }
 #undef X_BWD
     return Q8_OK;
+}
+
+}  // namespace q8
+
+using namespace q8;
+
+extern "C" int64_t q8_cross_attn_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
+    if (int e = x_sizes("q8_cross_attn_backward_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
+    return whole_bytes(B, H, Hkv, M, N, D);
+}
+
+extern "C" int64_t q8_cross_attn_train_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
+    if (int e = x_sizes("q8_cross_attn_train_backward_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
+    return plan_bytes(plan(B, H, Hkv, M, N, D));
+}
+
+extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides, const void* k,
+                                      const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* o, const int64_t* o_strides,
+                                      const float* lse, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                                      const int64_t* dv_strides, const int32_t* kv_lens, const uint8_t* key_mask, int64_t mask_row_stride, int dt,
+                                      float softmax_scale, int64_t B, int H, int Hkv, int M, int N, int D, void* workspace, int64_t workspace_bytes,
+                                      q8_stream_t stream) {
+    return cross_attn_backward("q8_cross_attn_backward",
+                               XBackward{grad, grad_strides, q, q_strides, k, k_strides, v, v_strides, o, o_strides, nullptr, lse, dq, dq_strides, dk, dk_strides, dv,
+                                         dv_strides, kv_lens, key_mask, mask_row_stride, dt, softmax_scale, B, H, Hkv, M, N, D, workspace, workspace_bytes,
+                                         static_cast<hipStream_t>(stream)});
+}
+
+extern "C" int q8_cross_attn_train_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides, const void* k,
+                                            const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* o, const int64_t* o_strides,
+                                            const void* o_low, const float* lse, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides,
+                                            void* dv, const int64_t* dv_strides, const int32_t* kv_lens, const uint8_t* key_mask, int64_t mask_row_stride,
+                                            int dt, float softmax_scale, int64_t B, int H, int Hkv, int M, int N, int D, void* workspace,
+                                            int64_t workspace_bytes, q8_stream_t stream) {
+    const char* who = "q8_cross_attn_train_backward";
+    if (int e = x_sizes(who, dt, B, H, Hkv, M, N, D, softmax_scale)) return e;
+    if (B && M && o_low == nullptr) return fail(Q8_ERR_NULL, "%s: o_low is NULL", who);
+    return cross_attn_backward(who, XBackward{grad, grad_strides, q, q_strides, k, k_strides, v, v_strides, o, o_strides, o_low, lse, dq, dq_strides, dk, dk_strides,
+                                              dv, dv_strides, kv_lens, key_mask, mask_row_stride, dt, softmax_scale, B, H, Hkv, M, N, D, workspace,
+                                              workspace_bytes, static_cast<hipStream_t>(stream)});
 }

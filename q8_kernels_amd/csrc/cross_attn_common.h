@@ -59,6 +59,36 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 template <int DT>
 __device__ __forceinline__ float unpack(uint32_t h) { return DT == Q8_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h); }
+// c + both values of a pair: exact products, one fp32 rounding to nearest
+template <int DT>
+__device__ __forceinline__ float add_pair(uint32_t p, float c) {
+    if constexpr (DT == Q8_BF16) {
+        typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, 0x3f803f80u), c, false);
+    } else {
+        typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, 0x3c003c00u), c, false);
+    }
+}
+// What rounding x to 16 bits, code h, left off, as one byte: 8 bits more of the mantissa, signed (values next to a tie give the
+// nearest byte there is). fp32 codes of one sign are in the order of their values, so it is a difference of codes, and with_rest
+// is an addition to one. Values whose 16-bit code has lost bits already (fp16 below 2^-14) get what a byte holds.
+template <int DT>
+constexpr int kRestShift = DT == Q8_BF16 ? 8 : 5;
+template <int DT>
+__device__ __forceinline__ uint32_t rest_of(float x, uint32_t h) {
+    const int d = (int)(__float_as_uint(x) - __float_as_uint(unpack<DT>(h))), r = (d + (1 << (kRestShift<DT> - 1))) >> kRestShift<DT>;
+    return (uint32_t)(r < -128 ? -128 : r > 127 ? 127 : r) & 0xffu;
+}
+template <int DT>
+__device__ __forceinline__ float with_rest(uint32_t h, uint32_t bytes, int k) {
+    return __uint_as_float(__float_as_uint(unpack<DT>(h)) + (uint32_t)(((int)(bytes << (24 - 8 * k)) >> 24) << kRestShift<DT>));
+}
+// the bytes of x0 .. x3, whose codes are in lo and hi
+template <int DT>
+__device__ __forceinline__ uint32_t rests_of(float x0, float x1, float x2, float x3, uint32_t lo, uint32_t hi) {
+    return rest_of<DT>(x0, lo & 0xffffu) | rest_of<DT>(x1, lo >> 16) << 8 | rest_of<DT>(x2, hi & 0xffffu) << 16 | rest_of<DT>(x3, hi >> 16) << 24;
+}
 
 __device__ __forceinline__ v16f splat16(float v) {
     v16f r;
@@ -371,6 +401,26 @@ __device__ __forceinline__ void store_rows(const v16f (&acc)[DP / 32], float sca
         }
 }
 
+// What that left off, 8 bytes of a lane in the same places
+template <int DT, int DP>
+__device__ __forceinline__ void store_rests(const v16f (&acc)[DP / 32], float scale, uint8_t* p, int D, int lane) {
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            uint32_t w[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = 4 * (i + k);
+                const float x0 = acc[t][r] * scale, x1 = acc[t][r + 1] * scale, x2 = acc[t][r + 2] * scale, x3 = acc[t][r + 3] * scale;
+                w[k] = rests_of<DT>(x0, x1, x2, x3, pack2<DT>(x0, x1), pack2<DT>(x2, x3));
+            }
+            const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false);
+            const int e = t * 32 + (i + (lane >> 5)) * 8;
+            if (p != nullptr && e < D) *reinterpret_cast<v2i*>(p + e) = v2i{(int)x[0], (int)x[1]};
+        }
+}
+
 // ---- host side ---------------------------------------------------------------------------------------------
 
 // strides of a [B, heads, tokens, D] tensor: 0 or more (outputs: as given by the caller, not checked for overlap), multiples
@@ -403,6 +453,23 @@ inline int x_sizes(const char* who, int dt, int64_t B, int H, int Hkv, int M, in
         return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
     return Q8_OK;
 }
+
+// The forward (cross_attn.hip) with every output optional but o or o_low; what the backward runs where it was not given o_low.
+struct XForward {
+    const void* q; const int64_t* q_strides;
+    const void* k; const int64_t* k_strides;
+    const void* v; const int64_t* v_strides;
+    void* o; const int64_t* o_strides;
+    void* o_low;
+    float* lse;
+    const int32_t* kv_lens; const uint8_t* key_mask; int64_t mask_row_stride;
+    int dt; float softmax_scale;
+    int64_t B; int H, Hkv, M, N, D;
+    void* workspace; int64_t workspace_bytes;
+    hipStream_t stream;
+};
+int cross_attn_forward(const char* who, const XForward& c);
+int64_t cross_attn_forward_workspace(int64_t B, int H, int Hkv, int M, int N, int D);  // bytes, of sizes that x_sizes takes
 
 inline int padded_head(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 

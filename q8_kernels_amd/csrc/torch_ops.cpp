@@ -309,7 +309,8 @@ Keys attn_check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
     return out;
 }
 
-std::array<Tensor, 2> attn_forward(Tensor q, Tensor k, Tensor v, double scale, const Tensor& lens, const Tensor& mask, bool stats) {
+// {o, lse, o_low}: the last two with stats, for a backward (o_low: what the rounding of o left off, [B, H, M, D] contiguous)
+std::array<Tensor, 3> attn_forward(Tensor q, Tensor k, Tensor v, double scale, const Tensor& lens, const Tensor& mask, bool stats, bool rest) {
     const Keys keys = attn_check(q, k, v, lens, mask, "cross_attention");
     const int64_t b = q.size(0);
     const int h = (int)q.size(1), hk = (int)k.size(1), m = (int)q.size(2), n = (int)k.size(2), d = (int)q.size(3);
@@ -317,17 +318,24 @@ std::array<Tensor, 2> attn_forward(Tensor q, Tensor k, Tensor v, double scale, c
     const int64_t size = q8_cross_attn_workspace(b, h, hk, m, n, d);
     check(size);
     q = chunks(q), k = chunks(k), v = chunks(v);
-    Tensor o = like(q), lse, work;
+    Tensor o = like(q), lse, low, work;
+    if (rest) low = at::empty(q.sizes(), q.options().dtype(at::kChar));
     if (stats) lse = at::empty({b, h, m}, q.options().dtype(at::kFloat));
     if (size) work = at::empty({size}, q.options().dtype(at::kByte));
-    check(q8_cross_attn(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), ptr(o), o.strides().data(), (float*)ptr(lse),
-                        (const int32_t*)ptr(keys.lens), (const uint8_t*)ptr(keys.mask), keys.row, type_of(q), (float)scale, b, h, hk, m, n, d, ptr(work), size,
-                        stream_of(q)));
-    return {o, lse};
+    if (rest)
+        check(q8_cross_attn_train(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), ptr(o), o.strides().data(), ptr(low),
+                                  (float*)ptr(lse), (const int32_t*)ptr(keys.lens), (const uint8_t*)ptr(keys.mask), keys.row, type_of(q), (float)scale, b, h, hk,
+                                  m, n, d, ptr(work), size, stream_of(q)));
+    else
+        check(q8_cross_attn(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), ptr(o), o.strides().data(), (float*)ptr(lse),
+                            (const int32_t*)ptr(keys.lens), (const uint8_t*)ptr(keys.mask), keys.row, type_of(q), (float)scale, b, h, hk, m, n, d, ptr(work),
+                            size, stream_of(q)));
+    return {o, lse, low};
 }
 
-std::array<Tensor, 3> attn_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor o, const Tensor& lse, double scale, const Tensor& lens,
-                                    const Tensor& mask) {
+// low: the forward's o_low, or undefined: it is formed again
+std::array<Tensor, 3> attn_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor o, const Tensor& low, const Tensor& lse, double scale,
+                                    const Tensor& lens, const Tensor& mask) {
     const char* who = "cross_attention_backward";
     const Keys keys = attn_check(q, k, v, lens, mask, who);
     const int64_t b = q.size(0);
@@ -336,16 +344,25 @@ std::array<Tensor, 3> attn_backward(Tensor grad, Tensor q, Tensor k, Tensor v, T
         TORCH_CHECK(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(), who, ": grad and o must match q");
     TORCH_CHECK(lse.sizes() == q.sizes().slice(0, 3) && lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.is_contiguous(), who,
                 ": lse must be the forward's");
+    if (low.defined())
+        TORCH_CHECK(low.sizes() == q.sizes() && low.scalar_type() == at::kChar && low.device() == q.device() && low.is_contiguous(), who,
+                    ": o_low must be the forward's");
     const c10::DeviceGuard guard(q.device());
-    const int64_t size = q8_cross_attn_backward_workspace(b, h, hk, m, n, d);
+    const int64_t size = low.defined() ? q8_cross_attn_train_backward_workspace(b, h, hk, m, n, d) : q8_cross_attn_backward_workspace(b, h, hk, m, n, d);
     check(size);
     q = chunks(q), k = chunks(k), v = chunks(v), o = chunks(o), grad = chunks(grad);
     Tensor dq = like(q), dk = like(k), dv = like(v), work;
     if (size) work = at::empty({size}, q.options().dtype(at::kByte));
-    check(q8_cross_attn_backward(ptr(grad), grad.strides().data(), ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), ptr(o),
-                                 o.strides().data(), (const float*)ptr(lse), ptr(dq), dq.strides().data(), ptr(dk), dk.strides().data(), ptr(dv),
-                                 dv.strides().data(), (const int32_t*)ptr(keys.lens), (const uint8_t*)ptr(keys.mask), keys.row, type_of(q), (float)scale, b, h,
-                                 hk, m, n, d, ptr(work), size, stream_of(q)));
+    if (low.defined())
+        check(q8_cross_attn_train_backward(ptr(grad), grad.strides().data(), ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(),
+                                           ptr(o), o.strides().data(), ptr(low), (const float*)ptr(lse), ptr(dq), dq.strides().data(), ptr(dk),
+                                           dk.strides().data(), ptr(dv), dv.strides().data(), (const int32_t*)ptr(keys.lens), (const uint8_t*)ptr(keys.mask),
+                                           keys.row, type_of(q), (float)scale, b, h, hk, m, n, d, ptr(work), size, stream_of(q)));
+    else
+        check(q8_cross_attn_backward(ptr(grad), grad.strides().data(), ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), ptr(o),
+                                     o.strides().data(), (const float*)ptr(lse), ptr(dq), dq.strides().data(), ptr(dk), dk.strides().data(), ptr(dv),
+                                     dv.strides().data(), (const int32_t*)ptr(keys.lens), (const uint8_t*)ptr(keys.mask), keys.row, type_of(q), (float)scale, b,
+                                     h, hk, m, n, d, ptr(work), size, stream_of(q)));
     return {dq, dk, dv};
 }
 
@@ -353,14 +370,14 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, double scale, const OptTensor& kv_lens,
                           const OptTensor& key_mask) {
         const Tensor lens = or_none(kv_lens), mask = or_none(key_mask);
-        auto out = attn_forward(q, k, v, scale, lens, mask, true);
-        ctx->save_for_backward({q, k, v, out[0], out[1], lens, mask});
+        auto out = attn_forward(q, k, v, scale, lens, mask, true, true);
+        ctx->save_for_backward({q, k, v, out[0], out[2], out[1], lens, mask});
         ctx->saved_data["scale"] = scale;
         return out[0];
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const auto s = ctx->get_saved_variables();
-        auto d = attn_backward(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), s[5], s[6]);
+        auto d = attn_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(), s[6], s[7]);
         return once({d[0], d[1], d[2], Tensor(), Tensor(), Tensor()});
     }
 };
@@ -374,7 +391,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, std::o
         no_eager_graph(q, {&q, &k, &v}, "cross_attention");
         return CrossAttention::apply(q, k, v, scale, given(lens), given(mask));
     }
-    return attn_forward(q, k, v, scale, lens, mask, false)[0];
+    return attn_forward(q, k, v, scale, lens, mask, false, false)[0];
 }
 
 }  // namespace
@@ -413,13 +430,15 @@ PYBIND11_MODULE(_torch_ops, m) {
     });
     m.def("cross_attention", &cross_attention);
     m.def("cross_attention_forward",
-          [](const Tensor& q, const Tensor& k, const Tensor& v, double scale, const OptTensor& lens, const OptTensor& mask, bool stats) {
-              auto r = attn_forward(q, k, v, scale, or_none(lens), or_none(mask), stats);
-              return std::vector<OptTensor>{r[0], given(r[1])};
+          [](const Tensor& q, const Tensor& k, const Tensor& v, double scale, const OptTensor& lens, const OptTensor& mask, bool stats, bool rest) {
+              auto r = attn_forward(q, k, v, scale, or_none(lens), or_none(mask), stats || rest, rest);
+              std::vector<OptTensor> out{r[0], given(r[1])};
+              if (rest) out.push_back(r[2]);
+              return out;
           });
     m.def("cross_attention_backward", [](const Tensor& g, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, double scale,
-                                         const OptTensor& lens, const OptTensor& mask) {
-        auto r = attn_backward(g, q, k, v, o, lse, scale, or_none(lens), or_none(mask));
+                                         const OptTensor& lens, const OptTensor& mask, const OptTensor& low) {
+        auto r = attn_backward(g, q, k, v, o, or_none(low), lse, scale, or_none(lens), or_none(mask));
         return std::vector<Tensor>{r[0], r[1], r[2]};
     });
 }

@@ -1,0 +1,141 @@
+"""16-bit cross attention: how exact its gradients are where the roundings inside it could show.
+
+Against the definition in float64, in two ways. u = half a step of the type (2^-8 bf16, 2^-11 fp16).
+
+Element by element: scores are fp32 sums, so p = exp(s) is off by at most es = 2 (D 2^-23 scale sum|q k| + 2^-22 max(4, |c s|)
++ N 2^-24) of itself (products, exponent and its difference from the log-sum, row sum); dS is rounded once where it enters a
+product, the result once at the end. delta = rowsum(dO O) has O from probabilities that were rounded for their product and are
+normalised by the sum of the rounded ones, so with relative roundings r_j it is off by sum_j r_j ds_j, and O itself, kept with 8
+bits more than its type has, by u / 2^8 |O| (next to a tie twice that):
+  edelta: sum_j (u + 2 es) |ds_j| + sum_d |g| (u / 2^7 |o| + 2 es sum_j p |v|) + D 2^-23 sum_d |g o|
+  ds: (u + 2 es) |ds| + p (D 2^-23 sum_d |g v| + edelta);  dq, dk: the sums of that and of fp32 additions, and half a step.
+
+All elements together: a value x that is rounded to 16 bits is off by h(x) / sqrt(3) in the square mean, where h(x) is half its
+step. dq has the roundings of its ds, of delta (u / sqrt(3) |ds_j| each, at most) and of the result. Their squares add up, for
+they are independent; the sum over some 10^4 elements scatters by a few percent, so the square mean error may be 1.1 times that
+root. Beside it stand the fp32 errors: a few 2^-24 of what is added up, with signs of their own, 2^-20 of p |g| |v| in a ds
+and of p in a dv."""
+import pytest
+import torch
+
+from q8_kernels_amd import _C, functional as Q8F
+
+pytestmark = pytest.mark.gpu
+attend = Q8F.cross_attention.cross_attention
+TYPES = [torch.bfloat16]
+
+
+def half_step(x, dtype):
+    info = torch.finfo(dtype)
+    e = torch.floor(torch.log2(x.abs().clamp_min(info.tiny)))
+    return torch.exp2(e) * (info.eps / 2)
+
+
+def definition(q, k, v, g, scale, valid):
+    """dq, dk, dv: value, element tolerance, square mean error allowed; and the same of o without the last"""
+    b, h, m, d = q.shape
+    hk, n = k.shape[1], k.shape[2]
+    dtype, u = q.dtype, torch.finfo(q.dtype).eps / 2
+    live = valid[:, None, :, None]
+    q6, g6 = (x.double().reshape(b, hk, h // hk * m, d) for x in (q, g))
+    k6, v6 = (torch.where(live, x.double(), 0.0) for x in (k, v))
+    s = q6 @ k6.transpose(2, 3) * scale
+    p = torch.softmax(torch.where(valid[:, None, None, :], s, float("-inf")), -1)
+    es = 2 * (d * 2.0 ** -23 * scale * (q6.abs() @ k6.abs().transpose(2, 3)) + 2.0 ** -22 * (1.45 * s.abs()).clamp_min(4.0).amax(-1, keepdim=True) + n * 2.0 ** -24)
+    o, dp = p @ v6, g6 @ v6.transpose(2, 3)
+    ds = p * (dp - (g6 * o).sum(-1, keepdim=True))
+    dq, dk, dv = scale * (ds @ k6), scale * (ds.transpose(2, 3) @ q6), p.transpose(2, 3) @ g6
+
+    mag = (p * (1 + es)) @ v6.abs()
+    edelta = ((u + 2 * es) * ds.abs()).sum(-1, keepdim=True) + (g6.abs() * (u / 128 * o.abs() + 2 * es.amax(-1, keepdim=True) * mag + d * 2.0 ** -23 * o.abs())).sum(-1, keepdim=True)
+    eds = ds.abs() * (u + 2 * es) + p * (d * 2.0 ** -23 * (g6.abs() @ v6.abs().transpose(2, 3)) + edelta)
+    edq = scale * (eds @ k6.abs() + n * 2.0 ** -24 * (ds.abs() @ k6.abs()))
+    edk = scale * (eds.transpose(2, 3) @ q6.abs() + q6.shape[2] * 2.0 ** -24 * (ds.abs().transpose(2, 3) @ q6.abs()))
+    edv = (p * (u + 2 * es)).transpose(2, 3) @ g6.abs() + q6.shape[2] * 2.0 ** -24 * (p.transpose(2, 3) @ g6.abs())
+    full = [e * (1 + u) + half_step(x, dtype) for e, x in zip((edq, edk, edv), (dq, dk, dv))]
+    small = 2.0 ** -20 * p * (g6.norm(dim=-1, keepdim=True) * v6.norm(dim=-1).unsqueeze(2))
+    fine = (scale * (small @ k6.abs()), scale * (small.transpose(2, 3) @ q6.abs()), 2.0 ** -20 * (p.transpose(2, 3) @ g6.abs()))
+    third = lambda x: half_step(x, dtype).square() / 3  # noqa: E731
+    # (a ds below the type's normal numbers is rounded like any other: it enters its product times a power of two)
+    step = lambda x: (torch.exp2(torch.floor(torch.log2(x.abs().clamp_min(1e-300)))) * u).square() / 3  # noqa: E731
+    delta = (u * u / 3) * ds.square().sum(-1, keepdim=True)
+    square = [scale ** 2 * (step(ds) @ k6.square() + delta * (p @ k6).square()) + third(dq),
+              scale ** 2 * (step(ds) + delta * p.square()).transpose(2, 3) @ q6.square() + third(dk),
+              step(p).transpose(2, 3) @ g6.square() + third(dv)]
+    mean = [1.1 * x.mean().sqrt() + e.square().mean().sqrt() for x, e in zip(square, fine)]
+    return [(w.reshape(x.shape), e.reshape(x.shape), a) for w, e, a, x in zip((dq, dk, dv), full, mean, (q, k, v))]
+
+
+def check(q, k, v, g, scale, lens=None, mask=None):
+    b, n = k.shape[0], k.shape[2]
+    valid = torch.ones(b, n, dtype=torch.bool, device=q.device)
+    if lens is not None:
+        valid = valid & (torch.arange(n, device=q.device) < lens[:, None])
+    if mask is not None:
+        valid = valid & mask
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    got = torch.autograd.grad(attend(*leaves, scale, lens, mask), leaves, g)
+    for name, x, (want, tol, mean) in zip(("dq", "dk", "dv"), got, definition(q, k, v, g, scale, valid)):
+        off = x.double() - want
+        assert float(off.square().mean().sqrt()) <= float(mean), "%s: %g off in the square mean, %g allowed" % (name, off.square().mean().sqrt(), mean)
+        assert (off.abs() <= tol).all(), "%s: off by %g" % (name, (off.abs() - tol).max())
+    return got
+
+
+def draw(dev, b, h, hk, m, n, d, dtype, seed):
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    one = lambda heads, t: torch.randn((b, t, heads, d), generator=gen, device=dev).transpose(1, 2)  # noqa: E731
+    return tuple(x.to(dtype) for x in (one(h, m), one(hk, n), one(hk, n), one(h, m)))
+
+
+# few keys and many rows (one pass over the rows, 4 or 8 waves, heads up to 64 and longer ones), long keys, divided walks
+SIZES = [(2, 4, 2, 130, 100, 64), (1, 4, 4, 300, 120, 128), (2, 32, 32, 1100, 200, 64), (1, 40, 40, 1700, 250, 80), (2, 4, 2, 200, 512, 64), (1, 4, 2, 150, 700, 128),
+         (1, 4, 1, 9, 3000, 64), (1, 8, 2, 3, 2100, 96)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_peaked_rows(dev, dtype, size):
+    """A few keys take most of a row, and the values have a mean: what is left of dS is small beside delta."""
+    q, k, v, g = draw(dev, *size, dtype, seed=1)
+    check(q, k, (v.float() + 3.0).to(dtype), g, 4 * size[5] ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_long_masks_that_leave_few_keys(dev, dtype, size):
+    q, k, v, g = draw(dev, *size, dtype, seed=2)
+    n = size[4]
+    for left in ([n - 1], [40, n - 3], [0, 33, 70]):
+        mask = torch.zeros(size[0], n, dtype=torch.bool, device=dev)
+        mask[:, left] = True
+        dq, dk, dv = check(q, k, v, g, size[5] ** -0.5, mask=mask)
+        if len(left) == 1:  # a softmax over one key has no gradient: what is left is the fp32 sums of dP and delta, of D products of about 1
+            assert float(dq.float().abs().max()) < 2.0 ** -14 and float(dk.float().abs().max()) < 2.0 ** -12
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", SIZES)
+def test_backward_with_and_without_the_rest(dev, dtype, size):
+    """o with o_low has 8 bits more, and a backward that is not given o_low forms the same one."""
+    q, k, v, g = draw(dev, *size, dtype, seed=3)
+    lens = torch.full((size[0],), size[4] - 1, dtype=torch.int32, device=dev)
+    o, lse, low = _C.cross_attention(q, k, v, 0.1, lens, rest=True)
+    assert all(torch.equal(a, b) for a, b in zip((o, lse), _C.cross_attention(q, k, v, 0.1, lens))) and torch.equal(o, attend(q, k, v, 0.1, lens))
+    assert low.is_contiguous() and low.dtype == torch.int8 and low.shape == o.shape and bool((low.float().std() > 60) & (low.float().mean().abs() < 10))
+    fine = (o.float().contiguous().view(torch.int32) + low.int() * (256 if dtype == torch.bfloat16 else 32)).view(torch.float32).double()
+    valid = torch.arange(size[4], device=dev) < size[4] - 1
+    k6, v6 = (x.double().repeat_interleave(size[1] // size[2], 1)[:, :, valid] for x in (k, v))
+    s = q.double() @ k6.transpose(2, 3) * 0.1
+    p = torch.softmax(s, -1)
+    # o's own roundings: P (sum_j r_j p_j (v_j - o), in the square mean) and what the 8 bits leave; a rounding of o would be u / sqrt(3) |o| or so
+    u = torch.finfo(dtype).eps / 2
+    spread = (p.square() @ v6.square() + p.square().sum(-1, keepdim=True) * (p @ v6).square()).sqrt()
+    assert float(((fine - p @ v6) / (u * (spread + (p @ v6).abs() / 128) + 2.0 ** -20)).square().mean().sqrt()) < 1.0
+    one = _C.cross_attention_backward(g, q, k, v, o, lse, 0.1, lens, o_low=low)
+    two = _C.cross_attention_backward(g, q, k, v, o, lse, 0.1, lens)
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    assert all(torch.equal(a, b) for a, b in zip(one, torch.autograd.grad(attend(*leaves, 0.1, lens), leaves, g)))
+    with pytest.raises(RuntimeError, match="o_low"):
+        _C.cross_attention_backward(g, q, k, v, o, lse, 0.1, lens, o_low=low[..., :8])
