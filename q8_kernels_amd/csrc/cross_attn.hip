@@ -4,8 +4,9 @@
 // stays in registers, K and V go through LDS in tiles of 64 keys (double-buffered, the next tile's loads in flight during the
 // present one's arithmetic). S^T = K Q^T leaves a query's scores in one lane pair, P^T = exp2(S^T c - m) goes on as the B
 // operand of O^T = V^T P^T without leaving registers. Scores, maxima, sums and O are fp32; P is rounded to 16 bits for the
-// product (as its operand has to be), relative to a maximum that trails the running one by at most 2^8, so the rounding is
-// a relative one. O is rescaled only when the maximum has grown beyond that.
+// product (as its operand has to be), relative to a maximum that trails the running one by at most 2^8 (fp16: to 2^-7 of it, so
+// what is 2^-21 of the largest is still a normal number), so the rounding is a relative one. O is rescaled only when the
+// maximum has grown beyond that.
 //
 // O is divided by the sum of the rounded P, so it is a mean of the values with weights that add up to one: with relative
 // roundings r_j it is off by sum_j r_j P_j (v_j - O), not by sum_j r_j P_j v_j, and what a training step forms from it,
@@ -40,7 +41,7 @@ struct Rows32 {
     static constexpr int KS = DP / 16, DTL = DP / 32;
     v4u qf[KS];
     v16f acc[DTL];
-    float m, w, l;  // m in units of log2; w, l: the sums of P as it is rounded and as it was, over this lane's half of the keys
+    float m, w, l;  // m, less kShiftM, in units of log2; w, l: the sums of P as it is rounded and as it was, over this lane's half of the keys
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -87,9 +88,9 @@ struct Rows32 {
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = max_ieee(top, s[1][i]);
         top = half_pair_max(top) * c;
-        const bool grown = top > m + 8.f;
+        const bool grown = top > m + (8 + kShiftM<DT>);
         if (__builtin_amdgcn_ballot_w64(grown) != 0) {
-            const float next = grown ? top : m, f = __builtin_amdgcn_exp2f(m - next);
+            const float next = grown ? top - kShiftM<DT> : m, f = __builtin_amdgcn_exp2f(m - next);
             m = next;
             w *= f;
             if constexpr (STATS) l *= f;

@@ -7,7 +7,8 @@
 // products instead of five; partial sums of dQ per key tile would move more time's worth of bytes than the two products
 // cost). The first owns 128 query rows and walks over the keys: it forms delta, writes it for the second, and dQ. The second
 // owns 128 keys and walks over the rows of all query heads of the group, so dK and dV of a shared head come out summed. P and
-// dS are rounded to 16 bits for the products they enter; scores, dP, sums and delta are fp32.
+// dS are rounded to 16 bits for the products they enter (P in fp16 times 2^14, which is taken off dV); scores, dP, sums and
+// delta are fp32.
 //
 // A key that does not count: in the first kernel its score is -infinity (P = 0 exactly, whatever lse is) and its rows of K
 // and V are zeros; in the second a key is a column of every product, whose garbage stays in its column, and its gradient is
@@ -28,6 +29,8 @@
 namespace q8 {
 
 constexpr int kXExact = 32;
+template <int DT>
+constexpr float kUnshiftP = 1.0f / (1 << kShiftP<DT>);
 
 // d + sum of g o over 8 elements, o with its rest
 template <int DT>
@@ -273,7 +276,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     auto finish = [&](float* lt, float* dt) {
         wait_loads();
         if (threadIdx.x < TR) {
-            lt[threadIdx.x] = (int)threadIdx.x < rows ? -row_lse : -__builtin_inff();
+            lt[threadIdx.x] = (int)threadIdx.x < rows ? kShiftP<DT> - row_lse : -__builtin_inff();
             dt[threadIdx.x] = (int)threadIdx.x < rows ? -row_delta : 0.f;
         }
     };
@@ -365,7 +368,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
                     for (int d = 0; d < ops.CG; ++d) dv[c * ops.CG + d] = mfma16<DT>(ops.f[w][d], p, dv[c * ops.CG + d]);
                     if (k == 0 && c == 0) {  // dS, beside them (P's second half is still needed as it is)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+                        for (int i = 0; i < 16; ++i) dp[i] *= DT == Q8_F16 ? s[i] * kUnshiftP<DT> : s[i];
                     }
                     keep();
                 }
@@ -395,6 +398,12 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     if (!counts) {  // a key that does not count has no gradient, whatever its column holds
 #pragma unroll
         for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
+    }
+    if constexpr (kShiftP<DT> != 0) {
+#pragma unroll
+        for (int t = 0; t < DTL; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dv[t][i] *= kUnshiftP<DT>;
     }
     const XBwd& z = arguments_again<XBwd>();
     if (of > 1) {
@@ -506,7 +515,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     };
     auto finish = [&](float* lt, float* dt) {
         wait_loads();
-        if (threadIdx.x < TR) lt[threadIdx.x] = (int)threadIdx.x < rows ? -row_lse : -__builtin_inff();
+        if (threadIdx.x < TR) lt[threadIdx.x] = (int)threadIdx.x < rows ? kShiftP<DT> - row_lse : -__builtin_inff();
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
             const float d = group_sum<CL>(dot_sum<DT>(dor[k], orr[k], lowr[k], 0.f));
@@ -593,10 +602,10 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
                             if constexpr (exact) {  // all keys are in this wave: what their dS adds up to is the error of delta
 #pragma unroll
                                 for (int i = 0; i < 16; ++i)
-                                    dp[i] -= group_sum<32>(__uint_as_float(__float_as_uint(dp[i] * s[i]) & keep));
+                                    dp[i] -= group_sum<32>(__uint_as_float(__float_as_uint(dp[i] * s[i]) & keep)) * kUnshiftP<DT>;
                             }
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+                            for (int i = 0; i < 16; ++i) dp[i] *= DT == Q8_F16 ? s[i] * kUnshiftP<DT> : s[i];
                         }
                         keep_apart();
                     }
@@ -679,6 +688,12 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     if (!counts) {  // a key that does not count has no gradient, whatever its column holds
 #pragma unroll
         for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
+    }
+    if constexpr (kShiftP<DT> != 0) {
+#pragma unroll
+        for (int t = 0; t < DTL; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dv[t][i] *= kUnshiftP<DT>;
     }
     const XBwd& z = arguments_again<XBwd>();
     if (key >= z.N) return;

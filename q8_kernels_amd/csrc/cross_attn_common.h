@@ -57,6 +57,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, f16x2));
 }
+// fp16 has its normal numbers down to 2^-14 only: probabilities enter their products times 2^kShiftP (backward, where they are at
+// most 1) or relative to 2^-kShiftM of the maximum (forward, where they are at most 2^8 beside it). bf16 has fp32's range.
+template <int DT>
+constexpr int kShiftP = DT == Q8_F16 ? 14 : 0;
+template <int DT>
+constexpr int kShiftM = DT == Q8_F16 ? 7 : 0;
 template <int DT>
 __device__ __forceinline__ float unpack(uint32_t h) { return DT == Q8_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h); }
 // c + both values of a pair: exact products, one fp32 rounding to nearest

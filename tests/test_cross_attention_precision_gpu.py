@@ -139,3 +139,31 @@ def test_backward_with_and_without_the_rest(dev, dtype, size):
     assert all(torch.equal(a, b) for a, b in zip(one, torch.autograd.grad(attend(*leaves, 0.1, lens), leaves, g)))
     with pytest.raises(RuntimeError, match="o_low"):
         _C.cross_attention_backward(g, q, k, v, o, lse, 0.1, lens, o_low=low[..., :8])
+
+
+def test_small_probabilities_in_float16(dev):
+    """Thousands of keys that share a row evenly: probabilities below float16's normal numbers enter the products of dV times a power of two."""
+    q, k, v, g = draw(dev, 1, 2, 1, 70, 50000, 64, torch.float16, seed=4)
+    check(q, k, v, g, 0.02)
+    q, k, v, g = draw(dev, 2, 4, 2, 40, 33, 64, torch.float16, seed=5)
+    check(q, k, v, g, 2.0)                                           # few keys, some of them with next to nothing
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [60, 250, 60001])
+def test_many_keys_far_below_the_largest(dev, dtype, n):
+    """One key of weight 1 and n - 1 of weight 2^-18.45 each: relative to the maximum they are below float16's normal numbers, and together
+    (n = 60001) a sixth as much. Each weight is rounded by u at most, the same for all: o is off by u times the sum of the parts, and half a step."""
+    gen = torch.Generator(device=dev).manual_seed(6)
+    d = 64
+    q = torch.ones(1, 1, 5, d, device=dev)
+    k = torch.zeros(1, 1, n, d, device=dev)
+    k[:, :, 0] = 18.45 * 0.6931471805599453 / 8
+    v = torch.randn((1, 1, n, d), generator=gen, device=dev) + 1.0
+    v[:, :, 0] = 0.0
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    u = torch.finfo(dtype).eps / 2
+    p = torch.softmax(q.double() @ k.double().transpose(2, 3) * 0.125, -1)
+    want = p @ v.double()
+    off = (attend(q, k, v, 0.125).double() - want).abs()
+    assert (off <= (u + 2.0 ** -17) * (p @ (v.double() - want[:, :, :1]).abs()) + 2.0 ** -17 * want.abs() + half_step(want, dtype)).all(), float(off.max())
