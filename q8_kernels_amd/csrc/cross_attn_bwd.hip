@@ -7,8 +7,14 @@
 // products instead of five; partial sums of dQ per key tile would move more time's worth of bytes than the two products
 // cost). The first owns 128 query rows and walks over the keys: it forms delta, writes it for the second, and dQ. The second
 // owns 128 keys and walks over the rows of all query heads of the group, so dK and dV of a shared head come out summed. P and
-// dS are rounded to 16 bits for the products they enter (P in fp16 times 2^14, which is taken off dV); scores, dP, sums and
-// delta are fp32.
+// dS are rounded to 16 bits for the products they enter (P in fp16 times 2^14, which is taken off dV); scores, dP, sums and delta
+// are fp32.
+//
+// fp16 holds neither the dS of small gradients (of 1e-3 with 2048 keys they are below 2^-14) nor those of scaled ones (above
+// 65504). There dS enters its products times a power of two, which is taken off the fp32 sums. In the two kernels every
+// column of a block has its own, a row of dQ or a key of dK: the largest |dS| of a block is looked at, and where it goes above
+// 2^15 the power is lowered so that it comes to 2^9, with the sums so far (as the forward does with its maximum). The kernel for
+// few keys has one for a tile, from a bound: |dS| <= |dO_i| max_j |V_j| / 2, for p (1 - p) is 1/4 at most.
 //
 // A key that does not count: in the first kernel its score is -infinity (P = 0 exactly, whatever lse is) and its rows of K
 // and V are zeros; in the second a key is a column of every product, whose garbage stays in its column, and its gradient is
@@ -31,6 +37,25 @@ namespace q8 {
 constexpr int kXExact = 32;
 template <int DT>
 constexpr float kUnshiftP = 1.0f / (1 << kShiftP<DT>);
+constexpr int kMostShift = 60;  // log2 of the largest factor of dS: P |dP| below 2^39 stays finite beside it
+
+// One column of a block of dS times a power of two, in 16 results of the lanes l and l + 32: the power's change (0 or less) where
+// the largest of them has grown beyond fp16's reach. NaN and infinity change nothing: their column is lost.
+__device__ __forceinline__ int shift_change(const v16f& ds) {
+    float top = max_ieee(__builtin_fabsf(ds[0]), __builtin_fabsf(ds[1]));
+#pragma unroll
+    for (int i = 2; i < 16; ++i) top = max_ieee(top, __builtin_fabsf(ds[i]));
+    top = half_pair_max(top);
+    const int to = 9 - __builtin_amdgcn_frexp_expf(top);
+    return top > 32768.f && to < 0 ? to : 0;
+}
+template <int N>
+__device__ __forceinline__ void scale_all(v16f (&x)[N], float f) {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[t][i] *= f;
+}
 
 // d + sum of g o over 8 elements, o with its rest
 template <int DT>
@@ -86,7 +111,7 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
     const bool few = kv.len > 0 && kv.len <= kXExact;
 
     v4u qf[KS], gf[KS];
-    float delta = 0.f, lse = __builtin_inff();
+    float delta = 0.f, lse = __builtin_inff();  // lse: less the power of two of the row's dS
     {
         const bool ok = row < a.R;
         const int g = ok ? row / a.M : 0, m = row - g * a.M;
@@ -108,6 +133,7 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
         if (ok) {
             const int64_t at = (int64_t)unit * a.R + row;
             lse = a.lse[at];
+            if constexpr (DT == Q8_F16) lse -= kMostShift;
             if (split == 0 && half == 0 && !few) a.delta[at] = delta;
         }
     }
@@ -172,6 +198,7 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
                     for (int i = 0; i < 16; ++i) sum += dp[i] * s[i];
                     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
                     sum = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+                    if constexpr (DT == Q8_F16) sum = __builtin_ldexpf(sum, -kMostShift);  // (the first block: no change so far)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) dp[i] -= sum;
                     if (const XBwd& z = arguments_again<XBwd>(); row < z.R && half == 0) z.delta[(int64_t)unit * z.R + row] = delta + sum;
@@ -179,6 +206,16 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+            if constexpr (DT == Q8_F16) {
+                const int change = shift_change(dp);
+                if (__builtin_amdgcn_ballot_w64(change != 0) != 0) {
+                    const float f = __builtin_ldexpf(1.0f, change);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dp[i] *= f;
+                    scale_all(acc, f);
+                    lse -= (float)change;
+                }
+            }
             int w = 0;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -204,6 +241,10 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
         if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
     }
     const XBwd& z = arguments_again<XBwd>();
+    if constexpr (DT == Q8_F16) {  // (where no key counts there are zeros)
+        const float whole = row < z.R ? z.lse[(int64_t)unit * z.R + row] : 0.f;
+        scale_all(acc, row < z.R && whole < __builtin_inff() ? __builtin_amdgcn_exp2f(lse - whole) : 1.0f);
+    }
     if (of > 1) {
         if (row < z.R) {
             float* p = z.part + (((int64_t)split * z.plan.tail + (block - z.plan.full)) * kXRows + wave * 32 + (lane & 31)) * z.D;
@@ -307,6 +348,7 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     __syncthreads();
     LaneOffsets<DP> at(lane);
     Operands<DP, V_IN_LDS ? 2 : 4> ops;
+    float factor = __builtin_ldexpf(kUnshiftP<DT>, kMostShift);  // fp16: of dS beside the shifted P's
     auto step = [&](int t, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
         at.fresh();
@@ -368,9 +410,19 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
                     for (int d = 0; d < ops.CG; ++d) dv[c * ops.CG + d] = mfma16<DT>(ops.f[w][d], p, dv[c * ops.CG + d]);
                     if (k == 0 && c == 0) {  // dS, beside them (P's second half is still needed as it is)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) dp[i] *= DT == Q8_F16 ? s[i] * kUnshiftP<DT> : s[i];
+                        for (int i = 0; i < 16; ++i) dp[i] *= DT == Q8_F16 ? s[i] * factor : s[i];
                     }
                     keep();
+                }
+            }
+            if constexpr (DT == Q8_F16) {
+                const int change = counts ? shift_change(dp) : 0;
+                if (__builtin_amdgcn_ballot_w64(change != 0) != 0) {
+                    const float f = __builtin_ldexpf(1.0f, change);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dp[i] *= f;
+                    scale_all(dk, f);
+                    factor *= f;
                 }
             }
 #pragma unroll
@@ -399,11 +451,9 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
 #pragma unroll
         for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
     }
-    if constexpr (kShiftP<DT> != 0) {
-#pragma unroll
-        for (int t = 0; t < DTL; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dv[t][i] *= kUnshiftP<DT>;
+    if constexpr (DT == Q8_F16) {
+        scale_all(dv, kUnshiftP<DT>);
+        scale_all(dk, kUnshiftP<DT> / factor);  // (a power of two)
     }
     const XBwd& z = arguments_again<XBwd>();
     if (of > 1) {
@@ -448,6 +498,8 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     constexpr int CHUNKS = TR * CL / (W * 64) > 0 ? TR * CL / (W * 64) : 1;
     __shared__ __align__(16) uint16_t q0[ELEMS], q1[ELEMS], g0[ELEMS], g1[ELEMS], kt[W * 32 * DP], ds[W * 32 * TR];
     __shared__ __align__(16) float lse0[TR], lse1[TR], delta0[TR], delta1[TR];  // -lse and -delta of the tile's rows
+    constexpr bool SHIFT = DT == Q8_F16;
+    __shared__ float size0[SHIFT ? TR : 1], size1[SHIFT ? TR : 1], vsize[SHIFT ? W : 1];  // |dO|^2 of the tile's rows, largest |V|^2 of a wave's keys
     __shared__ __align__(16) float sums[KG > 1 ? (KG - 1) * NB * 1024 : 4];
     const int unit = blockIdx.x / parts, part = blockIdx.x - unit * parts;
     const int b = unit / a.Hkv, hk = unit - b * a.Hkv;
@@ -473,6 +525,16 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
             vf[s] = in ? *reinterpret_cast<const v4u*>(vp + s * 16) : v4u{0u, 0u, 0u, 0u};
             *reinterpret_cast<v4u*>(kt + wave * 32 * DP + tile_at<DP>(lane & 31, 2 * s + half)) = x;
         }
+    }
+    if constexpr (SHIFT) {
+        float n = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n = square_sum<DT>(vf[s][i], n);
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(n), __float_as_uint(n), false, false);
+        n = group_max<32>(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+        if (lane == 0) vsize[wave] = n;
     }
     if (idle) {  // its part of dS stays zero
         for (int i = lane; i < 32 * TR / 8; i += 64) *reinterpret_cast<v4u*>(ds + wave * 32 * TR + i * 8) = v4u{0u, 0u, 0u, 0u};
@@ -513,7 +575,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
         const int g = t / head_tiles, m = (t - g * head_tiles) * TR;
         return XTile(p + g * x.sh + m * x.st, x.st, rows, a.D, TR);
     };
-    auto finish = [&](float* lt, float* dt) {
+    auto finish = [&](float* lt, float* dt, float* st) {
         wait_loads();
         if (threadIdx.x < TR) lt[threadIdx.x] = (int)threadIdx.x < rows ? kShiftP<DT> - row_lse : -__builtin_inff();
 #pragma unroll
@@ -521,6 +583,13 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
             const float d = group_sum<CL>(dot_sum<DT>(dor[k], orr[k], lowr[k], 0.f));
             const int r = crow + k * (W * 64 / CL);
             if (chunk == 0 && r < TR) dt[r] = r < rows ? -d : 0.f;
+            if constexpr (SHIFT) {
+                float n = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) n = square_sum<DT>(dor[k][i], n);
+                n = group_sum<CL>(n);
+                if (chunk == 0 && r < TR) st[r] = r < rows ? n : 0.f;
+            }
         }
     };
 
@@ -531,10 +600,16 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
         aim(t0);
         ask(t0);
         copies.group(0, 1, tile_of(qp, a.q, t0), tile_of(gp, a.g, t0), 0, q0, g0);
-        finish(lse0, delta0);
+        finish(lse0, delta0, size0);
     }
     wait_loads();
     __syncthreads();
+    float most_v = 0.f;
+    if constexpr (SHIFT) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) most_v = fmaxf(most_v, vsize[i]);
+    }
+    int shift = kMostShift, least = kMostShift;  // log2 of the present factor of dS, and the least that a tile so far asked for
 
     LaneOffsets<DP> at(lane);
     LaneOffsets<TR> ds_at(lane);
@@ -550,6 +625,22 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
         aim(t + 1);
         if constexpr (!LONG) ask(t + 1);
         copies.group(0, 1, tile_of(qp, a.q, t + 1), tile_of(gp, a.g, t + 1), 0, qnext, gnext);
+        float factor = 1.0f;  // of dS beside the shifted P's
+        if constexpr (SHIFT) {
+            // The power that brings the bound to 2^14 .. 2^15. It is kept while a tile loses no more than 6 bits by it; and it does not
+            // rise more than 40 above the least one, so that the sums so far stay in range.
+            const float rows_most = group_max<64>((BUF ? size1 : size0)[lane & (TR - 1)]);
+            const float bound = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(rows_most * most_v)));
+            const int x = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(bound));
+            const int own = bound > 0.f ? min(15 - ((x + 1) >> 1), kMostShift) : kMostShift;
+            least = min(least, own);
+            const int next = min(own, least + 40);
+            if (shift > own || shift < next - 6) {
+                scale_all(dk, __builtin_ldexpf(1.0f, next - shift));
+                shift = next;
+            }
+            factor = __builtin_ldexpf(kUnshiftP<DT>, shift);
+        }
         if (!idle) {
 #pragma unroll
             for (int u = 0; u < RB; ++u) {
@@ -605,7 +696,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
                                     dp[i] -= group_sum<32>(__uint_as_float(__float_as_uint(dp[i] * s[i]) & keep)) * kUnshiftP<DT>;
                             }
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) dp[i] *= DT == Q8_F16 ? s[i] * kUnshiftP<DT> : s[i];
+                            for (int i = 0; i < 16; ++i) dp[i] *= SHIFT ? s[i] * factor : s[i];
                         }
                         keep_apart();
                     }
@@ -646,16 +737,16 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
         auto store = [&] {
             const int r = rb * 32 + (lane & 31);
             uint16_t* p = a.dq.p + b * a.dq.sb + (int64_t)(hk * a.G + g) * a.dq.sh + (int64_t)(m + r) * a.dq.st + db * 32;
-            store_rows<DT, 32>({dq}, a.scale, r < here ? p : nullptr, a.D - db * 32, lane);
+            store_rows<DT, 32>({dq}, SHIFT ? __builtin_ldexpf(a.scale, -shift) : a.scale, r < here ? p : nullptr, a.D - db * 32, lane);
         };
         // Behind the barrier the next tile is whole and dS has been read. (The sums have been when their writers come back to them:
         // the barrier in front of the product lies between.)
         if constexpr (KG == 1) {
             if (kg == 0) store();
-            finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
+            finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1, BUF ? size0 : size1);
             barrier();
         } else {
-            finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1);
+            finish(BUF ? lse0 : lse1, BUF ? delta0 : delta1, BUF ? size0 : size1);
             if (kg > 0 && kg < KG) {
                 float* to = sums + ((kg - 1) * NB + block) * 1024 + lane * 4;
 #pragma unroll
@@ -689,11 +780,9 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
 #pragma unroll
         for (int t = 0; t < DTL; ++t) { dk[t] = splat16(0.f); dv[t] = splat16(0.f); }
     }
-    if constexpr (kShiftP<DT> != 0) {
-#pragma unroll
-        for (int t = 0; t < DTL; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dv[t][i] *= kUnshiftP<DT>;
+    if constexpr (SHIFT) {
+        scale_all(dv, kUnshiftP<DT>);
+        scale_all(dk, __builtin_ldexpf(1.0f, -shift));
     }
     const XBwd& z = arguments_again<XBwd>();
     if (key >= z.N) return;

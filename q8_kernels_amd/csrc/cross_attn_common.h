@@ -76,6 +76,17 @@ __device__ __forceinline__ float add_pair(uint32_t p, float c) {
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, 0x3c003c00u), c, false);
     }
 }
+// c + the squares of both values of a pair
+template <int DT>
+__device__ __forceinline__ float square_sum(uint32_t p, float c) {
+    if constexpr (DT == Q8_BF16) {
+        typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, p), c, false);
+    } else {
+        typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, p), c, false);
+    }
+}
 // What rounding x to 16 bits, code h, left off, as one byte: 8 bits more of the mantissa, signed (values next to a tie give the
 // nearest byte there is). fp32 codes of one sign are in the order of their values, so it is a difference of codes, and with_rest
 // is an addition to one. Values whose 16-bit code has lost bits already (fp16 below 2^-14) get what a byte holds.
