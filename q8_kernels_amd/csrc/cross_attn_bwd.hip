@@ -39,6 +39,8 @@ template <int DT>
 constexpr float kUnshiftP = 1.0f / (1 << kShiftP<DT>);
 constexpr int kMostShift = 60;  // log2 of the largest factor of dS: P |dP| below 2^39 stays finite beside it
 
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
+
 // One column of a block of dS times a power of two, in 16 results of the lanes l and l + 32: the power's change (0 or less) where
 // the largest of them has grown beyond fp16's reach. NaN and infinity change nothing: their column is lost.
 __device__ __forceinline__ int shift_change(const v16f& ds) {
@@ -604,11 +606,6 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
     }
     wait_loads();
     __syncthreads();
-    float most_v = 0.f;
-    if constexpr (SHIFT) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) most_v = fmaxf(most_v, vsize[i]);
-    }
     int shift = kMostShift, least = kMostShift;  // log2 of the present factor of dS, and the least that a tile so far asked for
 
     LaneOffsets<DP> at(lane);
@@ -629,6 +626,9 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
         if constexpr (SHIFT) {
             // The power that brings the bound to 2^14 .. 2^15. It is kept while a tile loses no more than 6 bits by it; and it does not
             // rise more than 40 above the least one, so that the sums so far stay in range.
+            float most_v = 0.f;  // (read again for every tile: no register for it between the products)
+#pragma unroll
+            for (int i = 0; i < W; ++i) most_v = fmaxf(most_v, vsize[i]);
             const float rows_most = group_max<64>((BUF ? size1 : size0)[lane & (TR - 1)]);
             const float bound = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(rows_most * most_v)));
             const int x = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(bound));
@@ -639,7 +639,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
                 scale_all(dk, __builtin_ldexpf(1.0f, next - shift));
                 shift = next;
             }
-            factor = __builtin_ldexpf(kUnshiftP<DT>, shift);
+            factor = power_of_two(shift - kShiftP<DT>);
         }
         if (!idle) {
 #pragma unroll

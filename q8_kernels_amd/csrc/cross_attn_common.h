@@ -89,13 +89,15 @@ __device__ __forceinline__ float square_sum(uint32_t p, float c) {
 }
 // What rounding x to 16 bits, code h, left off, as one byte: 8 bits more of the mantissa, signed (values next to a tie give the
 // nearest byte there is). fp32 codes of one sign are in the order of their values, so it is a difference of codes, and with_rest
-// is an addition to one. Values whose 16-bit code has lost bits already (fp16 below 2^-14) get what a byte holds.
+// is an addition to one. fp16 below 2^-14, whose step is 2^-24 whatever the value, gets the largest byte where that does not
+// reach: some of the way. (The difference to zero is 0 or more, so zero's byte is.)
 template <int DT>
 constexpr int kRestShift = DT == Q8_BF16 ? 8 : 5;
 template <int DT>
-__device__ __forceinline__ uint32_t rest_of(float x, uint32_t h) {
-    const int d = (int)(__float_as_uint(x) - __float_as_uint(unpack<DT>(h))), r = (d + (1 << (kRestShift<DT> - 1))) >> kRestShift<DT>;
-    return (uint32_t)(r < -128 ? -128 : r > 127 ? 127 : r) & 0xffu;
+__device__ __forceinline__ uint32_t rest_of(float x, uint32_t h) {  // in bits 8 .. 15
+    constexpr int up = 8 - kRestShift<DT>, most = 0x7f7f >> up, least = -(0x8000 >> up);
+    const int d = (int)(__float_as_uint(x) - __float_as_uint(unpack<DT>(h)));
+    return ((uint32_t)(d < least ? least : d < most ? d : most) << up) + 0x80u;
 }
 template <int DT>
 __device__ __forceinline__ float with_rest(uint32_t h, uint32_t bytes, int k) {
@@ -104,7 +106,9 @@ __device__ __forceinline__ float with_rest(uint32_t h, uint32_t bytes, int k) {
 // the bytes of x0 .. x3, whose codes are in lo and hi
 template <int DT>
 __device__ __forceinline__ uint32_t rests_of(float x0, float x1, float x2, float x3, uint32_t lo, uint32_t hi) {
-    return rest_of<DT>(x0, lo & 0xffffu) | rest_of<DT>(x1, lo >> 16) << 8 | rest_of<DT>(x2, hi & 0xffffu) << 16 | rest_of<DT>(x3, hi >> 16) << 24;
+    const uint32_t a = __builtin_amdgcn_perm(rest_of<DT>(x1, lo >> 16), rest_of<DT>(x0, lo & 0xffffu), 0x0c0c0501u);
+    const uint32_t b = __builtin_amdgcn_perm(rest_of<DT>(x3, hi >> 16), rest_of<DT>(x2, hi & 0xffffu), 0x05010c0cu);
+    return a | b;
 }
 
 __device__ __forceinline__ v16f splat16(float v) {
@@ -418,24 +422,27 @@ __device__ __forceinline__ void store_rows(const v16f (&acc)[DP / 32], float sca
         }
 }
 
-// What that left off, 8 bytes of a lane in the same places
+// What that left off: 16 bytes of a lane, elements 0 .. 15 of 32 in the low lane, 16 .. 31 in the high one
 template <int DT, int DP>
 __device__ __forceinline__ void store_rests(const v16f (&acc)[DP / 32], float scale, uint8_t* p, int D, int lane) {
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+    for (int t = 0; t < DP / 32; ++t) {
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            uint32_t w[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int r = 4 * (i + k);
-                const float x0 = acc[t][r] * scale, x1 = acc[t][r + 1] * scale, x2 = acc[t][r + 2] * scale, x3 = acc[t][r + 3] * scale;
-                w[k] = rests_of<DT>(x0, x1, x2, x3, pack2<DT>(x0, x1), pack2<DT>(x2, x3));
-            }
-            const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false);
-            const int e = t * 32 + (i + (lane >> 5)) * 8;
-            if (p != nullptr && e < D) *reinterpret_cast<v2i*>(p + e) = v2i{(int)x[0], (int)x[1]};
+        for (int i = 0; i < 4; ++i) {
+            const float x0 = acc[t][4 * i] * scale, x1 = acc[t][4 * i + 1] * scale, x2 = acc[t][4 * i + 2] * scale, x3 = acc[t][4 * i + 3] * scale;
+            w[i] = rests_of<DT>(x0, x1, x2, x3, pack2<DT>(x0, x1), pack2<DT>(x2, x3));
         }
+        // lanes l and l + 32: elements 8 i .. + 3 and 8 i + 4 .. + 7; first exchanged into 8 and 8, then into 16 and 16
+        const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false), b = __builtin_amdgcn_permlane32_swap(w[2], w[3], false, false);
+        const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false), y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+        typedef int v4i8 __attribute__((ext_vector_type(4), aligned(8)));
+        const int e = t * 32 + (lane >> 5) * 16;
+        if (p != nullptr) {  // (D is a multiple of 8)
+            if (e + 8 < D) *reinterpret_cast<v4i8*>(p + e) = v4i8{(int)x[0], (int)y[0], (int)x[1], (int)y[1]};
+            else if (e < D) *reinterpret_cast<v2i*>(p + e) = v2i{(int)x[0], (int)y[0]};
+        }
+    }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------

@@ -6,8 +6,9 @@ Element by element: scores are fp32 sums, so p = exp(s) is off by at most es = 2
 + N 2^-24) of itself (products, exponent and its difference from the log-sum, row sum); dS is rounded once where it enters a
 product, the result once at the end. delta = rowsum(dO O) has O from probabilities that were rounded for their product and are
 normalised by the sum of the rounded ones, so with relative roundings r_j it is off by sum_j r_j ds_j, and O itself, kept with 8
-bits more than its type has, by u / 2^8 |O| (next to a tie twice that):
-  edelta: sum_j (u + 2 es) |ds_j| + sum_d |g| (u / 2^7 |o| + 2 es sum_j p |v|) + D 2^-23 sum_d |g o|
+bits more than its type has, by eo = u / 2^8 |O| (next to a tie twice that). Those are bits of its fp32 code, which cannot reach
+across the step 2^-24 of float16 below 2^-14: there it is off by half that step, as O itself is.
+  edelta: sum_j (u + 2 es) |ds_j| + sum_d |g| (eo + 2 es sum_j p |v|) + D 2^-23 sum_d |g o|
   ds: (u + 2 es) |ds| + p (D 2^-23 sum_d |g v| + edelta);  dq, dk: the sums of that and of fp32 additions, and half a step.
 
 All elements together: a value x that is rounded to 16 bits is off by h(x) / sqrt(3) in the square mean, where h(x) is half its
@@ -22,7 +23,7 @@ from q8_kernels_amd import _C, functional as Q8F
 
 pytestmark = pytest.mark.gpu
 attend = Q8F.cross_attention.cross_attention
-TYPES = [torch.bfloat16]
+TYPES = [torch.bfloat16, torch.float16]
 
 
 def half_step(x, dtype):
@@ -46,8 +47,10 @@ def definition(q, k, v, g, scale, valid):
     ds = p * (dp - (g6 * o).sum(-1, keepdim=True))
     dq, dk, dv = scale * (ds @ k6), scale * (ds.transpose(2, 3) @ q6), p.transpose(2, 3) @ g6
 
+    eo = o.abs() * u / 128
+    rough = 2.0 ** -25 * (o.abs() < 2.0 ** -14) * (dtype == torch.float16)
     mag = (p * (1 + es)) @ v6.abs()
-    edelta = ((u + 2 * es) * ds.abs()).sum(-1, keepdim=True) + (g6.abs() * (u / 128 * o.abs() + 2 * es.amax(-1, keepdim=True) * mag + d * 2.0 ** -23 * o.abs())).sum(-1, keepdim=True)
+    edelta = ((u + 2 * es) * ds.abs()).sum(-1, keepdim=True) + (g6.abs() * (eo + rough + 2 * es.amax(-1, keepdim=True) * mag + d * 2.0 ** -23 * o.abs())).sum(-1, keepdim=True)
     eds = ds.abs() * (u + 2 * es) + p * (d * 2.0 ** -23 * (g6.abs() @ v6.abs().transpose(2, 3)) + edelta)
     edq = scale * (eds @ k6.abs() + n * 2.0 ** -24 * (ds.abs() @ k6.abs()))
     edk = scale * (eds.transpose(2, 3) @ q6.abs() + q6.shape[2] * 2.0 ** -24 * (ds.abs().transpose(2, 3) @ q6.abs()))
@@ -58,7 +61,7 @@ def definition(q, k, v, g, scale, valid):
     third = lambda x: half_step(x, dtype).square() / 3  # noqa: E731
     # (a ds below the type's normal numbers is rounded like any other: it enters its product times a power of two)
     step = lambda x: (torch.exp2(torch.floor(torch.log2(x.abs().clamp_min(1e-300)))) * u).square() / 3  # noqa: E731
-    delta = (u * u / 3) * ds.square().sum(-1, keepdim=True)
+    delta = (u * u / 3) * ds.square().sum(-1, keepdim=True) + (g6 * rough).square().sum(-1, keepdim=True) / 3
     square = [scale ** 2 * (step(ds) @ k6.square() + delta * (p @ k6).square()) + third(dq),
               scale ** 2 * (step(ds) + delta * p.square()).transpose(2, 3) @ q6.square() + third(dk),
               step(p).transpose(2, 3) @ g6.square() + third(dv)]
@@ -213,3 +216,13 @@ def test_values_that_are_not_finite_stay_in_their_rows(dev):
             dq, dq2 = (_C.cross_attention_backward(x, q, k, v, o, lse, 0.1, o_low=low)[0] for x in (g, g2))
             assert not torch.isfinite(dq2[:, :, -1].float()).any(-1).any() and torch.isfinite(dq2[:, :, :-32].float()).all()
             assert ((dq2[:, :, :-32].float() - dq[:, :, :-32].float()).abs() <= 2 * half_step(dq[:, :, :-32].float(), torch.float16)).all()
+
+
+@pytest.mark.parametrize("size", SIZES)
+def test_results_that_round_to_zero(dev, size):
+    """Values at the end of float16's range: the result is zero or a few steps, of either sign, and what its rounding left off is not."""
+    q, k, v, g = draw(dev, *size, torch.float16, seed=11)
+    for tiny in (2.0 ** -24, 2.0 ** -20, 0.0):
+        o = attend(q, k, (v.sign() * tiny).half(), 0.1)
+        assert bool((o == 0).any())
+        check(q, k, (v.sign() * tiny).half(), g, 0.1)
