@@ -50,6 +50,12 @@ q8_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.
 void require_gpu(const Tensor& t, const char* name) { TORCH_CHECK(t.is_cuda(), name, " must be a CUDA (HIP) tensor"); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// Forward-mode derivatives are not formed: a dual tensor would lose its tangent without a word where nothing requires a gradient
+// (where something does, torch's autograd refuses it).
+void no_tangents(std::initializer_list<const Tensor*> inputs, const char* who) {
+    for (const Tensor* t : inputs) TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), who, ": forward-mode derivatives are not formed");
+}
+
 // A leaf whose eager graph still lives keeps the stream that graph was built on for its gradients. If that is the default
 // stream, a backward captured on another one would make it wait inside the capture, which ends the process from the engine's
 // thread: refused here, before anything is recorded.
@@ -169,6 +175,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
     const Tensor w = or_none(weight), b = or_none(bias);
+    no_tangents({&x, &w, &b}, "layer_norm");
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) {
         require_gpu(x, "x");
         no_eager_graph(x, {&x, &w, &b}, "layer_norm");
@@ -259,6 +266,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 
 std::array<Tensor, 2> apply_rotary(const Tensor& q, const OptTensor& key, const OptTensor& positions, const Tensor& inv_freq, bool half, double factor) {
     const Tensor k = or_none(key), p = or_none(positions);
+    no_tangents({&q, &k, &inv_freq}, "rotary");
     TORCH_CHECK(!at::GradMode::is_enabled() || !inv_freq.requires_grad(), "rotary: no gradient of inv_freq is formed");
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k))) {
         require_gpu(q, "q and k");
@@ -386,6 +394,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, std::o
                        const OptTensor& key_mask) {
     const double scale = softmax_scale.has_value() ? *softmax_scale : q.dim() && q.size(-1) ? 1.0 / std::sqrt((double)q.size(-1)) : 1.0;
     const Tensor lens = or_none(kv_lens), mask = or_none(key_mask);
+    no_tangents({&q, &k, &v}, "cross_attention");
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v))) {
         require_gpu(q, "q, k and v");
         no_eager_graph(q, {&q, &k, &v}, "cross_attention");
