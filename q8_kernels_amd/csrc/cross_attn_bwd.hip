@@ -893,6 +893,7 @@ struct XBackward {
     hipStream_t stream;
 };
 
+static bool fits(const XPlan& p) { return p.units * p.dq_blocks <= kXMostBlocks && p.units * p.kv_blocks <= kXMostBlocks; }
 static int64_t plan_bytes(const XPlan& p) { return (delta_floats(p) + p.parts) * (int64_t)sizeof(float); }
 static int64_t low_bytes(int64_t B, int H, int M, int D) { return (B * H * M * D + 15) / 16 * 16; }
 // with o_low formed here: it, and behind it what the forward and then the backward use
@@ -928,7 +929,7 @@ static int cross_attn_backward(const char* who, const XBackward& c) {
     if (need && c.workspace == nullptr) return fail(Q8_ERR_NULL, "%s: a workspace of %lld bytes is needed", who, (long long)need);
     if (c.workspace_bytes < need) return fail(Q8_ERR_SHAPE, "%s: workspace of %lld bytes, %lld needed", who, (long long)c.workspace_bytes, (long long)need);
     if (!aligned16(c.workspace)) return fail(Q8_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
-    if (p.units * p.dq_blocks > kXMostBlocks || p.units * p.kv_blocks > kXMostBlocks) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
+    if (!fits(p)) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
     char* work = static_cast<char*>(c.workspace);
     const void* o_low = c.o_low;
     if (form_low) {
@@ -1035,13 +1036,17 @@ static int cross_attn_backward(const char* who, const XBackward& c) {
 using namespace q8;
 
 extern "C" int64_t q8_cross_attn_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
-    if (int e = x_sizes("q8_cross_attn_backward_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
+    const char* who = "q8_cross_attn_backward_workspace";
+    if (int e = x_sizes(who, Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
+    if (!fits(plan(B, H, Hkv, M, N, D))) return fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
     return whole_bytes(B, H, Hkv, M, N, D);
 }
 
 extern "C" int64_t q8_cross_attn_train_backward_workspace(int64_t B, int H, int Hkv, int M, int N, int D) {
-    if (int e = x_sizes("q8_cross_attn_train_backward_workspace", Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
-    return plan_bytes(plan(B, H, Hkv, M, N, D));
+    const char* who = "q8_cross_attn_train_backward_workspace";
+    if (int e = x_sizes(who, Q8_BF16, B, H, Hkv, M, N, D, 1.f)) return e;
+    const XPlan p = plan(B, H, Hkv, M, N, D);
+    return fits(p) ? plan_bytes(p) : fail(Q8_ERR_SHAPE, "%s: sizes out of range", who);
 }
 
 extern "C" int q8_cross_attn_backward(const void* grad, const int64_t* grad_strides, const void* q, const int64_t* q_strides, const void* k,

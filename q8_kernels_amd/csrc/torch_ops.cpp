@@ -2,12 +2,13 @@
 // attention. A training step of theirs is a few microseconds of device work for small tensors; as Python functions the same
 // checks, allocations and autograd bookkeeping cost 147 us a step on the host (22 us forward, the rest in the backward, which
 // runs on a thread of its own with cold caches), so they are done here. Checks raise RuntimeError, a status of libq8_hip
-// raises q8_kernels_amd.Q8Error. Everything runs on the current stream of the tensors' device; nothing synchronises.
+// raises q8_kernels_amd._lib.Q8Error, in a backward too. Everything runs on the current stream of the tensors' device; nothing synchronises.
 //
 // Host code only, compiled against torch; the kernels are reached through the C ABI (include/q8_hip.h).
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
@@ -24,15 +25,18 @@ using OptTensor = std::optional<Tensor>;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-struct StatusError : std::runtime_error {
-    int status;
-    StatusError(int s, const char* text) : std::runtime_error(text), status(s) {}
-};
+// A status becomes a Python error here, which torch carries through its engine's threads as it is (a C++ exception of this module
+// would reach the caller of a backward as a RuntimeError without the status). The error belongs to the thread that made the call.
 void check(int64_t status) {
-    if (status < 0) {
-        const char* text = q8_last_error();
-        throw StatusError((int)status, text && text[0] ? text : q8_strerror((int)status));
-    }
+    if (status >= 0) return;
+    const char* last = q8_last_error();
+    const std::string text = last && last[0] ? last : q8_strerror((int)status);
+    const pybind11::gil_scoped_acquire gil;
+    const pybind11::object type = pybind11::module_::import("q8_kernels_amd._lib").attr("Q8Error");
+    PyErr_SetObject(type.ptr(), type((int)status, text).ptr());
+    python_error error;
+    error.persist();
+    throw error;
 }
 
 int type_of(const Tensor& t) {
@@ -410,9 +414,8 @@ PYBIND11_MODULE(_torch_ops, m) {
     py::register_exception_translator([](std::exception_ptr p) {
         try {
             if (p) std::rethrow_exception(p);
-        } catch (const StatusError& e) {
-            const py::object type = py::module_::import("q8_kernels_amd._lib").attr("Q8Error");
-            PyErr_SetObject(type.ptr(), type(e.status, std::string(e.what())).ptr());
+        } catch (python_error& e) {
+            e.restore();
         }
     });
     m.def("layer_norm", &layer_norm);
