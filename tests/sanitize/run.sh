@@ -12,7 +12,7 @@ SAN="-Xarch_host -fsanitize=address -Xarch_host -fsanitize=undefined -Xarch_host
 FLAGS="--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops"
 pids=""
 newest_header="$(ls -t "$root"/q8_kernels_amd/csrc/*.h "$root"/include/*.h | head -1)"
-for f in api rows fused elementwise gemm attn; do
+for f in api rows fused elementwise gemm attn layernorm rotary cross_attn cross_attn_bwd; do
   src="$root/q8_kernels_amd/csrc/$f.hip"
   if [ -f "$out/$f.o" ] && [ "$out/$f.o" -nt "$src" ] && [ "$out/$f.o" -nt "$newest_header" ]; then continue; fi
   $HIPCC $FLAGS $SAN -c "$src" -o "$out/$f.o" 2> "$out/$f.log" &
