@@ -10,7 +10,7 @@ import torch.nn as nn
 
 from .. import _C
 from .. import functional as Q8F
-from .linear import Q8Linear
+from .linear import Q8Linear, Q8LinearLora
 from .rms_norm import RMSNorm
 
 
@@ -130,7 +130,7 @@ class Attention(nn.Module):
             if isinstance(x, tuple):  # already (int8 codes, row scales)
                 return [layer(x[0], x[1], out_dtype=mm_out_dtype) for layer in layers]
             if (self.fuse_prologue and len(layers) > 1 and x.is_cuda and Q8F.fused.can_fuse_hadamard_quantize(x)
-                    and all(type(layer) is Q8Linear for layer in layers)     # (an adapter's layer needs the values)
+                    and not any(isinstance(layer, Q8LinearLora) for layer in layers)  # (an adapter reads the values)
                     and not (torch.is_grad_enabled() and x.requires_grad)):  # the shared codes carry no gradient
                 xq, xs = Q8F.fused.hadamard_quantize(x)
                 return [layer(xq, xs, out_dtype=mm_out_dtype) for layer in layers]
