@@ -150,9 +150,10 @@ struct Rows32 {
     }
 };
 
-// bf16, us: 2 x 16 heads of 128 on 4, 4096 x 4096 275 to 290 (950 to 1000 TFLOP/s; the matrix instructions alone 131 at 2.1 GHz, a
-// rate that their own load does not leave the clock at), 2 x 16 of 64 on 4, 4096 x 4096 176; 8 single tokens, 32 heads of 128 on 8,
-// 8192 keys 32 to 37 (4.1 to 4.7 TB/s of keys and values: HBM).
+// us: 2 x 16 heads of 128 on 4, 4096 x 4096 fp16 298, with the log-sum and the rest of O 313, bf16 with both 303 to 318 (860 to 910
+// TFLOP/s; the matrix pipes are busy 45 % of the time, the vector units 52 %; the matrix instructions alone would take 131 at 2.1 GHz, a
+// rate that their own load does not leave the clock at); 2 x 16 of 64 on 4, 4096 x 4096 bf16 186, with both 190; 8 single tokens, 32 heads
+// of 128 on 8, 8192 ragged keys bf16 28 to 38 (4.0 to 5.3 TB/s of keys and values: HBM).
 template <int DT, int DP, bool STATS>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
     constexpr int ELEMS = kXTile * DP;
@@ -233,8 +234,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_fwd_kernel(XFwd a) {
 
 // Few keys (NT tiles at most): all of K and V stay in LDS, and a workgroup walks over the rows of its unit instead, each wave
 // by itself, without a barrier; the next 32 rows of Q are on their way meanwhile. The kernel above would fill LDS again for
-// every 128 rows. 2 x 32 heads of 64, ragged lengths: 6144 x 128 keys (NT = 2, three workgroups on a CU) 30 us here and 38 to
-// 48 us there, 6144 x 256 keys (NT = 4, two workgroups) 47 us here and 57 us there.
+// every 128 rows. bf16, 2 x 32 heads of 64: 6144 x 128 keys (NT = 2, three workgroups on a CU) 32 us here and 40 there (ragged lengths
+// 31, 40), 6144 x 256 keys (NT = 4, two workgroups) 52 and 53 (ragged 40, 52).
 template <int DT, int DP, int NT, bool STATS>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd a, int parts) {
     constexpr int ELEMS = kXTile * DP, KS = DP / 16;
@@ -286,8 +287,8 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_few_keys_kernel(XFwd 
 }
 
 // Joins the parts of a row: weights exp2(m_i - max m). D / 4 threads a row, 4 elements each, BATCH parts at a time, their loads
-// all under way together. Two parts of 2 x 23732 rows of 64: 7.8 us (30 MB; with batches
-// of 8 for them too 14 us), 16 parts of 8 x 1024 rows of 128 5.8 us.
+// all under way together. Two parts of 2 x 23732 rows of 64: 7.9 us (30 MB; with batches
+// of 8 for them too 9.7), 8 parts of 8 x 1024 rows of 128 5.6 us.
 template <int DT, int BATCH>
 __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
     const unsigned lanes = (unsigned)a.D / 4, id = blockIdx.x * 256 + threadIdx.x, n = id / lanes, all = a.plan.tail * kXRows;
@@ -340,9 +341,10 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(XFwd a) {
 }
 
 // The kernel for few keys: 256 for heads up to 64, 128 for longer ones (two workgroups on a CU, by LDS), and how many of its
-// workgroups run at once. us, this kernel and the general one, heads of 64: 16 heads, 1024 x 128 6.2, 6.6; 32 x 32, 64 x 64 8.8,
-// 10.7; 64 x 32 on 8, 1 x 100 5.9, 6.8; the other way round only 16 x 16, 300 x 128 11.4, 11.0. Of 128: 2 x 32, 6144 x 128 59, 71;
-// 32, 1 x 128 6.5, 7.2. Of 96: 2 x 32, 6144 x 128 42, 56; 32 x 32, 64 x 64 16.0, 15.5; 13 x 16 on 8, 3610 x 1 98, 93.
+// workgroups run at once. bf16, us, this kernel and the general one, heads of 64: 2 x 32, 6144 x 128 31.7, 39.9; 6144 x 256 51.7, 52.5;
+// 32 x 32, 64 x 64 11.8, 13.0; 64 x 32 on 8, 1 x 100 6.6, 7.0; the other way round 16, 1024 x 128 6.9, 6.4 and 16 x 16, 300 x 128 12.0, 11.4.
+// Of 128: 2 x 32, 6144 x 128 64, 67; 32, 1 x 128 7.2, 7.5. Of 96: 2 x 32, 6144 x 128 48, 61; 32 x 32, 64 x 64 16.9, 16.6; 13 x 16 on 8,
+// 3610 x 1 109, 89.
 static bool few_keys(int N, int D) { return N <= (D <= 64 ? 4 : 2) * kXTile; }
 static int few_blocks(int N, int D) { return D <= 64 && N <= 2 * kXTile ? 768 : 512; }
 

@@ -84,8 +84,8 @@ struct XBwd {
     float* part;         // divided blocks: [splits, tail, 128, D], or [splits, tail, 128, 2 D] (dK, dV)
 };
 
-// bf16, 2 x 16 heads of 128 on 4, 4096 x 4096: 370 us (three products, 1110 TFLOP/s); operands in groups of 2: with groups of 4, as
-// in the forward, 27 registers are spilled and it takes 392. Heads up to 64 fit three waves on a SIMD.
+// 2 x 16 heads of 128 on 4, 4096 x 4096: bf16 380 to 393 us (three products, 1050 to 1090 TFLOP/s), fp16 415; operands in groups of 2:
+// with groups of 4, as in the forward, 27 registers are spilled and it takes 432 to 440. Heads up to 64 fit three waves on a SIMD.
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_kernel(XBwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32, ELEMS = kXTile * DP;
@@ -266,8 +266,8 @@ __global__ __launch_bounds__(kXThreads, DP <= 64 ? 3 : 2) void cross_attn_dq_ker
 
 // A head of more than 96 leaves no registers for V beside K and the two sums (two waves a SIMD have 256 each): V stays in
 // LDS, the rows are walked in tiles of 32, and the order of the instructions is the compiler's (keeping the groups apart costs
-// registers that have to be spilled). bf16, 2 x 16 heads of 128 on 4, 4096 x 4096: 495 us (four products, 1110 TFLOP/s; 784 with V
-// in registers, staged through registers and spilled).
+// registers that have to be spilled). 2 x 16 heads of 128 on 4, 4096 x 4096: bf16 503 to 516 us (four products, 1065 to 1090 TFLOP/s;
+// an earlier build with V in registers, staged through registers and spilled, 784), fp16 557.
 template <int DT, int DP>
 __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
     constexpr int KS = DP / 16, DTL = DP / 32;
@@ -486,11 +486,11 @@ __global__ __launch_bounds__(kXThreads, 2) void cross_attn_dkdv_kernel(XBwd a) {
 // a part of its unit's tiles; the parts' dK and dV are added by the kernel below.
 //
 // Heads of more than 64 have tiles of 32 rows, K's operands from LDS, O and dO for delta only asked for behind the products and
-// the compiler's order of instructions: what two waves on a SIMD have registers for (43 spilled ones otherwise; 2 x 32 heads of
-// 128, 6144 rows, 128 keys: 166 us, with 9 spilled ones 138).
+// the compiler's order of instructions: what two waves on a SIMD have registers for, but for 14 (2 x 32 heads of 128, 6144 rows, 128
+// keys bf16: 130 to 142 us; with the groups kept apart 147 to 151; fp16, whose powers cost 14 more of them, 172).
 //
-// bf16, 2 x 32 heads of 64, 6144 rows, 256 keys: 97 us and 7 for the parts (200 MB at 2.1 TB/s; the matrix pipes are busy 29 % of
-// the time, the vector units 33 %, LDS 32 %: between the two barriers of a tile the two waves of a SIMD are in the same phase).
+// bf16, 2 x 32 heads of 64, 6144 rows, 256 keys, ragged: 93 to 118 us and 7 for the parts (274 MB; the matrix pipes are busy 27 % of
+// the time, the vector units 37 %, LDS 30 %: between the two barriers of a tile the two waves of a SIMD are in the same phase).
 template <int DT, int DP, int W>
 __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd a, int parts) {
     constexpr bool LONG = DP > 64;
@@ -849,12 +849,13 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     p.kv_blocks = ((int64_t)N + kXRows - 1) / kXRows;
     const int64_t tiles = (int64_t)(H / Hkv) * (((int64_t)M + kXTile - 1) / kXTile);
     // The kernel for few keys, a workgroup for four tiles of 64 rows or more: one of 8 waves on a CU, or two of 4 (LDS). bf16 times,
-    // this kernel against the other two (B x H x M x N x D), us:
-    //   2 x 32 x 6144 x 256 x 64   111, 146     2 x 32 x 6144 x 128 x 64   65, 97     2 x 32 x 6144 x 128 x 128   138, 229
-    //   2 x 32 x 6144 x 256 x 128  201, 292     2 x 32 x 6144 x 256 x 96  150, 211    11 x 4 x 8 x 2836 x 16 x 128  314, 424
-    //   1 x 32 x 2048 x 128 x 64   25, 34       1 x 16 x 1024 x 64 x 64    18, 19     16 x 32 x 256 x 128 x 64     28, 45
-    // With 129 to 256 keys it takes 1024 tiles to be faster: 8 x 8192 x 256 x 64 38 against 48, but 16 x 2048 x 256 x 64 (512
-    // tiles) 32.2 against 31.5, 8 x 512 x 256 x 64 24.6 against 22.5, 16 x 2048 x 256 x 128 51.3 against 51.0.
+    // this kernel against the other two, with their additions (B x H x M x N x D), us:
+    //   2 x 32 x 6144 x 256 x 64   120, 178     2 x 32 x 6144 x 128 x 64   81, 122    2 x 32 x 6144 x 128 x 128   154, 273
+    //   2 x 32 x 6144 x 256 x 128  233, 326     2 x 32 x 6144 x 256 x 96  155, 231    11 x 32 on 4 x 2836 x 16 x 128  368, 475
+    //   1 x 32 x 2048 x 128 x 64   28, 36       1 x 16 x 1024 x 64 x 64   20.6, 22.8  16 x 32 x 256 x 128 x 64   31, 51
+    // and in fp16 2 x 32 x 6144 x 256 x 64 145, 194; 6144 x 128 x 128 184, 272; 6144 x 256 x 128 292, 343. With 129 to 256 keys it takes
+    // 1024 tiles to be faster for certain: 8 x 8192 x 256 x 64 39.5 against 44.8; with 512 either is, 16 x 2048 x 256 x 64 31.2 against
+    // 32.6, 16 x 2048 x 256 x 128 54.9 against 55.0, and 8 x 512 x 256 x 64 (64 tiles) 26.3 against 26.1.
     const int at_once = N > kXRows ? 256 : 512;
     if (p.units > 0 && M > 0 && N > 0 && (N <= kXRows || (N <= 2 * kXRows && p.units * tiles >= 4 * at_once)) && p.units <= kXMostBlocks / 2) {
         p.few = N > kXRows ? 8 : 4;
@@ -866,7 +867,7 @@ static XPlan plan(int64_t B, int H, int Hkv, int M, int N, int D) {
     }
     // Workgroups that run at once on the 256 CUs, by the registers of a lane. A tile takes these kernels 1.3 and 1.7 times what it
     // takes the forward, which is what the floats of a part (for dK and dV twice as many) are weighed with: 8 heads of 128,
-    // 1024 x 1024 58 us with dK and dV in 4 parts, 71 in one.
+    // 1024 x 1024 60 us, dK and dV in 4 parts or more; 77 with none divided.
     p.dq = schedule(p.units * p.dq_blocks, N, D <= 32 ? 1024 : D <= 64 ? 768 : 512, 0.75 * (p.rows < kXRows ? p.rows : kXRows) * D);
     p.kv = schedule(p.units * p.kv_blocks, tiles * kXTile, D <= 32 ? 1024 : 512, (double)(N < kXRows ? N : kXRows) * D);
     const int64_t dq = p.dq.parts() * kXRows * D, kv = p.kv.parts() * kXRows * 2 * D;

@@ -364,8 +364,9 @@ struct XSchedule {
 // are divided (into parts of four tiles or more) with the number that ends first by this estimate, in tiles: a workgroup takes one
 // tile's time longer than its walk; a CU with one workgroup on it works a tile off faster than one with all its slots taken (half
 // the slots: 0.6 of the time); parts are written, read and joined: 6 tiles' time for 128 x 128 floats of every slot, and 2 for the
-// launch. Forward, us: 3 x 16 heads of 128, 700 x 700 (288 blocks) 22 whole, 41 in three parts; 8 x 16 heads of 64, 512 x 2048 (512
-// blocks) 46 whole, 62 in two; 8 single tokens, 8192 keys (64 blocks) 35 in 8 parts, 37 in 16, 43 in 32.
+// launch. Forward, bf16, us with the join: 3 x 16 heads of 128, 700 x 700 (288 blocks) 32 whole, 47 in two parts, 52 in three; 8 x 16
+// heads of 64, 512 x 2048 (512 blocks) 55 whole, 68 in two; 8 single tokens, 32 heads of 128 on 8, 8192 keys (64 blocks) 59 in 8 parts, 64
+// in 4, 63 in 16, 72 in 32.
 inline XSchedule schedule(int64_t blocks, int64_t length, int slots, double floats) {
     XSchedule s;
     s.full = (unsigned)(blocks / slots * slots);
@@ -386,7 +387,7 @@ inline XSchedule schedule(int64_t blocks, int64_t length, int slots, double floa
 }
 // Into how many parts each of `units` walks of `steps` goes, `least` steps each or more, when `slots` workgroups run at once: the
 // number with which the last one ends first, a workgroup costing about two steps beside its walk. (44 walks of 360 tiles on 512
-// slots, backward with 16 keys of 128: 11 parts 314 us; 12, whose last 16 workgroups wait for a free place, 476.)
+// slots, backward with 16 keys of 128: 11 parts 372 us; 12, whose last 16 workgroups wait for a free place, 548.)
 inline int walk_parts(int64_t units, int64_t steps, int slots, int least) {
     const int64_t most = steps > least ? (steps + least - 1) / least : 1;
     int64_t best = 1, cost = INT64_MAX;

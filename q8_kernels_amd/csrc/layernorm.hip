@@ -14,10 +14,10 @@
 // row of partial sums to the workspace; a second kernel adds those in a fixed order. No atomics: the same inputs give the
 // same bits. The number of workgroups (ln_blocks) trades rows in flight against the partial sums' traffic. Rows of more than
 // 16384 elements (8192 where accesses are by element) leave no registers for the sums: a kernel of its own reads x and g once
-// more for them (1000 x 30000: 61 us; with spilled registers in one kernel 172).
+// more for them (1000 x 30000 bf16: 37 and 30 us; in one kernel, an earlier build whose registers spilled, 172).
 //
-// bf16, 12288 x 2048: forward 19 us (5.3 TB/s, of data partly in the last-level cache), backward 36 us with the parameters' sums
-// (4 of them; 4.2 TB/s of what it has to move). What bounds it: HBM, and at the smallest sizes the launches.
+// bf16, 12288 x 2048, inputs that no cache holds: forward 22 to 23 us (4.4 TB/s), backward 33 and 4 to 5 for the parameters' sums
+// (4.0 TB/s of what it has to move; a copy reaches 5.1). What bounds it: HBM, and at the smallest sizes the launches.
 #include "q8_common.h"
 #include "q8_host.h"
 
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(ln_threads<T>()) void layernorm_kernel(const void* 
 
 // partials: [gridDim.x][2][dim] fp32 (sums of g h, sums of g), or NULL when no parameter needs a gradient.
 // dx NULL: not wanted. The next row is requested before the present one's sums are formed, where the registers
-// hold both (1000 x 16384 fp32, 1024 threads with 16 elements: 56 us without, 78 with).
+// hold both (1000 x 16384 fp32, 1024 threads with 16 elements: 62 us without, 85 with).
 template <int DT, int VEC, int T, int CH>
 __global__ __launch_bounds__(ln_threads<T>()) void layernorm_backward_kernel(const void* __restrict__ g, int64_t g_stride, const void* __restrict__ x,
                                                                            int64_t x_stride, const void* __restrict__ w, int w_f32,
@@ -389,17 +389,18 @@ __global__ __launch_bounds__(1024) void layernorm_params_kernel(const float* __r
 
 // The threads of a row, as LN_BY_DIM below chooses them with the chunks of 8 elements that each holds. The forward takes few
 // threads with up to 32 elements; the backward holds six times as many registers an element, so it takes more threads with 8
-// or 16, which leaves two waves or more on a SIMD. us of forward / backward with the parameters' sums, bf16 unless fp32 is said:
-//   12288 x 2048: 64 threads 20.1 / 37.1, 128 19.1 / 37.1, 256 22.3 / 37.9     4099 x 1155 fp32: 64 14.1 / 43.9, 128 11.0 / 23.6
-//   8192 x 4096:  256 24.6 / 49.0, 512 28.1 / 46.7                             4000 x 3001: 256 of 32 42.9 / 77.0, 512 of 8 22.9 / 27.8
-//   4096 x 8192:  256 26.8 / 66.1 (256 workgroups: 54), 1024 32.2 / 48.6       2000 x 5001: 256 30.3 / 53.0, 512 28.5 / 34.4, 1024 of 8 - / 39.7
-//   65536 x 128:  16 8.8 / 21.3, 64 22.5 / 34.6                                16000 x 601: 64 of 32 32.6 / 73.1, of 16 18.0 / 27.4
+// or 16, which leaves two waves or more on a SIMD. Kernel times in us, forward / backward and the parameters' sums, of threads that
+// each hold the fewest chunks that cover the row; bf16 unless fp32 is said, inputs that no cache holds:
+//   12288 x 2048: 64 threads 23.5 / 35.6, 128 22.1 / 37.2, 256 23.7 / 43.6     4099 x 1155 fp32: 64 15.2 / 37.4, 128 11.8 / 21.8
+//   8192 x 4096:  256 30.1 / 48.8, 512 31.8 / 48.3                             4000 x 3001: 256 28.6 / 30.7, 512 28.3 / 27.6
+//   4096 x 8192:  256 30.8 / 70.3 (256 workgroups: 60.7), 1024 35.2 / 55.4     2000 x 5001: 256 35.5 / 52.4, 512 36.7 / 34.9, 1024 26.1 / 27.0
+//   65536 x 128:  16 8.9 / 21.2, 64 21.4 / 38.3
 static int ln_fwd_threads(int dim) { return dim <= 128 ? 16 : dim <= 1024 ? 64 : dim <= 2048 ? 128 : dim <= 8192 ? 256 : 1024; }
 static int ln_threads_of(int dim, bool vec) { return dim <= 128 ? 16 : dim <= 1024 ? 64 : dim <= 2048 ? 128 : dim <= 4096 ? 512 : dim <= 8192 && !vec ? 512 : 1024; }
 
-// Workgroups of the backward: two rows or more for each group of threads (300 x 2048: 9.8 us, with four 11.4), and few enough
-// that the partial sums stay small beside the rows: 512 (12288 x 2048: 256 39.7 us, 512 37.1, 1024 43.7), 256 of 1024 threads
-// (4096 x 8192: 512 92 us with 256 threads, 256 54), 128 of the longest rows (2000 x 16384: 59 us).
+// Workgroups of the backward: two rows or more for each group of threads (300 x 2048: 10.3 us, with four 14.2), and few enough
+// that the partial sums stay small beside the rows: 512 (12288 x 2048: 256 49.5 us, 512 37.5, 1024 44.0), 256 of 1024 threads
+// (4096 x 8192 with 256 threads: 512 70 us, 256 61), 128 of the longest rows (2000 x 16384: 68 us).
 static int64_t ln_blocks(int64_t rows, int dim, bool vec) {
     const int t = ln_threads_of(dim, vec), groups = (t < 256 ? 256 : t) / t;
     const int64_t most = t < 1024 ? 512 : dim <= 8192 ? 256 : 128, b = (rows + 2 * groups - 1) / (2 * groups);

@@ -8,8 +8,8 @@
 // in fp64, whose whole turns are dropped there; the rest goes to the fp32 sine and cosine as two fp32 numbers, the second to first
 // order, so a far position's are as exact as a near one's, and no table limits the positions. fp32 results are 1.6 roundings off in
 // the square mean, as with tables from fp64 (of one fp32 number of turns: 2.1). A workgroup forms the R / 2 angles of
-// its tokens once, in LDS, and all heads of those tokens use them. bf16, 2 x 6144 tokens, 32 + 32 heads of 64: 41 us for 201 MB
-// (4.9 TB/s; a copy of them reaches 5.1), 16 single tokens of 32 + 8 heads 4.3 us, which is the launch.
+// its tokens once, in LDS, and all heads of those tokens use them. bf16, 2 x 6144 tokens, 32 + 32 heads of 64: 38 to 39 us for
+// 201 MB (5.2 TB/s; a large copy 5.1), 16 single tokens of 32 + 8 heads of 128 4.5 us, which is the launch.
 #include "q8_common.h"
 #include "q8_host.h"
 
@@ -267,7 +267,7 @@ extern "C" int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, c
     RotArgs a{};
     const int size = elem_size(dt), half = half_layout != 0;
     // The elements of an item: 8, or 4 where the pairs' second halves or the strides are not multiples of 8 (fp16, 10183 tokens of
-    // 10 heads of 48, 24 elements of them turned in the half layout: 10.4 us, by single elements 20.7), else one.
+    // 10 heads of 48, 24 elements of them turned in the half layout: 10.0 us, by single elements 20.6), else one.
     auto fits = [&](int n) { return dim % n == 0 && rotary_dim % (half ? 2 * n : n) == 0; };
     int vec = fits(8) ? 8 : fits(4) ? 4 : 1;
     const struct { const void* in; void* out; const int64_t *is, *os; int heads; RotTensor* to; } side[2] = {
@@ -301,8 +301,9 @@ extern "C" int q8_rotary(const void* q, const int64_t* q_strides, void* q_out, c
     a.pairs = rotary_dim / 2;
     a.tokens = tokens;
     a.all_tokens = all;
-    // tokens of a workgroup (63 at most): about 2048 items of 8 elements (2 x 6144 tokens of 64 heads of 64: 34.4 us; 1024 items
-    // 34.0, 4096 35.0), while 1024 workgroups remain (4099 tokens of 10 heads: 6.5 us; 256 workgroups 6.1) and the angles fit
+    // tokens of a workgroup (63 at most): about 2048 items of 8 elements (2 x 4099 tokens of 40 heads of 128: 38.1 us; 1024 items
+    // 42.0, 4096 38.0; of 2 x 6144 and 64 heads of 64 38.2, 38.5, 39.6), while 1024 workgroups remain (10183 tokens of 10 heads of 48:
+    // 10.0 us; 256 workgroups 14.4) and the angles fit
     const int64_t per_token = (int64_t)a.heads * ((dim + 7) / 8);
     int64_t per = 2048 / per_token;
     if (per > all / 1024) per = all / 1024;
