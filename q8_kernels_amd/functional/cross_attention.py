@@ -18,5 +18,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_s
     kv_lens: int32 [B], the keys of each batch element that count (clamped to 0 .. N); key_mask: bool [B, N], True where a key
     counts; both: keys that pass both. What stands in keys and values that do not count is not looked at, and their gradients
     are zeros. A query whose keys all do not count gets zeros. Scores, sums and the softmax are float32; the probabilities
-    (and, in the backward, their gradients) are rounded to the inputs' type where they enter a product. Differentiable once."""
+    (and, in the backward, their gradients) are rounded to the inputs' type where they enter a product, in float16 times a power
+    of two that keeps small and large ones in its range. Differentiable once; a call that is differentiated keeps a byte for
+    each element of the result beside what it was given. Forward-mode tangents are refused."""
     return _lib.ops().cross_attention(q, k, v, softmax_scale, kv_lens, key_mask)
