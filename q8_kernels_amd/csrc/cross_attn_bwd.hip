@@ -590,7 +590,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
 #pragma unroll
                 for (int i = 0; i < 4; ++i) n = square_sum<DT>(dor[k][i], n);
                 n = group_sum<CL>(n);
-                if (chunk == 0 && r < TR) st[r] = r < rows ? n : 0.f;
+                if (chunk == 0 && r < TR) st[r] = r < rows && n < __builtin_inff() ? n : 0.f;  // (a row that is not finite says nothing of the others)
             }
         }
     };

@@ -37,3 +37,5 @@ def test_dual_tensors_are_refused(dev):
     x = torch.randn(2, 2, 4, 64, device=dev).to(torch.bfloat16)
     with forward_ad.dual_level():  # tensors without a tangent: as ever
         assert torch.equal(norm(x), norm(x.clone())) and attend(x, x, x).shape == x.shape
+    with torch.inference_mode():
+        assert torch.equal(norm(x.clone()), norm(x)) and torch.equal(attend(x.clone(), x, x), attend(x, x, x))
