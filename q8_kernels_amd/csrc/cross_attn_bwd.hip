@@ -624,8 +624,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
         copies.group(0, 1, tile_of(qp, a.q, t + 1), tile_of(gp, a.g, t + 1), 0, qnext, gnext);
         float factor = 1.0f;  // of dS beside the shifted P's
         if constexpr (SHIFT) {
-            // The power that brings the bound to 2^14 .. 2^15. It is kept while a tile loses no more than 6 bits by it; and it does not
-            // rise more than 40 above the least one, so that the sums so far stay in range.
+            // The power that brings the bound to 2^14 .. 2^15, but no more than 40 above the least one, so that the sums so far stay in range.
             float most_v = 0.f;  // (read again for every tile: no register for it between the products)
 #pragma unroll
             for (int i = 0; i < W; ++i) most_v = fmaxf(most_v, vsize[i]);
@@ -635,7 +634,7 @@ __global__ __launch_bounds__(W * 64, 2) void cross_attn_bwd_few_keys_kernel(XBwd
             const int own = bound > 0.f ? min(15 - ((x + 1) >> 1), kMostShift) : kMostShift;
             least = min(least, own);
             const int next = min(own, least + 40);
-            if (shift > own || shift < next - 6) {
+            if (shift != next) {
                 scale_all(dk, __builtin_ldexpf(1.0f, next - shift));
                 shift = next;
             }
