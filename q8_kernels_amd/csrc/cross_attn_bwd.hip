@@ -22,9 +22,9 @@
 //
 // delta's error is that of every score's gradient in the row. It is formed from the forward's O with 8 bits
 // more than its result has, normalised by the sum of the rounded P: what is left of the error is sum_j r_j dS_j with the
-// roundings r_j of the forward's P, beside the root of 2 roundings that dS and the result cost nothing with many keys and
-// at most a sixth with few (from the rounded O alone: 512 keys, scores of deviation 4 2.0 roundings, with a mean of 3 in V 6.1, 2
-// keys 2.3). Up to kXExact keys, which one wave or one score tile holds, that goes too: the dS of a row are summed before they
+// roundings r_j of the forward's P. To the 1.4 roundings that dS and the result cost it adds nothing with many keys and at most
+// 0.2 with few (from the rounded O alone dQ is 2.0 off with 512 keys and scores of deviation 4, 6.1 with a mean of 3 in V as well,
+// 2.3 with 2 keys). Up to kXExact keys, which one wave or one score tile holds, that goes too: the dS of a row are summed before they
 // are rounded; the true ones add up to zero, so the sum is the error, and it is taken off.
 //
 // Few workgroups: the walk is divided over several of them, their fp32 sums are added by a third kernel in order.
